@@ -2,6 +2,13 @@
 grouped 4-bit gather_qmm with SwiGLU, down + top-k combine, gated shared
 expert), behind the C-ABI in include/fmx.h and built into libfmx.so."""
 from ._lib import FmxError, load  # noqa: F401
+from .cache import (  # noqa: F401
+    Rope,
+    RopeConfig,
+    attention_scored,
+    attention_shared_prefix,
+    cache_evict,
+)
 from .moe import (  # noqa: F401
     MoEBlock,
     MoEConfig,
@@ -23,6 +30,11 @@ __all__ = [
     "MoEConfig",
     "MoEWeights",
     "QWeight",
+    "Rope",
+    "RopeConfig",
+    "attention_scored",
+    "attention_shared_prefix",
+    "cache_evict",
     "dequantize",
     "gather_qmm",
     "load",

@@ -1,5 +1,5 @@
-"""ctypes binding of libfmx.so (the C-ABI declared in include/fmx.h and
-include/fmx_model.h).
+"""ctypes binding of libfmx.so (the C-ABI declared in include/fmx.h,
+include/fmx_model.h, include/fmx_nemotron.h and include/fmx_cache.h).
 
 This module only loads the library and declares its signatures. It raises
 ImportError when libfmx.so is missing: there is no fallback path.
@@ -135,6 +135,49 @@ class FmxNhMoEWeights(C.Structure):
     ]
 
 
+class FmxHeads(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("batch_stride", C.c_int64),
+        ("token_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+    ]
+
+
+class FmxRopeConfig(C.Structure):
+    _fields_ = [
+        ("dims", C.c_int64),
+        ("base", C.c_double),
+        ("scaling", C.c_int32),
+        ("factor", C.c_double),
+        ("original_max", C.c_int64),
+        ("low", C.c_double),
+        ("high", C.c_double),
+        ("attention_factor", C.c_double),
+    ]
+
+
+class FmxRopeAngles(C.Structure):
+    _fields_ = [
+        ("freqs", C.c_void_p),
+        ("dims", C.c_int64),
+        ("factor", C.c_double),
+        ("interleaved", C.c_int32),
+    ]
+
+
+class FmxAttentionShape(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("batch", C.c_int64),
+        ("seq_len", C.c_int64),
+        ("n_heads", C.c_int64),
+        ("n_kv_heads", C.c_int64),
+        ("head_dim", C.c_int64),
+        ("scale", C.c_float),
+    ]
+
+
 class FmxError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"{STATUS_NAMES.get(status, status)}: {message}")
@@ -153,6 +196,7 @@ STATUS_NAMES = {
 
 P = C.POINTER
 _A = P(FmxArray)
+_H = P(FmxHeads)
 _SIGS = {
     "fmx_abi_version": (C.c_int, []),
     "fmx_status_string": (C.c_char_p, [C.c_int]),
@@ -295,6 +339,31 @@ _SIGS = {
                   C.c_size_t, C.c_void_p, C.c_int]),
     "fmx_nh_moe_workspace_routing": (
         C.c_int, [P(FmxNhMoEConfig), C.c_int64, C.c_void_p, P(C.c_void_p), P(C.c_void_p), P(C.c_void_p)]),
+    # the cache's long-context operators (include/fmx_cache.h)
+    "fmx_rope_frequencies": (C.c_int, [P(FmxRopeConfig), C.c_void_p, P(C.c_double)]),
+    "fmx_rope": (
+        C.c_int,
+        [P(FmxRopeAngles), C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, _H, C.c_void_p, C.c_int, _H,
+         C.c_void_p]),
+    "fmx_rope_append": (
+        C.c_int,
+        [P(FmxRopeAngles), C.c_int] + [C.c_int64] * 5 + [_H] * 3 + [C.c_void_p] * 3 + [C.c_int64] * 2 + [_H] * 3 +
+        [C.c_void_p]),
+    "fmx_attention_shared_prefix_workspace_size": (C.c_size_t, [P(FmxAttentionShape), C.c_int64, C.c_int64]),
+    "fmx_attention_shared_prefix": (
+        C.c_int,
+        [P(FmxAttentionShape), _H, _H, _H, C.c_int64, _H, _H, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, _H,
+         C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fmx_attention_scored_workspace_size": (C.c_size_t, [P(FmxAttentionShape), C.c_int64]),
+    "fmx_attention_scored": (
+        C.c_int,
+        [P(FmxAttentionShape), _H, _H, _H, C.c_int64, C.c_int64] + [C.c_void_p] * 4 + [_H] +
+        [C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fmx_cache_evict_workspace_size": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
+    "fmx_cache_evict": (
+        C.c_int,
+        [C.c_int] + [C.c_int64] * 3 + [_H, _H, C.c_void_p] + [C.c_int64] * 2 + [C.c_void_p] * 2 + [C.c_int64] * 3 +
+        [_H, _H, C.c_void_p, C.c_int64] + [C.c_void_p] * 3 + [C.c_size_t, C.c_void_p]),
 }
 
 FMX_STATUS_WAIT_TIMEOUT = 1

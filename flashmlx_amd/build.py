@@ -33,6 +33,10 @@ SOURCES = [
     "csrc/fmx_sched.cpp",
     "csrc/fmx_nh_decode.hip",
     "csrc/fmx_nh.cpp",
+    "csrc/fmx_rope.hip",
+    "csrc/fmx_cache_attn.hip",
+    "csrc/fmx_evict.hip",
+    "csrc/fmx_cache.cpp",
 ]
 
 ARCH = os.environ.get("FMX_OFFLOAD_ARCH", "gfx950")
