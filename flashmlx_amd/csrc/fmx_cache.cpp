@@ -149,6 +149,7 @@ int check_attention(const fmx_attention_shape* s, int64_t prefix_len, int64_t ma
                 (long long)max_seq);
   if (s->batch * s->seq_len * s->n_heads > (int64_t{1} << 30))
     return fail(FMX_ERR_UNSUPPORTED, "more than 2^30 query rows");
+  if (s->batch * max_seq > (int64_t{1} << 36)) return fail(FMX_ERR_UNSUPPORTED, "more than 2^36 own positions");
   return FMX_OK;
 }
 

@@ -3,17 +3,607 @@
 // (no counterpart in the reference; mx::fast::scaled_dot_product_attention,
 // server/src/model.cpp:879-882, at their place).
 //
-// One workgroup per (query row, head): keys in tiles of 256, a thread per
-// key's score, the running maximum and sum of the softmax in fp32, a thread
-// per dimension for the values. The weights: a thread per key of a (sequence,
-// kv head), over the rows that see it, from the rows' ln sum exp.
+// The rows of one kv head (its query heads of every query) are taken
+// together, so keys and values are read once for all of them: the prefix for
+// the rows of the whole batch, a cache slot for the rows of its sequence.
+// Long axes of keys are cut into pieces; a piece leaves, for each row, the
+// largest score m, the sum l of exp2(t - m) and the values' sum o with the
+// same weights (t: score times log2 e), all fp32, and attn_join_kernel adds
+// the pieces of a row: sum of exp2(m_i - M) o_i over that of exp2(m_i - M) l_i.
+//
+//   attn_narrow_kernel   tiles of 16 or 32 rows, keys straight to registers
+//   attn_join_kernel     a row's pieces to its output; weights of the keys
+//                        from stored scores
+//   attn_weights_kernel  weights of the keys of many rows, scores formed again
+#include <algorithm>
+
 #include "fmx_cache_kernels.hpp"
+#include "fmx_dev.hpp"
 
 namespace fmx {
 
 namespace {
 
-constexpr int kRowThreads = 256;
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kStep = 32;                // keys of a wave's step
+constexpr int kPiece = kStep * kWaves;   // pieces are whole multiples of these
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+__device__ inline float neg_inf() { return -__builtin_huge_valf(); }
+
+// of the four lanes i16 + 16 j: their maximum, their sum, in each
+__device__ inline float quad_max(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ inline float quad_sum(float v) {
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// What a forward's launches agree on.
+struct Plan {
+  int R;                // rows of a sequence and kv head: L * rep
+  // the prefix: rows of all sequences, row b * R + l * rep + (head in group)
+  int p_tiles, p_splits;
+  int p_keys;           // of a split
+  float* p_o;           // [split][nkv][B R][hd]
+  float2* p_ml;         // [split][nkv][B R]
+  // own keys: o_grid pieces over all sequences
+  int o_tiles, o_grid;
+  float* o_o;           // [piece][nkv][R][hd]
+  float2* o_ml;         // [piece][nkv][R]
+  int2* table;          // [B] (first piece, pieces) of a sequence
+  int o_rows;           // rows of a tile
+  int* o_left;          // [piece][nkv][tile] values left out (L > 1 only), or null
+  // weights from stored scores: [B][nkv][R][s_ld] scores times log2 e
+  float* scores;
+  int64_t s_ld;
+  float* lse;           // [B, L, nh]: the caller's or the workspace's, or null
+};
+
+// Pieces of the own keys, found by every workgroup from the device's lengths:
+// sequence b has u_b = ceil(keys / kPiece) units and ceil(u_b / c) pieces of c
+// units, c the smallest that keeps all pieces within the grid: sum u_b / (grid
+// - B) rounded up. Lengths may differ as they like: all pieces but each
+// sequence's last are equally long. Returns the sequence of piece w (-1:
+// none), its piece number in *k and c in *units; workgroup 0 leaves the table.
+__device__ int find_piece(const CacheAttnArgs& a, const Plan& pl, int w, bool write_table, int* k, int* units,
+                          uint32_t* s_tmp) {
+  __shared__ int s_seq, s_k;
+  const int tid = threadIdx.x;
+  auto units_of = [&](int b) {
+    const int64_t n = own_keys(a, seq_slot(a.slots, a.n_slots, b), a.offs[b], a.L - 1);
+    return static_cast<uint32_t>((n + kPiece - 1) / kPiece);
+  };
+  uint32_t mine = 0;
+  for (int b = tid; b < a.B; b += kThreads) mine += units_of(b);
+  uint32_t total;
+  block_exclusive_scan<kThreads>(mine, s_tmp, &total);
+  const uint32_t room = static_cast<uint32_t>(pl.o_grid - a.B);
+  const uint32_t c = max(1u, (total + room - 1) / room);
+  if (tid == 0) s_seq = -1;
+  uint32_t base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+    const int b = b0 + tid;
+    const uint32_t n = b < a.B ? (units_of(b) + c - 1) / c : 0;
+    uint32_t sum;
+    const uint32_t first = base + block_exclusive_scan<kThreads>(n, s_tmp, &sum);
+    if (static_cast<uint32_t>(w) >= first && static_cast<uint32_t>(w) < first + n) {
+      s_seq = b;
+      s_k = w - static_cast<int>(first);
+    }
+    if (write_table && b < a.B) pl.table[b] = make_int2(static_cast<int>(first), static_cast<int>(n));
+    base += sum;
+  }
+  __syncthreads();
+  *k = s_k;
+  *units = static_cast<int>(c);
+  return s_seq;
+}
+
+// ------------------------------------------------------------------ narrow tiles
+//
+// One workgroup per (16 RT rows, piece of keys); each of its four waves takes
+// every fourth step of 32 keys, and they join in LDS at the end.
+//
+// S^T = K Q^T by v_mfma_f32_16x16x32: a lane's A operand is 16 bytes of key
+// i16 (+ 16), its B operand the row i16's query, which stays in registers.
+// The result leaves lane (i16, j) with row i16's scores of keys 4j + r (+ 16):
+// after exp2 the B operand of O^T += V^T P^T as it stands, if key 4j + r is
+// slot 8j + r and key 16 + 4j + r slot 8j + 4 + r of the 32. Its A operand
+// wants the same keys' values of one dimension: a lane loads VPL consecutive
+// dimensions of each of its eight keys (1 KB of four rows per load of a
+// wave), and pairs of keys are put together by v_perm. Nothing passes through
+// LDS and no load is narrower than a cache line's half.
+//
+// Bound by HBM: every key and value is read once, 512 bytes (heads of 128)
+// for 16 bytes of partial results per 128 keys and row. 16 sequences of up to
+// 16001 keys, 32 heads over 4, fp16, weights stored and added: 91 us, 3.0 TB/s;
+// one row per workgroup and head took 6.6 ms, the same values read for every
+// head and queried one after the other.
+template <int HD>
+struct Narrow {
+  static constexpr int KC = HD / 32;            // 32-dimension steps of a score
+  static constexpr int DT = HD / 16;            // 16-dimension tiles of the output
+  static constexpr int VPL = HD / 16;           // dimensions of a key per lane
+  static constexpr int VW = VPL / 2;            // 32-bit words of them
+  static constexpr int kRow = HD + 4;           // floats of a row in LDS
+};
+
+// dimension of A row `row`, tile dt (runs of up to 8 per lane)
+template <int HD>
+__device__ inline int out_dim(int row, int dt) {
+  constexpr int V8 = HD / 16 < 8 ? HD / 16 : 8;
+  return dt / V8 * (16 * V8) + row * V8 + dt % V8;
+}
+
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
+// the larger exponent field, half by half
+template <bool F16>
+__device__ inline u16x2_t top_exp(u16x2_t m, uint32_t w) {
+  return __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w & (F16 ? 0x7c007c00u : 0x7f807f80u)));
+}
+template <bool F16>
+__device__ inline bool is_top(u16x2_t m) {
+  constexpr uint16_t e = F16 ? 0x7c00 : 0x7f80;
+  return m[0] == e || m[1] == e;
+}
+
+// the halves of w that are infinite or NaN made 0
+template <bool F16>
+__device__ inline uint32_t word_finite(uint32_t w) {
+  constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
+  if ((w & e) == e) w &= 0xffff0000u;
+  if ((w & (e << 16)) == e << 16) w &= 0xffffu;
+  return w;
+}
+
+// ANY: hd may be below HD (chunks behind it read as zeros), and the rows of a
+// tile may see different keys (several queries per sequence)
+template <bool F16, int HD, int RT, bool ANY>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
+  using N = Narrow<HD>;
+  constexpr int KC = N::KC, DT = N::DT, VW = N::VW, VPL = N::VPL;
+  typedef act8_t<F16> frag_t;
+  // exp2's results are kept up to 2^10 for fp16 products, so that its
+  // smallest normal number is 2^-24 of the largest weight; bf16 needs none
+  constexpr float kBias = F16 ? 10.0f : 0.0f;
+  __shared__ __attribute__((aligned(16))) float s_o[2][16 * RT][N::kRow];
+  __shared__ float s_m[kWaves][16 * RT], s_l[kWaves][16 * RT];
+  __shared__ uint32_t s_tmp[kWaves + 1];
+  __shared__ int s_left[kWaves];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane & 15, j = lane >> 4;
+
+  // ---- the item: rows, keys
+  const bool prefix = static_cast<int>(blockIdx.x) < n_prefix;
+  const int tiles = prefix ? pl.p_tiles : pl.o_tiles;
+  int item = prefix ? blockIdx.x : blockIdx.x - n_prefix;
+  const int tile = item % tiles;
+  item /= tiles;
+  const int g = item % a.nkv;
+  const int piece = item / a.nkv;
+  int seq = 0, k0, k1;
+  const uint16_t* kb;
+  const uint16_t* vb;
+  int64_t kts, vts;
+  int off = 0;
+  int64_t slot = 0;
+  if (prefix) {
+    k0 = piece * pl.p_keys;
+    k1 = static_cast<int>(min(a.P, static_cast<int64_t>(k0) + pl.p_keys));
+    kb = static_cast<const uint16_t*>(a.kp.p) + g * a.kp.hs;
+    vb = static_cast<const uint16_t*>(a.vp.p) + g * a.vp.hs;
+    kts = a.kp.ts;
+    vts = a.vp.ts;
+  } else {
+    int k, units;
+    seq = find_piece(a, pl, piece, piece == 0 && g == 0 && tile == 0, &k, &units, s_tmp);
+    if (seq < 0) return;
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    slot = seq_slot(a.slots, a.n_slots, seq);
+    off = a.offs[seq];
+    k0 = __builtin_amdgcn_readfirstlane(k * units * kPiece);
+    k1 = static_cast<int>(min(own_keys(a, slot, off, a.L - 1), static_cast<int64_t>(k0) + units * kPiece));
+    k1 = __builtin_amdgcn_readfirstlane(k1);
+    kb = static_cast<const uint16_t*>(a.kc.p) + slot * a.kc.bs + g * a.kc.hs;
+    vb = static_cast<const uint16_t*>(a.vc.p) + slot * a.vc.bs + g * a.vc.hs;
+    kts = a.kc.ts;
+    vts = a.vc.ts;
+  }
+  const int rows = prefix ? a.B * pl.R : pl.R;
+  const int row0 = tile * 16 * RT;
+
+  // ---- queries, and how many keys a row may see
+  frag_t qf[RT][KC];
+  int limit[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int m = min(row0 + rt * 16 + i16, rows - 1);
+    const int b = prefix ? m / pl.R : seq;
+    const int r = prefix ? m - b * pl.R : m;
+    const int l = r / a.rep, h = g * a.rep + r - l * a.rep;
+    const uint16_t* q = static_cast<const uint16_t*>(a.q.p) + b * a.q.bs + l * a.q.ts + h * a.q.hs;
+#pragma unroll
+    for (int t = 0; t < KC; ++t) {
+      u32x4_t w = {0, 0, 0, 0};
+      if (!ANY || 32 * t + 8 * j < a.hd) w = *reinterpret_cast<const u32x4_t*>(q + 32 * t + 8 * j);
+      qf[rt][t] = __builtin_bit_cast(frag_t, w);
+    }
+    limit[rt] = prefix ? k1 : static_cast<int>(min(own_keys(a, slot, off, l), static_cast<int64_t>(k1)));
+  }
+  // keys below this are seen by every row of the tile
+  const int all =
+      prefix ? k1 : static_cast<int>(min(own_keys(a, slot, off, row0 / a.rep), static_cast<int64_t>(k1)));
+
+  f32x4_t o[RT][DT];
+  float mref[RT], lsum[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4_t{0, 0, 0, 0};
+    mref[rt] = neg_inf();
+    lsum[rt] = 0.0f;
+  }
+  const float c = a.scale * kLog2e;
+  float* sc_out[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+    sc_out[rt] = pl.scores && !prefix && row0 + rt * 16 + i16 < rows
+                     ? pl.scores + ((static_cast<int64_t>(seq) * a.nkv + g) * pl.R + row0 + rt * 16 + i16) * pl.s_ld
+                     : nullptr;
+
+  // rows behind the piece's last are read as its last
+  u32x4_t kw[2][KC];
+  uint32_t vw[8][VW];
+  auto load_k = [&](int kk) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint16_t* p = kb + min(kk + 16 * x + i16, k1 - 1) * kts + 8 * j;
+#pragma unroll
+      for (int t = 0; t < KC; ++t)
+        if (!ANY || 32 * t + 8 * j < a.hd) kw[x][t] = *reinterpret_cast<const u32x4_t*>(p + 32 * t);
+        else kw[x][t] = u32x4_t{0, 0, 0, 0};
+    }
+  };
+  auto load_v = [&](int kk) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const uint16_t* p = vb + min(kk + 16 * (s >> 2) + 4 * j + (s & 3), k1 - 1) * vts;
+      if constexpr (VPL == 4) {
+        const int d = 4 * i16;
+        u32x2_t w = {0, 0};
+        if (!ANY || d < a.hd) w = *reinterpret_cast<const u32x2_t*>(p + d);
+        vw[s][0] = w[0];
+        vw[s][1] = w[1];
+      } else {
+#pragma unroll
+        for (int q = 0; q < VPL / 8; ++q) {
+          const int d = 128 * q + 8 * i16;
+          u32x4_t w = {0, 0, 0, 0};
+          if (!ANY || d < a.hd) w = *reinterpret_cast<const u32x4_t*>(p + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vw[s][4 * q + i] = w[i];
+        }
+      }
+    }
+  };
+  // A operand of dimension tile dt from words w(slot)
+  auto v_frag = [&](int dt, auto&& word) {
+    u32x4_t f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = __builtin_amdgcn_perm(word(2 * i + 1, dt / 2), word(2 * i, dt / 2), dt % 2 ? 0x07060302u : 0x05040100u);
+    return __builtin_bit_cast(frag_t, f);
+  };
+
+  bool left_out = false;
+  int kk = k0 + wave * kStep;
+  if (kk < k1) load_k(kk);
+  for (; kk < k1; kk += kPiece) {
+    load_v(kk);
+    f32x4_t s[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        s[rt][x] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < KC; ++t) s[rt][x] = mfma16(__builtin_bit_cast(frag_t, kw[x][t]), qf[rt][t], s[rt][x]);
+      }
+    if (kk + kPiece < k1) load_k(kk + kPiece);
+    const bool part = kk + kStep > all;  // some row does not see all of the step
+    frag_t ph[RT], pw[RT];               // weights: their leading bits and the rest
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float mt = neg_inf();
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[rt][x][r] *= c;
+      if (sc_out[rt]) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          *reinterpret_cast<f32x4_t*>(sc_out[rt] + kk + 16 * x + 4 * j) = s[rt][x];
+      }
+      if (part) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (kk + 16 * x + 4 * j + r >= limit[rt]) s[rt][x][r] = neg_inf();
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[rt][x][r]);
+      mt = quad_max(mt) - kBias;
+      if (__any(mt > mref[rt])) {
+        const float mn = fmaxf(mt, mref[rt]);
+        const float f = __builtin_amdgcn_exp2f(mref[rt] - (mn == neg_inf() ? 0.0f : mn));
+        mref[rt] = mn;
+        lsum[rt] *= f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
+      }
+      const float ms = mref[rt] == neg_inf() ? 0.0f : mref[rt];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(s[rt][x][r] - ms);
+          lsum[rt] += p;
+          typedef typename std::conditional<F16, _Float16, __bf16>::type half_t;
+          const half_t hi = static_cast<half_t>(p);
+          ph[rt][4 * x + r] = hi;
+          pw[rt][4 * x + r] = static_cast<half_t>(p - static_cast<float>(hi));
+        }
+    }
+    if (part) {
+      // values behind the piece count nothing, whatever they hold
+      u16x2_t top = {0, 0};
+#pragma unroll
+      for (int sl = 0; sl < 8; ++sl) {
+        const bool in = kk + 16 * (sl >> 2) + 4 * j + (sl & 3) < k1;
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          vw[sl][w] = in ? vw[sl][w] : 0u;
+          if (ANY && a.L > 1) top = top_exp<F16>(top, vw[sl][w]);
+        }
+      }
+      if (ANY && __any(is_top<F16>(top))) {
+        // infinite or NaN values that some rows see and others do not, whose
+        // weight of 0 makes no 0 of them: left out here, the join adds them
+        // to the rows that see them
+        left_out = true;
+#pragma unroll
+        for (int sl = 0; sl < 8; ++sl)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vw[sl][w] = word_finite<F16>(vw[sl][w]);
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const frag_t f = v_frag(dt, [&](int sl, int w) { return vw[sl][w]; });
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        o[rt][dt] = mfma16(f, ph[rt], o[rt][dt]);
+        o[rt][dt] = mfma16(f, pw[rt], o[rt][dt]);
+      }
+    }
+  }
+
+  if (ANY && lane == 0) s_left[wave] = left_out;
+  // ---- the waves' sums together: waves 0 and 1 leave theirs, 2 and 3 add
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const float l = quad_sum(lsum[rt]);
+    if (j == 0) {
+      s_m[wave][rt * 16 + i16] = mref[rt];
+      s_l[wave][rt * 16 + i16] = l;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float m = s_m[0][rt * 16 + i16];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][rt * 16 + i16]);
+    const float f = __builtin_amdgcn_exp2f(mref[rt] - (m == neg_inf() ? 0.0f : m));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
+  }
+  constexpr int V4 = DT < 8 ? DT : 8;  // consecutive dimensions of a lane and row
+  auto leave = [&](bool add) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int d4 = 0; d4 < DT; d4 += 4) {
+          f32x4_t* p = reinterpret_cast<f32x4_t*>(&s_o[wave & 1][rt * 16 + i16][out_dim<HD>(4 * j + r, d4)]);
+          f32x4_t v = {o[rt][d4][r], o[rt][d4 + 1][r], o[rt][d4 + 2][r], o[rt][d4 + 3][r]};
+          *p = add ? *p + v : v;
+        }
+  };
+  static_assert(V4 % 4 == 0, "dimensions in fours");
+  if (wave < 2) leave(false);
+  __syncthreads();
+  if (wave >= 2) leave(true);
+  __syncthreads();
+
+  const int64_t first = prefix ? (static_cast<int64_t>(piece) * a.nkv + g) * rows + row0
+                               : (static_cast<int64_t>(piece) * a.nkv + g) * pl.R + row0;
+  const int nr = min(16 * RT, rows - row0);
+  float* po = (prefix ? pl.p_o : pl.o_o) + first * a.hd;
+  const int h4 = a.hd / 4;
+  for (int i = tid; i < nr * h4; i += kThreads) {
+    const int r = i / h4, d = (i - r * h4) * 4;
+    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(&s_o[0][r][d]) +
+                      *reinterpret_cast<const f32x4_t*>(&s_o[1][r][d]);
+    *reinterpret_cast<f32x4_t*>(po + static_cast<int64_t>(i) * 4) = v;
+  }
+  if (tid < nr) {
+    float m = s_m[0][tid];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][tid]);
+    float l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      l += s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - (m == neg_inf() ? 0.0f : m));
+    (prefix ? pl.p_ml : pl.o_ml)[first + tid] = make_float2(m, l);
+  }
+  if (ANY && !prefix && tid == 0 && pl.o_left)
+    pl.o_left[(static_cast<int64_t>(piece) * a.nkv + g) * pl.o_tiles + tile] =
+        s_left[0] | s_left[1] | s_left[2] | s_left[3];
+}
+
+// ------------------------------------------------------------------ join
+
+// (m, l) of piece i of a row: the prefix's splits first, then its own pieces
+struct RowPieces {
+  const CacheAttnArgs& a;
+  const Plan& pl;
+  int64_t p_at, o_at, p_stride, o_stride;  // rows
+  int np, n, g, r, first;
+  __device__ RowPieces(const CacheAttnArgs& a_, const Plan& pl_, int b, int g_, int r_)
+      : a(a_), pl(pl_), g(g_), r(r_) {
+    p_stride = static_cast<int64_t>(a.nkv) * a.B * pl.R;
+    o_stride = static_cast<int64_t>(a.nkv) * pl.R;
+    np = pl.p_splits;
+    p_at = (static_cast<int64_t>(g) * a.B + b) * pl.R + r;
+    const int2 t = pl.o_grid ? pl.table[b] : make_int2(0, 0);
+    o_at = t.x * o_stride + static_cast<int64_t>(g) * pl.R + r;
+    n = np + t.y;
+    first = t.x;
+  }
+  // whether a piece left values of the row's tile out
+  __device__ bool left_out() const {
+    int any = 0;
+    for (int i = 0; i < n - np; ++i)
+      any |= pl.o_left[(static_cast<int64_t>(first + i) * a.nkv + g) * pl.o_tiles + r / pl.o_rows];
+    return any != 0;
+  }
+  __device__ float2 ml(int i) const {
+    return i < np ? pl.p_ml[p_at + i * p_stride] : pl.o_ml[o_at + (i - np) * o_stride];
+  }
+  __device__ const float* o(int i) const {
+    return (i < np ? pl.p_o + (p_at + i * p_stride) * a.hd : pl.o_o + (o_at + (i - np) * o_stride) * a.hd);
+  }
+};
+
+constexpr int kJoinLanes = 32;  // per row
+constexpr int kJoinRows = kThreads / kJoinLanes;
+constexpr int kWeightKeys = 1024;  // of a weights workgroup
+
+// Workgroups below n_join: kJoinRows rows each. The others: the weights of
+// kWeightKeys keys of a (sequence, kv head) from the stored scores.
+template <bool F16>
+__global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Plan pl, int n_join, int w_tiles) {
+  const int tid = threadIdx.x;
+  if (static_cast<int>(blockIdx.x) < n_join) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinRows + tid / kJoinLanes;
+    if (row >= static_cast<int64_t>(a.B) * a.L * a.nh) return;
+    const int lane = tid % kJoinLanes;
+    const int t = static_cast<int>(row / a.nh), h = static_cast<int>(row % a.nh);
+    const int b = t / a.L, l = t - b * a.L, g = h / a.rep;
+    const RowPieces ps(a, pl, b, g, l * a.rep + h - g * a.rep);
+    float m = neg_inf();
+    for (int i = lane; i < ps.n; i += kJoinLanes) m = fmaxf(m, ps.ml(i).x);
+#pragma unroll
+    for (int o = kJoinLanes / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float ms = m == neg_inf() ? 0.0f : m;
+    f32x4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    float z = 0.0f;
+    const int d = lane * 4;
+#pragma unroll 4
+    for (int i = 0; i < ps.n; ++i) {
+      const float2 ml = ps.ml(i);
+      const float f = __builtin_amdgcn_exp2f(ml.x - ms);
+      const float* o = ps.o(i);
+      z += ml.y * f;
+      if (d < a.hd) acc[0] += *reinterpret_cast<const f32x4_t*>(o + d) * f;
+      if (d + 128 < a.hd) acc[1] += *reinterpret_cast<const f32x4_t*>(o + d + 128) * f;
+    }
+    if (pl.o_left && ps.left_out()) {
+      // infinite and NaN values among the keys that not all rows of the
+      // tile see (steps of kStep keys): added to the rows that do
+      const int64_t slot = seq_slot(a.slots, a.n_slots, b);
+      const int l0 = ps.r / pl.o_rows * pl.o_rows / a.rep;
+      const int64_t lo = own_keys(a, slot, a.offs[b], l0) / kStep * kStep, hi = own_keys(a, slot, a.offs[b], l);
+      const uint16_t* v = static_cast<const uint16_t*>(a.vc.p) + slot * a.vc.bs + g * a.vc.hs;
+      for (int64_t k = lo; k < hi; ++k)
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (d + 128 * q < a.hd) {
+            const u32x2_t w = *reinterpret_cast<const u32x2_t*>(v + k * a.vc.ts + d + 128 * q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float x = Act<F16>::ld(static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1))));
+              if (!(fabsf(x) < -neg_inf())) acc[q][i] += x;
+            }
+          }
+    }
+    uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + l * a.out.ts + h * a.out.hs;
+    const float inv = z == 0.0f ? 0.0f : 1.0f / z;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (d + 128 * q < a.hd) {
+        u32x2_t w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          w[i] = Act<F16>::st(acc[q][2 * i] * inv) | static_cast<uint32_t>(Act<F16>::st(acc[q][2 * i + 1] * inv)) << 16;
+        *reinterpret_cast<u32x2_t*>(out + d + 128 * q) = w;
+      }
+    if (pl.lse && lane == 0) pl.lse[row] = z == 0.0f ? neg_inf() : (m + __log2f(z)) * kLn2;
+    return;
+  }
+  __shared__ float2 s_row[2 * 16];
+  int item = static_cast<int>(blockIdx.x) - n_join;
+  const int64_t j0 = static_cast<int64_t>(item % w_tiles) * kWeightKeys;
+  item /= w_tiles;
+  const int g = item % a.nkv, b = item / a.nkv;
+  const int64_t slot = seq_slot(a.slots, a.n_slots, b);
+  if (slot < 0) return;
+  const int off = a.offs[b];
+  const int64_t n = own_keys(a, slot, off, a.L - 1);
+  if (j0 < n) {
+    if (tid < pl.R) {
+      const RowPieces ps(a, pl, b, g, tid);
+      float m = neg_inf(), z = 0.0f;
+      for (int i = 0; i < ps.n; ++i) m = fmaxf(m, ps.ml(i).x);
+      const float ms = m == neg_inf() ? 0.0f : m;
+      for (int i = 0; i < ps.n; ++i) {
+        const float2 ml = ps.ml(i);
+        z += ml.y * __builtin_amdgcn_exp2f(ml.x - ms);
+      }
+      s_row[tid] = make_float2(ms, z == 0.0f ? 0.0f : 1.0f / z);
+    }
+    __syncthreads();
+  }
+  const int64_t at = (slot * a.nkv + g) * a.S;
+  const float* sc = pl.scores + (static_cast<int64_t>(b) * a.nkv + g) * pl.R * pl.s_ld;
+  for (int64_t j = j0 + tid; j < min(a.S, j0 + kWeightKeys); j += kThreads) {
+    float w = 0.0f;
+    if (j < n)
+      for (int r = 0; r < pl.R; ++r)
+        if (j < own_keys(a, slot, off, r / a.rep))
+          w += __builtin_amdgcn_exp2f(sc[r * pl.s_ld + j] - s_row[r].x) * s_row[r].y;
+    if (j < n || a.w_in != a.w_out) a.w_out[at + j] = (a.w_in ? a.w_in[at + j] : 0.0f) + w;
+  }
+}
+
+// ------------------------------------------------------------------ weights, scores formed again
 
 template <bool F16>
 __device__ inline float dot8(const float* q, const uint16_t* k, int hd) {
@@ -29,66 +619,15 @@ __device__ inline float dot8(const float* q, const uint16_t* k, int hd) {
   return s;
 }
 
-__device__ inline float block_reduce(float v, bool is_max, float* s_red) {
-  for (int o = 32; o >= 1; o >>= 1) {
-    const float w = __shfl_xor(v, o);
-    v = is_max ? fmaxf(v, w) : v + w;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = s_red[0];
-  for (int w = 1; w < kRowThreads / kWave; ++w) v = is_max ? fmaxf(v, s_red[w]) : v + s_red[w];
-  return v;
-}
-
 template <bool F16>
-__global__ __launch_bounds__(kRowThreads) void attn_rows_kernel(CacheAttnArgs a, float* lse) {
-  __shared__ float s_q[kCacheMaxHd], s_p[kRowThreads], s_red[kRowThreads / kWave];
-  const int tid = threadIdx.x;
-  const int t = blockIdx.x, h = blockIdx.y, b = t / a.L, l = t - b * a.L, g = h / a.rep;
-  const uint16_t* q = static_cast<const uint16_t*>(a.q.p) + b * a.q.bs + l * a.q.ts + h * a.q.hs;
-  if (tid < a.hd) s_q[tid] = Act<F16>::ld(q[tid]);
-  const int64_t slot = a.S > 0 ? seq_slot(a.slots, a.n_slots, b) : -1;
-  const int64_t own = a.S > 0 ? own_keys(a, slot, a.offs[b], l) : 0;
-  float m = -__builtin_huge_valf(), z = 0.0f, o = 0.0f;
-  for (int part = 0; part < 2; ++part) {
-    const int64_t n = part ? own : a.P;
-    if (n == 0) continue;
-    const HeadsView& kv = part ? a.kc : a.kp;
-    const HeadsView& vv = part ? a.vc : a.vp;
-    const uint16_t* kb = static_cast<const uint16_t*>(kv.p) + (part ? slot * kv.bs : 0) + g * kv.hs;
-    const uint16_t* vb = static_cast<const uint16_t*>(vv.p) + (part ? slot * vv.bs : 0) + g * vv.hs;
-    for (int64_t j0 = 0; j0 < n; j0 += kRowThreads) {
-      __syncthreads();
-      const int64_t j = j0 + tid;
-      const float s = j < n ? dot8<F16>(s_q, kb + j * kv.ts, a.hd) * a.scale : -__builtin_huge_valf();
-      const float mt = fmaxf(m, block_reduce(s, true, s_red));
-      const float mu = mt == -__builtin_huge_valf() ? 0.0f : mt;
-      const float p = j < n ? expf(s - mu) : 0.0f;
-      s_p[tid] = p;
-      const float f = expf(m - mu);
-      z = z * f + block_reduce(p, false, s_red);
-      o *= f;
-      m = mt;
-      const int c = static_cast<int>(n - j0 < kRowThreads ? n - j0 : kRowThreads);
-      if (tid < a.hd)
-        for (int i = 0; i < c; ++i) o = __builtin_fmaf(s_p[i], Act<F16>::ld(vb[(j0 + i) * vv.ts + tid]), o);
-    }
-  }
-  uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + l * a.out.ts + h * a.out.hs;
-  if (tid < a.hd) out[tid] = Act<F16>::st(z == 0.0f ? 0.0f : o / z);
-  if (tid == 0 && lse) lse[static_cast<int64_t>(t) * a.nh + h] = z == 0.0f ? -__builtin_huge_valf() : m + logf(z);
-}
-
-template <bool F16>
-__global__ __launch_bounds__(kRowThreads) void attn_weights_kernel(CacheAttnArgs a, const float* lse) {
+__global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a, Plan pl, int tiles) {
   __shared__ float s_q[kCacheMaxHd];
   const int tid = threadIdx.x;
-  const int b = blockIdx.y / a.nkv, g = blockIdx.y % a.nkv;
+  const int bg = blockIdx.x / tiles;
+  const int b = bg / a.nkv, g = bg % a.nkv;
   const int64_t slot = seq_slot(a.slots, a.n_slots, b);
   if (slot < 0) return;
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * kRowThreads + tid;
+  const int64_t j = static_cast<int64_t>(blockIdx.x % tiles) * kThreads + tid;
   const uint16_t* kb = static_cast<const uint16_t*>(a.kc.p) + slot * a.kc.bs + g * a.kc.hs;
   const int off = a.offs[b];
   float sum = 0.0f;
@@ -102,7 +641,7 @@ __global__ __launch_bounds__(kRowThreads) void attn_weights_kernel(CacheAttnArgs
       __syncthreads();
       if (j < n)
         sum += expf(dot8<F16>(s_q, kb + j * a.kc.ts, a.hd) * a.scale -
-                    lse[(static_cast<int64_t>(b) * a.L + l) * a.nh + h]);
+                    pl.lse[(static_cast<int64_t>(b) * a.L + l) * a.nh + h]);
     }
   }
   if (j < a.S) {
@@ -111,27 +650,126 @@ __global__ __launch_bounds__(kRowThreads) void attn_weights_kernel(CacheAttnArgs
   }
 }
 
-}  // namespace
+// ------------------------------------------------------------------ plan
 
-size_t cache_attn_workspace(const CacheAttnArgs& a) {
-  return a.w_out ? static_cast<size_t>(align_up(static_cast<int64_t>(a.B) * a.L * a.nh * 4, 256)) : 0;
+// workgroups that fill the card: three of 256 threads per CU
+constexpr int64_t kFill = 768;
+
+struct Layout {
+  Plan pl;
+  int rt;
+  size_t bytes;
+};
+
+Layout make_plan(const CacheAttnArgs& a, char* ws) {
+  Layout y{};
+  Plan& pl = y.pl;
+  size_t used = 0;
+  auto take = [&](int64_t n) {
+    char* p = ws ? ws + used : nullptr;
+    used = static_cast<size_t>(align_up(static_cast<int64_t>(used) + n, 256));
+    return p;
+  };
+  pl.R = a.L * a.rep;
+  const int64_t rows_p = static_cast<int64_t>(a.B) * pl.R;
+  const int64_t rt_rows = std::max<int64_t>(a.P > 0 ? rows_p : 0, a.S > 0 ? pl.R : 0);
+  // (heads beyond 128: two tiles' sums leave no registers for the keys)
+  y.rt = rt_rows > 16 && a.hd <= 128 ? 2 : 1;
+  const int tr = 16 * y.rt;
+  if (a.P > 0) {
+    pl.p_tiles = static_cast<int>((rows_p + tr - 1) / tr);
+    const int64_t units = (a.P + kPiece - 1) / kPiece;
+    int64_t splits = std::max<int64_t>(1, kFill / (static_cast<int64_t>(pl.p_tiles) * a.nkv));
+    splits = std::min(splits, units);
+    const int64_t per = (units + splits - 1) / splits;
+    pl.p_keys = static_cast<int>(per * kPiece);
+    pl.p_splits = static_cast<int>((units + per - 1) / per);
+    pl.p_o = reinterpret_cast<float*>(take(pl.p_splits * rows_p * a.nkv * a.hd * 4));
+    pl.p_ml = reinterpret_cast<float2*>(take(pl.p_splits * rows_p * a.nkv * 8));
+  }
+  if (a.S > 0) {
+    pl.o_tiles = (pl.R + tr - 1) / tr;
+    const int64_t units = (a.S + kPiece - 1) / kPiece;
+    // no more pieces than units of 128 keys, and the table's room
+    const int64_t fill = std::max<int64_t>(1, kFill / (static_cast<int64_t>(pl.o_tiles) * a.nkv));
+    pl.o_grid = static_cast<int>(a.B + std::min<int64_t>(fill, a.B * units));
+    pl.o_o = reinterpret_cast<float*>(take(static_cast<int64_t>(pl.o_grid) * a.nkv * pl.R * a.hd * 4));
+    pl.o_ml = reinterpret_cast<float2*>(take(static_cast<int64_t>(pl.o_grid) * a.nkv * pl.R * 8));
+    pl.table = reinterpret_cast<int2*>(take(static_cast<int64_t>(a.B) * 8));
+    pl.o_rows = tr;
+    if (a.L > 1) pl.o_left = reinterpret_cast<int*>(take(static_cast<int64_t>(pl.o_grid) * a.nkv * pl.o_tiles * 4));
+  }
+  if (a.w_out) {
+    if (pl.R <= 32) {
+      pl.s_ld = align_up(a.S, kStep);
+      pl.scores = reinterpret_cast<float*>(take(rows_p * a.nkv * pl.s_ld * 4));
+    } else {
+      pl.lse = reinterpret_cast<float*>(take(static_cast<int64_t>(a.B) * a.L * a.nh * 4));
+    }
+  } else {
+    pl.lse = a.lse;
+  }
+  y.bytes = used;
+  return y;
 }
 
-hipError_t launch_cache_attn(const CacheAttnArgs& a, bool f16, void* ws, hipStream_t stream) {
-  float* lse = a.w_out ? static_cast<float*>(ws) : a.lse;
-  const dim3 grid(static_cast<uint32_t>(a.B * a.L), static_cast<uint32_t>(a.nh));
-  if (f16)
-    hipLaunchKernelGGL(attn_rows_kernel<true>, grid, dim3(kRowThreads), 0, stream, a, lse);
-  else
-    hipLaunchKernelGGL(attn_rows_kernel<false>, grid, dim3(kRowThreads), 0, stream, a, lse);
-  if (a.w_out) {
-    const dim3 wg(static_cast<uint32_t>((a.S + kRowThreads - 1) / kRowThreads), static_cast<uint32_t>(a.B * a.nkv));
-    if (f16)
-      hipLaunchKernelGGL(attn_weights_kernel<true>, wg, dim3(kRowThreads), 0, stream, a, lse);
-    else
-      hipLaunchKernelGGL(attn_weights_kernel<false>, wg, dim3(kRowThreads), 0, stream, a, lse);
+template <bool F16, int HD, bool ANY>
+hipError_t launch_narrow(const CacheAttnArgs& a, const Plan& pl, int rt, hipStream_t stream) {
+  const int64_t n_prefix = static_cast<int64_t>(pl.p_splits) * a.nkv * pl.p_tiles;
+  const int64_t n = n_prefix + static_cast<int64_t>(pl.o_grid) * a.nkv * pl.o_tiles;
+  if (n > 0x7fffffff) return hipErrorInvalidValue;
+  if (n == 0) return hipSuccess;
+  const dim3 grid(static_cast<uint32_t>(n)), wg(kThreads);
+  if constexpr (HD <= 128) {
+    if (rt == 2) {
+      hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, 2, ANY>), grid, wg, 0, stream, a, pl,
+                         static_cast<int>(n_prefix));
+      return hipGetLastError();
+    }
   }
+  hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, 1, ANY>), grid, wg, 0, stream, a, pl, static_cast<int>(n_prefix));
   return hipGetLastError();
+}
+
+template <bool F16>
+hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
+  const Layout y = make_plan(a, static_cast<char*>(ws));
+  const Plan& pl = y.pl;
+  hipError_t e;
+  const bool any = a.L > 1;
+  if (a.hd <= 64)
+    e = a.hd == 64 && !any ? launch_narrow<F16, 64, false>(a, pl, y.rt, stream)
+                           : launch_narrow<F16, 64, true>(a, pl, y.rt, stream);
+  else if (a.hd <= 128)
+    e = a.hd == 128 && !any ? launch_narrow<F16, 128, false>(a, pl, y.rt, stream)
+                            : launch_narrow<F16, 128, true>(a, pl, y.rt, stream);
+  else
+    e = a.hd == 256 && !any ? launch_narrow<F16, 256, false>(a, pl, y.rt, stream)
+                            : launch_narrow<F16, 256, true>(a, pl, y.rt, stream);
+  if (e != hipSuccess) return e;
+  const int64_t n_join = (static_cast<int64_t>(a.B) * a.L * a.nh + kJoinRows - 1) / kJoinRows;
+  const int64_t w_tiles = pl.scores ? (a.S + kWeightKeys - 1) / kWeightKeys : 0;
+  const int64_t grid = n_join + w_tiles * a.nkv * a.B;
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(attn_join_kernel<F16>, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a, pl,
+                     static_cast<int>(n_join), static_cast<int>(w_tiles));
+  e = hipGetLastError();
+  if (e == hipSuccess && a.w_out && !pl.scores) {
+    const int64_t tiles = (a.S + kThreads - 1) / kThreads;
+    if (tiles * a.B * a.nkv > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(attn_weights_kernel<F16>, dim3(static_cast<uint32_t>(tiles * a.B * a.nkv)), dim3(kThreads), 0,
+                       stream, a, pl, static_cast<int>(tiles));
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+}  // namespace
+
+size_t cache_attn_workspace(const CacheAttnArgs& a) { return make_plan(a, nullptr).bytes; }
+
+hipError_t launch_cache_attn(const CacheAttnArgs& a, bool f16, void* ws, hipStream_t stream) {
+  return f16 ? launch<true>(a, ws, stream) : launch<false>(a, ws, stream);
 }
 
 }  // namespace fmx
