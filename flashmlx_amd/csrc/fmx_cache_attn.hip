@@ -12,6 +12,7 @@
 // the pieces of a row: sum of exp2(m_i - M) o_i over that of exp2(m_i - M) l_i.
 //
 //   attn_narrow_kernel   tiles of 16 or 32 rows, keys straight to registers
+//   attn_wide_kernel     tiles of 128 rows, keys and values staged in LDS
 //   attn_join_kernel     a row's pieces to its output; weights of the keys
 //                        from stored scores
 //   attn_weights_kernel  weights of the keys of many rows, scores formed again
@@ -55,17 +56,18 @@ struct Plan {
   int p_keys;           // of a split
   float* p_o;           // [split][nkv][B R][hd]
   float2* p_ml;         // [split][nkv][B R]
-  // own keys: o_grid pieces over all sequences
-  int o_tiles, o_grid;
+  // own keys: o_grid pieces over all sequences, or (wide tiles) o_splits
+  // pieces of every row tile's keys, [split][B][nkv][R]
+  bool p_wide, o_wide;
+  int o_tiles, o_grid, o_splits;
   float* o_o;           // [piece][nkv][R][hd]
   float2* o_ml;         // [piece][nkv][R]
   int2* table;          // [B] (first piece, pieces) of a sequence
-  int o_rows;           // rows of a tile
-  int* o_left;          // [piece][nkv][tile] values left out (L > 1 only), or null
   // weights from stored scores: [B][nkv][R][s_ld] scores times log2 e
   float* scores;
   int64_t s_ld;
   float* lse;           // [B, L, nh]: the caller's or the workspace's, or null
+  bool direct;          // one piece per row: the wide tiles write the output
 };
 
 // Pieces of the own keys, found by every workgroup from the device's lengths:
@@ -164,6 +166,18 @@ __device__ inline uint32_t word_finite(uint32_t w) {
   if ((w & e) == e) w &= 0xffff0000u;
   if ((w & (e << 16)) == e << 16) w &= 0xffffu;
   return w;
+}
+
+// The infinite and NaN values of keys [lo, hi), four dimensions at v, added
+// to a row's sums
+template <bool F16>
+__device__ __attribute__((noinline)) void add_left_out(f32x4_t& acc, const uint16_t* v, int64_t ts, int lo, int hi) {
+  for (int k = lo; k < hi; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = Act<F16>::ld(v[k * ts + i]);
+      if (!(fabsf(x) < -neg_inf())) acc[i] += x;
+    }
 }
 
 // ANY: hd may be below HD (chunks behind it read as zeros), and the rows of a
@@ -383,8 +397,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       }
       if (ANY && __any(is_top<F16>(top))) {
         // infinite or NaN values that some rows see and others do not, whose
-        // weight of 0 makes no 0 of them: left out here, the join adds them
-        // to the rows that see them
+        // weight of 0 makes no 0 of them: left out here, added to the rows
+        // that see them at the end
         left_out = true;
 #pragma unroll
         for (int sl = 0; sl < 8; ++sl)
@@ -449,8 +463,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int h4 = a.hd / 4;
   for (int i = tid; i < nr * h4; i += kThreads) {
     const int r = i / h4, d = (i - r * h4) * 4;
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(&s_o[0][r][d]) +
-                      *reinterpret_cast<const f32x4_t*>(&s_o[1][r][d]);
+    f32x4_t v = *reinterpret_cast<const f32x4_t*>(&s_o[0][r][d]) + *reinterpret_cast<const f32x4_t*>(&s_o[1][r][d]);
+    if (ANY && (s_left[0] | s_left[1] | s_left[2] | s_left[3]))
+      add_left_out<F16>(v, vb + d, vts, max(k0, all / kStep * kStep),
+                        prefix ? k1
+                               : static_cast<int>(min(own_keys(a, slot, off, (row0 + r) / a.rep),
+                                                      static_cast<int64_t>(k1))));
     *reinterpret_cast<f32x4_t*>(po + static_cast<int64_t>(i) * 4) = v;
   }
   if (tid < nr) {
@@ -463,9 +481,330 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       l += s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - (m == neg_inf() ? 0.0f : m));
     (prefix ? pl.p_ml : pl.o_ml)[first + tid] = make_float2(m, l);
   }
-  if (ANY && !prefix && tid == 0 && pl.o_left)
-    pl.o_left[(static_cast<int64_t>(piece) * a.nkv + g) * pl.o_tiles + tile] =
-        s_left[0] | s_left[1] | s_left[2] | s_left[3];
+}
+
+// ------------------------------------------------------------------ wide tiles
+//
+// One workgroup per (128 rows, piece of keys): 32 rows per wave, the keys and
+// values of kWideKeys positions staged in LDS for all four.
+//
+// S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16. Register 8u + 4v + r
+// of a lane (row c of the 32, half h) is the score of key 16u + 8v + 4h + r:
+// after exp2 the B operand of the value product over those 16 keys, if key 16u
+// + 8v + 4h + r is its slot 8h + 4v + r. Values are staged dimension by
+// dimension with the keys in slot order, so that the A operand of a dimension
+// is 16 consecutive bytes: a thread loads 16 bytes of four keys, transposes
+// them by v_perm and writes four keys of each of its eight dimensions. Rows of
+// both arrays are padded by 16 bytes: the 16 lanes that an LDS access serves
+// at a time fall on different banks. The next positions are loaded while
+// these are multiplied.
+//
+// The weights are rounded to the inputs' type for the value product (2^-9 or
+// 2^-12 of each, as random as the values' own rounding); their sum is formed
+// before the rounding. The maximum is only raised when a score lies more than
+// kLazy above it: the weights reach 2^kLazy times kBias' 2^8 at most, in fp16
+// 2^14 of 65504.
+constexpr int kWideRows = 32 * kWaves;
+constexpr int kWideKeys = 64;
+constexpr float kLazy = 6.0f;
+
+__device__ inline f32x16_t mfma32(const bf16x8_t& a, const bf16x8_t& b, const f32x16_t& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x16_t mfma32(const f16x8_t& a, const f16x8_t& b, const f32x16_t& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// of the two lanes c and c + 32
+__device__ inline float half_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ inline float half_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// what a wide launch goes over: pairs (of keys: piece, kv head [, sequence])
+// times row tiles. Blocks go to the 8 XCDs in turn; with the pairs a divisor
+// or a multiple of 8 a pair's tiles meet in one L2.
+struct WideGrid {
+  bool prefix;
+  int pairs, padded, tiles, splits;
+};
+
+template <bool F16, int HD, bool ANY>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD > 128 ? 1 : 2)))
+void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
+  typedef act8_t<F16> frag_t;
+  constexpr int KS = HD / 16;              // score steps
+  constexpr int DT = HD / 32;              // dimension tiles
+  constexpr int kKRow = HD + 8;            // elements of a key's row
+  constexpr int kVRow = kWideKeys + 8;     // of a dimension's
+  constexpr int kBuf = kWideKeys * kKRow + HD * kVRow;
+  constexpr int NK = kWideKeys * HD / 8 / kThreads;       // 16-byte loads of keys per thread
+  constexpr int NV = (kWideKeys / 4 * HD / 8 + kThreads - 1) / kThreads;  // 4-key blocks of values
+  constexpr float kBias = F16 ? 8.0f : 0.0f;
+  __shared__ __attribute__((aligned(16))) uint16_t s_kv[2][kBuf];
+  __shared__ int s_left;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c32 = lane & 31, h2 = lane >> 5;
+
+  // ---- the item
+  const int pair = blockIdx.x % wg.padded;
+  if (pair >= wg.pairs) return;
+  const int tile = wg.tiles - 1 - static_cast<int>(blockIdx.x / wg.padded);  // the rows that see most first
+  const int g = pair % a.nkv;
+  const int split = wg.prefix ? pair / a.nkv : pair / a.nkv % wg.splits;
+  const int seq = wg.prefix ? 0 : pair / a.nkv / wg.splits;
+  const int rows = wg.prefix ? a.B * pl.R : pl.R;
+  const int row0 = tile * kWideRows;
+  int64_t slot = 0;
+  int off = 0, k0, k1, all;
+  const uint16_t* kb;
+  const uint16_t* vb;
+  int64_t kts, vts;
+  if (wg.prefix) {
+    k0 = split * pl.p_keys;
+    k1 = static_cast<int>(min(a.P, static_cast<int64_t>(k0) + pl.p_keys));
+    all = k1;
+    kb = static_cast<const uint16_t*>(a.kp.p) + g * a.kp.hs;
+    vb = static_cast<const uint16_t*>(a.vp.p) + g * a.vp.hs;
+    kts = a.kp.ts;
+    vts = a.vp.ts;
+  } else {
+    slot = seq_slot(a.slots, a.n_slots, seq);
+    off = a.offs[seq];
+    const int n = static_cast<int>(own_keys(a, slot, off, (min(row0 + kWideRows, rows) - 1) / a.rep));
+    const int per = (n + wg.splits * kWideKeys - 1) / (wg.splits * kWideKeys) * kWideKeys;
+    k0 = min(split * per, n);
+    k1 = min(k0 + per, n);
+    all = min(k1, static_cast<int>(own_keys(a, slot, off, row0 / a.rep)));
+    kb = static_cast<const uint16_t*>(a.kc.p) + (slot < 0 ? 0 : slot) * a.kc.bs + g * a.kc.hs;
+    vb = static_cast<const uint16_t*>(a.vc.p) + (slot < 0 ? 0 : slot) * a.vc.bs + g * a.vc.hs;
+    kts = a.kc.ts;
+    vts = a.vc.ts;
+  }
+  k0 = __builtin_amdgcn_readfirstlane(k0);
+  k1 = __builtin_amdgcn_readfirstlane(k1);
+  all = __builtin_amdgcn_readfirstlane(all);
+  if (ANY && tid == 0) s_left = 0;
+
+  // ---- this lane's row
+  const int m = row0 + wave * 32 + c32;
+  const int mr = min(m, rows - 1);
+  const int b = wg.prefix ? mr / pl.R : seq;
+  const int r = wg.prefix ? mr - b * pl.R : mr;
+  const int l = r / a.rep, h = g * a.rep + r - l * a.rep;
+  const int limit = wg.prefix ? k1 : min(k1, static_cast<int>(own_keys(a, slot, off, l)));
+  // of the wave's rows: the fewest and the most keys one sees
+  const int w_all = wg.prefix ? k1 : __builtin_amdgcn_readfirstlane(limit);
+  const int w_end = wg.prefix ? k1 : __builtin_amdgcn_readlane(limit, 31);
+  frag_t qf[KS];
+  {
+    const uint16_t* q = static_cast<const uint16_t*>(a.q.p) + b * a.q.bs + l * a.q.ts + h * a.q.hs;
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      u32x4_t w = {0, 0, 0, 0};
+      if (!ANY || 16 * t + 8 * h2 < a.hd) w = *reinterpret_cast<const u32x4_t*>(q + 16 * t + 8 * h2);
+      qf[t] = __builtin_bit_cast(frag_t, w);
+    }
+  }
+
+  // ---- staging
+  u32x4_t kr[NK], vr[NV][4];
+  const int kg = tid & 15;
+  auto load = [&](int kt) {
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int x = tid + i * kThreads;
+      const int key = x / (HD / 8), ch = x % (HD / 8);
+      kr[i] = u32x4_t{0, 0, 0, 0};
+      if (!ANY || 8 * ch < a.hd)
+        kr[i] = *reinterpret_cast<const u32x4_t*>(kb + min(kt + key, k1 - 1) * kts + 8 * ch);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int ch = (tid >> 4) + i * (kThreads / 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        vr[i][e] = u32x4_t{0, 0, 0, 0};
+        if (8 * ch < (ANY ? a.hd : HD))
+          vr[i][e] = *reinterpret_cast<const u32x4_t*>(vb + min(kt + 4 * kg + e, k1 - 1) * vts + 8 * ch);
+      }
+    }
+  };
+  auto store = [&](int kt, int buf) {
+    uint16_t* sk = s_kv[buf];
+    uint16_t* sv = s_kv[buf] + kWideKeys * kKRow;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int x = tid + i * kThreads;
+      *reinterpret_cast<u32x4_t*>(sk + x / (HD / 8) * kKRow + x % (HD / 8) * 8) = kr[i];
+    }
+    if (kt + kWideKeys > all) {
+      // values behind the piece count nothing, whatever they hold; infinite
+      // and NaN ones that not all rows see are left out and added at the end
+      u16x2_t top = {0, 0};
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = kt + 4 * kg + e < k1;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            vr[i][e][w] = in ? vr[i][e][w] : 0u;
+            if (ANY && a.L > 1) top = top_exp<F16>(top, vr[i][e][w]);
+          }
+        }
+      if (ANY && is_top<F16>(top)) {
+        s_left = 1;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) vr[i][e][w] = word_finite<F16>(vr[i][e][w]);
+      }
+    }
+    // keys 4 kg ..: 16 u + 8 v + 4 h of the 64, at 16 u + 8 h + 4 v
+    const int pos = (kg >> 2) * 16 + (kg & 1) * 8 + (kg >> 1 & 1) * 4;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int ch = (tid >> 4) + i * (kThreads / 16);
+      if (ch < HD / 8) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
+          const u32x2_t w = {__builtin_amdgcn_perm(vr[i][1][d / 2], vr[i][0][d / 2], sel),
+                             __builtin_amdgcn_perm(vr[i][3][d / 2], vr[i][2][d / 2], sel)};
+          *reinterpret_cast<u32x2_t*>(sv + (8 * ch + d) * kVRow + pos) = w;
+        }
+      }
+    }
+  };
+
+  f32x16_t o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
+  float mref = neg_inf(), lsum = 0.0f;
+  const float sc = a.scale * kLog2e;
+
+  if (k0 < k1) {
+    load(k0);
+    store(k0, 0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (int kt = k0; kt < k1; kt += kWideKeys, buf ^= 1) {
+    const bool more = kt + kWideKeys < k1;
+    if (more) load(kt + kWideKeys);
+    if (kt < w_end) {
+      const uint16_t* sk = s_kv[buf];
+      const uint16_t* sv = s_kv[buf] + kWideKeys * kKRow;
+      f32x16_t s[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < KS; ++t)
+          s[x] = mfma32(*reinterpret_cast<const frag_t*>(sk + (32 * x + c32) * kKRow + 16 * t + 8 * h2), qf[t], s[x]);
+      }
+      if (kt + kWideKeys > w_all) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (kt + 32 * x + 8 * (i >> 2) + 4 * h2 + (i & 3) >= limit) s[x][i] = neg_inf();
+      }
+      float mt = neg_inf();
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[x][i]);
+      mt = half_max(mt) * sc - kBias;
+      if (__any(mt > mref + kLazy)) {
+        const float mn = fmaxf(mt, mref);
+        const float f = __builtin_amdgcn_exp2f(mref - (mn == neg_inf() ? 0.0f : mn));
+        mref = mn;
+        lsum *= f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+      }
+      const float ms = mref == neg_inf() ? 0.0f : mref;
+      frag_t pf[4];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], sc, -ms));
+          lsum += p;
+          typedef typename std::conditional<F16, _Float16, __bf16>::type half_t;
+          pf[2 * x + (i >> 3)][i & 7] = static_cast<half_t>(p);
+        }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          o[dt] = mfma32(*reinterpret_cast<const frag_t*>(sv + (32 * dt + c32) * kVRow + 16 * t + 8 * h2), pf[t], o[dt]);
+    }
+    if (more) store(kt + kWideKeys, buf ^ 1);
+    __syncthreads();
+  }
+
+  if (m >= rows) return;
+  if (ANY && s_left) {
+    const int lo = max(k0, k0 + (max(all, k0) - k0) / kWideKeys * kWideKeys);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = 32 * dt + 8 * q + 4 * h2;
+        if (d >= a.hd) continue;
+        f32x4_t v = {o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
+        add_left_out<F16>(v, vb + d, vts, lo, limit);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[dt][4 * q + i] = v[i];
+      }
+  }
+  const float z = half_sum(lsum);
+  if (pl.direct) {
+    const float inv = z == 0.0f ? 0.0f : 1.0f / z;
+    uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + l * a.out.ts + h * a.out.hs;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = 32 * dt + 8 * q + 4 * h2;
+        u32x2_t w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          w[i] = Act<F16>::st(o[dt][4 * q + 2 * i] * inv) |
+                 static_cast<uint32_t>(Act<F16>::st(o[dt][4 * q + 2 * i + 1] * inv)) << 16;
+        if (!ANY || d < a.hd) *reinterpret_cast<u32x2_t*>(out + d) = w;
+      }
+    if (pl.lse && h2 == 0)
+      pl.lse[(static_cast<int64_t>(b) * a.L + l) * a.nh + h] = z == 0.0f ? neg_inf() : (mref + __log2f(z)) * kLn2;
+    return;
+  }
+  const int64_t at = wg.prefix ? (static_cast<int64_t>(split) * a.nkv + g) * rows + m
+                               : ((static_cast<int64_t>(split) * a.B + seq) * a.nkv + g) * pl.R + m;
+  float* po = (wg.prefix ? pl.p_o : pl.o_o) + at * a.hd;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * dt + 8 * q + 4 * h2;
+      if (!ANY || d < a.hd)
+        *reinterpret_cast<f32x4_t*>(po + d) =
+            f32x4_t{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
+    }
+  if (h2 == 0) (wg.prefix ? pl.p_ml : pl.o_ml)[at] = make_float2(mref, z);
 }
 
 // ------------------------------------------------------------------ join
@@ -475,24 +814,21 @@ struct RowPieces {
   const CacheAttnArgs& a;
   const Plan& pl;
   int64_t p_at, o_at, p_stride, o_stride;  // rows
-  int np, n, g, r, first;
-  __device__ RowPieces(const CacheAttnArgs& a_, const Plan& pl_, int b, int g_, int r_)
-      : a(a_), pl(pl_), g(g_), r(r_) {
+  int np, n;
+  __device__ RowPieces(const CacheAttnArgs& a_, const Plan& pl_, int b, int g, int r) : a(a_), pl(pl_) {
     p_stride = static_cast<int64_t>(a.nkv) * a.B * pl.R;
     o_stride = static_cast<int64_t>(a.nkv) * pl.R;
     np = pl.p_splits;
     p_at = (static_cast<int64_t>(g) * a.B + b) * pl.R + r;
-    const int2 t = pl.o_grid ? pl.table[b] : make_int2(0, 0);
+    int2 t = make_int2(0, 0);
+    if (pl.o_wide) {
+      t = make_int2(b, pl.o_splits);
+    } else if (pl.o_grid) {
+      t = pl.table[b];
+    }
     o_at = t.x * o_stride + static_cast<int64_t>(g) * pl.R + r;
+    if (pl.o_wide) o_stride *= a.B;
     n = np + t.y;
-    first = t.x;
-  }
-  // whether a piece left values of the row's tile out
-  __device__ bool left_out() const {
-    int any = 0;
-    for (int i = 0; i < n - np; ++i)
-      any |= pl.o_left[(static_cast<int64_t>(first + i) * a.nkv + g) * pl.o_tiles + r / pl.o_rows];
-    return any != 0;
   }
   __device__ float2 ml(int i) const {
     return i < np ? pl.p_ml[p_at + i * p_stride] : pl.o_ml[o_at + (i - np) * o_stride];
@@ -534,25 +870,6 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Pl
       z += ml.y * f;
       if (d < a.hd) acc[0] += *reinterpret_cast<const f32x4_t*>(o + d) * f;
       if (d + 128 < a.hd) acc[1] += *reinterpret_cast<const f32x4_t*>(o + d + 128) * f;
-    }
-    if (pl.o_left && ps.left_out()) {
-      // infinite and NaN values among the keys that not all rows of the
-      // tile see (steps of kStep keys): added to the rows that do
-      const int64_t slot = seq_slot(a.slots, a.n_slots, b);
-      const int l0 = ps.r / pl.o_rows * pl.o_rows / a.rep;
-      const int64_t lo = own_keys(a, slot, a.offs[b], l0) / kStep * kStep, hi = own_keys(a, slot, a.offs[b], l);
-      const uint16_t* v = static_cast<const uint16_t*>(a.vc.p) + slot * a.vc.bs + g * a.vc.hs;
-      for (int64_t k = lo; k < hi; ++k)
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          if (d + 128 * q < a.hd) {
-            const u32x2_t w = *reinterpret_cast<const u32x2_t*>(v + k * a.vc.ts + d + 128 * q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float x = Act<F16>::ld(static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1))));
-              if (!(fabsf(x) < -neg_inf())) acc[q][i] += x;
-            }
-          }
     }
     uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + l * a.out.ts + h * a.out.hs;
     const float inv = z == 0.0f ? 0.0f : 1.0f / z;
@@ -654,6 +971,11 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a,
 
 // workgroups that fill the card: three of 256 threads per CU
 constexpr int64_t kFill = 768;
+// and of wide tiles: two
+constexpr int64_t kWideFill = 512;
+
+// from more rows on (of a kv head) wide tiles take over
+constexpr int64_t kNarrowRows = 32;
 
 struct Layout {
   Plan pl;
@@ -672,35 +994,50 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
   };
   pl.R = a.L * a.rep;
   const int64_t rows_p = static_cast<int64_t>(a.B) * pl.R;
-  const int64_t rt_rows = std::max<int64_t>(a.P > 0 ? rows_p : 0, a.S > 0 ? pl.R : 0);
+  pl.p_wide = a.P > 0 && rows_p > kNarrowRows;
+  pl.o_wide = a.S > 0 && pl.R > kNarrowRows;
+  const int64_t rt_rows =
+      std::max<int64_t>(a.P > 0 && !pl.p_wide ? rows_p : 0, a.S > 0 && !pl.o_wide ? pl.R : 0);
   // (heads beyond 128: two tiles' sums leave no registers for the keys)
   y.rt = rt_rows > 16 && a.hd <= 128 ? 2 : 1;
   const int tr = 16 * y.rt;
   if (a.P > 0) {
-    pl.p_tiles = static_cast<int>((rows_p + tr - 1) / tr);
+    const int rows = pl.p_wide ? kWideRows : tr;
+    pl.p_tiles = static_cast<int>((rows_p + rows - 1) / rows);
     const int64_t units = (a.P + kPiece - 1) / kPiece;
-    int64_t splits = std::max<int64_t>(1, kFill / (static_cast<int64_t>(pl.p_tiles) * a.nkv));
+    const int64_t fill = pl.p_wide ? kWideFill : kFill;
+    int64_t splits = std::max<int64_t>(1, fill / (static_cast<int64_t>(pl.p_tiles) * a.nkv));
     splits = std::min(splits, units);
     const int64_t per = (units + splits - 1) / splits;
     pl.p_keys = static_cast<int>(per * kPiece);
     pl.p_splits = static_cast<int>((units + per - 1) / per);
+  }
+  if (a.S > 0) {
+    const int64_t units = (a.S + kPiece - 1) / kPiece;
+    if (pl.o_wide) {
+      pl.o_tiles = (pl.R + kWideRows - 1) / kWideRows;
+      const int64_t fill = kWideFill / (static_cast<int64_t>(pl.o_tiles) * a.nkv * a.B);
+      pl.o_splits = static_cast<int>(std::max<int64_t>(1, std::min(fill, units)));
+    } else {
+      pl.o_tiles = (pl.R + tr - 1) / tr;
+      // no more pieces than units of 128 keys, and the table's room
+      const int64_t fill = std::max<int64_t>(1, kFill / (static_cast<int64_t>(pl.o_tiles) * a.nkv));
+      pl.o_grid = static_cast<int>(a.B + std::min<int64_t>(fill, a.B * units));
+      pl.table = reinterpret_cast<int2*>(take(static_cast<int64_t>(a.B) * 8));
+    }
+  }
+  pl.direct = (pl.o_wide && pl.o_splits == 1 && a.P == 0) || (pl.p_wide && pl.p_splits == 1 && a.S == 0);
+  if (a.P > 0 && !pl.direct) {
     pl.p_o = reinterpret_cast<float*>(take(pl.p_splits * rows_p * a.nkv * a.hd * 4));
     pl.p_ml = reinterpret_cast<float2*>(take(pl.p_splits * rows_p * a.nkv * 8));
   }
-  if (a.S > 0) {
-    pl.o_tiles = (pl.R + tr - 1) / tr;
-    const int64_t units = (a.S + kPiece - 1) / kPiece;
-    // no more pieces than units of 128 keys, and the table's room
-    const int64_t fill = std::max<int64_t>(1, kFill / (static_cast<int64_t>(pl.o_tiles) * a.nkv));
-    pl.o_grid = static_cast<int>(a.B + std::min<int64_t>(fill, a.B * units));
-    pl.o_o = reinterpret_cast<float*>(take(static_cast<int64_t>(pl.o_grid) * a.nkv * pl.R * a.hd * 4));
-    pl.o_ml = reinterpret_cast<float2*>(take(static_cast<int64_t>(pl.o_grid) * a.nkv * pl.R * 8));
-    pl.table = reinterpret_cast<int2*>(take(static_cast<int64_t>(a.B) * 8));
-    pl.o_rows = tr;
-    if (a.L > 1) pl.o_left = reinterpret_cast<int*>(take(static_cast<int64_t>(pl.o_grid) * a.nkv * pl.o_tiles * 4));
+  if (a.S > 0 && !pl.direct) {
+    const int64_t pieces = pl.o_wide ? static_cast<int64_t>(pl.o_splits) * a.B : pl.o_grid;
+    pl.o_o = reinterpret_cast<float*>(take(pieces * a.nkv * pl.R * a.hd * 4));
+    pl.o_ml = reinterpret_cast<float2*>(take(pieces * a.nkv * pl.R * 8));
   }
   if (a.w_out) {
-    if (pl.R <= 32) {
+    if (!pl.o_wide) {
       pl.s_ld = align_up(a.S, kStep);
       pl.scores = reinterpret_cast<float*>(take(rows_p * a.nkv * pl.s_ld * 4));
     } else {
@@ -714,9 +1051,26 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
 }
 
 template <bool F16, int HD, bool ANY>
-hipError_t launch_narrow(const CacheAttnArgs& a, const Plan& pl, int rt, hipStream_t stream) {
-  const int64_t n_prefix = static_cast<int64_t>(pl.p_splits) * a.nkv * pl.p_tiles;
-  const int64_t n = n_prefix + static_cast<int64_t>(pl.o_grid) * a.nkv * pl.o_tiles;
+hipError_t launch_parts(const CacheAttnArgs& a, const Plan& pl, int rt, hipStream_t stream) {
+  // wide tiles first: a prefix of many rows, or own keys of many queries
+  for (int part = 0; part < 2; ++part) {
+    if (!(part ? pl.o_wide : pl.p_wide)) continue;
+    WideGrid wg{};
+    wg.prefix = part == 0;
+    wg.splits = part ? pl.o_splits : pl.p_splits;
+    wg.tiles = part ? pl.o_tiles : pl.p_tiles;
+    const int64_t pairs = static_cast<int64_t>(wg.splits) * a.nkv * (part ? a.B : 1);
+    const int64_t padded = pairs <= 8 ? pairs : align_up(pairs, 8);
+    if (padded * wg.tiles > 0x7fffffff) return hipErrorInvalidValue;
+    wg.pairs = static_cast<int>(pairs);
+    wg.padded = static_cast<int>(padded);
+    hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(static_cast<uint32_t>(padded * wg.tiles)),
+                       dim3(kThreads), 0, stream, a, pl, wg);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  const int64_t n_prefix = pl.p_wide ? 0 : static_cast<int64_t>(pl.p_splits) * a.nkv * pl.p_tiles;
+  const int64_t n = n_prefix + (pl.o_wide ? 0 : static_cast<int64_t>(pl.o_grid) * a.nkv * pl.o_tiles);
   if (n > 0x7fffffff) return hipErrorInvalidValue;
   if (n == 0) return hipSuccess;
   const dim3 grid(static_cast<uint32_t>(n)), wg(kThreads);
@@ -738,22 +1092,24 @@ hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
   hipError_t e;
   const bool any = a.L > 1;
   if (a.hd <= 64)
-    e = a.hd == 64 && !any ? launch_narrow<F16, 64, false>(a, pl, y.rt, stream)
-                           : launch_narrow<F16, 64, true>(a, pl, y.rt, stream);
+    e = a.hd == 64 && !any ? launch_parts<F16, 64, false>(a, pl, y.rt, stream)
+                           : launch_parts<F16, 64, true>(a, pl, y.rt, stream);
   else if (a.hd <= 128)
-    e = a.hd == 128 && !any ? launch_narrow<F16, 128, false>(a, pl, y.rt, stream)
-                            : launch_narrow<F16, 128, true>(a, pl, y.rt, stream);
+    e = a.hd == 128 && !any ? launch_parts<F16, 128, false>(a, pl, y.rt, stream)
+                            : launch_parts<F16, 128, true>(a, pl, y.rt, stream);
   else
-    e = a.hd == 256 && !any ? launch_narrow<F16, 256, false>(a, pl, y.rt, stream)
-                            : launch_narrow<F16, 256, true>(a, pl, y.rt, stream);
+    e = a.hd == 256 && !any ? launch_parts<F16, 256, false>(a, pl, y.rt, stream)
+                            : launch_parts<F16, 256, true>(a, pl, y.rt, stream);
   if (e != hipSuccess) return e;
-  const int64_t n_join = (static_cast<int64_t>(a.B) * a.L * a.nh + kJoinRows - 1) / kJoinRows;
+  const int64_t n_join = pl.direct ? 0 : (static_cast<int64_t>(a.B) * a.L * a.nh + kJoinRows - 1) / kJoinRows;
   const int64_t w_tiles = pl.scores ? (a.S + kWeightKeys - 1) / kWeightKeys : 0;
   const int64_t grid = n_join + w_tiles * a.nkv * a.B;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(attn_join_kernel<F16>, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a, pl,
-                     static_cast<int>(n_join), static_cast<int>(w_tiles));
-  e = hipGetLastError();
+  if (grid > 0) {
+    hipLaunchKernelGGL(attn_join_kernel<F16>, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a, pl,
+                       static_cast<int>(n_join), static_cast<int>(w_tiles));
+    e = hipGetLastError();
+  }
   if (e == hipSuccess && a.w_out && !pl.scores) {
     const int64_t tiles = (a.S + kThreads - 1) / kThreads;
     if (tiles * a.B * a.nkv > 0x7fffffff) return hipErrorInvalidValue;
