@@ -15,7 +15,8 @@
 //   attn_wide_kernel     tiles of 128 rows, keys and values staged in LDS
 //   attn_join_kernel     a row's pieces to its output; weights of the keys
 //                        from stored scores
-//   attn_weights_kernel  weights of the keys of many rows, scores formed again
+//   attn_weights_kernel, attn_weights_sum_kernel
+//                        weights of the keys of many rows, scores formed again
 #include <algorithm>
 
 #include "fmx_cache_kernels.hpp"
@@ -66,7 +67,12 @@ struct Plan {
   // weights from stored scores: [B][nkv][R][s_ld] scores times log2 e
   float* scores;
   int64_t s_ld;
-  float* lse;           // [B, L, nh]: the caller's or the workspace's, or null
+  float* lse;           // [B, L, nh]: the caller's, or null
+  // weights of many rows: ln sum exp by log2 e of [B, nkv, R], and sums over
+  // w_rows rows each, [w_parts][B][nkv][S]
+  float* lse2;
+  float* w_part;
+  int w_rows, w_parts;
   bool direct;          // one piece per row: the wide tiles write the output
 };
 
@@ -788,8 +794,11 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
                  static_cast<uint32_t>(Act<F16>::st(o[dt][4 * q + 2 * i + 1] * inv)) << 16;
         if (!ANY || d < a.hd) *reinterpret_cast<u32x2_t*>(out + d) = w;
       }
-    if (pl.lse && h2 == 0)
-      pl.lse[(static_cast<int64_t>(b) * a.L + l) * a.nh + h] = z == 0.0f ? neg_inf() : (mref + __log2f(z)) * kLn2;
+    if (h2 == 0) {
+      const float l2 = z == 0.0f ? neg_inf() : mref + __log2f(z);
+      if (pl.lse) pl.lse[(static_cast<int64_t>(b) * a.L + l) * a.nh + h] = l2 * kLn2;
+      if (pl.lse2) pl.lse2[(static_cast<int64_t>(b) * a.nkv + g) * pl.R + r] = l2;
+    }
     return;
   }
   const int64_t at = wg.prefix ? (static_cast<int64_t>(split) * a.nkv + g) * rows + m
@@ -838,51 +847,75 @@ struct RowPieces {
   }
 };
 
-constexpr int kJoinLanes = 32;  // per row
-constexpr int kJoinRows = kThreads / kJoinLanes;
 constexpr int kWeightKeys = 1024;  // of a weights workgroup
 
-// Workgroups below n_join: kJoinRows rows each. The others: the weights of
-// kWeightKeys keys of a (sequence, kv head) from the stored scores.
+// Workgroups below n_join: one row per wave. The pieces' (m, l) are read a
+// lane each, so that a row waits for two rounds of loads, whatever its number
+// of pieces (a thread of 32 per row walking them one by one took 27 us for 34
+// pieces of 1024 rows). The others: the weights of kWeightKeys keys of a
+// (sequence, kv head) from the stored scores.
 template <bool F16>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Plan pl, int n_join, int w_tiles) {
   const int tid = threadIdx.x;
   if (static_cast<int>(blockIdx.x) < n_join) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinRows + tid / kJoinLanes;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + wave;
     if (row >= static_cast<int64_t>(a.B) * a.L * a.nh) return;
-    const int lane = tid % kJoinLanes;
     const int t = static_cast<int>(row / a.nh), h = static_cast<int>(row % a.nh);
     const int b = t / a.L, l = t - b * a.L, g = h / a.rep;
     const RowPieces ps(a, pl, b, g, l * a.rep + h - g * a.rep);
     float m = neg_inf();
-    for (int i = lane; i < ps.n; i += kJoinLanes) m = fmaxf(m, ps.ml(i).x);
-#pragma unroll
-    for (int o = kJoinLanes / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const float ms = m == neg_inf() ? 0.0f : m;
-    f32x4_t acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    float z = 0.0f;
-    const int d = lane * 4;
-#pragma unroll 4
-    for (int i = 0; i < ps.n; ++i) {
-      const float2 ml = ps.ml(i);
-      const float f = __builtin_amdgcn_exp2f(ml.x - ms);
-      const float* o = ps.o(i);
-      z += ml.y * f;
-      if (d < a.hd) acc[0] += *reinterpret_cast<const f32x4_t*>(o + d) * f;
-      if (d + 128 < a.hd) acc[1] += *reinterpret_cast<const f32x4_t*>(o + d + 128) * f;
+    float2 mine = make_float2(neg_inf(), 0.0f);
+    for (int i = lane; i < ps.n; i += kWave) {
+      mine = ps.ml(i);
+      m = fmaxf(m, mine.x);
     }
+    m = wave_max_f32(m);
+    const float ms = m == neg_inf() ? 0.0f : m;
+    float acc[4] = {0, 0, 0, 0};
+    float z = 0.0f;
+    const int vd = a.hd > 128 ? 4 : 2;  // dimensions of a lane
+    const int d = lane * vd;
+    const bool in = d < a.hd;
+    for (int i0 = 0; i0 < ps.n; i0 += kWave) {
+      if (ps.n > kWave) mine = i0 + lane < ps.n ? ps.ml(i0 + lane) : make_float2(neg_inf(), 0.0f);
+      const float f = __builtin_amdgcn_exp2f(mine.x - ms);
+      z += mine.y * f;
+      const int c = min(kWave, ps.n - i0);
+#pragma unroll 8
+      for (int i = 0; i < c; ++i) {
+        const float fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
+        const float* o = ps.o(i0 + i);
+        if (!in) o -= d;  // lanes behind the row read its start and keep nothing
+        if (vd == 2) {
+          const float2 v = *reinterpret_cast<const float2*>(o + d);
+          acc[0] = __builtin_fmaf(v.x, fi, acc[0]);
+          acc[1] = __builtin_fmaf(v.y, fi, acc[1]);
+        } else {
+          const f32x4_t v = *reinterpret_cast<const f32x4_t*>(o + d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], fi, acc[e]);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o);
     uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + l * a.out.ts + h * a.out.hs;
     const float inv = z == 0.0f ? 0.0f : 1.0f / z;
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-      if (d + 128 * q < a.hd) {
-        u32x2_t w;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          w[i] = Act<F16>::st(acc[q][2 * i] * inv) | static_cast<uint32_t>(Act<F16>::st(acc[q][2 * i + 1] * inv)) << 16;
-        *reinterpret_cast<u32x2_t*>(out + d + 128 * q) = w;
-      }
-    if (pl.lse && lane == 0) pl.lse[row] = z == 0.0f ? neg_inf() : (m + __log2f(z)) * kLn2;
+    if (in) {
+      const auto pair = [&](int e) {
+        return Act<F16>::st(acc[e] * inv) | static_cast<uint32_t>(Act<F16>::st(acc[e + 1] * inv)) << 16;
+      };
+      if (vd == 2)
+        *reinterpret_cast<uint32_t*>(out + d) = pair(0);
+      else
+        *reinterpret_cast<u32x2_t*>(out + d) = u32x2_t{pair(0), pair(2)};
+    }
+    if (lane == 0) {
+      const float l2 = z == 0.0f ? neg_inf() : m + __log2f(z);
+      if (pl.lse) pl.lse[row] = l2 * kLn2;
+      if (pl.lse2) pl.lse2[(static_cast<int64_t>(b) * a.nkv + g) * pl.R + l * a.rep + h - g * a.rep] = l2;
+    }
     return;
   }
   __shared__ float2 s_row[2 * 16];
@@ -921,50 +954,150 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Pl
 }
 
 // ------------------------------------------------------------------ weights, scores formed again
+//
+// One workgroup per (128 keys, part of the rows): a wave keeps 32 keys as the
+// B operand of S = Q K^T and goes over the rows, kSumRows at a time staged in
+// LDS for all four waves with their ln sum exp. A lane then has 16 rows'
+// scores of one key: exp2(t - lse) added up in the lane, over rows in order,
+// in sums of kSumRows rows that are added to the total (a thousand rows' sum
+// is off by tens of roundings, not by a thousand). The parts' sums are added
+// by attn_weights_sum_kernel, in order.
+constexpr int kSumRows = 64;
+constexpr int kSumKeys = 32 * kWaves;
 
-template <bool F16>
-__device__ inline float dot8(const float* q, const uint16_t* k, int hd) {
-  float s = 0.0f;
-  for (int c = 0; c < hd; c += 8) {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(k + c);
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      s = __builtin_fmaf(q[c + 2 * m], Act<F16>::lo(w[m]), s);
-      s = __builtin_fmaf(q[c + 2 * m + 1], Act<F16>::hi(w[m]), s);
-    }
-  }
-  return s;
-}
-
-template <bool F16>
+template <bool F16, int HD, bool ANY>
 __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a, Plan pl, int tiles) {
-  __shared__ float s_q[kCacheMaxHd];
-  const int tid = threadIdx.x;
-  const int bg = blockIdx.x / tiles;
-  const int b = bg / a.nkv, g = bg % a.nkv;
+  typedef act8_t<F16> frag_t;
+  constexpr int KS = HD / 16;
+  constexpr int kRow = HD + 8;
+  constexpr int NQ = kSumRows * HD / 8 / kThreads;
+  __shared__ __attribute__((aligned(16))) uint16_t s_q[2][kSumRows * kRow];
+  __shared__ __attribute__((aligned(16))) float s_lse[2][kSumRows];
+  __shared__ __attribute__((aligned(16))) int s_lim[2][kSumRows];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c32 = lane & 31, h2 = lane >> 5;
+  int item = blockIdx.x;
+  const int tile = item % tiles;
+  item /= tiles;
+  const int part = item % pl.w_parts;
+  item /= pl.w_parts;
+  const int g = item % a.nkv, b = item / a.nkv;
   const int64_t slot = seq_slot(a.slots, a.n_slots, b);
   if (slot < 0) return;
-  const int64_t j = static_cast<int64_t>(blockIdx.x % tiles) * kThreads + tid;
-  const uint16_t* kb = static_cast<const uint16_t*>(a.kc.p) + slot * a.kc.bs + g * a.kc.hs;
   const int off = a.offs[b];
-  float sum = 0.0f;
-  for (int l = 0; l < a.L; ++l) {
-    const int64_t n = own_keys(a, slot, off, l);
-    for (int r = 0; r < a.rep; ++r) {
-      const int h = g * a.rep + r;
-      const uint16_t* q = static_cast<const uint16_t*>(a.q.p) + b * a.q.bs + l * a.q.ts + h * a.q.hs;
-      __syncthreads();
-      if (tid < a.hd) s_q[tid] = Act<F16>::ld(q[tid]);
-      __syncthreads();
-      if (j < n)
-        sum += expf(dot8<F16>(s_q, kb + j * a.kc.ts, a.hd) * a.scale -
-                    pl.lse[(static_cast<int64_t>(b) * a.L + l) * a.nh + h]);
+  const int key0 = tile * kSumKeys;
+  const int n = static_cast<int>(own_keys(a, slot, off, a.L - 1));
+  // rows [r0, r1) of the part, from the first that sees the tile's first key
+  const int64_t l0 = max(static_cast<int64_t>(key0) - off, static_cast<int64_t>(0));
+  int r0 = part * pl.w_rows;
+  const int r1 = min(pl.R, r0 + pl.w_rows);
+  if (key0 >= n || l0 >= a.L) return;
+  r0 = max(r0, static_cast<int>(l0) * a.rep);
+  if (r0 >= r1) return;
+
+  const int key = key0 + wave * 32 + c32;
+  frag_t kf[KS];
+  {
+    const uint16_t* k = static_cast<const uint16_t*>(a.kc.p) + slot * a.kc.bs + g * a.kc.hs + min(key, n - 1) * a.kc.ts;
+#pragma unroll
+    for (int t = 0; t < KS; ++t) {
+      u32x4_t w = {0, 0, 0, 0};
+      if (!ANY || 16 * t + 8 * h2 < a.hd) w = *reinterpret_cast<const u32x4_t*>(k + 16 * t + 8 * h2);
+      kf[t] = __builtin_bit_cast(frag_t, w);
     }
   }
-  if (j < a.S) {
-    const int64_t w = (slot * a.nkv + g) * a.S + j;
-    a.w_out[w] = (a.w_in ? a.w_in[w] : 0.0f) + sum;
+  u32x4_t qr[NQ];
+  float lr = 0.0f;
+  int mr = 0;
+  const uint16_t* qb = static_cast<const uint16_t*>(a.q.p) + b * a.q.bs;
+  const float* lb = pl.lse2 + (static_cast<int64_t>(b) * a.nkv + g) * pl.R;
+  auto load = [&](int r) {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int x = tid + i * kThreads;
+      const int row = min(r + x / (HD / 8), r1 - 1), ch = x % (HD / 8);
+      const int l = row / a.rep;
+      qr[i] = u32x4_t{0, 0, 0, 0};
+      if (!ANY || 8 * ch < a.hd)
+        qr[i] = *reinterpret_cast<const u32x4_t*>(qb + l * a.q.ts + (g * a.rep + row - l * a.rep) * a.q.hs + 8 * ch);
+    }
+    if (tid < kSumRows) {
+      lr = lb[min(r + tid, r1 - 1)];
+      mr = r + tid < r1 ? static_cast<int>(own_keys(a, slot, off, (r + tid) / a.rep)) : 0;
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int x = tid + i * kThreads;
+      *reinterpret_cast<u32x4_t*>(&s_q[buf][x / (HD / 8) * kRow + x % (HD / 8) * 8]) = qr[i];
+    }
+    if (tid < kSumRows) {
+      s_lse[buf][tid] = lr;
+      s_lim[buf][tid] = mr;
+    }
+  };
+  const float c = a.scale * kLog2e;
+  float total = 0.0f;
+  load(r0);
+  store(0);
+  __syncthreads();
+  int buf = 0;
+  for (int r = r0; r < r1; r += kSumRows, buf ^= 1) {
+    const bool more = r + kSumRows < r1;
+    if (more) load(r + kSumRows);
+    // the rows' first sees the fewest keys
+    const bool some = r + kSumRows > r1 || own_keys(a, slot, off, r / a.rep) < key0 + kSumKeys;
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kSumRows / 32; ++x) {
+      f32x16_t s;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+      for (int t = 0; t < KS; ++t)
+        s = mfma32(*reinterpret_cast<const frag_t*>(&s_q[buf][(32 * x + c32) * kRow + 16 * t + 8 * h2]), kf[t], s);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4_t z = *reinterpret_cast<const f32x4_t*>(&s_lse[buf][32 * x + 8 * q + 4 * h2]);
+        f32x4_t p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + i], c, -z[i]));
+        if (some) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key >= s_lim[buf][32 * x + 8 * q + 4 * h2 + i]) p[i] = 0.0f;
+        }
+        sum += (p[0] + p[1]) + (p[2] + p[3]);
+      }
+    }
+    total += sum;
+    if (more) store(buf ^ 1);
+    __syncthreads();
   }
+  total = half_sum(total);
+  if (h2 == 0 && key < n)
+    pl.w_part[((static_cast<int64_t>(part) * a.B + b) * a.nkv + g) * a.S + key] = total;
+}
+
+__global__ __launch_bounds__(kThreads) void attn_weights_sum_kernel(CacheAttnArgs a, Plan pl, int tiles) {
+  const int64_t j = static_cast<int64_t>(blockIdx.x % tiles) * kThreads + threadIdx.x;
+  const int bg = blockIdx.x / tiles, b = bg / a.nkv, g = bg % a.nkv;
+  const int64_t slot = seq_slot(a.slots, a.n_slots, b);
+  if (slot < 0 || j >= a.S) return;
+  const int off = a.offs[b];
+  float w = 0.0f;
+  const bool seen = j < own_keys(a, slot, off, a.L - 1);
+  if (seen) {
+    // the parts that hold rows seeing the tile's first key have left a sum
+    const int64_t l0 = max(j / kSumKeys * kSumKeys - off, static_cast<int64_t>(0));
+    for (int p = static_cast<int>(l0 * a.rep / pl.w_rows); p < pl.w_parts; ++p)
+      w += pl.w_part[((static_cast<int64_t>(p) * a.B + b) * a.nkv + g) * a.S + j];
+  }
+  const int64_t at = (slot * a.nkv + g) * a.S + j;
+  if (seen || a.w_in != a.w_out) a.w_out[at] = (a.w_in ? a.w_in[at] : 0.0f) + w;
 }
 
 // ------------------------------------------------------------------ plan
@@ -973,6 +1106,9 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a,
 constexpr int64_t kFill = 768;
 // and of wide tiles: two
 constexpr int64_t kWideFill = 512;
+// workgroups for a prompt's weights, of which about half have no rows that
+// see their keys; a part has at least 256 rows
+constexpr int64_t kSumFill = 1024;
 
 // from more rows on (of a kv head) wide tiles take over
 constexpr int64_t kNarrowRows = 32;
@@ -1041,7 +1177,12 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
       pl.s_ld = align_up(a.S, kStep);
       pl.scores = reinterpret_cast<float*>(take(rows_p * a.nkv * pl.s_ld * 4));
     } else {
-      pl.lse = reinterpret_cast<float*>(take(static_cast<int64_t>(a.B) * a.L * a.nh * 4));
+      pl.lse2 = reinterpret_cast<float*>(take(rows_p * a.nkv * 4));
+      const int64_t tiles = (a.S + kSumKeys - 1) / kSumKeys * a.nkv * a.B;
+      const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(kSumFill / tiles, (pl.R + 255) / 256));
+      pl.w_rows = static_cast<int>(align_up((pl.R + parts - 1) / parts, kSumRows));
+      pl.w_parts = (pl.R + pl.w_rows - 1) / pl.w_rows;
+      pl.w_part = reinterpret_cast<float*>(take(pl.w_parts * static_cast<int64_t>(a.B) * a.nkv * a.S * 4));
     }
   } else {
     pl.lse = a.lse;
@@ -1085,6 +1226,34 @@ hipError_t launch_parts(const CacheAttnArgs& a, const Plan& pl, int rt, hipStrea
   return hipGetLastError();
 }
 
+template <bool F16, int HD>
+void launch_weight_parts(const CacheAttnArgs& a, const Plan& pl, uint32_t grid, int tiles, hipStream_t stream) {
+  if (a.hd == HD)
+    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, false>), dim3(grid), dim3(kThreads), 0, stream, a, pl, tiles);
+  else
+    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, true>), dim3(grid), dim3(kThreads), 0, stream, a, pl, tiles);
+}
+
+template <bool F16>
+hipError_t launch_weights(const CacheAttnArgs& a, const Plan& pl, hipStream_t stream) {
+  const int64_t tiles = (a.S + kSumKeys - 1) / kSumKeys;
+  const int64_t grid = tiles * pl.w_parts * a.nkv * a.B;
+  const int64_t sum_tiles = (a.S + kThreads - 1) / kThreads;
+  if (grid > 0x7fffffff || sum_tiles * a.nkv * a.B > 0x7fffffff) return hipErrorInvalidValue;
+  const uint32_t n = static_cast<uint32_t>(grid);
+  if (a.hd <= 64)
+    launch_weight_parts<F16, 64>(a, pl, n, static_cast<int>(tiles), stream);
+  else if (a.hd <= 128)
+    launch_weight_parts<F16, 128>(a, pl, n, static_cast<int>(tiles), stream);
+  else
+    launch_weight_parts<F16, 256>(a, pl, n, static_cast<int>(tiles), stream);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(attn_weights_sum_kernel, dim3(static_cast<uint32_t>(sum_tiles * a.nkv * a.B)), dim3(kThreads), 0,
+                     stream, a, pl, static_cast<int>(sum_tiles));
+  return hipGetLastError();
+}
+
 template <bool F16>
 hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
   const Layout y = make_plan(a, static_cast<char*>(ws));
@@ -1101,7 +1270,7 @@ hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
     e = a.hd == 256 && !any ? launch_parts<F16, 256, false>(a, pl, y.rt, stream)
                             : launch_parts<F16, 256, true>(a, pl, y.rt, stream);
   if (e != hipSuccess) return e;
-  const int64_t n_join = pl.direct ? 0 : (static_cast<int64_t>(a.B) * a.L * a.nh + kJoinRows - 1) / kJoinRows;
+  const int64_t n_join = pl.direct ? 0 : (static_cast<int64_t>(a.B) * a.L * a.nh + kWaves - 1) / kWaves;
   const int64_t w_tiles = pl.scores ? (a.S + kWeightKeys - 1) / kWeightKeys : 0;
   const int64_t grid = n_join + w_tiles * a.nkv * a.B;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
@@ -1110,13 +1279,7 @@ hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
                        static_cast<int>(n_join), static_cast<int>(w_tiles));
     e = hipGetLastError();
   }
-  if (e == hipSuccess && a.w_out && !pl.scores) {
-    const int64_t tiles = (a.S + kThreads - 1) / kThreads;
-    if (tiles * a.B * a.nkv > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(attn_weights_kernel<F16>, dim3(static_cast<uint32_t>(tiles * a.B * a.nkv)), dim3(kThreads), 0,
-                       stream, a, pl, static_cast<int>(tiles));
-    e = hipGetLastError();
-  }
+  if (e == hipSuccess && a.w_out && !pl.scores) e = launch_weights<F16>(a, pl, stream);
   return e;
 }
 

@@ -9,6 +9,8 @@
 //                        positions in order, and the weights moved
 //   evict_move_kernel    the kept keys and values, into another cache
 //   evict_shift_kernel   the same within one cache
+#include <algorithm>
+
 #include "fmx_cache_kernels.hpp"
 
 namespace fmx {
@@ -18,6 +20,8 @@ namespace {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kSelBins = 2048;
+// positions whose images a thread keeps in registers (position tid + 1024 i)
+constexpr int kSelKeep = 16;
 
 // unsigned image of a weight: larger weight, larger image; -0 as 0, any NaN
 // above infinity
@@ -28,25 +32,65 @@ __device__ inline uint32_t weight_key(float f) {
 }
 
 // inclusive scan over the workgroup's threads
-__device__ inline uint64_t block_scan(uint64_t v, uint64_t* s_tmp) {
+__device__ inline uint32_t block_scan(uint32_t v, uint32_t* s_tmp) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
-    const uint64_t o = __shfl_up(v, d);
+    const uint32_t o = __shfl_up(v, d);
     if (lane >= d) v += o;
   }
   __syncthreads();
   if (lane == kWave - 1) s_tmp[wave] = v;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) v += s_tmp[w];
+#pragma unroll
+  for (int w = 0; w < kSelWaves; ++w) v += w < wave ? s_tmp[w] : 0;
   return v;
 }
 
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-  __shared__ uint32_t s_bin[kSelBins];
-  __shared__ uint64_t s_tmp[kSelWaves];
-  __shared__ uint32_t s_digit, s_above;
+struct SelShared {
+  uint32_t bin[kSelBins];
+  uint32_t tmp[kSelWaves];
+  uint32_t digit, above;
+  uint32_t sure[kSelWaves], equal[kSelWaves];
+};
+
+// One round: bins of the digit at `shift` of the images that agree with
+// `found` above it, then the digit of the need-th largest, from the top.
+template <typename F>
+__device__ inline void select_round(SelShared& s, int shift, int bits, uint32_t& found, uint32_t& need,
+                                    F&& each) {
   const int tid = threadIdx.x;
+  for (int i = tid; i < kSelBins; i += kSelThreads) s.bin[i] = 0;
+  __syncthreads();
+  each([&](uint32_t u) {
+    if (shift + bits == 32 || u >> (shift + bits) == found >> (shift + bits))
+      atomicAdd(&s.bin[u >> shift & ((1u << bits) - 1)], 1u);
+  });
+  __syncthreads();
+  // from the largest digit down: thread t has digits top - 2 t, top - 2 t - 1
+  const int top = (1 << bits) - 1;
+  const uint32_t c0 = 2 * tid <= top ? s.bin[top - 2 * tid] : 0;
+  const uint32_t c1 = 2 * tid + 1 <= top ? s.bin[top - 2 * tid - 1] : 0;
+  const uint32_t end = block_scan(c0 + c1, s.tmp);
+  const uint32_t start = end - c0 - c1;
+  if (start < need && need <= end) {
+    const bool first = need <= start + c0;
+    s.digit = static_cast<uint32_t>(top - 2 * tid - (first ? 0 : 1));
+    s.above = first ? start : start + c0;
+  }
+  __syncthreads();
+  found |= s.digit << shift;
+  need -= s.above;
+  __syncthreads();
+}
+
+// Bound by its chain of rounds: the weights are read once (up to 16384
+// positions: kept in registers as images), a round is an LDS histogram and a
+// scan. 64 rows of 2000 to 16384 positions cut to 4000: 38 us with every round
+// reading the weights again, .. us so.
+__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
+  __shared__ SelShared s;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / a.nkv, g = blockIdx.x % a.nkv;
   int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
   const int64_t slot = seq_slot(a.slots, a.n_slots, b);
@@ -58,132 +102,235 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   if (slot < 0) return;
   const float* w = a.w + (slot * a.nkv + g) * a.S;
   float* wo = a.w_out + (slot * a.nkv + g) * a.S_out;
-  const bool move_w = wo != w;
   if (n <= budget) {
     for (int i = tid; i < n; i += kSelThreads) kept[i] = i;
-    for (int64_t i = move_w ? tid : n + tid; i < a.S_out; i += kSelThreads) wo[i] = i < n ? w[i] : 0.0f;
+    for (int64_t i = wo != w ? tid : n + tid; i < a.S_out; i += kSelThreads) wo[i] = i < n ? w[i] : 0.0f;
     return;
   }
   // middle positions [lo, hi), `need` of them kept
   const int lo = static_cast<int>(a.sinks), hi = n - static_cast<int>(a.recent);
   uint32_t need = static_cast<uint32_t>(budget - a.sinks - a.recent);
-  uint32_t found = 0;  // digits of the need-th largest image, from the top
-  int shift = 32;
-  for (int round = 0; round < 3 && need > 0; ++round) {
-    const int bits = round < 2 ? 11 : 10;
-    shift -= bits;
-    for (int i = tid; i < kSelBins; i += kSelThreads) s_bin[i] = 0;
-    __syncthreads();
-    for (int i = lo + tid; i < hi; i += kSelThreads) {
-      const uint32_t u = weight_key(w[i]);
-      if (round == 0 || u >> (shift + bits) == found >> (shift + bits))
-        atomicAdd(&s_bin[u >> shift & ((1u << bits) - 1)], 1u);
-    }
-    __syncthreads();
-    // from the largest digit down: thread t has digits top - 2 t, top - 2 t - 1
-    const int top = (1 << bits) - 1;
-    const uint32_t c0 = 2 * tid <= top ? s_bin[top - 2 * tid] : 0;
-    const uint32_t c1 = 2 * tid + 1 <= top ? s_bin[top - 2 * tid - 1] : 0;
-    const uint32_t end = static_cast<uint32_t>(block_scan(c0 + c1, s_tmp));
-    const uint32_t start = end - c0 - c1;
-    if (start < need && need <= end) {
-      const bool first = need <= start + c0;
-      s_digit = static_cast<uint32_t>(top - 2 * tid - (first ? 0 : 1));
-      s_above = first ? start : start + c0;
-    }
-    __syncthreads();
-    found |= s_digit << shift;
-    need -= s_above;
-    __syncthreads();
-  }
-  // kept: images above `found`, and the first `need` equal to it. Thread t
-  // has a run of positions; counts of both kinds are scanned together.
-  const bool some = budget > a.sinks + a.recent;
-  const int run = (n + kSelThreads - 1) / kSelThreads;
-  const int i0 = min(tid * run, n), i1 = min(i0 + run, n);
-  uint64_t mine = 0;  // sure ones | equal ones << 32
-  for (int i = i0; i < i1; ++i) {
-    if (i < lo || i >= hi) {
-      ++mine;
-    } else if (some) {
-      const uint32_t u = weight_key(w[i]);
-      mine += (u > found ? 1ull : 0ull) + (u == found ? 1ull << 32 : 0ull);
+  uint32_t found = 0;  // the need-th largest image, from its top digit down
+  const bool in_regs = n <= kSelThreads * kSelKeep;
+  float v[kSelKeep];
+  if (in_regs) {
+#pragma unroll
+    for (int i = 0; i < kSelKeep; ++i) {
+      const int p = tid + i * kSelThreads;
+      v[i] = p < n ? w[p] : 0.0f;
     }
   }
-  const uint64_t before = block_scan(mine, s_tmp) - mine;
-  uint32_t eq = static_cast<uint32_t>(before >> 32);
-  uint32_t at = static_cast<uint32_t>(before) + min(eq, need);
-  for (int i = i0; i < i1; ++i) {
-    bool keep = i < lo || i >= hi;
-    if (!keep && some) {
-      const uint32_t u = weight_key(w[i]);
-      keep = u > found;
-      if (u == found) keep = eq++ < need;
-    }
-    if (keep) kept[at++] = i;
-  }
-  __threadfence_block();
-  __syncthreads();
-  // the weights in order: position i comes from kept[i] >= i, so a tile's
-  // reads are behind every earlier tile's writes
-  for (int64_t i0w = 0; i0w < a.S_out; i0w += kSelThreads) {
-    const int64_t i = i0w + tid;
-    const float v = i < cnt ? w[kept[i]] : 0.0f;
-    __syncthreads();
-    if (i < a.S_out) wo[i] = v;
-  }
-}
-
-__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
-  const int b = blockIdx.y / a.nkv, g = blockIdx.y % a.nkv;
-  const int64_t slot = seq_slot(a.slots, a.n_slots, b);
-  const int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.y) * a.budget;
-  const int64_t per = a.row_bytes / 2, total = a.budget * per;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total && slot >= 0; i += gridDim.x * 256ll) {
-    const int64_t row = i / per, e = i % per;
-    const int32_t s = kept[row];
-    if (s < 0) break;
-    const int64_t ko = slot * a.ko_bs + g * a.ko_hs + row * a.ko_ts, ki = slot * a.k_bs + g * a.k_hs + s * a.k_ts;
-    const int64_t vo = slot * a.vo_bs + g * a.vo_hs + row * a.vo_ts, vi = slot * a.v_bs + g * a.v_hs + s * a.v_ts;
-    reinterpret_cast<uint16_t*>(a.k_out + ko)[e] = reinterpret_cast<const uint16_t*>(a.k + ki)[e];
-    reinterpret_cast<uint16_t*>(a.v_out + vo)[e] = reinterpret_cast<const uint16_t*>(a.v + vi)[e];
-  }
-  if (blockIdx.x == 0 && g == 0 && threadIdx.x == 0) {
-    int n = 0;
-    if (slot >= 0) {
-      int lo = 0, hi = static_cast<int>(a.budget);  // kept's entries from here on are -1
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (kept[mid] >= 0) lo = mid + 1; else hi = mid;
+  if (need > 0) {
+    auto all = [&](auto&& f) {
+      if (in_regs) {
+#pragma unroll
+        for (int i = 0; i < kSelKeep; ++i) {
+          const int p = tid + i * kSelThreads;
+          if (p >= lo && p < hi) f(weight_key(v[i]));
+        }
+      } else {
+        for (int p = lo + tid; p < hi; p += kSelThreads) f(weight_key(w[p]));
       }
-      n = lo;
+    };
+    select_round(s, 21, 11, found, need, all);
+    select_round(s, 10, 11, found, need, all);
+    select_round(s, 0, 10, found, need, all);
+  } else {
+    found = 0xffffffffu;  // nothing above it, none of its equals wanted
+  }
+  // In order, 1024 positions at a time: images above `found` and the first
+  // `need` equal to it go behind those before them.
+  uint32_t at = 0, eq = 0;  // kept and equal ones of earlier positions
+  for (int p0 = 0; p0 < n; p0 += kSelThreads) {
+    const int p = p0 + tid;
+    float x = 0.0f;
+    if (in_regs) {
+#pragma unroll
+      for (int i = 0; i < kSelKeep; ++i)
+        if (p0 == i * kSelThreads) x = v[i];
+    } else if (p < n) {
+      x = w[p];
     }
-    a.lens_out[b] = n;
+    const bool mid = p >= lo && p < hi;
+    const uint32_t u = weight_key(x);
+    const bool sure = p < n && (!mid || u > found), same = mid && u == found;
+    const uint64_t ms = __ballot(sure), me = __ballot(same);
+    if (lane == 0) {
+      s.sure[wave] = static_cast<uint32_t>(__popcll(ms));
+      s.equal[wave] = static_cast<uint32_t>(__popcll(me));
+    }
+    __syncthreads();
+    uint32_t bs = 0, be = 0, ts = 0, te = 0;
+#pragma unroll
+    for (int q = 0; q < kSelWaves; ++q) {
+      const uint32_t cs = s.sure[q], ce = s.equal[q];
+      bs += q < wave ? cs : 0;
+      be += q < wave ? ce : 0;
+      ts += cs;
+      te += ce;
+    }
+    const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+    const uint32_t es = bs + static_cast<uint32_t>(__popcll(ms & below));
+    const uint32_t ee = eq + be + static_cast<uint32_t>(__popcll(me & below));
+    const uint32_t pos = at + es + min(ee, need) - min(eq, need);
+    const bool keep = sure || (same && ee < need);
+    // (in place: position pos <= p, whose weight has been read by now)
+    if (keep) {
+      kept[pos] = p;
+      wo[pos] = x;
+    }
+    at += ts + min(eq + te, need) - min(eq, need);
+    eq += te;
+    __syncthreads();
+  }
+  for (int64_t i = cnt + tid; i < a.S_out; i += kSelThreads) wo[i] = 0.0f;
+}
+
+// ------------------------------------------------------------------ keys and values
+
+constexpr int kMoveThreads = 256;
+constexpr int kMoveUnits = 4;  // of a thread, keys and values each: loads in flight
+
+template <int VB>
+struct Unit;
+template <>
+struct Unit<16> {
+  typedef u32x4_t T;
+};
+template <>
+struct Unit<2> {
+  typedef uint16_t T;
+};
+
+// Bound by HBM: kept rows are read and written once. 16 bytes per lane where
+// rows and strides allow.
+template <int VB>
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, int chunks, int chunk_rows) {
+  typedef typename Unit<VB>::T T;
+  const int bg = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int b = bg / a.nkv, g = bg % a.nkv;
+  const int64_t slot = seq_slot(a.slots, a.n_slots, b);
+  const int32_t* kept = a.kept + static_cast<int64_t>(bg) * a.budget;
+  const int per = static_cast<int>(a.row_bytes / VB);
+  const int r0 = chunk * chunk_rows, r1 = min(static_cast<int>(a.budget), r0 + chunk_rows);
+  if (slot >= 0) {
+    const uint8_t* k = a.k + slot * a.k_bs + g * a.k_hs;
+    const uint8_t* v = a.v + slot * a.v_bs + g * a.v_hs;
+    uint8_t* ko = a.k_out + slot * a.ko_bs + g * a.ko_hs;
+    uint8_t* vo = a.v_out + slot * a.vo_bs + g * a.vo_hs;
+    const int units = (r1 - r0) * per;
+    for (int u0 = threadIdx.x; u0 < units; u0 += kMoveThreads * kMoveUnits) {
+      T kv[kMoveUnits], vv[kMoveUnits];
+      int src[kMoveUnits], row[kMoveUnits], e[kMoveUnits];
+#pragma unroll
+      for (int i = 0; i < kMoveUnits; ++i) {
+        const int u = u0 + i * kMoveThreads;
+        row[i] = r0 + u / per;
+        e[i] = u % per * VB;
+        src[i] = u < units ? kept[row[i]] : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < kMoveUnits; ++i)
+        if (src[i] >= 0) {
+          kv[i] = *reinterpret_cast<const T*>(k + src[i] * a.k_ts + e[i]);
+          vv[i] = *reinterpret_cast<const T*>(v + src[i] * a.v_ts + e[i]);
+        }
+#pragma unroll
+      for (int i = 0; i < kMoveUnits; ++i)
+        if (src[i] >= 0) {
+          *reinterpret_cast<T*>(ko + row[i] * a.ko_ts + e[i]) = kv[i];
+          *reinterpret_cast<T*>(vo + row[i] * a.vo_ts + e[i]) = vv[i];
+        }
+    }
+  }
+  if (chunk == 0 && g == 0 && threadIdx.x == 0) {
+    const int64_t len = slot < 0 ? 0 : a.lens[b];
+    const int64_t n = len < 0 ? 0 : (len > a.S ? a.S : len);
+    a.lens_out[b] = static_cast<int32_t>(n < a.budget ? n : a.budget);
   }
 }
 
-// One workgroup per (sequence, kv head, keys or values), rows in order: row i
-// comes from row kept[i] >= i, so what a step reads lies behind all that
-// earlier steps wrote, and what it writes is read by no later step.
-__global__ __launch_bounds__(256) void evict_shift_kernel(EvictArgs a) {
-  const int b = blockIdx.y / a.nkv, g = blockIdx.y % a.nkv;
+// One workgroup per (sequence, kv head, keys or values, slice of the row), a
+// block of rows after the other. Row i comes from row kept[i] >= i, so what a
+// block reads lies behind all that earlier blocks wrote, and what it writes is
+// read by no later block: only a block's own reads have to end before its
+// writes begin.
+template <int VB>
+__global__ __launch_bounds__(kMoveThreads) void evict_shift_kernel(EvictArgs a, int slices, int slice_units) {
+  typedef typename Unit<VB>::T T;
+  constexpr int kUnits = 8;
+  int item = blockIdx.x;
+  const int slice = item % slices;
+  item /= slices;
+  const bool isv = item & 1;
+  const int bg = item >> 1, b = bg / a.nkv, g = bg % a.nkv;
   const int64_t slot = seq_slot(a.slots, a.n_slots, b);
-  const int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.y) * a.budget;
-  const bool isv = blockIdx.x != 0;
-  uint8_t* base = isv ? a.v_out + slot * a.v_bs + g * a.v_hs : a.k_out + slot * a.k_bs + g * a.k_hs;
-  const int64_t ts = isv ? a.v_ts : a.k_ts;
-  const int per = static_cast<int>(a.row_bytes / 2);
-  int64_t n = 0;
-  if (slot >= 0)
-    for (int64_t row = 0; row < a.budget; ++row) {
-      const int32_t s = kept[row];
-      if (s < 0) break;
-      ++n;
-      if (s == row) continue;
-      for (int e = threadIdx.x; e < per; e += 256)
-        reinterpret_cast<uint16_t*>(base + row * ts)[e] = reinterpret_cast<const uint16_t*>(base + s * ts)[e];
+  const int32_t* kept = a.kept + static_cast<int64_t>(bg) * a.budget;
+  if (slot >= 0) {
+    uint8_t* base = (isv ? a.v_out + slot * a.v_bs + g * a.v_hs : a.k_out + slot * a.k_bs + g * a.k_hs) +
+                    static_cast<int64_t>(slice) * slice_units * VB;
+    const int64_t ts = isv ? a.v_ts : a.k_ts;
+    const int per = min(slice_units, static_cast<int>(a.row_bytes / VB) - slice * slice_units);
+    // lanes beyond the whole rows of a block idle
+    const int rows = kMoveThreads / per, r = threadIdx.x / per, e = threadIdx.x % per * VB;
+    const int budget = static_cast<int>(a.budget);
+    for (int r0 = 0; r0 < budget; r0 += rows * kUnits) {
+      if (kept[r0] < 0) break;
+      T x[kUnits];
+      int src[kUnits];
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int row = r0 + i * rows + r;
+        src[i] = r < rows && row < budget ? kept[row] : -1;
+        if (src[i] == row) src[i] = -1;
+      }
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        x[i] = T{};
+        if (src[i] >= 0) x[i] = *reinterpret_cast<const T*>(base + src[i] * ts + e);
+      }
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) asm volatile("" : "+v"(x[i]));  // in registers, not on their way
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i)
+        if (src[i] >= 0) *reinterpret_cast<T*>(base + (r0 + i * rows + r) * ts + e) = x[i];
     }
-  if (!isv && g == 0 && threadIdx.x == 0) a.lens_out[b] = static_cast<int32_t>(n);
+  }
+  if (slice == 0 && !isv && g == 0 && threadIdx.x == 0) {
+    // as many as are kept (lens may be lens_out, but nothing else reads it here)
+    const int64_t len = slot < 0 ? 0 : a.lens[b];
+    const int64_t n = len < 0 ? 0 : (len > a.S ? a.S : len);
+    a.lens_out[b] = static_cast<int32_t>(n < a.budget ? n : a.budget);
+  }
+}
+
+template <int VB>
+hipError_t move_rows(const EvictArgs& a, hipStream_t stream) {
+  const int64_t heads = static_cast<int64_t>(a.B) * a.nkv;
+  const int per = static_cast<int>(a.row_bytes / VB);
+  const dim3 wg(kMoveThreads);
+  if (a.in_place) {
+    // slices of a row, each at least 64 bytes, until 512 workgroups are busy
+    int slices = 1;
+    while (slices * 2 * 64 <= a.row_bytes && heads * 2 * slices < 512 && per % (slices * 2) == 0) slices *= 2;
+    // (and no longer than a block of threads)
+    while (per / slices > kMoveThreads) ++slices;
+    const int units = (per + slices - 1) / slices;
+    slices = (per + units - 1) / units;
+    const int64_t n = heads * 2 * slices;
+    if (n > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(evict_shift_kernel<VB>, dim3(static_cast<uint32_t>(n)), wg, 0, stream, a, slices, units);
+    return hipGetLastError();
+  }
+  // rows of a workgroup: about two rounds of its threads
+  const int rows = std::max(1, 2 * kMoveThreads * kMoveUnits / per);
+  const int64_t chunks = (a.budget + rows - 1) / rows;
+  if (chunks * heads > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(evict_move_kernel<VB>, dim3(static_cast<uint32_t>(chunks * heads)), wg, 0, stream, a,
+                     static_cast<int>(chunks), rows);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -191,12 +338,15 @@ __global__ __launch_bounds__(256) void evict_shift_kernel(EvictArgs a) {
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
   const uint32_t heads = static_cast<uint32_t>(a.B) * static_cast<uint32_t>(a.nkv);
   hipLaunchKernelGGL(evict_select_kernel, dim3(heads), dim3(kSelThreads), 0, stream, a);
-  if (a.in_place) {
-    hipLaunchKernelGGL(evict_shift_kernel, dim3(2, heads), dim3(256), 0, stream, a);
-  } else {
-    hipLaunchKernelGGL(evict_move_kernel, dim3(64, heads), dim3(256), 0, stream, a);
-  }
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  int64_t all = a.row_bytes;
+  for (int64_t s : {a.k_bs, a.k_ts, a.k_hs, a.v_bs, a.v_ts, a.v_hs, a.ko_bs, a.ko_ts, a.ko_hs, a.vo_bs, a.vo_ts, a.vo_hs})
+    all |= s;
+  for (const void* p : {static_cast<const void*>(a.k), static_cast<const void*>(a.v),
+                        static_cast<const void*>(a.k_out), static_cast<const void*>(a.v_out)})
+    all |= static_cast<int64_t>(reinterpret_cast<uintptr_t>(p) & 15);
+  return all % 16 == 0 ? move_rows<16>(a, stream) : move_rows<2>(a, stream);
 }
 
 }  // namespace fmx
