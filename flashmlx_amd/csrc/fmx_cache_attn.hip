@@ -35,6 +35,19 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 __device__ inline float neg_inf() { return -__builtin_huge_valf(); }
 
+// The fragments are in registers from here on: a load still counted as on its
+// way at a loop's entry would make every round wait for the loads that it has
+// just issued.
+template <typename T, int N>
+__device__ inline void settle(T (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    u32x4_t w = __builtin_bit_cast(u32x4_t, f[i]);
+    asm volatile("" : "+v"(w));
+    f[i] = __builtin_bit_cast(T, w);
+  }
+}
+
 // of the four lanes i16 + 16 j: their maximum, their sum, in each
 __device__ inline float quad_max(float v) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -286,10 +299,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   // rows behind the piece's last are read as its last
   u32x4_t kw[2][KC];
   uint32_t vw[8][VW];
+  // (a lane's 64-bit row products are formed once; a step adds a scalar one)
+  const int kk0 = k0 + wave * kStep;
+  const uint16_t* kp0 = kb + min(kk0 + i16, k1 - 1) * kts + 8 * j;
+  const uint16_t* vp0 = vb + min(kk0 + 4 * j, k1 - 1) * vts + (VPL == 4 ? 4 : 8) * i16;
   auto load_k = [&](int kk) {
+    const bool whole = kk + kStep <= k1;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const uint16_t* p = kb + min(kk + 16 * x + i16, k1 - 1) * kts + 8 * j;
+      const uint16_t* p = whole ? kp0 + (kk - kk0 + 16 * x) * kts : kb + min(kk + 16 * x + i16, k1 - 1) * kts + 8 * j;
 #pragma unroll
       for (int t = 0; t < KC; ++t)
         if (!ANY || 32 * t + 8 * j < a.hd) kw[x][t] = *reinterpret_cast<const u32x4_t*>(p + 32 * t);
@@ -297,21 +315,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     }
   };
   auto load_v = [&](int kk) {
+    const bool whole = kk + kStep <= k1;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      const uint16_t* p = vb + min(kk + 16 * (s >> 2) + 4 * j + (s & 3), k1 - 1) * vts;
+      const int row = 16 * (s >> 2) + (s & 3);
+      const uint16_t* p = whole ? vp0 + (kk - kk0 + row) * vts
+                                : vb + min(kk + row + 4 * j, k1 - 1) * vts + (VPL == 4 ? 4 : 8) * i16;
       if constexpr (VPL == 4) {
-        const int d = 4 * i16;
         u32x2_t w = {0, 0};
-        if (!ANY || d < a.hd) w = *reinterpret_cast<const u32x2_t*>(p + d);
+        if (!ANY || 4 * i16 < a.hd) w = *reinterpret_cast<const u32x2_t*>(p);
         vw[s][0] = w[0];
         vw[s][1] = w[1];
       } else {
 #pragma unroll
         for (int q = 0; q < VPL / 8; ++q) {
-          const int d = 128 * q + 8 * i16;
           u32x4_t w = {0, 0, 0, 0};
-          if (!ANY || d < a.hd) w = *reinterpret_cast<const u32x4_t*>(p + d);
+          if (!ANY || 128 * q + 8 * i16 < a.hd) w = *reinterpret_cast<const u32x4_t*>(p + 128 * q);
 #pragma unroll
           for (int i = 0; i < 4; ++i) vw[s][4 * q + i] = w[i];
         }
@@ -328,7 +347,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   };
 
   bool left_out = false;
-  int kk = k0 + wave * kStep;
+  int kk = kk0;
   if (kk < k1) load_k(kk);
   for (; kk < k1; kk += kPiece) {
     load_v(kk);
@@ -622,23 +641,30 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
   // ---- staging
   u32x4_t kr[NK], vr[NV][4];
   const int kg = tid & 15;
+  constexpr int kKStep = kThreads / (HD / 8);      // keys between a thread's loads
+  constexpr bool kVWhole = HD / 8 % (kThreads / 16) == 0;
+  const int kch = tid % (HD / 8), kkey = tid / (HD / 8);
+  // (a thread's 64-bit row products are formed once; a step adds a scalar one)
+  const uint16_t* kp0 = kb + min(k0 + kkey, max(k1 - 1, 0)) * kts + 8 * kch;
+  const uint16_t* vp0 = vb + min(k0 + 4 * kg, max(k1 - 1, 0)) * vts + 8 * (tid >> 4);
   auto load = [&](int kt) {
+    const bool whole = kt + kWideKeys <= k1;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int x = tid + i * kThreads;
-      const int key = x / (HD / 8), ch = x % (HD / 8);
-      kr[i] = u32x4_t{0, 0, 0, 0};
-      if (!ANY || 8 * ch < a.hd)
-        kr[i] = *reinterpret_cast<const u32x4_t*>(kb + min(kt + key, k1 - 1) * kts + 8 * ch);
+      const uint16_t* p =
+          whole ? kp0 + (kt - k0 + i * kKStep) * kts : kb + min(kt + kkey + i * kKStep, k1 - 1) * kts + 8 * kch;
+      if (ANY) kr[i] = u32x4_t{0, 0, 0, 0};
+      if (!ANY || 8 * kch < a.hd) kr[i] = *reinterpret_cast<const u32x4_t*>(p);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int ch = (tid >> 4) + i * (kThreads / 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        vr[i][e] = u32x4_t{0, 0, 0, 0};
-        if (8 * ch < (ANY ? a.hd : HD))
-          vr[i][e] = *reinterpret_cast<const u32x4_t*>(vb + min(kt + 4 * kg + e, k1 - 1) * vts + 8 * ch);
+        const uint16_t* p = whole ? vp0 + (kt - k0 + e) * vts + i * (kThreads / 2)
+                                  : vb + min(kt + 4 * kg + e, k1 - 1) * vts + 8 * ch;
+        if (ANY || !kVWhole) vr[i][e] = u32x4_t{0, 0, 0, 0};
+        if ((!ANY && kVWhole) || 8 * ch < (ANY ? a.hd : HD)) vr[i][e] = *reinterpret_cast<const u32x4_t*>(p);
       }
     }
   };
@@ -647,8 +673,7 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
     uint16_t* sv = s_kv[buf] + kWideKeys * kKRow;
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int x = tid + i * kThreads;
-      *reinterpret_cast<u32x4_t*>(sk + x / (HD / 8) * kKRow + x % (HD / 8) * 8) = kr[i];
+      *reinterpret_cast<u32x4_t*>(sk + (kkey + i * kKStep) * kKRow + kch * 8) = kr[i];
     }
     if (kt + kWideKeys > all) {
       // values behind the piece count nothing, whatever they hold; infinite
@@ -680,7 +705,7 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int ch = (tid >> 4) + i * (kThreads / 16);
-      if (ch < HD / 8) {
+      if (kVWhole || ch < HD / 8) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
           const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
@@ -704,6 +729,7 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
     load(k0);
     store(k0, 0);
   }
+  settle(qf);
   __syncthreads();
   int buf = 0;
   for (int kt = k0; kt < k1; kt += kWideKeys, buf ^= 1) {
@@ -714,13 +740,16 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
       const uint16_t* sv = s_kv[buf] + kWideKeys * kKRow;
       f32x16_t s[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int t = 0; t < KS; ++t)
+      for (int t = 0; t < KS; ++t)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
           s[x] = mfma32(*reinterpret_cast<const frag_t*>(sk + (32 * x + c32) * kKRow + 16 * t + 8 * h2), qf[t], s[x]);
-      }
+      __builtin_amdgcn_s_setprio(0);
       if (kt + kWideKeys > w_all) {
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -753,11 +782,13 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
           typedef typename std::conditional<F16, _Float16, __bf16>::type half_t;
           pf[2 * x + (i >> 3)][i & 7] = static_cast<half_t>(p);
         }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int dt = 0; dt < DT; ++dt)
           o[dt] = mfma32(*reinterpret_cast<const frag_t*>(sv + (32 * dt + c32) * kVRow + 16 * t + 8 * h2), pf[t], o[dt]);
+      __builtin_amdgcn_s_setprio(0);
     }
     if (more) store(kt + kWideKeys, buf ^ 1);
     __syncthreads();
@@ -928,16 +959,20 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Pl
   const int off = a.offs[b];
   const int64_t n = own_keys(a, slot, off, a.L - 1);
   if (j0 < n) {
-    if (tid < pl.R) {
-      const RowPieces ps(a, pl, b, g, tid);
+    const int lane = tid & 63;
+    for (int r = __builtin_amdgcn_readfirstlane(tid >> 6); r < pl.R; r += kWaves) {
+      const RowPieces ps(a, pl, b, g, r);
       float m = neg_inf(), z = 0.0f;
-      for (int i = 0; i < ps.n; ++i) m = fmaxf(m, ps.ml(i).x);
+      for (int i = lane; i < ps.n; i += kWave) m = fmaxf(m, ps.ml(i).x);
+      m = wave_max_f32(m);
       const float ms = m == neg_inf() ? 0.0f : m;
-      for (int i = 0; i < ps.n; ++i) {
+      for (int i = lane; i < ps.n; i += kWave) {
         const float2 ml = ps.ml(i);
         z += ml.y * __builtin_amdgcn_exp2f(ml.x - ms);
       }
-      s_row[tid] = make_float2(ms, z == 0.0f ? 0.0f : 1.0f / z);
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o);
+      if (lane == 0) s_row[r] = make_float2(ms, z == 0.0f ? 0.0f : 1.0f / z);
     }
     __syncthreads();
   }
@@ -1008,32 +1043,52 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a,
       kf[t] = __builtin_bit_cast(frag_t, w);
     }
   }
-  u32x4_t qr[NQ];
+  u32x4_t qr[NQ] = {};
   float lr = 0.0f;
   int mr = 0;
   const uint16_t* qb = static_cast<const uint16_t*>(a.q.p) + b * a.q.bs;
   const float* lb = pl.lse2 + (static_cast<int64_t>(b) * a.nkv + g) * pl.R;
+  // (query, head in group) of the thread's rows, kept by steps of kSumRows
+  constexpr int kQStep = kThreads / (HD / 8);  // rows between a thread's loads
+  const int qch = tid % (HD / 8), qrow = tid / (HD / 8);
+  const int dl = kSumRows / a.rep, dr = kSumRows % a.rep;
+  int ql[NQ], qh[NQ];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    ql[i] = (r0 + qrow + i * kQStep) / a.rep;
+    qh[i] = (r0 + qrow + i * kQStep) % a.rep;
+  }
+  int ml = (r0 + tid) / a.rep, mh = (r0 + tid) % a.rep;
+  auto advance = [&](int& l, int& h) {
+    l += dl;
+    h += dr;
+    if (h >= a.rep) {
+      h -= a.rep;
+      ++l;
+    }
+  };
+  // rows behind the part's are not loaded: no key counts for them
   auto load = [&](int r) {
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      const int x = tid + i * kThreads;
-      const int row = min(r + x / (HD / 8), r1 - 1), ch = x % (HD / 8);
-      const int l = row / a.rep;
-      qr[i] = u32x4_t{0, 0, 0, 0};
-      if (!ANY || 8 * ch < a.hd)
-        qr[i] = *reinterpret_cast<const u32x4_t*>(qb + l * a.q.ts + (g * a.rep + row - l * a.rep) * a.q.hs + 8 * ch);
+      if (ANY) qr[i] = u32x4_t{0, 0, 0, 0};
+      if (r + qrow + i * kQStep < r1 && (!ANY || 8 * qch < a.hd))
+        qr[i] = *reinterpret_cast<const u32x4_t*>(qb + ql[i] * a.q.ts + (g * a.rep + qh[i]) * a.q.hs + 8 * qch);
+      advance(ql[i], qh[i]);
     }
     if (tid < kSumRows) {
-      lr = lb[min(r + tid, r1 - 1)];
-      mr = r + tid < r1 ? static_cast<int>(own_keys(a, slot, off, (r + tid) / a.rep)) : 0;
+      mr = 0;
+      if (r + tid < r1) {
+        lr = lb[r + tid];
+        mr = static_cast<int>(own_keys(a, slot, off, ml));
+      }
+      advance(ml, mh);
     }
   };
   auto store = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int x = tid + i * kThreads;
-      *reinterpret_cast<u32x4_t*>(&s_q[buf][x / (HD / 8) * kRow + x % (HD / 8) * 8]) = qr[i];
-    }
+    for (int i = 0; i < NQ; ++i)
+      *reinterpret_cast<u32x4_t*>(&s_q[buf][(qrow + i * kQStep) * kRow + qch * 8]) = qr[i];
     if (tid < kSumRows) {
       s_lse[buf][tid] = lr;
       s_lim[buf][tid] = mr;
@@ -1043,13 +1098,15 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a,
   float total = 0.0f;
   load(r0);
   store(0);
+  settle(kf);
   __syncthreads();
   int buf = 0;
   for (int r = r0; r < r1; r += kSumRows, buf ^= 1) {
     const bool more = r + kSumRows < r1;
     if (more) load(r + kSumRows);
-    // the rows' first sees the fewest keys
-    const bool some = r + kSumRows > r1 || own_keys(a, slot, off, r / a.rep) < key0 + kSumKeys;
+    // whether a row of these may not see all of the keys: the first sees the
+    // fewest (one of the buffer's limits, the same in every thread)
+    const bool some = r + kSumRows > r1 || __builtin_amdgcn_readfirstlane(s_lim[buf][0]) < key0 + kSumKeys;
     float sum = 0.0f;
 #pragma unroll
     for (int x = 0; x < kSumRows / 32; ++x) {
