@@ -28,57 +28,68 @@ _SCALING = {"none": 0, "linear": 1, "ntk": 2, "parts": 3, "yarn": 4}
 _TURNS = {"parts": (1.0, 4.0), "yarn": (1.0, 32.0)}
 
 
-def _heads(t: torch.Tensor, name: str, like: torch.Tensor, shape: tuple, order=(0, 1, 2)) -> FmxHeads:
-    """The view of a 4-d tensor whose batch, token and head axes are `order`."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
-    if t.dtype != like.dtype:
-        raise TypeError(f"{name}: {t.dtype}, expected {like.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, not {like.device}")
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
-        raise ValueError(f"{name}: the head's elements must be contiguous")
-    st = t.stride()
-    # the stride of an axis of one entry is never used: 0, whatever torch says
-    b, l, h = (st[i] if t.shape[i] > 1 else 0 for i in order)
-    return FmxHeads(t.data_ptr(), b, l, h)
+_byref = C.byref
 
 
-def _cache(t: torch.Tensor, name: str, like: torch.Tensor, nkv: int, hd: int) -> FmxHeads:
-    if t.dim() != 4 or t.shape[1] != nkv or t.shape[3] != hd:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [slots, {nkv}, positions, {hd}]")
-    return _heads(t, name, like, tuple(t.shape), (0, 2, 1))
+def _refuse(t, name: str, shape: tuple, dtype, dev: int) -> None:
+    """Says which of an argument's shape, dtype, device or layout is wrong."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor expected, got {type(t).__name__}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: {t.dtype}, expected {dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
+    raise ValueError(f"{name}: strides {t.stride()}, expected contiguous " +
+                     ("elements of a head" if t.is_floating_point() and t.dim() > 2 else "memory"))
 
 
-def _ints(t: Optional[torch.Tensor], name: str, like: torch.Tensor, shape: tuple) -> Optional[int]:
+def _heads(t: torch.Tensor, name: str, shape, dtype, dev: int):
+    """The view of a [batch, token, head, element] tensor."""
+    s = t.stride()
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev or s[3] != 1 and shape[3] != 1:
+        _refuse(t, name, shape, dtype, dev)
+    return _byref(FmxHeads(t.data_ptr(), s[0], s[1], s[2]))
+
+
+def _cache(t: torch.Tensor, name: str, shape, dtype, dev: int):
+    """The view of a [slot, head, position, element] tensor."""
+    s = t.stride()
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev or s[3] != 1 and shape[3] != 1:
+        _refuse(t, name, shape, dtype, dev)
+    return _byref(FmxHeads(t.data_ptr(), s[0], s[2], s[1]))
+
+
+def _flat(t: Optional[torch.Tensor], name: str, shape, dtype, dev: int) -> Optional[int]:
+    """The address of a contiguous array, or None."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != like.device:
-        raise ValueError(f"{name}: a contiguous int32 tensor {shape} on {like.device} expected")
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
+        _refuse(t, name, shape, dtype, dev)
     return t.data_ptr()
 
 
-def _floats(t: Optional[torch.Tensor], name: str, like: torch.Tensor, shape: tuple) -> Optional[int]:
-    if t is None:
-        return None
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != like.device:
-        raise ValueError(f"{name}: a contiguous float32 tensor {shape} on {like.device} expected")
-    return t.data_ptr()
-
-
-def _rows(t: torch.Tensor, name: str) -> tuple:
-    """(batch, seq_len, heads, head_dim) of a query-like tensor on the current device."""
+def _device(t: torch.Tensor, name: str, dims: str) -> int:
+    """The index of the current device, on which t, of four axes, has to be."""
     if t.dim() != 4:
-        raise ValueError(f"{name}: [batch, seq_len, heads, head_dim] expected, got {tuple(t.shape)}")
+        raise ValueError(f"{name}: [{dims}] expected, got {tuple(t.shape)}")
     if t.dtype not in _DT:
         raise TypeError(f"{name}: {t.dtype} (bfloat16, float16 or float32)")
-    _on_device(t, name)
-    return tuple(t.shape)
-
-
-def _on_device(t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    dev = t.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
         raise ValueError(f"{name} is on {t.device}, which is not the current HIP device")
+    return dev
+
+
+_ROWS, _SLOTS = "batch, seq_len, heads, head_dim", "slots, kv_heads, positions, head_dim"
+
+
+def _pool(k: torch.Tensor, hd: int) -> tuple:
+    """(slots, kv heads, positions) of the caches."""
+    if k.dim() != 4 or k.shape[3] != hd:
+        raise ValueError(f"k_cache: shape {tuple(k.shape)}, expected [slots, kv_heads, positions, {hd}]")
+    return k.shape[0], k.shape[1], k.shape[2]
 
 
 def _stream() -> int:
@@ -87,8 +98,8 @@ def _stream() -> int:
 
 def _workspace(ws: Optional[torch.Tensor], need: int, like: torch.Tensor) -> torch.Tensor:
     if ws is None:
-        return torch.empty(max(need, 1), dtype=torch.uint8, device=like.device)
-    if ws.device != like.device or not ws.is_contiguous() or ws.dtype != torch.uint8:
+        return like.new_empty(max(need, 1), dtype=torch.uint8)
+    if ws.get_device() != like.get_device() or not ws.is_contiguous() or ws.dtype != torch.uint8:
         raise ValueError(f"workspace: a contiguous uint8 tensor on {like.device} expected")
     return ws
 
@@ -138,23 +149,26 @@ class Rope:
         dev = device or torch.device("cuda", torch.cuda.current_device())
         self.freqs = torch.from_numpy(freqs).to(dev)
         self._c = FmxRopeAngles(self.freqs.data_ptr(), cfg.dims, self.factor, int(cfg.interleaved))
+        self._dev = self.freqs.get_device()
 
-    def _check(self, t: torch.Tensor) -> None:
-        if t.device != self.freqs.device:
-            raise ValueError(f"the frequencies are on {self.freqs.device}, the rows on {t.device}")
+    def _check(self, dev: int) -> None:
+        if dev != self._dev:
+            raise ValueError(f"the frequencies are on cuda:{self._dev}, the rows on cuda:{dev}")
 
     def __call__(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None,
                  inverse: bool = False) -> torch.Tensor:
         """x [batch, seq_len, heads, head_dim] turned to positions [batch,
         seq_len] (int32); inverse: back, which is the gradient of the forward
         call with respect to x. out may be x."""
-        B, L, nh, hd = shape = _rows(x, "x")
-        self._check(x)
+        dev, shape, dt = _device(x, "x", _ROWS), x.shape, x.dtype
+        self._check(dev)
+        B, L, nh, hd = shape
         if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=x.device)
+            out = x.new_empty(shape)
         _lib.check(self.lib.fmx_rope(
-            C.byref(self._c), _DT[x.dtype], B, L, nh, hd, C.byref(_heads(x, "x", x, shape)),
-            _ints(positions, "positions", x, (B, L)), int(inverse), C.byref(_heads(out, "out", x, shape)), _stream()))
+            _byref(self._c), _DT[dt], B, L, nh, hd, _heads(x, "x", shape, dt, dev),
+            _flat(positions, "positions", (B, L), torch.int32, dev), int(inverse),
+            _heads(out, "out", shape, dt, dev), _stream()))
         return out
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -163,20 +177,19 @@ class Rope:
         """One step's new tokens: returns q rotated; k, rotated, and v go to
         cache positions offsets[b] + l of slot slots[b] (or b). Rows outside
         the cache are not written. out may be q."""
-        B, L, nh, hd = shape = _rows(q, "q")
-        self._check(q)
-        nkv = k.shape[2] if k.dim() == 4 else 0
+        dev, shape, dt, i32 = _device(q, "q", _ROWS), q.shape, q.dtype, torch.int32
+        self._check(dev)
+        B, L, nh, hd = shape
+        n_slots, nkv, S = _pool(k_cache, hd)
+        new, pool = (B, L, nkv, hd), k_cache.shape
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        kc, vc = _cache(k_cache, "k_cache", q, nkv, hd), _cache(v_cache, "v_cache", q, nkv, hd)
-        if v_cache.shape[:3] != k_cache.shape[:3]:
-            raise ValueError("k_cache and v_cache differ in shape")
+            out = q.new_empty(shape)
         _lib.check(self.lib.fmx_rope_append(
-            C.byref(self._c), _DT[q.dtype], B, L, nh, nkv, hd, C.byref(_heads(q, "q", q, shape)),
-            C.byref(_heads(k, "k", q, (B, L, nkv, hd))), C.byref(_heads(v, "v", q, (B, L, nkv, hd))),
-            _ints(positions, "positions", q, (B, L)), _ints(offsets, "offsets", q, (B,)),
-            _ints(slots, "slots", q, (B,)), k_cache.shape[0], k_cache.shape[2],
-            C.byref(_heads(out, "out", q, shape)), C.byref(kc), C.byref(vc), _stream()))
+            _byref(self._c), _DT[dt], B, L, nh, nkv, hd, _heads(q, "q", shape, dt, dev), _heads(k, "k", new, dt, dev),
+            _heads(v, "v", new, dt, dev), _flat(positions, "positions", (B, L), i32, dev),
+            _flat(offsets, "offsets", (B,), i32, dev), _flat(slots, "slots", (B,), i32, dev), n_slots, S,
+            _heads(out, "out", shape, dt, dev), _cache(k_cache, "k_cache", pool, dt, dev),
+            _cache(v_cache, "v_cache", pool, dt, dev), _stream()))
         return out
 
 
@@ -192,28 +205,28 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v
     them see the whole prefix (None: no prefix), and of their own slot the
     positions up to their own. A query that sees no key gets 0 and -inf."""
     lib = _lib.load()
-    B, L, nh, hd = shape = _rows(q, "q")
-    nkv = k_cache.shape[1] if k_cache.dim() == 4 else 0
-    kc, vc = _cache(k_cache, "k_cache", q, nkv, hd), _cache(v_cache, "v_cache", q, nkv, hd)
-    if v_cache.shape[:3] != k_cache.shape[:3]:
-        raise ValueError("k_cache and v_cache differ in shape")
+    dev, shape, dt, i32 = _device(q, "q", _ROWS), q.shape, q.dtype, torch.int32
+    B, L, nh, hd = shape
+    n_slots, nkv, S = _pool(k_cache, hd)
+    pool = k_cache.shape
     P, kp, vp = 0, None, None
     if (k_prefix is None) != (v_prefix is None):
         raise ValueError("k_prefix and v_prefix: both or neither")
     if k_prefix is not None:
         P = k_prefix.shape[1] if k_prefix.dim() == 3 else -1
-        kp = C.byref(_heads(k_prefix.unsqueeze(0), "k_prefix", q, (1, nkv, P, hd), (0, 2, 1)))
-        vp = C.byref(_heads(v_prefix.unsqueeze(0), "v_prefix", q, (1, nkv, P, hd), (0, 2, 1)))
+        prefix = (1, nkv, P, hd)
+        kp = _cache(k_prefix.unsqueeze(0), "k_prefix", prefix, dt, dev)
+        vp = _cache(v_prefix.unsqueeze(0), "v_prefix", prefix, dt, dev)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, L, nh), dtype=torch.float32, device=q.device)
-    c = FmxAttentionShape(_DT[q.dtype], B, L, nh, nkv, hd, scale)
-    S = k_cache.shape[2]
-    ws = _workspace(workspace, lib.fmx_attention_shared_prefix_workspace_size(C.byref(c), P, S), q)
+        out = q.new_empty(shape)
+    lse = q.new_empty((B, L, nh), dtype=torch.float32)
+    c = _byref(FmxAttentionShape(_DT[dt], B, L, nh, nkv, hd, scale))
+    ws = _workspace(workspace, lib.fmx_attention_shared_prefix_workspace_size(c, P, S), q)
     _lib.check(lib.fmx_attention_shared_prefix(
-        C.byref(c), C.byref(_heads(q, "q", q, shape)), kp, vp, P, C.byref(kc), C.byref(vc), k_cache.shape[0], S,
-        _ints(offsets, "offsets", q, (B,)), _ints(slots, "slots", q, (B,)), C.byref(_heads(out, "out", q, shape)),
-        lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream()))
+        c, _heads(q, "q", shape, dt, dev), kp, vp, P, _cache(k_cache, "k_cache", pool, dt, dev),
+        _cache(v_cache, "v_cache", pool, dt, dev), n_slots, S, _flat(offsets, "offsets", (B,), i32, dev),
+        _flat(slots, "slots", (B,), i32, dev), _heads(out, "out", shape, dt, dev), lse.data_ptr(), ws.data_ptr(),
+        ws.numel(), _stream()))
     return out, lse
 
 
@@ -226,29 +239,27 @@ def attention_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     position, summed over a kv head's query heads. weights_out may be weights;
     a new one made here holds `weights` (or 0) in the slots of no sequence."""
     lib = _lib.load()
-    B, L, nh, hd = shape = _rows(q, "q")
-    nkv = k_cache.shape[1] if k_cache.dim() == 4 else 0
-    kc, vc = _cache(k_cache, "k_cache", q, nkv, hd), _cache(v_cache, "v_cache", q, nkv, hd)
-    if v_cache.shape[:3] != k_cache.shape[:3]:
-        raise ValueError("k_cache and v_cache differ in shape")
-    n_slots, S = k_cache.shape[0], k_cache.shape[2]
-    w_in = _floats(weights, "weights", q, (n_slots, nkv, S))
+    dev, shape, dt, i32, f32 = _device(q, "q", _ROWS), q.shape, q.dtype, torch.int32, torch.float32
+    B, L, nh, hd = shape
+    n_slots, nkv, S = _pool(k_cache, hd)
+    pool, wsh = k_cache.shape, (n_slots, nkv, S)
+    w_in = _flat(weights, "weights", wsh, f32, dev)
     if weights_out is None:
         if slots is None and n_slots == B and L > 0:
-            weights_out = torch.empty((n_slots, nkv, S), dtype=torch.float32, device=q.device)
+            weights_out = q.new_empty(wsh, dtype=f32)
         elif weights is not None:
             weights_out = weights.clone()
         else:
-            weights_out = torch.zeros((n_slots, nkv, S), dtype=torch.float32, device=q.device)
+            weights_out = q.new_zeros(wsh, dtype=f32)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    c = FmxAttentionShape(_DT[q.dtype], B, L, nh, nkv, hd, scale)
-    ws = _workspace(workspace, lib.fmx_attention_scored_workspace_size(C.byref(c), S), q)
+        out = q.new_empty(shape)
+    c = _byref(FmxAttentionShape(_DT[dt], B, L, nh, nkv, hd, scale))
+    ws = _workspace(workspace, lib.fmx_attention_scored_workspace_size(c, S), q)
     _lib.check(lib.fmx_attention_scored(
-        C.byref(c), C.byref(_heads(q, "q", q, shape)), C.byref(kc), C.byref(vc), n_slots, S,
-        _ints(offsets, "offsets", q, (B,)), _ints(slots, "slots", q, (B,)), w_in,
-        _floats(weights_out, "weights_out", q, (n_slots, nkv, S)), C.byref(_heads(out, "out", q, shape)),
-        ws.data_ptr(), ws.numel(), _stream()))
+        c, _heads(q, "q", shape, dt, dev), _cache(k_cache, "k_cache", pool, dt, dev),
+        _cache(v_cache, "v_cache", pool, dt, dev), n_slots, S, _flat(offsets, "offsets", (B,), i32, dev),
+        _flat(slots, "slots", (B,), i32, dev), w_in, _flat(weights_out, "weights_out", wsh, f32, dev),
+        _heads(out, "out", shape, dt, dev), ws.data_ptr(), ws.numel(), _stream()))
     return out, weights_out
 
 
@@ -263,33 +274,27 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     (lengths_out int32 [batch], kept int32 [batch, kv_heads, budget]: the kept
     positions, -1 behind the last). lengths_out may be lengths."""
     lib = _lib.load()
-    if k_cache.dim() != 4:
-        raise ValueError(f"k_cache: shape {tuple(k_cache.shape)}, expected [slots, kv_heads, positions, head_dim]")
-    if k_cache.dtype not in _DT:
-        raise TypeError(f"k_cache: {k_cache.dtype}")
-    _on_device(k_cache, "k_cache")
-    n_slots, nkv, S, hd = k_cache.shape
-    B = lengths.shape[0] if lengths.dim() == 1 else -1
-    kc, vc = _cache(k_cache, "k_cache", k_cache, nkv, hd), _cache(v_cache, "v_cache", k_cache, nkv, hd)
-    if v_cache.shape != k_cache.shape:
-        raise ValueError("k_cache and v_cache differ in shape")
-    w = _floats(weights, "weights", k_cache, (n_slots, nkv, S))
+    dev, pool, dt, i32, f32 = _device(k_cache, "k_cache", _SLOTS), k_cache.shape, k_cache.dtype, torch.int32, torch.float32
+    n_slots, nkv, S, hd = pool
+    if lengths.dim() != 1:
+        raise ValueError(f"lengths: shape {tuple(lengths.shape)}, expected [batch]")
+    if budget < 1:
+        raise ValueError(f"budget {budget}")
+    B = lengths.shape[0]
     ko = vo = wo = None
     S_out = 0
     if out is not None:
         k_out, v_out, w_out = out
         S_out = k_out.shape[2] if k_out.dim() == 4 else -1
-        want = (n_slots, nkv, S_out, hd)
-        ko = C.byref(_heads(k_out, "out[0]", k_cache, want, (0, 2, 1)))
-        vo = C.byref(_heads(v_out, "out[1]", k_cache, want, (0, 2, 1)))
-        wo = _floats(w_out, "out[2]", k_cache, want[:3])
-    if budget < 1:
-        raise ValueError(f"budget {budget}")
+        to = (n_slots, nkv, S_out, hd)
+        ko, vo = _cache(k_out, "out[0]", to, dt, dev), _cache(v_out, "out[1]", to, dt, dev)
+        wo = _flat(w_out, "out[2]", to[:3], f32, dev)
     if lengths_out is None:
-        lengths_out = torch.empty((max(B, 0),), dtype=torch.int32, device=k_cache.device)
-    kept = torch.empty((max(B, 0), nkv, budget), dtype=torch.int32, device=k_cache.device)
+        lengths_out = lengths.new_empty((B,))
+    kept = lengths.new_empty((B, nkv, budget))
     _lib.check(lib.fmx_cache_evict(
-        _DT[k_cache.dtype], B, nkv, hd, C.byref(kc), C.byref(vc), w, n_slots, S,
-        _ints(lengths, "lengths", k_cache, (B,)), _ints(slots, "slots", k_cache, (B,)), budget, sinks, recent, ko, vo,
-        wo, S_out, _ints(lengths_out, "lengths_out", k_cache, (B,)), kept.data_ptr(), None, 0, _stream()))
+        _DT[dt], B, nkv, hd, _cache(k_cache, "k_cache", pool, dt, dev), _cache(v_cache, "v_cache", pool, dt, dev),
+        _flat(weights, "weights", (n_slots, nkv, S), f32, dev), n_slots, S, _flat(lengths, "lengths", (B,), i32, dev),
+        _flat(slots, "slots", (B,), i32, dev), budget, sinks, recent, ko, vo, wo, S_out,
+        _flat(lengths_out, "lengths_out", (B,), i32, dev), kept.data_ptr(), None, 0, _stream()))
     return lengths_out, kept

@@ -84,12 +84,18 @@ int check_counts(int64_t batch, int64_t seq_len, int64_t n_heads, int64_t n_kv_h
   return FMX_OK;
 }
 
-// data: `align` bytes (the element's size, or 16 with strides in whole 8s)
-int check_view(const fmx_heads* v, const char* name, size_t align, int stride_mult) {
+// A view of [nb, nt, nh] rows into *out (strides of axes with one entry are
+// never used and taken as 0). data: aligned to `align` bytes (the element's
+// size, or 16 with strides in whole 8s).
+int check_view(const fmx_heads* v, const char* name, int64_t nb, int64_t nt, int64_t nh, size_t align,
+               int stride_mult, fmx_heads* out) {
   if (!v || !v->data) return fail(FMX_ERR_ARG, "%s is NULL", name);
   if (!aligned(v->data, align)) return fail(FMX_ERR_ARG, "%s: data not %zu-byte aligned", name, align);
-  for (int64_t s : {v->batch_stride, v->token_stride, v->head_stride}) {
-    if (s < 0 || s > kMaxStride) return fail(FMX_ERR_SHAPE, "%s: stride %lld", name, (long long)s);
+  if (v->batch_stride < 0 || v->token_stride < 0 || v->head_stride < 0)
+    return fail(FMX_ERR_SHAPE, "%s: negative stride", name);
+  *out = fmx_heads{v->data, nb > 1 ? v->batch_stride : 0, nt > 1 ? v->token_stride : 0, nh > 1 ? v->head_stride : 0};
+  for (int64_t s : {out->batch_stride, out->token_stride, out->head_stride}) {
+    if (s > kMaxStride) return fail(FMX_ERR_SHAPE, "%s: stride %lld", name, (long long)s);
     if (s % stride_mult) return fail(FMX_ERR_UNSUPPORTED, "%s: strides must be multiples of %d", name, stride_mult);
   }
   return FMX_OK;
@@ -236,8 +242,11 @@ int fmx_rope(const fmx_rope_angles* angles, int dtype, int64_t batch, int64_t se
   if (batch * seq_len == 0) return ok();
   if (!angles->freqs || !positions) return fail(FMX_ERR_ARG, "NULL freqs or positions");
   const int es = elem_size(dtype);
-  FMX_RC(check_view(x, "x", es, 1));
-  FMX_RC(check_view(out, "out", es, 1));
+  fmx_heads x_v, out_v;
+  FMX_RC(check_view(x, "x", batch, seq_len, n_heads, es, 1, &x_v));
+  FMX_RC(check_view(out, "out", batch, seq_len, n_heads, es, 1, &out_v));
+  x = &x_v;
+  out = &out_v;
   if (!same(x, out) && overlap(span(x, batch, seq_len, n_heads, head_dim, es),
                                span(out, batch, seq_len, n_heads, head_dim, es)))
     return fail(FMX_ERR_ARG, "out overlaps x with other strides or another start");
@@ -272,12 +281,19 @@ int fmx_rope_append(const fmx_rope_angles* angles, int dtype, int64_t batch, int
   if (batch * seq_len == 0) return ok();
   if (!angles->freqs || !positions || !offsets) return fail(FMX_ERR_ARG, "NULL freqs, positions or offsets");
   const int es = elem_size(dtype);
-  FMX_RC(check_view(q, "q", es, 1));
-  FMX_RC(check_view(k, "k", es, 1));
-  FMX_RC(check_view(v, "v", es, 1));
-  FMX_RC(check_view(q_out, "q_out", es, 1));
-  FMX_RC(check_view(k_cache, "k_cache", es, 1));
-  FMX_RC(check_view(v_cache, "v_cache", es, 1));
+  fmx_heads q_v, k_v, v_v, qo_v, kc_v, vc_v;
+  FMX_RC(check_view(q, "q", batch, seq_len, n_heads, es, 1, &q_v));
+  FMX_RC(check_view(k, "k", batch, seq_len, n_kv_heads, es, 1, &k_v));
+  FMX_RC(check_view(v, "v", batch, seq_len, n_kv_heads, es, 1, &v_v));
+  FMX_RC(check_view(q_out, "q_out", batch, seq_len, n_heads, es, 1, &qo_v));
+  FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, n_kv_heads, es, 1, &kc_v));
+  FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, n_kv_heads, es, 1, &vc_v));
+  q = &q_v;
+  k = &k_v;
+  v = &v_v;
+  q_out = &qo_v;
+  k_cache = &kc_v;
+  v_cache = &vc_v;
   const Span ins[3] = {span(q, batch, seq_len, n_heads, head_dim, es),
                        span(k, batch, seq_len, n_kv_heads, head_dim, es),
                        span(v, batch, seq_len, n_kv_heads, head_dim, es)};
@@ -332,31 +348,28 @@ int fmx_attention_shared_prefix(const fmx_attention_shape* shape, const fmx_head
   if (max_seq > 0 && !slots && n_slots < shape->batch)
     return fail(FMX_ERR_SHAPE, "n_slots below batch without slots");
   if (shape->batch * shape->seq_len == 0) return ok();
-  FMX_RC(check_view(q, "q", 16, 8));
-  FMX_RC(check_view(out, "out", 16, 8));
+  fmx_heads q_v, out_v, kp_v, vp_v, kc_v, vc_v;
+  FMX_RC(check_view(q, "q", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &q_v));
+  FMX_RC(check_view(out, "out", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &out_v));
   if (prefix_len > 0) {
-    FMX_RC(check_view(k_prefix, "k_prefix", 16, 8));
-    FMX_RC(check_view(v_prefix, "v_prefix", 16, 8));
+    FMX_RC(check_view(k_prefix, "k_prefix", 1, prefix_len, shape->n_kv_heads, 16, 8, &kp_v));
+    FMX_RC(check_view(v_prefix, "v_prefix", 1, prefix_len, shape->n_kv_heads, 16, 8, &vp_v));
+    a.kp = view(&kp_v);
+    a.vp = view(&vp_v);
   }
   if (max_seq > 0) {
-    FMX_RC(check_view(k_cache, "k_cache", 16, 8));
-    FMX_RC(check_view(v_cache, "v_cache", 16, 8));
-    if (!offsets) return fail(FMX_ERR_ARG, "offsets is NULL");
-  }
-  hipStream_t stream = static_cast<hipStream_t>(stream_);
-  a.q = view(q);
-  a.out = view(out);
-  if (prefix_len > 0) {
-    a.kp = view(k_prefix);
-    a.vp = view(v_prefix);
-  }
-  if (max_seq > 0) {
-    a.kc = view(k_cache);
-    a.vc = view(v_cache);
+    FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &kc_v));
+    FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &vc_v));
+    a.kc = view(&kc_v);
+    a.vc = view(&vc_v);
     a.offs = offsets;
     a.slots = slots;
     a.n_slots = n_slots;
+    if (!offsets) return fail(FMX_ERR_ARG, "offsets is NULL");
   }
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  a.q = view(&q_v);
+  a.out = view(&out_v);
   a.lse = lse;
   Workspace ws;
   FMX_RC(ws.bind(workspace, workspace_bytes, cache_attn_workspace(a), stream));
@@ -379,10 +392,11 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
   CacheAttnArgs a = attention_args(shape, 0, max_seq, true);
   if (!slots && n_slots < shape->batch) return fail(FMX_ERR_SHAPE, "n_slots below batch without slots");
   if (shape->batch * shape->seq_len == 0) return ok();
-  FMX_RC(check_view(q, "q", 16, 8));
-  FMX_RC(check_view(out, "out", 16, 8));
-  FMX_RC(check_view(k_cache, "k_cache", 16, 8));
-  FMX_RC(check_view(v_cache, "v_cache", 16, 8));
+  fmx_heads q_v, out_v, kc_v, vc_v;
+  FMX_RC(check_view(q, "q", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &q_v));
+  FMX_RC(check_view(out, "out", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &out_v));
+  FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &kc_v));
+  FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &vc_v));
   if (!offsets || !weights_out) return fail(FMX_ERR_ARG, "NULL offsets or weights_out");
   if (!aligned(weights_in, 4) || !aligned(weights_out, 4)) return fail(FMX_ERR_ARG, "weights not 4-byte aligned");
   if (weights_in && weights_in != weights_out) {
@@ -392,10 +406,10 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
     if (overlap({i, i + n}, {o, o + n})) return fail(FMX_ERR_ARG, "weights_out overlaps weights_in in part");
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);
-  a.q = view(q);
-  a.out = view(out);
-  a.kc = view(k_cache);
-  a.vc = view(v_cache);
+  a.q = view(&q_v);
+  a.out = view(&out_v);
+  a.kc = view(&kc_v);
+  a.vc = view(&vc_v);
   a.offs = offsets;
   a.slots = slots;
   a.n_slots = n_slots;
@@ -437,13 +451,18 @@ int fmx_cache_evict(int dtype, int64_t batch, int64_t n_kv_heads, int64_t head_d
     return fail(FMX_ERR_SHAPE, "out_max_seq %lld", (long long)out_max_seq);
   if (!slots && n_slots < batch) return fail(FMX_ERR_SHAPE, "n_slots below batch without slots");
   if (batch == 0) return ok();
-  FMX_RC(check_view(k_cache, "k_cache", 2, 1));
-  FMX_RC(check_view(v_cache, "v_cache", 2, 1));
+  fmx_heads kc_v, vc_v, ko_v, vo_v;
+  FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, n_kv_heads, 2, 1, &kc_v));
+  FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, n_kv_heads, 2, 1, &vc_v));
+  k_cache = &kc_v;
+  v_cache = &vc_v;
   if (!weights || !lengths || !lengths_out) return fail(FMX_ERR_ARG, "NULL weights, lengths or lengths_out");
   if (!aligned(weights, 4) || !aligned(weights_out, 4)) return fail(FMX_ERR_ARG, "weights not 4-byte aligned");
   if (!in_place) {
-    FMX_RC(check_view(k_out, "k_out", 2, 1));
-    FMX_RC(check_view(v_out, "v_out", 2, 1));
+    FMX_RC(check_view(k_out, "k_out", n_slots, out_max_seq, n_kv_heads, 2, 1, &ko_v));
+    FMX_RC(check_view(v_out, "v_out", n_slots, out_max_seq, n_kv_heads, 2, 1, &vo_v));
+    k_out = &ko_v;
+    v_out = &vo_v;
     const uintptr_t w = reinterpret_cast<uintptr_t>(weights), wo = reinterpret_cast<uintptr_t>(weights_out);
     const uintptr_t rows = static_cast<uintptr_t>(n_slots) * static_cast<uintptr_t>(n_kv_heads) * 4;
     const Span ins[3] = {span(k_cache, n_slots, max_seq, n_kv_heads, head_dim, 2),

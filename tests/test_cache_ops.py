@@ -254,14 +254,19 @@ def test_python_refusals(fmx):
     with pytest.raises(ValueError, match="HIP device"):
         fmx.cache_evict(kc, kc, torch.zeros(2, 2, 10), offs, 5)
     from flashmlx_amd import cache as M
+    bf, dev = torch.bfloat16, -1  # (CPU tensors)
     with pytest.raises(ValueError, match="k_cache: shape"):
-        M._cache(kc, "k_cache", q, 4, 64)
+        M._cache(kc, "k_cache", (2, 4, 10, 64), bf, dev)
     with pytest.raises(TypeError, match="k_cache"):
-        M._cache(kc.half(), "k_cache", q, 2, 64)
+        M._cache(kc.half(), "k_cache", kc.shape, bf, dev)
+    with pytest.raises(ValueError, match="k_cache is on cpu"):
+        M._cache(kc, "k_cache", kc.shape, bf, 0)
     with pytest.raises(ValueError, match="contiguous"):
-        M._cache(torch.zeros(2, 2, 10, 128, dtype=torch.bfloat16)[..., ::2], "k_cache", q, 2, 64)
-    for bad in (offs.long(), offs[:1], torch.zeros(4, dtype=torch.int32)[::2]):
+        M._cache(torch.zeros(2, 2, 10, 128, dtype=bf)[..., ::2], "k_cache", kc.shape, bf, dev)
+    for bad in (offs[:1], torch.zeros(4, dtype=torch.int32)[::2]):
         with pytest.raises(ValueError, match="offsets"):
-            M._ints(bad, "offsets", q, (2,))
-    with pytest.raises(ValueError, match="weights"):
-        M._floats(torch.zeros(2, 2, 10).half(), "weights", q, (2, 2, 10))
+            M._flat(bad, "offsets", (2,), torch.int32, dev)
+    with pytest.raises(TypeError, match="offsets"):
+        M._flat(offs.long(), "offsets", (2,), torch.int32, dev)
+    with pytest.raises(TypeError, match="weights"):
+        M._flat(torch.zeros(2, 2, 10).half(), "weights", (2, 2, 10), torch.float32, dev)
