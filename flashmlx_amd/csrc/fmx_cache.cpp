@@ -75,6 +75,8 @@ constexpr int64_t kMaxHeads = 65535;
 // strides: element offsets, and sums of a few of them, stay within 63 bits
 // whatever the rows' count
 constexpr int64_t kMaxStride = int64_t{1} << 34;
+// of the positions that attention reads: 64 rows' byte offsets within 32 bits
+constexpr int64_t kMaxKeyStride = int64_t{1} << 24;
 
 int check_counts(int64_t batch, int64_t seq_len, int64_t n_heads, int64_t n_kv_heads) {
   if (batch < 0 || seq_len < 0 || batch > kMaxRows || seq_len > kMaxRows || batch * seq_len > kMaxRows)
@@ -103,6 +105,12 @@ int check_view(const fmx_heads* v, const char* name, int64_t nb, int64_t nt, int
 
 HeadsView view(const fmx_heads* v) {
   return v ? HeadsView{v->data, v->batch_stride, v->token_stride, v->head_stride} : HeadsView{nullptr, 0, 0, 0};
+}
+
+int check_key_stride(const fmx_heads& k, const fmx_heads& v, const char* name) {
+  if (k.token_stride > kMaxKeyStride || v.token_stride > kMaxKeyStride)
+    return fail(FMX_ERR_UNSUPPORTED, "%s: token strides above 2^24", name);
+  return FMX_OK;
 }
 
 bool same(const fmx_heads* a, const fmx_heads* b) {
@@ -354,12 +362,14 @@ int fmx_attention_shared_prefix(const fmx_attention_shape* shape, const fmx_head
   if (prefix_len > 0) {
     FMX_RC(check_view(k_prefix, "k_prefix", 1, prefix_len, shape->n_kv_heads, 16, 8, &kp_v));
     FMX_RC(check_view(v_prefix, "v_prefix", 1, prefix_len, shape->n_kv_heads, 16, 8, &vp_v));
+    FMX_RC(check_key_stride(kp_v, vp_v, "prefix"));
     a.kp = view(&kp_v);
     a.vp = view(&vp_v);
   }
   if (max_seq > 0) {
     FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &kc_v));
     FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &vc_v));
+    FMX_RC(check_key_stride(kc_v, vc_v, "caches"));
     a.kc = view(&kc_v);
     a.vc = view(&vc_v);
     a.offs = offsets;
@@ -397,6 +407,7 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
   FMX_RC(check_view(out, "out", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &out_v));
   FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &kc_v));
   FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &vc_v));
+  FMX_RC(check_key_stride(kc_v, vc_v, "caches"));
   if (!offsets || !weights_out) return fail(FMX_ERR_ARG, "NULL offsets or weights_out");
   if (!aligned(weights_in, 4) || !aligned(weights_out, 4)) return fail(FMX_ERR_ARG, "weights not 4-byte aligned");
   if (weights_in && weights_in != weights_out) {

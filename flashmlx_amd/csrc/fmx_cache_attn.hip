@@ -13,6 +13,7 @@
 //
 //   attn_narrow_kernel   tiles of 16 or 32 rows, keys straight to registers
 //   attn_wide_kernel     tiles of 128 rows, keys and values staged in LDS
+//   attn_both_kernel     both in one grid
 //   attn_join_kernel     a row's pieces to its output; weights of the keys
 //                        from stored scores
 //   attn_weights_kernel, attn_weights_sum_kernel
@@ -30,6 +31,8 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kStep = 32;                // keys of a wave's step
 constexpr int kPiece = kStep * kWaves;   // pieces are whole multiples of these
+// up to so many rows of a kv head run in narrow tiles
+constexpr int kNarrowRows = 32;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -95,9 +98,12 @@ struct Plan {
 // - B) rounded up. Lengths may differ as they like: all pieces but each
 // sequence's last are equally long. Returns the sequence of piece w (-1:
 // none), its piece number in *k and c in *units; workgroup 0 leaves the table.
+struct PieceLds {
+  uint32_t tmp[kWaves + 1];
+  int seq, k;
+};
 __device__ int find_piece(const CacheAttnArgs& a, const Plan& pl, int w, bool write_table, int* k, int* units,
-                          uint32_t* s_tmp) {
-  __shared__ int s_seq, s_k;
+                          PieceLds& s) {
   const int tid = threadIdx.x;
   auto units_of = [&](int b) {
     const int64_t n = own_keys(a, seq_slot(a.slots, a.n_slots, b), a.offs[b], a.L - 1);
@@ -106,27 +112,27 @@ __device__ int find_piece(const CacheAttnArgs& a, const Plan& pl, int w, bool wr
   uint32_t mine = 0;
   for (int b = tid; b < a.B; b += kThreads) mine += units_of(b);
   uint32_t total;
-  block_exclusive_scan<kThreads>(mine, s_tmp, &total);
+  block_exclusive_scan<kThreads>(mine, s.tmp, &total);
   const uint32_t room = static_cast<uint32_t>(pl.o_grid - a.B);
   const uint32_t c = max(1u, (total + room - 1) / room);
-  if (tid == 0) s_seq = -1;
+  if (tid == 0) s.seq = -1;
   uint32_t base = 0;
   for (int b0 = 0; b0 < a.B; b0 += kThreads) {
     const int b = b0 + tid;
     const uint32_t n = b < a.B ? (units_of(b) + c - 1) / c : 0;
     uint32_t sum;
-    const uint32_t first = base + block_exclusive_scan<kThreads>(n, s_tmp, &sum);
+    const uint32_t first = base + block_exclusive_scan<kThreads>(n, s.tmp, &sum);
     if (static_cast<uint32_t>(w) >= first && static_cast<uint32_t>(w) < first + n) {
-      s_seq = b;
-      s_k = w - static_cast<int>(first);
+      s.seq = b;
+      s.k = w - static_cast<int>(first);
     }
     if (write_table && b < a.B) pl.table[b] = make_int2(static_cast<int>(first), static_cast<int>(n));
     base += sum;
   }
   __syncthreads();
-  *k = s_k;
+  *k = s.k;
   *units = static_cast<int>(c);
-  return s_seq;
+  return s.seq;
 }
 
 // ------------------------------------------------------------------ narrow tiles
@@ -155,8 +161,21 @@ struct Narrow {
   static constexpr int DT = HD / 16;            // 16-dimension tiles of the output
   static constexpr int VPL = HD / 16;           // dimensions of a key per lane
   static constexpr int VW = VPL / 2;            // 32-bit words of them
-  static constexpr int kRow = HD + 4;           // floats of a row in LDS
 };
+
+template <int RT>
+struct NarrowLds {
+  float m[kWaves][16 * RT], l[kWaves][16 * RT];
+  int left[kWaves];
+  PieceLds piece;
+};
+
+// where four dimensions from d on of a row's sums lie in LDS (rows one after
+// the other: shifted against each other by the row, for the banks)
+template <int HD>
+__device__ inline f32x4_t* sums_at(float* o, int row, int d) {
+  return reinterpret_cast<f32x4_t*>(o + row * HD + ((d >> 2) ^ (row & 7)) * 4);
+}
 
 // dimension of A row `row`, tile dt (runs of up to 8 per lane)
 template <int HD>
@@ -202,26 +221,23 @@ __device__ __attribute__((noinline)) void add_left_out(f32x4_t& acc, const uint1
 // ANY: hd may be below HD (chunks behind it read as zeros), and the rows of a
 // tile may see different keys (several queries per sequence)
 template <bool F16, int HD, int RT, bool ANY>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
+__device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& a, const Plan& pl, int n_prefix,
+                                                           int block, float* o0, float* o1,
+                                                           NarrowLds<RT>& s) {
   using N = Narrow<HD>;
   constexpr int KC = N::KC, DT = N::DT, VW = N::VW, VPL = N::VPL;
   typedef act8_t<F16> frag_t;
   // exp2's results are kept up to 2^10 for fp16 products, so that its
   // smallest normal number is 2^-24 of the largest weight; bf16 needs none
   constexpr float kBias = F16 ? 10.0f : 0.0f;
-  __shared__ __attribute__((aligned(16))) float s_o[2][16 * RT][N::kRow];
-  __shared__ float s_m[kWaves][16 * RT], s_l[kWaves][16 * RT];
-  __shared__ uint32_t s_tmp[kWaves + 1];
-  __shared__ int s_left[kWaves];
-
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i16 = lane & 15, j = lane >> 4;
 
   // ---- the item: rows, keys
-  const bool prefix = static_cast<int>(blockIdx.x) < n_prefix;
+  const bool prefix = block < n_prefix;
   const int tiles = prefix ? pl.p_tiles : pl.o_tiles;
-  int item = prefix ? blockIdx.x : blockIdx.x - n_prefix;
+  int item = prefix ? block : block - n_prefix;
   const int tile = item % tiles;
   item /= tiles;
   const int g = item % a.nkv;
@@ -241,7 +257,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     vts = a.vp.ts;
   } else {
     int k, units;
-    seq = find_piece(a, pl, piece, piece == 0 && g == 0 && tile == 0, &k, &units, s_tmp);
+    seq = find_piece(a, pl, piece, piece == 0 && g == 0 && tile == 0, &k, &units, s.piece);
     if (seq < 0) return;
     seq = __builtin_amdgcn_readfirstlane(seq);
     slot = seq_slot(a.slots, a.n_slots, seq);
@@ -317,22 +333,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   auto load_v = [&](int kk) {
     const bool whole = kk + kStep <= k1;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const int row = 16 * (s >> 2) + (s & 3);
+    for (int sl = 0; sl < 8; ++sl) {
+      const int row = 16 * (sl >> 2) + (sl & 3);
       const uint16_t* p = whole ? vp0 + (kk - kk0 + row) * vts
                                 : vb + min(kk + row + 4 * j, k1 - 1) * vts + (VPL == 4 ? 4 : 8) * i16;
       if constexpr (VPL == 4) {
         u32x2_t w = {0, 0};
         if (!ANY || 4 * i16 < a.hd) w = *reinterpret_cast<const u32x2_t*>(p);
-        vw[s][0] = w[0];
-        vw[s][1] = w[1];
+        vw[sl][0] = w[0];
+        vw[sl][1] = w[1];
       } else {
 #pragma unroll
         for (int q = 0; q < VPL / 8; ++q) {
           u32x4_t w = {0, 0, 0, 0};
           if (!ANY || 128 * q + 8 * i16 < a.hd) w = *reinterpret_cast<const u32x4_t*>(p + 128 * q);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vw[s][4 * q + i] = w[i];
+          for (int i = 0; i < 4; ++i) vw[sl][4 * q + i] = w[i];
         }
       }
     }
@@ -351,14 +367,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   if (kk < k1) load_k(kk);
   for (; kk < k1; kk += kPiece) {
     load_v(kk);
-    f32x4_t s[RT][2];
+    f32x4_t sc[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        s[rt][x] = f32x4_t{0, 0, 0, 0};
+        sc[rt][x] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < KC; ++t) s[rt][x] = mfma16(__builtin_bit_cast(frag_t, kw[x][t]), qf[rt][t], s[rt][x]);
+        for (int t = 0; t < KC; ++t) sc[rt][x] = mfma16(__builtin_bit_cast(frag_t, kw[x][t]), qf[rt][t], sc[rt][x]);
       }
     if (kk + kPiece < k1) load_k(kk + kPiece);
     const bool part = kk + kStep > all;  // some row does not see all of the step
@@ -369,23 +385,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[rt][x][r] *= c;
+        for (int r = 0; r < 4; ++r) sc[rt][x][r] *= c;
       if (sc_out[rt]) {
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-          *reinterpret_cast<f32x4_t*>(sc_out[rt] + kk + 16 * x + 4 * j) = s[rt][x];
+          *reinterpret_cast<f32x4_t*>(sc_out[rt] + kk + 16 * x + 4 * j) = sc[rt][x];
       }
       if (part) {
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (kk + 16 * x + 4 * j + r >= limit[rt]) s[rt][x][r] = neg_inf();
+            if (kk + 16 * x + 4 * j + r >= limit[rt]) sc[rt][x][r] = neg_inf();
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[rt][x][r]);
+        for (int r = 0; r < 4; ++r) mt = fmaxf(mt, sc[rt][x][r]);
       mt = quad_max(mt) - kBias;
       if (__any(mt > mref[rt])) {
         const float mn = fmaxf(mt, mref[rt]);
@@ -400,7 +416,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(s[rt][x][r] - ms);
+          const float p = __builtin_amdgcn_exp2f(sc[rt][x][r] - ms);
           lsum[rt] += p;
           typedef typename std::conditional<F16, _Float16, __bf16>::type half_t;
           const half_t hi = static_cast<half_t>(p);
@@ -442,22 +458,22 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     }
   }
 
-  if (ANY && lane == 0) s_left[wave] = left_out;
+  if (ANY && lane == 0) s.left[wave] = left_out;
   // ---- the waves' sums together: waves 0 and 1 leave theirs, 2 and 3 add
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const float l = quad_sum(lsum[rt]);
     if (j == 0) {
-      s_m[wave][rt * 16 + i16] = mref[rt];
-      s_l[wave][rt * 16 + i16] = l;
+      s.m[wave][rt * 16 + i16] = mref[rt];
+      s.l[wave][rt * 16 + i16] = l;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    float m = s_m[0][rt * 16 + i16];
+    float m = s.m[0][rt * 16 + i16];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][rt * 16 + i16]);
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s.m[w][rt * 16 + i16]);
     const float f = __builtin_amdgcn_exp2f(mref[rt] - (m == neg_inf() ? 0.0f : m));
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
@@ -470,7 +486,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int d4 = 0; d4 < DT; d4 += 4) {
-          f32x4_t* p = reinterpret_cast<f32x4_t*>(&s_o[wave & 1][rt * 16 + i16][out_dim<HD>(4 * j + r, d4)]);
+          f32x4_t* p = sums_at<HD>(wave & 1 ? o1 : o0, rt * 16 + i16, out_dim<HD>(4 * j + r, d4));
           f32x4_t v = {o[rt][d4][r], o[rt][d4 + 1][r], o[rt][d4 + 2][r], o[rt][d4 + 3][r]};
           *p = add ? *p + v : v;
         }
@@ -488,8 +504,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   const int h4 = a.hd / 4;
   for (int i = tid; i < nr * h4; i += kThreads) {
     const int r = i / h4, d = (i - r * h4) * 4;
-    f32x4_t v = *reinterpret_cast<const f32x4_t*>(&s_o[0][r][d]) + *reinterpret_cast<const f32x4_t*>(&s_o[1][r][d]);
-    if (ANY && (s_left[0] | s_left[1] | s_left[2] | s_left[3]))
+    f32x4_t v = *sums_at<HD>(o0, r, d) + *sums_at<HD>(o1, r, d);
+    if (ANY && (s.left[0] | s.left[1] | s.left[2] | s.left[3]))
       add_left_out<F16>(v, vb + d, vts, max(k0, all / kStep * kStep),
                         prefix ? k1
                                : static_cast<int>(min(own_keys(a, slot, off, (row0 + r) / a.rep),
@@ -497,15 +513,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
     *reinterpret_cast<f32x4_t*>(po + static_cast<int64_t>(i) * 4) = v;
   }
   if (tid < nr) {
-    float m = s_m[0][tid];
+    float m = s.m[0][tid];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][tid]);
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s.m[w][tid]);
     float l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
-      l += s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - (m == neg_inf() ? 0.0f : m));
+      l += s.l[w][tid] * __builtin_amdgcn_exp2f(s.m[w][tid] - (m == neg_inf() ? 0.0f : m));
     (prefix ? pl.p_ml : pl.o_ml)[first + tid] = make_float2(m, l);
   }
+}
+
+template <bool F16, int HD, int RT, bool ANY>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
+void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
+  __shared__ __attribute__((aligned(16))) float s_o[2][16 * RT * HD];
+  __shared__ NarrowLds<RT> s;
+  narrow_item<F16, HD, RT, ANY>(a, pl, n_prefix, blockIdx.x, s_o[0], s_o[1], s);
 }
 
 // ------------------------------------------------------------------ wide tiles
@@ -558,29 +582,60 @@ struct WideGrid {
   int pairs, padded, tiles, splits;
 };
 
+// Arrays of their own, so that the compiler can tell the buffers that loads are
+// on their way to from those being read (it would wait for the loads before
+// every read otherwise).
+template <int HD>
+struct WideLds {
+  uint16_t *k0, *k1, *v0, *v1;  // kWideKeys * HD each
+  int* left;
+};
+#define FMX_WIDE_LDS(HD, name)                                                       \
+  __shared__ __attribute__((aligned(16))) uint16_t name##_k0[kWideKeys * HD];        \
+  __shared__ __attribute__((aligned(16))) uint16_t name##_k1[kWideKeys * HD];        \
+  __shared__ __attribute__((aligned(16))) uint16_t name##_v0[kWideKeys * HD];        \
+  __shared__ __attribute__((aligned(16))) uint16_t name##_v1[kWideKeys * HD];        \
+  __shared__ int name##_left;                                                        \
+  const WideLds<HD> name{name##_k0, name##_k1, name##_v0, name##_v1, &name##_left}
+
+// Rows of both arrays lie one after the other, their 16-byte chunks in an
+// order of the row's own, so that the lanes that LDS serves together fall on
+// different banks: a key's chunk c at c ^ swz_k (16 rows' same chunk), a
+// value's 32-byte segment at segment ^ swz_v (8 rows' same segment).
+template <int HD>
+__device__ inline int swz_k(int row) {
+  return HD == 64 ? row >> 1 & 7 : row & 15;
+}
+template <int HD>
+__device__ inline int swz_v(int row) {
+  return HD == 64 ? row >> 1 & 3 : row & 7;
+}
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+// 4 x 16 elements across 16 lanes: lane i gets element i % 4 of the lanes i / 4 + 4 e
+__device__ inline s16x4_t lds_read_tr(const uint16_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4_t*)const_cast<uint16_t*>(p));
+}
+
 template <bool F16, int HD, bool ANY>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD > 128 ? 1 : 2)))
-void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
+__device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a, const Plan& pl, const WideGrid& wg,
+                                                         int block, const WideLds<HD>& sh) {
   typedef act8_t<F16> frag_t;
   constexpr int KS = HD / 16;              // score steps
   constexpr int DT = HD / 32;              // dimension tiles
-  constexpr int kKRow = HD + 8;            // elements of a key's row
-  constexpr int kVRow = kWideKeys + 8;     // of a dimension's
-  constexpr int kBuf = kWideKeys * kKRow + HD * kVRow;
-  constexpr int NK = kWideKeys * HD / 8 / kThreads;       // 16-byte loads of keys per thread
-  constexpr int NV = (kWideKeys / 4 * HD / 8 + kThreads - 1) / kThreads;  // 4-key blocks of values
+  constexpr int kRowChunks = HD / 8;
+  constexpr int kDmaRows = kWave / kRowChunks;             // rows of a wave's load
+  constexpr int NL = kWideKeys / kWaves / kDmaRows;        // loads of a wave per array
   constexpr float kBias = F16 ? 8.0f : 0.0f;
-  __shared__ __attribute__((aligned(16))) uint16_t s_kv[2][kBuf];
-  __shared__ int s_left;
-
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, h2 = lane >> 5;
 
   // ---- the item
-  const int pair = blockIdx.x % wg.padded;
+  const int pair = block % wg.padded;
   if (pair >= wg.pairs) return;
-  const int tile = wg.tiles - 1 - static_cast<int>(blockIdx.x / wg.padded);  // the rows that see most first
+  const int tile = wg.tiles - 1 - block / wg.padded;  // the rows that see most first
   const int g = pair % a.nkv;
   const int split = wg.prefix ? pair / a.nkv : pair / a.nkv % wg.splits;
   const int seq = wg.prefix ? 0 : pair / a.nkv / wg.splits;
@@ -615,7 +670,7 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
   k0 = __builtin_amdgcn_readfirstlane(k0);
   k1 = __builtin_amdgcn_readfirstlane(k1);
   all = __builtin_amdgcn_readfirstlane(all);
-  if (ANY && tid == 0) s_left = 0;
+  if (ANY && tid == 0) *sh.left = 0;
 
   // ---- this lane's row
   const int m = row0 + wave * 32 + c32;
@@ -638,84 +693,67 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
     }
   }
 
-  // ---- staging
-  u32x4_t kr[NK], vr[NV][4];
-  const int kg = tid & 15;
-  constexpr int kKStep = kThreads / (HD / 8);      // keys between a thread's loads
-  constexpr bool kVWhole = HD / 8 % (kThreads / 16) == 0;
-  const int kch = tid % (HD / 8), kkey = tid / (HD / 8);
-  // (a thread's 64-bit row products are formed once; a step adds a scalar one)
-  const uint16_t* kp0 = kb + min(k0 + kkey, max(k1 - 1, 0)) * kts + 8 * kch;
-  const uint16_t* vp0 = vb + min(k0 + 4 * kg, max(k1 - 1, 0)) * vts + 8 * (tid >> 4);
-  auto load = [&](int kt) {
+  // ---- staging: straight to LDS, wave w rows 16 w .. of both arrays
+  const int lr = lane / kRowChunks, lc = lane % kRowChunks;
+  auto k_chunk = [&](int i) { return lc ^ swz_k<HD>(i * kDmaRows + lr); };
+  auto v_chunk = [&](int i) { return lc ^ swz_v<HD>(i * kDmaRows + lr) << 1; };
+  uint32_t ko[NL], vo[NL];  // byte offsets from the first position's row
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const uint32_t row = wave * 16 + i * kDmaRows + lr;
+    ko[i] = (row * static_cast<uint32_t>(kts) + 8 * k_chunk(i)) * 2;
+    vo[i] = (row * static_cast<uint32_t>(vts) + 8 * v_chunk(i)) * 2;
+  }
+  auto dma = [&](const uint16_t* base, int64_t ts, const uint32_t (&off_b)[NL], bool keys, int kt, uint16_t* to) {
+    const uint8_t* at = reinterpret_cast<const uint8_t*>(base + kt * ts);
     const bool whole = kt + kWideKeys <= k1;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      const uint16_t* p =
-          whole ? kp0 + (kt - k0 + i * kKStep) * kts : kb + min(kt + kkey + i * kKStep, k1 - 1) * kts + 8 * kch;
-      if (ANY) kr[i] = u32x4_t{0, 0, 0, 0};
-      if (!ANY || 8 * kch < a.hd) kr[i] = *reinterpret_cast<const u32x4_t*>(p);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int ch = (tid >> 4) + i * (kThreads / 16);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint16_t* p = whole ? vp0 + (kt - k0 + e) * vts + i * (kThreads / 2)
-                                  : vb + min(kt + 4 * kg + e, k1 - 1) * vts + 8 * ch;
-        if (ANY || !kVWhole) vr[i][e] = u32x4_t{0, 0, 0, 0};
-        if ((!ANY && kVWhole) || 8 * ch < (ANY ? a.hd : HD)) vr[i][e] = *reinterpret_cast<const u32x4_t*>(p);
-      }
+    for (int i = 0; i < NL; ++i) {
+      const int row = wave * 16 + i * kDmaRows + lr, ch = keys ? k_chunk(i) : v_chunk(i);
+      uint32_t o = off_b[i];
+      // rows behind the piece's last are read as its last
+      if (!whole) o = (static_cast<uint32_t>(min(row, k1 - 1 - kt)) * static_cast<uint32_t>(ts) + 8 * ch) * 2;
+      if (!ANY || 8 * ch < a.hd)
+        __builtin_amdgcn_global_load_lds(
+            at + o, (__attribute__((address_space(3))) void*)(to + (wave * 16 + i * kDmaRows) * HD), 16, 0, 0);
     }
   };
-  auto store = [&](int kt, int buf) {
-    uint16_t* sk = s_kv[buf];
-    uint16_t* sv = s_kv[buf] + kWideKeys * kKRow;
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      *reinterpret_cast<u32x4_t*>(sk + (kkey + i * kKStep) * kKRow + kch * 8) = kr[i];
-    }
-    if (kt + kWideKeys > all) {
-      // values behind the piece count nothing, whatever they hold; infinite
-      // and NaN ones that not all rows see are left out and added at the end
+  auto load_k = [&](int kt, int buf) { dma(kb, kts, ko, true, kt, buf ? sh.k1 : sh.k0); };
+  auto load_v = [&](int kt, int buf) { dma(vb, vts, vo, false, kt, buf ? sh.v1 : sh.v0); };
+  // Values behind the piece count nothing, whatever they hold; infinite and
+  // NaN ones that not all rows see are left out and added at the end.
+  auto clean_v = [&](int kt, int buf) {
+    for (int x = tid; x < kWideKeys * kRowChunks; x += kThreads) {
+      u32x4_t* at = reinterpret_cast<u32x4_t*>(buf ? sh.v1 : sh.v0) + x;
+      u32x4_t w = *at;
       u16x2_t top = {0, 0};
+      const bool in = kt + x / kRowChunks < k1;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool in = kt + 4 * kg + e < k1;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            vr[i][e][w] = in ? vr[i][e][w] : 0u;
-            if (ANY && a.L > 1) top = top_exp<F16>(top, vr[i][e][w]);
-          }
-        }
-      if (ANY && is_top<F16>(top)) {
-        s_left = 1;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) vr[i][e][w] = word_finite<F16>(vr[i][e][w]);
+      for (int i = 0; i < 4; ++i) {
+        w[i] = in ? w[i] : 0u;
+        if (a.L > 1) top = top_exp<F16>(top, w[i]);
       }
-    }
-    // keys 4 kg ..: 16 u + 8 v + 4 h of the 64, at 16 u + 8 h + 4 v
-    const int pos = (kg >> 2) * 16 + (kg & 1) * 8 + (kg >> 1 & 1) * 4;
+      const bool bad = is_top<F16>(top);
+      if (bad) {
+        *sh.left = 1;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int ch = (tid >> 4) + i * (kThreads / 16);
-      if (kVWhole || ch < HD / 8) {
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const uint32_t sel = d % 2 ? 0x07060302u : 0x05040100u;
-          const u32x2_t w = {__builtin_amdgcn_perm(vr[i][1][d / 2], vr[i][0][d / 2], sel),
-                             __builtin_amdgcn_perm(vr[i][3][d / 2], vr[i][2][d / 2], sel)};
-          *reinterpret_cast<u32x2_t*>(sv + (8 * ch + d) * kVRow + pos) = w;
-        }
+        for (int i = 0; i < 4; ++i) w[i] = word_finite<F16>(w[i]);
       }
+      if (bad || !in) *at = w;
     }
+    __syncthreads();
   };
+
+  // ---- operands in LDS, in elements from a buffer's start
+  int ka[KS], va[DT];
+#pragma unroll
+  for (int t = 0; t < KS; ++t) ka[t] = c32 * HD + ((2 * t + h2) ^ swz_k<HD>(c32)) * 8;
+  {
+    const int row = 4 * h2 + (lane & 15) / 4;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      va[dt] = row * HD + ((2 * dt + (lane >> 4 & 1)) ^ swz_v<HD>(row)) * 16 + (lane & 3) * 4;
+  }
 
   f32x16_t o[DT];
 #pragma unroll
@@ -725,77 +763,120 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
   float mref = neg_inf(), lsum = 0.0f;
   const float sc = a.scale * kLog2e;
 
-  if (k0 < k1) {
-    load(k0);
-    store(k0, 0);
-  }
-  settle(qf);
-  __syncthreads();
-  int buf = 0;
-  for (int kt = k0; kt < k1; kt += kWideKeys, buf ^= 1) {
-    const bool more = kt + kWideKeys < k1;
-    if (more) load(kt + kWideKeys);
-    if (kt < w_end) {
-      const uint16_t* sk = s_kv[buf];
-      const uint16_t* sv = s_kv[buf] + kWideKeys * kKRow;
-      f32x16_t s[2];
+  // scores of half x of the keys
+  auto scores = [&](int x, int buf) {
+    f32x16_t s;
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
-      __builtin_amdgcn_s_setprio(1);
+    for (int t = 0; t < KS; ++t)
+      s = mfma32(*reinterpret_cast<const frag_t*>((buf ? sh.k1 : sh.k0) + ka[t] + 32 * x * HD), qf[t], s);
+    return s;
+  };
+  // those that the row sees, and the maximum raised to them
+  auto raise = [&](f32x16_t& s, int kx) {
+    if (kx + 32 > w_all) {
 #pragma unroll
-      for (int t = 0; t < KS; ++t)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          s[x] = mfma32(*reinterpret_cast<const frag_t*>(sk + (32 * x + c32) * kKRow + 16 * t + 8 * h2), qf[t], s[x]);
-      __builtin_amdgcn_s_setprio(0);
-      if (kt + kWideKeys > w_all) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (kt + 32 * x + 8 * (i >> 2) + 4 * h2 + (i & 3) >= limit) s[x][i] = neg_inf();
-      }
-      float mt = neg_inf();
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[x][i]);
-      mt = half_max(mt) * sc - kBias;
-      if (__any(mt > mref + kLazy)) {
-        const float mn = fmaxf(mt, mref);
-        const float f = __builtin_amdgcn_exp2f(mref - (mn == neg_inf() ? 0.0f : mn));
-        mref = mn;
-        lsum *= f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
-      }
-      const float ms = mref == neg_inf() ? 0.0f : mref;
-      frag_t pf[4];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], sc, -ms));
-          lsum += p;
-          typedef typename std::conditional<F16, _Float16, __bf16>::type half_t;
-          pf[2 * x + (i >> 3)][i & 7] = static_cast<half_t>(p);
-        }
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          o[dt] = mfma32(*reinterpret_cast<const frag_t*>(sv + (32 * dt + c32) * kVRow + 16 * t + 8 * h2), pf[t], o[dt]);
-      __builtin_amdgcn_s_setprio(0);
+      for (int i = 0; i < 16; ++i)
+        if (kx + 8 * (i >> 2) + 4 * h2 + (i & 3) >= limit) s[i] = neg_inf();
     }
-    if (more) store(kt + kWideKeys, buf ^ 1);
+    float mt = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[i]);
+    mt = half_max(mt) * sc - kBias;
+    if (__any(mt > mref + kLazy)) {
+      const float mn = fmaxf(mt, mref);
+      const float f = __builtin_amdgcn_exp2f(mref - (mn == neg_inf() ? 0.0f : mn));
+      mref = mn;
+      lsum *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= f;
+    }
+  };
+  // the half's weights, and the values' sums with them
+  auto values = [&](const f32x16_t& s, int x, int buf) {
+    const float ms = mref == neg_inf() ? 0.0f : mref;
+    float ls[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      frag_t pf;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + i], sc, -ms));
+        ls[i & 1] += p;
+        typedef typename std::conditional<F16, _Float16, __bf16>::type half_t;
+        pf[i] = static_cast<half_t>(p);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        typedef short s16x8_t __attribute__((ext_vector_type(8)));
+        const uint16_t* v = (buf ? sh.v1 : sh.v0) + va[dt] + (32 * x + 16 * t) * HD;
+        const s16x4_t lo = lds_read_tr(v), hi = lds_read_tr(v + 8 * HD);
+        const s16x8_t f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        o[dt] = mfma32(__builtin_bit_cast(frag_t, f), pf, o[dt]);
+      }
+    }
+    lsum += ls[0] + ls[1];
+  };
+  // The keys at kt, in buffers buf. The second half's scores are formed among
+  // the first's exponentials, so that a wave's matrix and vector instructions
+  // overlap (the scheduler is told to deal them out in turn).
+  auto step = [&](int kt, int buf) {
+    // these keys and values have landed, and every wave is done with the
+    // other buffers
+    wait_vmcnt0();
+    wait_lgkmcnt0();
+    lds_dma_barrier();
+    if (kt + kWideKeys < k1) {
+      load_k(kt + kWideKeys, buf ^ 1);
+      load_v(kt + kWideKeys, buf ^ 1);
+    }
+    if (kt + kWideKeys > all) clean_v(kt, buf);
+    if (kt >= w_end) return;
+    f32x16_t s0 = scores(0, buf);
+    raise(s0, kt);
+    f32x16_t s1 = scores(1, buf);
+    values(s0, 0, buf);
+    // (LDS reads run four matrix instructions ahead)
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // four vector ones
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * DT; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    raise(s1, kt + 32);
+    values(s1, 1, buf);
+  };
+
+  if (ANY && a.hd < HD) {  // chunks behind the heads' end, which no load writes
+    for (uint16_t* buf : {sh.k0, sh.k1, sh.v0, sh.v1})
+      for (int i = tid; i < kWideKeys * kRowChunks; i += kThreads)
+        reinterpret_cast<u32x4_t*>(buf)[i] = u32x4_t{0, 0, 0, 0};
     __syncthreads();
   }
+  if (k0 < k1) {
+    load_k(k0, 0);
+    load_v(k0, 0);
+  }
+  settle(qf);
+  for (int kt = k0; kt < k1;) {
+    step(kt, 0);
+    kt += kWideKeys;
+    if (kt >= k1) break;
+    step(kt, 1);
+    kt += kWideKeys;
+  }
+  __syncthreads();
 
   if (m >= rows) return;
-  if (ANY && s_left) {
+  if (ANY && *sh.left) {
     const int lo = max(k0, k0 + (max(all, k0) - k0) / kWideKeys * kWideKeys);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -847,6 +928,31 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
   if (h2 == 0) (wg.prefix ? pl.p_ml : pl.o_ml)[at] = make_float2(mref, z);
 }
 
+template <bool F16, int HD, bool ANY>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD > 128 ? 1 : 2)))
+void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
+  FMX_WIDE_LDS(HD, s);
+  wide_item<F16, HD, ANY>(a, pl, wg, blockIdx.x, s);
+}
+
+// A prefix in wide tiles and own keys in narrow ones in one grid: the former
+// keep the matrix cores busy, the latter HBM. Groups of 8 workgroups (one per
+// XCD) of both kinds take turns until one kind has run out.
+template <bool F16, int HD, int RT, bool ANY>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD > 128 ? 1 : 2)))
+void attn_both_kernel(CacheAttnArgs a, Plan pl, WideGrid wg, int n_wide, int n_narrow) {
+  FMX_WIDE_LDS(HD, s);
+  const int base = (n_wide + 7) / 8 * 8;
+  const bool wide = static_cast<int>(blockIdx.x) < base;
+  const int item = wide ? blockIdx.x : blockIdx.x - base;
+  if (wide) {
+    if (item < n_wide) wide_item<F16, HD, ANY>(a, pl, wg, item, s);
+  } else {
+    if (item < n_narrow) narrow_item<F16, HD, RT, ANY>(a, pl, 0, item, reinterpret_cast<float*>(s.k0), reinterpret_cast<float*>(s.k1),
+                                    *reinterpret_cast<NarrowLds<RT>*>(s.v0));
+  }
+}
+
 // ------------------------------------------------------------------ join
 
 // (m, l) of piece i of a row: the prefix's splits first, then its own pieces
@@ -878,114 +984,140 @@ struct RowPieces {
   }
 };
 
-constexpr int kWeightKeys = 1024;  // of a weights workgroup
+constexpr int kWeightKeys = 1024;  // of a weights workgroup: four per thread
+constexpr int kWeightAhead = 8;    // rows whose scores are loaded ahead
 
-// Workgroups below n_join: one row per wave. The pieces' (m, l) are read a
-// lane each, so that a row waits for two rounds of loads, whatever its number
-// of pieces (a thread of 32 per row walking them one by one took 27 us for 34
-// pieces of 1024 rows). The others: the weights of kWeightKeys keys of a
-// (sequence, kv head) from the stored scores.
+// M and 1 / sum of a row from its pieces' (m, l), a lane each; one wave. f:
+// this lane's piece's factor, where there are no more than 64.
+__device__ inline void row_stats(const RowPieces& ps, int lane, float* m_out, float* z_out, float* f) {
+  float m = neg_inf(), z = 0.0f;
+  float2 mine = make_float2(neg_inf(), 0.0f);
+  for (int i = lane; i < ps.n; i += kWave) {
+    mine = ps.ml(i);
+    m = fmaxf(m, mine.x);
+  }
+  m = wave_max_f32(m);
+  const float ms = m == neg_inf() ? 0.0f : m;
+  *f = __builtin_amdgcn_exp2f(mine.x - ms);
+  if (ps.n <= kWave) {
+    z = mine.y * *f;
+  } else {
+    for (int i = lane; i < ps.n; i += kWave) {
+      const float2 ml = ps.ml(i);
+      z += ml.y * __builtin_amdgcn_exp2f(ml.x - ms);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o);
+  *m_out = ms;
+  *z_out = z;
+}
+
+// Workgroups below n_join: one row each. The pieces' (m, l) are read a lane
+// each and their values' sums dealt to the four waves, so a row waits for two
+// or three rounds of loads, whatever its number of pieces (34 pieces of 1024
+// rows: 27 us with 32 threads per row that walk them one by one, 18 us with a
+// wave per row). The others: the weights of kWeightKeys keys of a (sequence,
+// kv head) from the stored scores, a thread's loads issued before the rows'
+// statistics are there.
 template <bool F16>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Plan pl, int n_join, int w_tiles) {
-  const int tid = threadIdx.x;
+  __shared__ float s_acc[kWaves][kCacheMaxHd];
+  __shared__ float2 s_row[kNarrowRows];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (static_cast<int>(blockIdx.x) < n_join) {
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + wave;
-    if (row >= static_cast<int64_t>(a.B) * a.L * a.nh) return;
+    const int64_t row = blockIdx.x;
     const int t = static_cast<int>(row / a.nh), h = static_cast<int>(row % a.nh);
     const int b = t / a.L, l = t - b * a.L, g = h / a.rep;
     const RowPieces ps(a, pl, b, g, l * a.rep + h - g * a.rep);
-    float m = neg_inf();
-    float2 mine = make_float2(neg_inf(), 0.0f);
-    for (int i = lane; i < ps.n; i += kWave) {
-      mine = ps.ml(i);
-      m = fmaxf(m, mine.x);
-    }
-    m = wave_max_f32(m);
-    const float ms = m == neg_inf() ? 0.0f : m;
+    float ms, z, f;
+    row_stats(ps, lane, &ms, &z, &f);
     float acc[4] = {0, 0, 0, 0};
-    float z = 0.0f;
     const int vd = a.hd > 128 ? 4 : 2;  // dimensions of a lane
     const int d = lane * vd;
-    const bool in = d < a.hd;
-    for (int i0 = 0; i0 < ps.n; i0 += kWave) {
-      if (ps.n > kWave) mine = i0 + lane < ps.n ? ps.ml(i0 + lane) : make_float2(neg_inf(), 0.0f);
-      const float f = __builtin_amdgcn_exp2f(mine.x - ms);
-      z += mine.y * f;
-      const int c = min(kWave, ps.n - i0);
-#pragma unroll 8
-      for (int i = 0; i < c; ++i) {
-        const float fi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
-        const float* o = ps.o(i0 + i);
-        if (!in) o -= d;  // lanes behind the row read its start and keep nothing
-        if (vd == 2) {
-          const float2 v = *reinterpret_cast<const float2*>(o + d);
-          acc[0] = __builtin_fmaf(v.x, fi, acc[0]);
-          acc[1] = __builtin_fmaf(v.y, fi, acc[1]);
-        } else {
-          const f32x4_t v = *reinterpret_cast<const f32x4_t*>(o + d);
+    const int at = d < a.hd ? d : 0;    // lanes behind the row keep nothing
+    auto add = [&](int i, float fi) {
+      const float* o = ps.o(i) + at;
+      if (vd == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(o);
+        acc[0] = __builtin_fmaf(v.x, fi, acc[0]);
+        acc[1] = __builtin_fmaf(v.y, fi, acc[1]);
+      } else {
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(o);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], fi, acc[e]);
-        }
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], fi, acc[e]);
       }
+    };
+    if (ps.n <= kWave) {
+#pragma unroll 8
+      for (int i = wave; i < ps.n; i += kWaves)
+        add(i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i)));
+    } else {
+#pragma unroll 4
+      for (int i = wave; i < ps.n; i += kWaves) add(i, __builtin_amdgcn_exp2f(ps.ml(i).x - ms));
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o);
-    uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + l * a.out.ts + h * a.out.hs;
+    if (d < a.hd)
+      for (int e = 0; e < vd; ++e) s_acc[wave][d + e] = acc[e];
+    __syncthreads();
     const float inv = z == 0.0f ? 0.0f : 1.0f / z;
-    if (in) {
-      const auto pair = [&](int e) {
-        return Act<F16>::st(acc[e] * inv) | static_cast<uint32_t>(Act<F16>::st(acc[e + 1] * inv)) << 16;
-      };
-      if (vd == 2)
-        *reinterpret_cast<uint32_t*>(out + d) = pair(0);
-      else
-        *reinterpret_cast<u32x2_t*>(out + d) = u32x2_t{pair(0), pair(2)};
+    uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + l * a.out.ts + h * a.out.hs;
+    if (2 * tid < a.hd) {
+      float v[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        v[e] = (s_acc[0][2 * tid + e] + s_acc[1][2 * tid + e] + (s_acc[2][2 * tid + e] + s_acc[3][2 * tid + e])) * inv;
+      reinterpret_cast<uint32_t*>(out)[tid] = Act<F16>::st(v[0]) | static_cast<uint32_t>(Act<F16>::st(v[1])) << 16;
     }
-    if (lane == 0) {
-      const float l2 = z == 0.0f ? neg_inf() : m + __log2f(z);
+    if (tid == 0) {
+      const float l2 = z == 0.0f ? neg_inf() : ms + __log2f(z);
       if (pl.lse) pl.lse[row] = l2 * kLn2;
       if (pl.lse2) pl.lse2[(static_cast<int64_t>(b) * a.nkv + g) * pl.R + l * a.rep + h - g * a.rep] = l2;
     }
     return;
   }
-  __shared__ float2 s_row[2 * 16];
   int item = static_cast<int>(blockIdx.x) - n_join;
-  const int64_t j0 = static_cast<int64_t>(item % w_tiles) * kWeightKeys;
+  const int64_t j = static_cast<int64_t>(item % w_tiles) * kWeightKeys + 4 * tid;
   item /= w_tiles;
   const int g = item % a.nkv, b = item / a.nkv;
   const int64_t slot = seq_slot(a.slots, a.n_slots, b);
   if (slot < 0) return;
   const int off = a.offs[b];
   const int64_t n = own_keys(a, slot, off, a.L - 1);
-  if (j0 < n) {
-    const int lane = tid & 63;
-    for (int r = __builtin_amdgcn_readfirstlane(tid >> 6); r < pl.R; r += kWaves) {
-      const RowPieces ps(a, pl, b, g, r);
-      float m = neg_inf(), z = 0.0f;
-      for (int i = lane; i < ps.n; i += kWave) m = fmaxf(m, ps.ml(i).x);
-      m = wave_max_f32(m);
-      const float ms = m == neg_inf() ? 0.0f : m;
-      for (int i = lane; i < ps.n; i += kWave) {
-        const float2 ml = ps.ml(i);
-        z += ml.y * __builtin_amdgcn_exp2f(ml.x - ms);
-      }
+  const bool some = j - 4 * tid < n;  // of the workgroup's keys are seen
+  // rows of scores are multiples of 32 long: four at a time stay within
+  const float* sc = pl.scores + (static_cast<int64_t>(b) * a.nkv + g) * pl.R * pl.s_ld + j;
+  f32x4_t ahead[kWeightAhead];
 #pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o);
+  for (int r = 0; r < kWeightAhead; ++r)
+    if (j < n && r < pl.R) ahead[r] = *reinterpret_cast<const f32x4_t*>(sc + r * pl.s_ld);
+  if (some) {
+    for (int r = wave; r < pl.R; r += kWaves) {
+      float ms, z, f;
+      row_stats(RowPieces(a, pl, b, g, r), lane, &ms, &z, &f);
       if (lane == 0) s_row[r] = make_float2(ms, z == 0.0f ? 0.0f : 1.0f / z);
     }
     __syncthreads();
   }
-  const int64_t at = (slot * a.nkv + g) * a.S;
-  const float* sc = pl.scores + (static_cast<int64_t>(b) * a.nkv + g) * pl.R * pl.s_ld;
-  for (int64_t j = j0 + tid; j < min(a.S, j0 + kWeightKeys); j += kThreads) {
-    float w = 0.0f;
-    if (j < n)
-      for (int r = 0; r < pl.R; ++r)
-        if (j < own_keys(a, slot, off, r / a.rep))
-          w += __builtin_amdgcn_exp2f(sc[r * pl.s_ld + j] - s_row[r].x) * s_row[r].y;
-    if (j < n || a.w_in != a.w_out) a.w_out[at + j] = (a.w_in ? a.w_in[at + j] : 0.0f) + w;
+  f32x4_t w = {0, 0, 0, 0};
+  if (j < n) {
+    auto add = [&](int r, const f32x4_t& v) {
+      const int64_t lim = own_keys(a, slot, off, r / a.rep);
+      const float2 st = s_row[r];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] += j + e < lim ? __builtin_amdgcn_exp2f(v[e] - st.x) * st.y : 0.0f;
+    };
+#pragma unroll
+    for (int r = 0; r < kWeightAhead; ++r)
+      if (r < pl.R) add(r, ahead[r]);
+    for (int r = kWeightAhead; r < pl.R; ++r) add(r, *reinterpret_cast<const f32x4_t*>(sc + r * pl.s_ld));
   }
+  const int64_t at = (slot * a.nkv + g) * a.S + j;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j + e < a.S && (j + e < n || a.w_in != a.w_out))
+      a.w_out[at + e] = (a.w_in ? a.w_in[at + e] : 0.0f) + w[e];
 }
 
 // ------------------------------------------------------------------ weights, scores formed again
@@ -1167,9 +1299,6 @@ constexpr int64_t kWideFill = 512;
 // see their keys; a part has at least 256 rows
 constexpr int64_t kSumFill = 1024;
 
-// from more rows on (of a kv head) wide tiles take over
-constexpr int64_t kNarrowRows = 32;
-
 struct Layout {
   Plan pl;
   int rt;
@@ -1198,7 +1327,7 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
     const int rows = pl.p_wide ? kWideRows : tr;
     pl.p_tiles = static_cast<int>((rows_p + rows - 1) / rows);
     const int64_t units = (a.P + kPiece - 1) / kPiece;
-    const int64_t fill = pl.p_wide ? kWideFill : kFill;
+    const int64_t fill = !pl.p_wide ? kFill : a.S > 0 && !pl.o_wide ? kWideFill / 2 : kWideFill;
     int64_t splits = std::max<int64_t>(1, fill / (static_cast<int64_t>(pl.p_tiles) * a.nkv));
     splits = std::min(splits, units);
     const int64_t per = (units + splits - 1) / splits;
@@ -1248,39 +1377,58 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
   return y;
 }
 
-template <bool F16, int HD, bool ANY>
-hipError_t launch_parts(const CacheAttnArgs& a, const Plan& pl, int rt, hipStream_t stream) {
-  // wide tiles first: a prefix of many rows, or own keys of many queries
-  for (int part = 0; part < 2; ++part) {
-    if (!(part ? pl.o_wide : pl.p_wide)) continue;
-    WideGrid wg{};
-    wg.prefix = part == 0;
-    wg.splits = part ? pl.o_splits : pl.p_splits;
-    wg.tiles = part ? pl.o_tiles : pl.p_tiles;
-    const int64_t pairs = static_cast<int64_t>(wg.splits) * a.nkv * (part ? a.B : 1);
-    const int64_t padded = pairs <= 8 ? pairs : align_up(pairs, 8);
-    if (padded * wg.tiles > 0x7fffffff) return hipErrorInvalidValue;
-    wg.pairs = static_cast<int>(pairs);
-    wg.padded = static_cast<int>(padded);
-    hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(static_cast<uint32_t>(padded * wg.tiles)),
-                       dim3(kThreads), 0, stream, a, pl, wg);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
+bool wide_grid(const CacheAttnArgs& a, const Plan& pl, bool prefix, WideGrid* wg, int* blocks) {
+  wg->prefix = prefix;
+  wg->splits = prefix ? pl.p_splits : pl.o_splits;
+  wg->tiles = prefix ? pl.p_tiles : pl.o_tiles;
+  const int64_t pairs = static_cast<int64_t>(wg->splits) * a.nkv * (prefix ? 1 : a.B);
+  const int64_t padded = pairs <= 8 ? pairs : align_up(pairs, 8);
+  wg->pairs = static_cast<int>(pairs);
+  wg->padded = static_cast<int>(padded);
+  *blocks = static_cast<int>(padded * wg->tiles);
+  return padded * wg->tiles <= 0x3fffffff;
+}
+
+template <bool F16, int HD, int RT, bool ANY>
+hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stream) {
+  WideGrid pg{}, og{};
+  int np = 0, no = 0;
+  if (pl.p_wide && !wide_grid(a, pl, true, &pg, &np)) return hipErrorInvalidValue;
+  if (pl.o_wide && !wide_grid(a, pl, false, &og, &no)) return hipErrorInvalidValue;
   const int64_t n_prefix = pl.p_wide ? 0 : static_cast<int64_t>(pl.p_splits) * a.nkv * pl.p_tiles;
   const int64_t n = n_prefix + (pl.o_wide ? 0 : static_cast<int64_t>(pl.o_grid) * a.nkv * pl.o_tiles);
-  if (n > 0x7fffffff) return hipErrorInvalidValue;
-  if (n == 0) return hipSuccess;
-  const dim3 grid(static_cast<uint32_t>(n)), wg(kThreads);
-  if constexpr (HD <= 128) {
-    if (rt == 2) {
-      hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, 2, ANY>), grid, wg, 0, stream, a, pl,
-                         static_cast<int>(n_prefix));
-      return hipGetLastError();
-    }
+  if (n > 0x3fffffff) return hipErrorInvalidValue;
+  const dim3 wg(kThreads);
+  // (heads beyond 128: a wide workgroup fills a CU's LDS, and so would narrow
+  // ones in its grid)
+  if (HD <= 128 && pl.p_wide && n > 0) {
+    const int groups = (np + 7) / 8 + static_cast<int>((n + 7) / 8);
+    if constexpr (HD <= 128)
+      hipLaunchKernelGGL((attn_both_kernel<F16, HD, RT, ANY>), dim3(static_cast<uint32_t>(groups) * 8), wg, 0, stream,
+                         a, pl, pg, np, static_cast<int>(n));
+    return hipGetLastError();
   }
-  hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, 1, ANY>), grid, wg, 0, stream, a, pl, static_cast<int>(n_prefix));
-  return hipGetLastError();
+  hipError_t e = hipSuccess;
+  if (np) hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(np), wg, 0, stream, a, pl, pg);
+  if (np) e = hipGetLastError();
+  if (e == hipSuccess && no) {
+    hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(no), wg, 0, stream, a, pl, og);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && n) {
+    hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, RT, ANY>), dim3(static_cast<uint32_t>(n)), wg, 0, stream, a, pl,
+                       static_cast<int>(n_prefix));
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+template <bool F16, int HD, bool ANY>
+hipError_t launch_parts(const CacheAttnArgs& a, const Plan& pl, int rt, hipStream_t stream) {
+  if constexpr (HD <= 128) {
+    if (rt == 2) return launch_tiles<F16, HD, 2, ANY>(a, pl, stream);
+  }
+  return launch_tiles<F16, HD, 1, ANY>(a, pl, stream);
 }
 
 template <bool F16, int HD>
@@ -1327,7 +1475,7 @@ hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
     e = a.hd == 256 && !any ? launch_parts<F16, 256, false>(a, pl, y.rt, stream)
                             : launch_parts<F16, 256, true>(a, pl, y.rt, stream);
   if (e != hipSuccess) return e;
-  const int64_t n_join = pl.direct ? 0 : (static_cast<int64_t>(a.B) * a.L * a.nh + kWaves - 1) / kWaves;
+  const int64_t n_join = pl.direct ? 0 : static_cast<int64_t>(a.B) * a.L * a.nh;
   const int64_t w_tiles = pl.scores ? (a.S + kWeightKeys - 1) / kWeightKeys : 0;
   const int64_t grid = n_join + w_tiles * a.nkv * a.B;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;

@@ -118,7 +118,8 @@ int fmx_rope_append(const fmx_rope_angles* angles, int dtype, int64_t batch, int
 /* n_heads a multiple of n_kv_heads (query head h reads kv head
  * h / (n_heads / n_kv_heads)); head_dim a multiple of 8, at most 256; scale
  * finite and positive. q, out, keys and values are FMX_BF16 or FMX_F16;
- * their data 16-byte aligned, strides multiples of 8. */
+ * their data 16-byte aligned, strides multiples of 8, and the token strides
+ * of keys and values at most 2^24. */
 typedef struct fmx_attention_shape {
   int32_t dtype;
   int64_t batch;
