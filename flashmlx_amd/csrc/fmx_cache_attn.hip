@@ -51,6 +51,14 @@ __device__ inline void settle(T (&f)[N]) {
   }
 }
 
+// 16 or 4 bytes of every lane straight to LDS, lane after lane from `to` on
+__device__ inline void load_to_lds16(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+__device__ inline void load_to_lds4(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds(from, (__attribute__((address_space(3))) void*)to, 4, 0, 0);
+}
+
 // of the four lanes i16 + 16 j: their maximum, their sum, in each
 __device__ inline float quad_max(float v) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -85,10 +93,10 @@ struct Plan {
   int64_t s_ld;
   float* lse;           // [B, L, nh]: the caller's, or null
   // weights of many rows: ln sum exp by log2 e of [B, nkv, R], and sums over
-  // w_rows rows each, [w_parts][B][nkv][S]
+  // every w_parts-th block of kSumRows rows, [w_parts][B][nkv][S]
   float* lse2;
   float* w_part;
-  int w_rows, w_parts;
+  int w_parts;
   bool direct;          // one piece per row: the wide tiles write the output
 };
 
@@ -554,6 +562,7 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 // kLazy above it: the weights reach 2^kLazy times kBias' 2^8 at most, in fp16
 // 2^14 of 65504.
 constexpr int kWideRows = 32 * kWaves;
+constexpr int kCus = 256;
 constexpr int kWideKeys = 64;
 constexpr float kLazy = 6.0f;
 
@@ -601,14 +610,14 @@ struct WideLds {
 // Rows of both arrays lie one after the other, their 16-byte chunks in an
 // order of the row's own, so that the lanes that LDS serves together fall on
 // different banks: a key's chunk c at c ^ swz_k (16 rows' same chunk), a
-// value's 32-byte segment at segment ^ swz_v (8 rows' same segment).
+// value's 32-byte segment at segment ^ swz_v (four rows' two segments).
 template <int HD>
 __device__ inline int swz_k(int row) {
   return HD == 64 ? row >> 1 & 7 : row & 15;
 }
 template <int HD>
 __device__ inline int swz_v(int row) {
-  return HD == 64 ? row >> 1 & 3 : row & 7;
+  return HD == 64 ? row & 2 : (row & 3) * 2;
 }
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -635,7 +644,15 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
   // ---- the item
   const int pair = block % wg.padded;
   if (pair >= wg.pairs) return;
-  const int tile = wg.tiles - 1 - block / wg.padded;  // the rows that see most first
+  // Rows that see the most keys first; of the tiles that one round of the CUs
+  // takes, every other round's in reverse, so that a CU's tiles are long and
+  // short ones.
+  int tile = block / wg.padded;
+  {
+    const int per = max(kCus / wg.padded, 1), round = tile / per;
+    if (round & 1) tile = round * per + min(per, wg.tiles - round * per) - 1 - (tile - round * per);
+  }
+  tile = wg.tiles - 1 - tile;
   const int g = pair % a.nkv;
   const int split = wg.prefix ? pair / a.nkv : pair / a.nkv % wg.splits;
   const int seq = wg.prefix ? 0 : pair / a.nkv / wg.splits;
@@ -713,9 +730,7 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
       uint32_t o = off_b[i];
       // rows behind the piece's last are read as its last
       if (!whole) o = (static_cast<uint32_t>(min(row, k1 - 1 - kt)) * static_cast<uint32_t>(ts) + 8 * ch) * 2;
-      if (!ANY || 8 * ch < a.hd)
-        __builtin_amdgcn_global_load_lds(
-            at + o, (__attribute__((address_space(3))) void*)(to + (wave * 16 + i * kDmaRows) * HD), 16, 0, 0);
+      if (!ANY || 8 * ch < a.hd) load_to_lds16(at + o, to + (wave * 16 + i * kDmaRows) * HD);
     }
   };
   auto load_k = [&](int kt, int buf) { dma(kb, kts, ko, true, kt, buf ? sh.k1 : sh.k0); };
@@ -842,14 +857,14 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
-      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);  // four vector ones
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
+      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // vector ones
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
     }
 #pragma unroll
     for (int i = 0; i < 2 * DT; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
     raise(s1, kt + 32);
     values(s1, 1, buf);
@@ -1123,31 +1138,40 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Pl
 // ------------------------------------------------------------------ weights, scores formed again
 //
 // One workgroup per (128 keys, part of the rows): a wave keeps 32 keys as the
-// B operand of S = Q K^T and goes over the rows, kSumRows at a time staged in
-// LDS for all four waves with their ln sum exp. A lane then has 16 rows'
-// scores of one key: exp2(t - lse) added up in the lane, over rows in order,
-// in sums of kSumRows rows that are added to the total (a thousand rows' sum
-// is off by tens of roundings, not by a thousand). The parts' sums are added
-// by attn_weights_sum_kernel, in order.
+// B operand of S = Q K^T and goes over the rows, kSumRows at a time, which
+// come straight to LDS (three buffers, loads two ahead) with their ln sum exp
+// and how many keys they see. A lane then has 16 rows' scores of one key:
+// exp2(t - lse) added up in the lane, over rows in order, in sums of kSumRows
+// rows that are added to the total (a thousand rows' sum is off by tens of
+// roundings, not by a thousand). A part is every w_parts-th block of rows, so
+// that all parts of a causal triangle are equally long (parts of consecutive
+// rows left some XCDs with 2.4 times the work of others: 64 us for a prompt of
+// 2000 tokens, 32 heads over 4). The parts' sums are added by
+// attn_weights_sum_kernel, in order. Workgroups over one part's rows run on
+// one XCD.
 constexpr int kSumRows = 64;
 constexpr int kSumKeys = 32 * kWaves;
 
 template <bool F16, int HD, bool ANY>
-__global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a, Plan pl, int tiles) {
+__global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a, Plan pl, int pairs, int padded) {
   typedef act8_t<F16> frag_t;
   constexpr int KS = HD / 16;
-  constexpr int kRow = HD + 8;
-  constexpr int NQ = kSumRows * HD / 8 / kThreads;
-  __shared__ __attribute__((aligned(16))) uint16_t s_q[2][kSumRows * kRow];
-  __shared__ __attribute__((aligned(16))) float s_lse[2][kSumRows];
-  __shared__ __attribute__((aligned(16))) int s_lim[2][kSumRows];
+  constexpr int kRowChunks = HD / 8;
+  constexpr int kDmaRows = kWave / kRowChunks;
+  constexpr int NL = kSumRows / kWaves / kDmaRows;
+  __shared__ __attribute__((aligned(16))) uint16_t s_q0[kSumRows * HD], s_q1[kSumRows * HD], s_q2[kSumRows * HD];
+  __shared__ __attribute__((aligned(16))) float s_lse0[kSumRows], s_lse1[kSumRows], s_lse2[kSumRows];
+  __shared__ __attribute__((aligned(16))) int s_lim0[kSumRows], s_lim1[kSumRows], s_lim2[kSumRows];
+  uint16_t* const s_q[3] = {s_q0, s_q1, s_q2};
+  float* const s_lse[3] = {s_lse0, s_lse1, s_lse2};
+  int* const s_lim[3] = {s_lim0, s_lim1, s_lim2};
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, h2 = lane >> 5;
-  int item = blockIdx.x;
-  const int tile = item % tiles;
-  item /= tiles;
+  int item = static_cast<int>(blockIdx.x % padded);
+  if (item >= pairs) return;
+  const int tile = static_cast<int>(blockIdx.x / padded);
   const int part = item % pl.w_parts;
   item /= pl.w_parts;
   const int g = item % a.nkv, b = item / a.nkv;
@@ -1156,12 +1180,13 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a,
   const int off = a.offs[b];
   const int key0 = tile * kSumKeys;
   const int n = static_cast<int>(own_keys(a, slot, off, a.L - 1));
-  // rows [r0, r1) of the part, from the first that sees the tile's first key
+  // the part's blocks of rows from the one with the first row that sees the
+  // tile's first key
   const int64_t l0 = max(static_cast<int64_t>(key0) - off, static_cast<int64_t>(0));
-  int r0 = part * pl.w_rows;
-  const int r1 = min(pl.R, r0 + pl.w_rows);
   if (key0 >= n || l0 >= a.L) return;
-  r0 = max(r0, static_cast<int>(l0) * a.rep);
+  const int first = static_cast<int>(l0) * a.rep / kSumRows;
+  const int r0 = (first + (part - first % pl.w_parts + pl.w_parts) % pl.w_parts) * kSumRows;
+  const int r1 = pl.R, stride = kSumRows * pl.w_parts;
   if (r0 >= r1) return;
 
   const int key = key0 + wave * 32 + c32;
@@ -1175,85 +1200,93 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a,
       kf[t] = __builtin_bit_cast(frag_t, w);
     }
   }
-  u32x4_t qr[NQ] = {};
-  float lr = 0.0f;
-  int mr = 0;
-  const uint16_t* qb = static_cast<const uint16_t*>(a.q.p) + b * a.q.bs;
-  const float* lb = pl.lse2 + (static_cast<int64_t>(b) * a.nkv + g) * pl.R;
-  // (query, head in group) of the thread's rows, kept by steps of kSumRows
-  constexpr int kQStep = kThreads / (HD / 8);  // rows between a thread's loads
-  const int qch = tid % (HD / 8), qrow = tid / (HD / 8);
-  const int dl = kSumRows / a.rep, dr = kSumRows % a.rep;
-  int ql[NQ], qh[NQ];
+  // A lane's rows' addresses, moved on to the next block: dl queries and dr
+  // heads, one query more where that passes the group's last head.
+  const int lr = lane / kRowChunks, lc = lane % kRowChunks;
+  const int dl = stride / a.rep, dr = stride % a.rep;
+  const int64_t move = dl * a.q.ts + dr * a.q.hs, carry = a.q.ts - a.rep * a.q.hs;
+  const uint16_t* qp[NL];
+  int qh[NL];
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    ql[i] = (r0 + qrow + i * kQStep) / a.rep;
-    qh[i] = (r0 + qrow + i * kQStep) % a.rep;
+  for (int i = 0; i < NL; ++i) {
+    const int row = wave * 16 + i * kDmaRows + lr, l = (r0 + row) / a.rep;
+    qh[i] = (r0 + row) % a.rep;
+    qp[i] = static_cast<const uint16_t*>(a.q.p) + b * a.q.bs + l * a.q.ts + (g * a.rep + qh[i]) * a.q.hs +
+            8 * (lc ^ swz_k<HD>(i * kDmaRows + lr));
   }
   int ml = (r0 + tid) / a.rep, mh = (r0 + tid) % a.rep;
-  auto advance = [&](int& l, int& h) {
-    l += dl;
-    h += dr;
-    if (h >= a.rep) {
-      h -= a.rep;
-      ++l;
-    }
-  };
-  // rows behind the part's are not loaded: no key counts for them
-  auto load = [&](int r) {
+  const float* lb = pl.lse2 + (static_cast<int64_t>(b) * a.nkv + g) * pl.R;
+  // (rows behind the last are not loaded: no key counts for them, whatever the
+  // buffer holds)
+  auto load = [&](int r, int buf) {
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      if (ANY) qr[i] = u32x4_t{0, 0, 0, 0};
-      if (r + qrow + i * kQStep < r1 && (!ANY || 8 * qch < a.hd))
-        qr[i] = *reinterpret_cast<const u32x4_t*>(qb + ql[i] * a.q.ts + (g * a.rep + qh[i]) * a.q.hs + 8 * qch);
-      advance(ql[i], qh[i]);
+    for (int i = 0; i < NL; ++i) {
+      if (r + wave * 16 + i * kDmaRows + lr < r1 && (!ANY || 8 * (lc ^ swz_k<HD>(i * kDmaRows + lr)) < a.hd))
+        load_to_lds16(qp[i], s_q[buf] + (wave * 16 + i * kDmaRows) * HD);
+      qh[i] += dr;
+      const bool over = qh[i] >= a.rep;
+      qh[i] -= over ? a.rep : 0;
+      qp[i] += over ? move + carry : move;
     }
+    // (all waves: the same values, and the same number of loads in each)
+    if (r + lane < r1) load_to_lds4(lb + r + lane, s_lse[buf]);
     if (tid < kSumRows) {
-      mr = 0;
-      if (r + tid < r1) {
-        lr = lb[r + tid];
-        mr = static_cast<int>(own_keys(a, slot, off, ml));
+      s_lim[buf][tid] = r + tid < r1 ? static_cast<int>(own_keys(a, slot, off, ml)) : 0;
+      ml += dl;
+      mh += dr;
+      if (mh >= a.rep) {
+        mh -= a.rep;
+        ++ml;
       }
-      advance(ml, mh);
     }
   };
-  auto store = [&](int buf) {
+  int qa[KS];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i)
-      *reinterpret_cast<u32x4_t*>(&s_q[buf][(qrow + i * kQStep) * kRow + qch * 8]) = qr[i];
-    if (tid < kSumRows) {
-      s_lse[buf][tid] = lr;
-      s_lim[buf][tid] = mr;
-    }
-  };
+  for (int t = 0; t < KS; ++t) qa[t] = c32 * HD + ((2 * t + h2) ^ swz_k<HD>(c32)) * 8;
   const float c = a.scale * kLog2e;
   float total = 0.0f;
-  load(r0);
-  store(0);
+  if (ANY && a.hd < HD) {  // chunks behind the heads' end, which no load writes
+    for (uint16_t* q : s_q)
+      for (int i = tid; i < kSumRows * kRowChunks; i += kThreads)
+        reinterpret_cast<u32x4_t*>(q)[i] = u32x4_t{0, 0, 0, 0};
+    __syncthreads();
+  }
   settle(kf);
-  __syncthreads();
-  int buf = 0;
-  for (int r = r0; r < r1; r += kSumRows, buf ^= 1) {
-    const bool more = r + kSumRows < r1;
-    if (more) load(r + kSumRows);
+  load(r0, 0);
+  if (r0 + stride < r1) load(r0 + stride, 1);
+  auto step = [&](int r, int buf) {
+    // these rows have landed (the next ones, NL + 1 loads where they are
+    // whole, may be on their way), and every wave is done with the third
+    // buffer
+    if (r + stride + kSumRows <= r1)
+      wait_vmcnt<NL + 1>();
+    else
+      wait_vmcnt0();
+    wait_lgkmcnt0();
+    lds_dma_barrier();
+    if (r + 2 * stride < r1) load(r + 2 * stride, (buf + 2) % 3);
     // whether a row of these may not see all of the keys: the first sees the
     // fewest (one of the buffer's limits, the same in every thread)
     const bool some = r + kSumRows > r1 || __builtin_amdgcn_readfirstlane(s_lim[buf][0]) < key0 + kSumKeys;
+    f32x16_t s[kSumRows / 32];
+#pragma unroll
+    for (int x = 0; x < kSumRows / 32; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < KS; ++t)
+#pragma unroll
+      for (int x = 0; x < kSumRows / 32; ++x)
+        s[x] = mfma32(*reinterpret_cast<const frag_t*>(s_q[buf] + qa[t] + 32 * x * HD), kf[t], s[x]);
     float sum = 0.0f;
 #pragma unroll
-    for (int x = 0; x < kSumRows / 32; ++x) {
-      f32x16_t s;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < KS; ++t)
-        s = mfma32(*reinterpret_cast<const frag_t*>(&s_q[buf][(32 * x + c32) * kRow + 16 * t + 8 * h2]), kf[t], s);
+    for (int x = 0; x < kSumRows / 32; ++x)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const f32x4_t z = *reinterpret_cast<const f32x4_t*>(&s_lse[buf][32 * x + 8 * q + 4 * h2]);
+        const f32x4_t z = *reinterpret_cast<const f32x4_t*>(s_lse[buf] + 32 * x + 8 * q + 4 * h2);
         f32x4_t p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + i], c, -z[i]));
+        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][4 * q + i], c, -z[i]));
         if (some) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -1261,10 +1294,15 @@ __global__ __launch_bounds__(kThreads) void attn_weights_kernel(CacheAttnArgs a,
         }
         sum += (p[0] + p[1]) + (p[2] + p[3]);
       }
-    }
     total += sum;
-    if (more) store(buf ^ 1);
-    __syncthreads();
+  };
+  for (int r = r0;;) {
+    step(r, 0);
+    if ((r += stride) >= r1) break;
+    step(r, 1);
+    if ((r += stride) >= r1) break;
+    step(r, 2);
+    if ((r += stride) >= r1) break;
   }
   total = half_sum(total);
   if (h2 == 0 && key < n)
@@ -1280,10 +1318,13 @@ __global__ __launch_bounds__(kThreads) void attn_weights_sum_kernel(CacheAttnArg
   float w = 0.0f;
   const bool seen = j < own_keys(a, slot, off, a.L - 1);
   if (seen) {
-    // the parts that hold rows seeing the tile's first key have left a sum
+    // the parts with a block from the first row on that sees the tile's first
+    // key have left a sum
     const int64_t l0 = max(j / kSumKeys * kSumKeys - off, static_cast<int64_t>(0));
-    for (int p = static_cast<int>(l0 * a.rep / pl.w_rows); p < pl.w_parts; ++p)
-      w += pl.w_part[((static_cast<int64_t>(p) * a.B + b) * a.nkv + g) * a.S + j];
+    const int first = static_cast<int>(l0) * a.rep / kSumRows, last = (pl.R - 1) / kSumRows;
+    for (int p = 0; p < pl.w_parts; ++p)
+      if (last - (last - p) % pl.w_parts >= first)
+        w += pl.w_part[((static_cast<int64_t>(p) * a.B + b) * a.nkv + g) * a.S + j];
   }
   const int64_t at = (slot * a.nkv + g) * a.S + j;
   if (seen || a.w_in != a.w_out) a.w_out[at] = (a.w_in ? a.w_in[at] : 0.0f) + w;
@@ -1295,9 +1336,8 @@ __global__ __launch_bounds__(kThreads) void attn_weights_sum_kernel(CacheAttnArg
 constexpr int64_t kFill = 768;
 // and of wide tiles: two
 constexpr int64_t kWideFill = 512;
-// workgroups for a prompt's weights, of which about half have no rows that
-// see their keys; a part has at least 256 rows
-constexpr int64_t kSumFill = 1024;
+// workgroups for a prompt's weights; a part has at least 256 rows or so
+constexpr int64_t kSumFill = 768;
 
 struct Layout {
   Plan pl;
@@ -1365,9 +1405,7 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
     } else {
       pl.lse2 = reinterpret_cast<float*>(take(rows_p * a.nkv * 4));
       const int64_t tiles = (a.S + kSumKeys - 1) / kSumKeys * a.nkv * a.B;
-      const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(kSumFill / tiles, (pl.R + 255) / 256));
-      pl.w_rows = static_cast<int>(align_up((pl.R + parts - 1) / parts, kSumRows));
-      pl.w_parts = (pl.R + pl.w_rows - 1) / pl.w_rows;
+      pl.w_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kSumFill / tiles, (pl.R + 255) / 256)));
       pl.w_part = reinterpret_cast<float*>(take(pl.w_parts * static_cast<int64_t>(a.B) * a.nkv * a.S * 4));
     }
   } else {
@@ -1432,26 +1470,32 @@ hipError_t launch_parts(const CacheAttnArgs& a, const Plan& pl, int rt, hipStrea
 }
 
 template <bool F16, int HD>
-void launch_weight_parts(const CacheAttnArgs& a, const Plan& pl, uint32_t grid, int tiles, hipStream_t stream) {
+void launch_weight_parts(const CacheAttnArgs& a, const Plan& pl, uint32_t grid, int pairs, int padded,
+                         hipStream_t stream) {
   if (a.hd == HD)
-    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, false>), dim3(grid), dim3(kThreads), 0, stream, a, pl, tiles);
+    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, false>), dim3(grid), dim3(kThreads), 0, stream, a, pl, pairs,
+                       padded);
   else
-    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, true>), dim3(grid), dim3(kThreads), 0, stream, a, pl, tiles);
+    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, true>), dim3(grid), dim3(kThreads), 0, stream, a, pl, pairs,
+                       padded);
 }
 
 template <bool F16>
 hipError_t launch_weights(const CacheAttnArgs& a, const Plan& pl, hipStream_t stream) {
   const int64_t tiles = (a.S + kSumKeys - 1) / kSumKeys;
-  const int64_t grid = tiles * pl.w_parts * a.nkv * a.B;
+  const int64_t pairs = static_cast<int64_t>(pl.w_parts) * a.nkv * a.B;
+  const int64_t padded = pairs <= 8 ? pairs : align_up(pairs, 8);
+  const int64_t grid = tiles * padded;
   const int64_t sum_tiles = (a.S + kThreads - 1) / kThreads;
   if (grid > 0x7fffffff || sum_tiles * a.nkv * a.B > 0x7fffffff) return hipErrorInvalidValue;
   const uint32_t n = static_cast<uint32_t>(grid);
+  const int np = static_cast<int>(pairs), npad = static_cast<int>(padded);
   if (a.hd <= 64)
-    launch_weight_parts<F16, 64>(a, pl, n, static_cast<int>(tiles), stream);
+    launch_weight_parts<F16, 64>(a, pl, n, np, npad, stream);
   else if (a.hd <= 128)
-    launch_weight_parts<F16, 128>(a, pl, n, static_cast<int>(tiles), stream);
+    launch_weight_parts<F16, 128>(a, pl, n, np, npad, stream);
   else
-    launch_weight_parts<F16, 256>(a, pl, n, static_cast<int>(tiles), stream);
+    launch_weight_parts<F16, 256>(a, pl, n, np, npad, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(attn_weights_sum_kernel, dim3(static_cast<uint32_t>(sum_tiles * a.nkv * a.B)), dim3(kThreads), 0,

@@ -20,6 +20,11 @@ namespace {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kSelBins = 2048;
+// copies of a histogram, lanes in turn: weights crowd in few digits, and a
+// wave's additions to one address come one after the other. From kSelMany
+// positions on; fewer take less time than clearing and adding up the copies.
+constexpr int kSelCopies = 8;
+constexpr int kSelMany = 4096;
 // positions whose images a thread keeps in registers (position tid + 1024 i)
 constexpr int kSelKeep = 16;
 
@@ -48,29 +53,45 @@ __device__ inline uint32_t block_scan(uint32_t v, uint32_t* s_tmp) {
 }
 
 struct SelShared {
-  uint32_t bin[kSelBins];
+  __attribute__((aligned(16))) uint32_t bin[kSelBins * kSelCopies];
   uint32_t tmp[kSelWaves];
   uint32_t digit, above;
-  uint32_t sure[kSelWaves], equal[kSelWaves];
+  uint32_t cnt[kSelKeep * kSelWaves];
 };
 
 // One round: bins of the digit at `shift` of the images that agree with
 // `found` above it, then the digit of the need-th largest, from the top.
-template <typename F>
+template <int COPIES, typename F>
 __device__ inline void select_round(SelShared& s, int shift, int bits, uint32_t& found, uint32_t& need,
                                     F&& each) {
   const int tid = threadIdx.x;
-  for (int i = tid; i < kSelBins; i += kSelThreads) s.bin[i] = 0;
+  u32x4_t* quads = reinterpret_cast<u32x4_t*>(s.bin);
+#pragma unroll
+  for (int i = 0; i < kSelBins * COPIES / 4; i += kSelThreads)
+    if (i + tid < kSelBins * COPIES / 4) quads[i + tid] = u32x4_t{0, 0, 0, 0};
   __syncthreads();
   each([&](uint32_t u) {
     if (shift + bits == 32 || u >> (shift + bits) == found >> (shift + bits))
-      atomicAdd(&s.bin[u >> shift & ((1u << bits) - 1)], 1u);
+      atomicAdd(&s.bin[(u >> shift & ((1u << bits) - 1)) * COPIES + tid % COPIES], 1u);
   });
   __syncthreads();
   // from the largest digit down: thread t has digits top - 2 t, top - 2 t - 1
   const int top = (1 << bits) - 1;
-  const uint32_t c0 = 2 * tid <= top ? s.bin[top - 2 * tid] : 0;
-  const uint32_t c1 = 2 * tid + 1 <= top ? s.bin[top - 2 * tid - 1] : 0;
+  auto count = [&](int digit) {
+    if (digit < 0) return 0u;
+    uint32_t c = 0;
+    if constexpr (COPIES == 1) {
+      c = s.bin[digit];
+    } else {
+#pragma unroll
+      for (int i = 0; i < COPIES / 4; ++i) {
+        const u32x4_t x = quads[digit * (COPIES / 4) + i];
+        c += x[0] + x[1] + x[2] + x[3];
+      }
+    }
+    return c;
+  };
+  const uint32_t c0 = count(top - 2 * tid), c1 = count(top - 2 * tid - 1);
   const uint32_t end = block_scan(c0 + c1, s.tmp);
   const uint32_t start = end - c0 - c1;
   if (start < need && need <= end) {
@@ -126,62 +147,89 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
 #pragma unroll
         for (int i = 0; i < kSelKeep; ++i) {
           const int p = tid + i * kSelThreads;
-          if (p >= lo && p < hi) f(weight_key(v[i]));
+          if (i * kSelThreads < n && p >= lo && p < hi) f(weight_key(v[i]));
         }
       } else {
         for (int p = lo + tid; p < hi; p += kSelThreads) f(weight_key(w[p]));
       }
     };
-    select_round(s, 21, 11, found, need, all);
-    select_round(s, 10, 11, found, need, all);
-    select_round(s, 0, 10, found, need, all);
+    // (the later digits of few weights agree with the first: no crowds)
+    if (hi - lo >= kSelMany)
+      select_round<kSelCopies>(s, 21, 11, found, need, all);
+    else
+      select_round<1>(s, 21, 11, found, need, all);
+    select_round<1>(s, 10, 11, found, need, all);
+    select_round<1>(s, 0, 10, found, need, all);
   } else {
     found = 0xffffffffu;  // nothing above it, none of its equals wanted
   }
-  // In order, 1024 positions at a time: images above `found` and the first
-  // `need` equal to it go behind those before them.
-  uint32_t at = 0, eq = 0;  // kept and equal ones of earlier positions
-  for (int p0 = 0; p0 < n; p0 += kSelThreads) {
-    const int p = p0 + tid;
-    float x = 0.0f;
-    if (in_regs) {
-#pragma unroll
-      for (int i = 0; i < kSelKeep; ++i)
-        if (p0 == i * kSelThreads) x = v[i];
-    } else if (p < n) {
-      x = w[p];
-    }
+  // In order: images above `found` and the first `need` equal to it go behind
+  // those before them. In place a weight moves to a position <= its own, all
+  // weights up to which have been read by then.
+  const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+  auto kinds = [&](int p, float x, bool* sure, bool* same) {
     const bool mid = p >= lo && p < hi;
     const uint32_t u = weight_key(x);
-    const bool sure = p < n && (!mid || u > found), same = mid && u == found;
-    const uint64_t ms = __ballot(sure), me = __ballot(same);
-    if (lane == 0) {
-      s.sure[wave] = static_cast<uint32_t>(__popcll(ms));
-      s.equal[wave] = static_cast<uint32_t>(__popcll(me));
-    }
-    __syncthreads();
-    uint32_t bs = 0, be = 0, ts = 0, te = 0;
-#pragma unroll
-    for (int q = 0; q < kSelWaves; ++q) {
-      const uint32_t cs = s.sure[q], ce = s.equal[q];
-      bs += q < wave ? cs : 0;
-      be += q < wave ? ce : 0;
-      ts += cs;
-      te += ce;
-    }
-    const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
-    const uint32_t es = bs + static_cast<uint32_t>(__popcll(ms & below));
-    const uint32_t ee = eq + be + static_cast<uint32_t>(__popcll(me & below));
-    const uint32_t pos = at + es + min(ee, need) - min(eq, need);
-    const bool keep = sure || (same && ee < need);
-    // (in place: position pos <= p, whose weight has been read by now)
-    if (keep) {
+    *sure = p < n && (!mid || u > found);
+    *same = mid && u == found;
+  };
+  auto put = [&](int p, float x, bool sure, bool same, uint32_t at, uint32_t eq) {
+    // at, eq: sure and equal ones before p
+    if (sure || (same && eq < need)) {
+      const uint32_t pos = at + min(eq, need);
       kept[pos] = p;
       wo[pos] = x;
     }
-    at += ts + min(eq + te, need) - min(eq, need);
-    eq += te;
+  };
+  if (in_regs) {
+    // counts of (1024 positions, wave), sure ones | equal ones << 16, scanned
+    // in the positions' order
+#pragma unroll
+    for (int i = 0; i < kSelKeep; ++i) {
+      bool sure = false, same = false;
+      if (i * kSelThreads < n) kinds(tid + i * kSelThreads, v[i], &sure, &same);
+      const uint32_t c = static_cast<uint32_t>(__popcll(__ballot(sure)) | __popcll(__ballot(same)) << 16);
+      if (lane == 0) s.cnt[i * kSelWaves + wave] = c;
+    }
     __syncthreads();
+    static_assert(kSelKeep * kSelWaves <= kSelThreads, "one thread per count");
+    const uint32_t c = tid < kSelKeep * kSelWaves ? s.cnt[tid] : 0;
+    const uint32_t before = block_scan(c, s.tmp) - c;
+    if (tid < kSelKeep * kSelWaves) s.cnt[tid] = before;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSelKeep; ++i) {
+      const int p = tid + i * kSelThreads;
+      if (i * kSelThreads >= n) continue;
+      bool sure, same;
+      kinds(p, v[i], &sure, &same);
+      const uint64_t ms = __ballot(sure), me = __ballot(same);
+      const uint32_t base = s.cnt[i * kSelWaves + wave];
+      put(p, v[i], sure, same, (base & 0xffffu) + static_cast<uint32_t>(__popcll(ms & below)),
+          (base >> 16) + static_cast<uint32_t>(__popcll(me & below)));
+    }
+  } else {
+    uint32_t at = 0, eq = 0;  // of earlier positions
+    for (int p0 = 0; p0 < n; p0 += kSelThreads) {
+      const int p = p0 + tid;
+      const float x = p < n ? w[p] : 0.0f;
+      bool sure, same;
+      kinds(p, x, &sure, &same);
+      const uint64_t ms = __ballot(sure), me = __ballot(same);
+      if (lane == 0) s.cnt[wave] = static_cast<uint32_t>(__popcll(ms) | __popcll(me) << 16);
+      __syncthreads();
+      uint32_t base = 0, all = 0;
+#pragma unroll
+      for (int q = 0; q < kSelWaves; ++q) {
+        base += q < wave ? s.cnt[q] : 0;
+        all += s.cnt[q];
+      }
+      put(p, x, sure, same, at + (base & 0xffffu) + static_cast<uint32_t>(__popcll(ms & below)),
+          eq + (base >> 16) + static_cast<uint32_t>(__popcll(me & below)));
+      at += all & 0xffffu;
+      eq += all >> 16;
+      __syncthreads();
+    }
   }
   for (int64_t i = cnt + tid; i < a.S_out; i += kSelThreads) wo[i] = 0.0f;
 }
