@@ -12,6 +12,7 @@
 #include <algorithm>
 
 #include "fmx_cache_kernels.hpp"
+#include "fmx_dev.hpp"
 
 namespace fmx {
 
@@ -20,11 +21,9 @@ namespace {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kSelBins = 2048;
-// copies of a histogram, lanes in turn: weights crowd in few digits, and a
-// wave's additions to one address come one after the other. From kSelMany
-// positions on; fewer take less time than clearing and adding up the copies.
+// copies of a long row's first histogram, lanes in turn: weights crowd in few
+// digits, and a wave's additions to one address come one after the other
 constexpr int kSelCopies = 8;
-constexpr int kSelMany = 4096;
 // positions whose images a thread keeps in registers (position tid + 1024 i)
 constexpr int kSelKeep = 16;
 
@@ -39,11 +38,7 @@ __device__ inline uint32_t weight_key(float f) {
 // inclusive scan over the workgroup's threads
 __device__ inline uint32_t block_scan(uint32_t v, uint32_t* s_tmp) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const uint32_t o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+  v = tree_to_last<64>(v, 0u, [](uint32_t a, uint32_t b) { return a + b; });  // (an inclusive scan)
   __syncthreads();
   if (lane == kWave - 1) s_tmp[wave] = v;
   __syncthreads();
@@ -105,59 +100,34 @@ __device__ inline void select_round(SelShared& s, int shift, int bits, uint32_t&
   __syncthreads();
 }
 
-// Bound by its chain of rounds: the weights are read once (up to 16384
-// positions: kept in registers as images), a round is an LDS histogram and a
-// scan. 64 rows of 2000 to 16384 positions cut to 4000: 38 us with every round
-// reading the weights again, .. us so.
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-  __shared__ SelShared s;
+// A row of n > budget weights: the kept positions in order, and their weights.
+// KEEP: so many positions per thread are kept in registers (n <= 1024 KEEP),
+// 0: every round reads the weights again.
+template <int KEEP, int COPIES>
+__device__ void cut_row(const EvictArgs& a, SelShared& s, const float* w, float* wo, int32_t* kept, int n) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = blockIdx.x / a.nkv, g = blockIdx.x % a.nkv;
-  int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
-  const int64_t slot = seq_slot(a.slots, a.n_slots, b);
-  const int64_t len = slot < 0 ? 0 : a.lens[b];
-  const int n = static_cast<int>(len < 0 ? 0 : (len > a.S ? a.S : len));
-  const int budget = static_cast<int>(a.budget);
-  const int cnt = min(n, budget);
-  for (int i = cnt + tid; i < budget; i += kSelThreads) kept[i] = -1;
-  if (slot < 0) return;
-  const float* w = a.w + (slot * a.nkv + g) * a.S;
-  float* wo = a.w_out + (slot * a.nkv + g) * a.S_out;
-  if (n <= budget) {
-    for (int i = tid; i < n; i += kSelThreads) kept[i] = i;
-    for (int64_t i = wo != w ? tid : n + tid; i < a.S_out; i += kSelThreads) wo[i] = i < n ? w[i] : 0.0f;
-    return;
-  }
   // middle positions [lo, hi), `need` of them kept
   const int lo = static_cast<int>(a.sinks), hi = n - static_cast<int>(a.recent);
-  uint32_t need = static_cast<uint32_t>(budget - a.sinks - a.recent);
+  uint32_t need = static_cast<uint32_t>(a.budget - a.sinks - a.recent);
   uint32_t found = 0;  // the need-th largest image, from its top digit down
-  const bool in_regs = n <= kSelThreads * kSelKeep;
-  float v[kSelKeep];
-  if (in_regs) {
+  float v[KEEP ? KEEP : 1];
 #pragma unroll
-    for (int i = 0; i < kSelKeep; ++i) {
-      const int p = tid + i * kSelThreads;
-      v[i] = p < n ? w[p] : 0.0f;
-    }
+  for (int i = 0; i < KEEP; ++i) {
+    const int p = tid + i * kSelThreads;
+    v[i] = p < n ? w[p] : 0.0f;
   }
   if (need > 0) {
     auto all = [&](auto&& f) {
-      if (in_regs) {
 #pragma unroll
-        for (int i = 0; i < kSelKeep; ++i) {
-          const int p = tid + i * kSelThreads;
-          if (i * kSelThreads < n && p >= lo && p < hi) f(weight_key(v[i]));
-        }
-      } else {
-        for (int p = lo + tid; p < hi; p += kSelThreads) f(weight_key(w[p]));
+      for (int i = 0; i < KEEP; ++i) {
+        const int p = tid + i * kSelThreads;
+        if (p >= lo && p < hi) f(weight_key(v[i]));
       }
+      if (KEEP == 0)
+        for (int p = lo + tid; p < hi; p += kSelThreads) f(weight_key(w[p]));
     };
-    // (the later digits of few weights agree with the first: no crowds)
-    if (hi - lo >= kSelMany)
-      select_round<kSelCopies>(s, 21, 11, found, need, all);
-    else
-      select_round<1>(s, 21, 11, found, need, all);
+    select_round<COPIES>(s, 21, 11, found, need, all);
+    // (few weights agree in the first digit: no crowds)
     select_round<1>(s, 10, 11, found, need, all);
     select_round<1>(s, 0, 10, found, need, all);
   } else {
@@ -166,7 +136,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   // In order: images above `found` and the first `need` equal to it go behind
   // those before them. In place a weight moves to a position <= its own, all
   // weights up to which have been read by then.
-  const uint64_t below = lane == 0 ? 0ull : ~0ull >> (64 - lane);
+  const uint64_t below = lanes_below(lane);
   auto kinds = [&](int p, float x, bool* sure, bool* same) {
     const bool mid = p >= lo && p < hi;
     const uint32_t u = weight_key(x);
@@ -181,26 +151,25 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       wo[pos] = x;
     }
   };
-  if (in_regs) {
+  if constexpr (KEEP > 0) {
     // counts of (1024 positions, wave), sure ones | equal ones << 16, scanned
     // in the positions' order
+    static_assert(KEEP * kSelWaves <= kSelThreads && KEEP <= kSelKeep, "one thread per count, sums in 16 bits");
 #pragma unroll
-    for (int i = 0; i < kSelKeep; ++i) {
-      bool sure = false, same = false;
-      if (i * kSelThreads < n) kinds(tid + i * kSelThreads, v[i], &sure, &same);
+    for (int i = 0; i < KEEP; ++i) {
+      bool sure, same;
+      kinds(tid + i * kSelThreads, v[i], &sure, &same);
       const uint32_t c = static_cast<uint32_t>(__popcll(__ballot(sure)) | __popcll(__ballot(same)) << 16);
       if (lane == 0) s.cnt[i * kSelWaves + wave] = c;
     }
     __syncthreads();
-    static_assert(kSelKeep * kSelWaves <= kSelThreads, "one thread per count");
-    const uint32_t c = tid < kSelKeep * kSelWaves ? s.cnt[tid] : 0;
+    const uint32_t c = tid < KEEP * kSelWaves ? s.cnt[tid] : 0;
     const uint32_t before = block_scan(c, s.tmp) - c;
-    if (tid < kSelKeep * kSelWaves) s.cnt[tid] = before;
+    if (tid < KEEP * kSelWaves) s.cnt[tid] = before;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kSelKeep; ++i) {
+    for (int i = 0; i < KEEP; ++i) {
       const int p = tid + i * kSelThreads;
-      if (i * kSelThreads >= n) continue;
       bool sure, same;
       kinds(p, v[i], &sure, &same);
       const uint64_t ms = __ballot(sure), me = __ballot(same);
@@ -218,19 +187,48 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       const uint64_t ms = __ballot(sure), me = __ballot(same);
       if (lane == 0) s.cnt[wave] = static_cast<uint32_t>(__popcll(ms) | __popcll(me) << 16);
       __syncthreads();
-      uint32_t base = 0, all = 0;
+      uint32_t base = 0, sum = 0;
 #pragma unroll
       for (int q = 0; q < kSelWaves; ++q) {
         base += q < wave ? s.cnt[q] : 0;
-        all += s.cnt[q];
+        sum += s.cnt[q];
       }
       put(p, x, sure, same, at + (base & 0xffffu) + static_cast<uint32_t>(__popcll(ms & below)),
           eq + (base >> 16) + static_cast<uint32_t>(__popcll(me & below)));
-      at += all & 0xffffu;
-      eq += all >> 16;
+      at += sum & 0xffffu;
+      eq += sum >> 16;
       __syncthreads();
     }
   }
+}
+
+// Bound by its chain of rounds: the weights are read once (up to 16384
+// positions: kept in registers), a round is an LDS histogram and a scan.
+__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
+  __shared__ SelShared s;
+  const int tid = threadIdx.x;
+  const int b = blockIdx.x / a.nkv, g = blockIdx.x % a.nkv;
+  int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
+  const int64_t slot = seq_slot(a.slots, a.n_slots, b);
+  const int64_t len = slot < 0 ? 0 : a.lens[b];
+  const int n = static_cast<int>(len < 0 ? 0 : (len > a.S ? a.S : len));
+  const int budget = static_cast<int>(a.budget);
+  const int cnt = min(n, budget);
+  for (int i = cnt + tid; i < budget; i += kSelThreads) kept[i] = -1;
+  if (slot < 0) return;
+  const float* w = a.w + (slot * a.nkv + g) * a.S;
+  float* wo = a.w_out + (slot * a.nkv + g) * a.S_out;
+  if (n <= budget) {
+    for (int i = tid; i < n; i += kSelThreads) kept[i] = i;
+    for (int64_t i = wo != w ? tid : n + tid; i < a.S_out; i += kSelThreads) wo[i] = i < n ? w[i] : 0.0f;
+    return;
+  }
+  if (n <= 2 * kSelThreads)
+    cut_row<2, 1>(a, s, w, wo, kept, n);
+  else if (n <= kSelKeep * kSelThreads)
+    cut_row<kSelKeep, kSelCopies>(a, s, w, wo, kept, n);
+  else
+    cut_row<0, kSelCopies>(a, s, w, wo, kept, n);
   for (int64_t i = cnt + tid; i < a.S_out; i += kSelThreads) wo[i] = 0.0f;
 }
 
