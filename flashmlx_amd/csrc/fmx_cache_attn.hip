@@ -543,7 +543,7 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 // ------------------------------------------------------------------ wide tiles
 //
 // One workgroup per (128 rows, piece of keys): 32 rows per wave, the keys and
-// values of kWideKeys positions staged in LDS for all four.
+// values of KT positions staged in LDS for all four.
 //
 // S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16. Register 8u + 4v + r
 // of a lane (row c of the 32, half h) is the score of key 16u + 8v + 4h + r:
@@ -563,7 +563,6 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 // 2^14 of 65504.
 constexpr int kWideRows = 32 * kWaves;
 constexpr int kCus = 256;
-constexpr int kWideKeys = 64;
 constexpr float kLazy = 6.0f;
 
 __device__ inline f32x16_t mfma32(const bf16x8_t& a, const bf16x8_t& b, const f32x16_t& c) {
@@ -596,15 +595,15 @@ struct WideGrid {
 // every read otherwise).
 template <int HD>
 struct WideLds {
-  uint16_t *k0, *k1, *v0, *v1;  // kWideKeys * HD each
+  uint16_t *k0, *k1, *v0, *v1;  // KT * HD each
   int* left;
 };
-#define FMX_WIDE_LDS(HD, name)                                                       \
-  __shared__ __attribute__((aligned(16))) uint16_t name##_k0[kWideKeys * HD];        \
-  __shared__ __attribute__((aligned(16))) uint16_t name##_k1[kWideKeys * HD];        \
-  __shared__ __attribute__((aligned(16))) uint16_t name##_v0[kWideKeys * HD];        \
-  __shared__ __attribute__((aligned(16))) uint16_t name##_v1[kWideKeys * HD];        \
-  __shared__ int name##_left;                                                        \
+#define FMX_WIDE_LDS(HD, KT, name)                                             \
+  __shared__ __attribute__((aligned(16))) uint16_t name##_k0[KT * HD];         \
+  __shared__ __attribute__((aligned(16))) uint16_t name##_k1[KT * HD];         \
+  __shared__ __attribute__((aligned(16))) uint16_t name##_v0[KT * HD];         \
+  __shared__ __attribute__((aligned(16))) uint16_t name##_v1[KT * HD];         \
+  __shared__ int name##_left;                                                  \
   const WideLds<HD> name{name##_k0, name##_k1, name##_v0, name##_v1, &name##_left}
 
 // Rows of both arrays lie one after the other, their 16-byte chunks in an
@@ -627,7 +626,7 @@ __device__ inline s16x4_t lds_read_tr(const uint16_t* p) {
       (__attribute__((address_space(3))) s16x4_t*)const_cast<uint16_t*>(p));
 }
 
-template <bool F16, int HD, bool ANY>
+template <bool F16, int HD, int KT, bool ANY>
 __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a, const Plan& pl, const WideGrid& wg,
                                                          int block, const WideLds<HD>& sh) {
   typedef act8_t<F16> frag_t;
@@ -635,7 +634,8 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
   constexpr int DT = HD / 32;              // dimension tiles
   constexpr int kRowChunks = HD / 8;
   constexpr int kDmaRows = kWave / kRowChunks;             // rows of a wave's load
-  constexpr int NL = kWideKeys / kWaves / kDmaRows;        // loads of a wave per array
+  constexpr int kWaveRows = KT / kWaves;
+  constexpr int NL = kWaveRows / kDmaRows;                 // loads of a wave per array
   constexpr float kBias = F16 ? 8.0f : 0.0f;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -675,7 +675,7 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
     slot = seq_slot(a.slots, a.n_slots, seq);
     off = a.offs[seq];
     const int n = static_cast<int>(own_keys(a, slot, off, (min(row0 + kWideRows, rows) - 1) / a.rep));
-    const int per = (n + wg.splits * kWideKeys - 1) / (wg.splits * kWideKeys) * kWideKeys;
+    const int per = (n + wg.splits * KT - 1) / (wg.splits * KT) * KT;
     k0 = min(split * per, n);
     k1 = min(k0 + per, n);
     all = min(k1, static_cast<int>(own_keys(a, slot, off, row0 / a.rep)));
@@ -710,27 +710,27 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
     }
   }
 
-  // ---- staging: straight to LDS, wave w rows 16 w .. of both arrays
+  // ---- staging: straight to LDS, a quarter of both arrays' rows per wave
   const int lr = lane / kRowChunks, lc = lane % kRowChunks;
-  auto k_chunk = [&](int i) { return lc ^ swz_k<HD>(i * kDmaRows + lr); };
-  auto v_chunk = [&](int i) { return lc ^ swz_v<HD>(i * kDmaRows + lr) << 1; };
+  auto k_chunk = [&](int i) { return lc ^ swz_k<HD>(wave * kWaveRows + i * kDmaRows + lr); };
+  auto v_chunk = [&](int i) { return lc ^ swz_v<HD>(wave * kWaveRows + i * kDmaRows + lr) << 1; };
   uint32_t ko[NL], vo[NL];  // byte offsets from the first position's row
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const uint32_t row = wave * 16 + i * kDmaRows + lr;
+    const uint32_t row = wave * kWaveRows + i * kDmaRows + lr;
     ko[i] = (row * static_cast<uint32_t>(kts) + 8 * k_chunk(i)) * 2;
     vo[i] = (row * static_cast<uint32_t>(vts) + 8 * v_chunk(i)) * 2;
   }
   auto dma = [&](const uint16_t* base, int64_t ts, const uint32_t (&off_b)[NL], bool keys, int kt, uint16_t* to) {
     const uint8_t* at = reinterpret_cast<const uint8_t*>(base + kt * ts);
-    const bool whole = kt + kWideKeys <= k1;
+    const bool whole = kt + KT <= k1;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int row = wave * 16 + i * kDmaRows + lr, ch = keys ? k_chunk(i) : v_chunk(i);
+      const int row = wave * kWaveRows + i * kDmaRows + lr, ch = keys ? k_chunk(i) : v_chunk(i);
       uint32_t o = off_b[i];
       // rows behind the piece's last are read as its last
       if (!whole) o = (static_cast<uint32_t>(min(row, k1 - 1 - kt)) * static_cast<uint32_t>(ts) + 8 * ch) * 2;
-      if (!ANY || 8 * ch < a.hd) load_to_lds16(at + o, to + (wave * 16 + i * kDmaRows) * HD);
+      if (!ANY || 8 * ch < a.hd) load_to_lds16(at + o, to + (wave * kWaveRows + i * kDmaRows) * HD);
     }
   };
   auto load_k = [&](int kt, int buf) { dma(kb, kts, ko, true, kt, buf ? sh.k1 : sh.k0); };
@@ -738,7 +738,7 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
   // Values behind the piece count nothing, whatever they hold; infinite and
   // NaN ones that not all rows see are left out and added at the end.
   auto clean_v = [&](int kt, int buf) {
-    for (int x = tid; x < kWideKeys * kRowChunks; x += kThreads) {
+    for (int x = tid; x < KT * kRowChunks; x += kThreads) {
       u32x4_t* at = reinterpret_cast<u32x4_t*>(buf ? sh.v1 : sh.v0) + x;
       u32x4_t w = *at;
       u16x2_t top = {0, 0};
@@ -842,37 +842,41 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
     wait_vmcnt0();
     wait_lgkmcnt0();
     lds_dma_barrier();
-    if (kt + kWideKeys < k1) {
-      load_k(kt + kWideKeys, buf ^ 1);
-      load_v(kt + kWideKeys, buf ^ 1);
+    if (kt + KT < k1) {
+      load_k(kt + KT, buf ^ 1);
+      load_v(kt + KT, buf ^ 1);
     }
-    if (kt + kWideKeys > all) clean_v(kt, buf);
+    if (kt + KT > all) clean_v(kt, buf);
     if (kt >= w_end) return;
     f32x16_t s0 = scores(0, buf);
     raise(s0, kt);
-    f32x16_t s1 = scores(1, buf);
-    values(s0, 0, buf);
-    // (LDS reads run four matrix instructions ahead)
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+    if constexpr (KT == 32) {
+      values(s0, 0, buf);
+    } else {
+      f32x16_t s1 = scores(1, buf);
+      values(s0, 0, buf);
+      // (LDS reads run four matrix instructions ahead)
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
-      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // vector ones
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
-    }
+      for (int i = 0; i < KS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // vector ones
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+      }
 #pragma unroll
-    for (int i = 0; i < 2 * DT; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      for (int i = 0; i < 2 * DT; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      raise(s1, kt + 32);
+      values(s1, 1, buf);
     }
-    raise(s1, kt + 32);
-    values(s1, 1, buf);
   };
 
   if (ANY && a.hd < HD) {  // chunks behind the heads' end, which no load writes
     for (uint16_t* buf : {sh.k0, sh.k1, sh.v0, sh.v1})
-      for (int i = tid; i < kWideKeys * kRowChunks; i += kThreads)
+      for (int i = tid; i < KT * kRowChunks; i += kThreads)
         reinterpret_cast<u32x4_t*>(buf)[i] = u32x4_t{0, 0, 0, 0};
     __syncthreads();
   }
@@ -883,16 +887,16 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
   settle(qf);
   for (int kt = k0; kt < k1;) {
     step(kt, 0);
-    kt += kWideKeys;
+    kt += KT;
     if (kt >= k1) break;
     step(kt, 1);
-    kt += kWideKeys;
+    kt += KT;
   }
   __syncthreads();
 
   if (m >= rows) return;
   if (ANY && *sh.left) {
-    const int lo = max(k0, k0 + (max(all, k0) - k0) / kWideKeys * kWideKeys);
+    const int lo = max(k0, k0 + (max(all, k0) - k0) / KT * KT);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -943,28 +947,33 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
   if (h2 == 0) (wg.prefix ? pl.p_ml : pl.o_ml)[at] = make_float2(mref, z);
 }
 
+// keys of a step: 64 where a CU has two workgroups at most (64.5 us for a prompt
+// of 2000 tokens; 73 with 32), 32 where there are enough for three
 template <bool F16, int HD, bool ANY>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD > 128 ? 1 : 2)))
 void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
-  FMX_WIDE_LDS(HD, s);
-  wide_item<F16, HD, ANY>(a, pl, wg, blockIdx.x, s);
+  FMX_WIDE_LDS(HD, 64, s);
+  wide_item<F16, HD, 64, ANY>(a, pl, wg, blockIdx.x, s);
 }
 
 // A prefix in wide tiles and own keys in narrow ones in one grid: the former
-// keep the matrix cores busy, the latter HBM. Groups of 8 workgroups (one per
-// XCD) of both kinds take turns until one kind has run out.
+// keep the matrix cores busy, the latter HBM, as workgroups end at different
+// times. With 32 keys per step both fit three times on a CU (narrow tiles of
+// two row sets do not: then 64 keys, twice). 128 sequences behind 32768 shared
+// positions: 90 + 65 us as two grids, 121 us so; 140 us with 64 keys.
 template <bool F16, int HD, int RT, bool ANY>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD > 128 ? 1 : 2)))
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(RT == 1 ? 3 : 2)))
 void attn_both_kernel(CacheAttnArgs a, Plan pl, WideGrid wg, int n_wide, int n_narrow) {
-  FMX_WIDE_LDS(HD, s);
+  constexpr int KT = RT == 1 ? 32 : 64;
+  FMX_WIDE_LDS(HD, KT, s);
+  static_assert(16 * RT * HD * 4 <= KT * HD * 2 && sizeof(NarrowLds<RT>) <= KT * HD * 2, "narrow tiles' LDS");
   const int base = (n_wide + 7) / 8 * 8;
-  const bool wide = static_cast<int>(blockIdx.x) < base;
-  const int item = wide ? blockIdx.x : blockIdx.x - base;
-  if (wide) {
-    if (item < n_wide) wide_item<F16, HD, ANY>(a, pl, wg, item, s);
+  if (static_cast<int>(blockIdx.x) < base) {
+    if (static_cast<int>(blockIdx.x) < n_wide) wide_item<F16, HD, KT, ANY>(a, pl, wg, blockIdx.x, s);
   } else {
-    if (item < n_narrow) narrow_item<F16, HD, RT, ANY>(a, pl, 0, item, reinterpret_cast<float*>(s.k0), reinterpret_cast<float*>(s.k1),
-                                    *reinterpret_cast<NarrowLds<RT>*>(s.v0));
+    if (static_cast<int>(blockIdx.x) - base < n_narrow)
+      narrow_item<F16, HD, RT, ANY>(a, pl, 0, blockIdx.x - base, reinterpret_cast<float*>(s.k0),
+                                    reinterpret_cast<float*>(s.k1), *reinterpret_cast<NarrowLds<RT>*>(s.v0));
   }
 }
 
@@ -1367,7 +1376,8 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
     const int rows = pl.p_wide ? kWideRows : tr;
     pl.p_tiles = static_cast<int>((rows_p + rows - 1) / rows);
     const int64_t units = (a.P + kPiece - 1) / kPiece;
-    const int64_t fill = !pl.p_wide ? kFill : a.S > 0 && !pl.o_wide ? kWideFill / 2 : kWideFill;
+    // (beside narrow tiles of two row sets a CU takes one wide workgroup)
+    const int64_t fill = !pl.p_wide ? kFill : a.S > 0 && !pl.o_wide && y.rt == 2 ? kWideFill / 2 : kWideFill;
     int64_t splits = std::max<int64_t>(1, fill / (static_cast<int64_t>(pl.p_tiles) * a.nkv));
     splits = std::min(splits, units);
     const int64_t per = (units + splits - 1) / splits;
