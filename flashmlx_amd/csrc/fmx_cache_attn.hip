@@ -643,7 +643,7 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
 
   // ---- the item
   const int pair = block % wg.padded;
-  if (pair >= wg.pairs) return;
+  if (pair >= wg.pairs || block >= wg.padded * wg.tiles) return;
   // Rows that see the most keys first; of the tiles that one round of the CUs
   // takes, every other round's in reverse, so that a CU's tiles are long and
   // short ones.
@@ -951,9 +951,11 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
 // of 2000 tokens; 73 with 32), 32 where there are enough for three
 template <bool F16, int HD, bool ANY>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD > 128 ? 1 : 2)))
-void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid wg) {
+void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid pg, WideGrid og, int n_prefix) {
   FMX_WIDE_LDS(HD, 64, s);
-  wide_item<F16, HD, 64, ANY>(a, pl, wg, blockIdx.x, s);
+  // (the prefix's blocks, then the own keys')
+  const bool prefix = static_cast<int>(blockIdx.x) < n_prefix;
+  wide_item<F16, HD, 64, ANY>(a, pl, prefix ? pg : og, prefix ? blockIdx.x : blockIdx.x - n_prefix, s);
 }
 
 // A prefix in wide tiles and own keys in narrow ones in one grid: the former
@@ -1041,17 +1043,19 @@ __device__ inline void row_stats(const RowPieces& ps, int lane, float* m_out, fl
 // each and their values' sums dealt to the four waves, so a row waits for two
 // or three rounds of loads, whatever its number of pieces (34 pieces of 1024
 // rows: 27 us with 32 threads per row that walk them one by one, 18 us with a
-// wave per row). The others: the weights of kWeightKeys keys of a (sequence,
+// wave per row, 8 us so). PER_WAVE: four rows each, where there are rows
+// enough to fill the card. The others: the weights of kWeightKeys keys of a (sequence,
 // kv head) from the stored scores, a thread's loads issued before the rows'
 // statistics are there.
-template <bool F16>
+template <bool F16, bool PER_WAVE>
 __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Plan pl, int n_join, int w_tiles) {
   __shared__ float s_acc[kWaves][kCacheMaxHd];
   __shared__ float2 s_row[kNarrowRows];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (static_cast<int>(blockIdx.x) < n_join) {
-    const int64_t row = blockIdx.x;
+    const int64_t row = PER_WAVE ? static_cast<int64_t>(blockIdx.x) * kWaves + wave : blockIdx.x;
+    if (PER_WAVE && row >= static_cast<int64_t>(a.B) * a.L * a.nh) return;
     const int t = static_cast<int>(row / a.nh), h = static_cast<int>(row % a.nh);
     const int b = t / a.L, l = t - b * a.L, g = h / a.rep;
     const RowPieces ps(a, pl, b, g, l * a.rep + h - g * a.rep);
@@ -1073,27 +1077,40 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Pl
         for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], fi, acc[e]);
       }
     };
-    if (ps.n <= kWave) {
+    constexpr int kStride = PER_WAVE ? 1 : kWaves;
+    for (int i0 = 0; i0 < ps.n; i0 += kWave) {
+      // 64 pieces' factors, a lane each
+      if (ps.n > kWave) f = i0 + lane < ps.n ? __builtin_amdgcn_exp2f(ps.ml(i0 + lane).x - ms) : 0.0f;
+      const int c = min(kWave, ps.n - i0);
 #pragma unroll 8
-      for (int i = wave; i < ps.n; i += kWaves)
-        add(i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i)));
-    } else {
-#pragma unroll 4
-      for (int i = wave; i < ps.n; i += kWaves) add(i, __builtin_amdgcn_exp2f(ps.ml(i).x - ms));
+      for (int i = PER_WAVE ? 0 : wave; i < c; i += kStride)
+        add(i0 + i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i)));
     }
-    if (d < a.hd)
-      for (int e = 0; e < vd; ++e) s_acc[wave][d + e] = acc[e];
-    __syncthreads();
     const float inv = z == 0.0f ? 0.0f : 1.0f / z;
     uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + l * a.out.ts + h * a.out.hs;
-    if (2 * tid < a.hd) {
-      float v[2];
+    const auto pair = [&](float x, float y) {
+      return Act<F16>::st(x * inv) | static_cast<uint32_t>(Act<F16>::st(y * inv)) << 16;
+    };
+    if constexpr (PER_WAVE) {
+      if (d < a.hd) {
+        if (vd == 2)
+          *reinterpret_cast<uint32_t*>(out + d) = pair(acc[0], acc[1]);
+        else
+          *reinterpret_cast<u32x2_t*>(out + d) = u32x2_t{pair(acc[0], acc[1]), pair(acc[2], acc[3])};
+      }
+    } else {
+      if (d < a.hd)
+        for (int e = 0; e < vd; ++e) s_acc[wave][d + e] = acc[e];
+      __syncthreads();
+      if (2 * tid < a.hd) {
+        float v[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        v[e] = (s_acc[0][2 * tid + e] + s_acc[1][2 * tid + e] + (s_acc[2][2 * tid + e] + s_acc[3][2 * tid + e])) * inv;
-      reinterpret_cast<uint32_t*>(out)[tid] = Act<F16>::st(v[0]) | static_cast<uint32_t>(Act<F16>::st(v[1])) << 16;
+        for (int e = 0; e < 2; ++e)
+          v[e] = s_acc[0][2 * tid + e] + s_acc[1][2 * tid + e] + (s_acc[2][2 * tid + e] + s_acc[3][2 * tid + e]);
+        reinterpret_cast<uint32_t*>(out)[tid] = pair(v[0], v[1]);
+      }
     }
-    if (tid == 0) {
+    if (PER_WAVE ? lane == 0 : tid == 0) {
       const float l2 = z == 0.0f ? neg_inf() : ms + __log2f(z);
       if (pl.lse) pl.lse[row] = l2 * kLn2;
       if (pl.lse2) pl.lse2[(static_cast<int64_t>(b) * a.nkv + g) * pl.R + l * a.rep + h - g * a.rep] = l2;
@@ -1345,6 +1362,12 @@ __global__ __launch_bounds__(kThreads) void attn_weights_sum_kernel(CacheAttnArg
 constexpr int64_t kFill = 768;
 // and of wide tiles: two
 constexpr int64_t kWideFill = 512;
+// rows from which a wave of the join takes one of its own: 32 waves per CU
+constexpr int64_t kJoinWaves = 8192;
+// keys of a wide tile's piece at least: shorter ones cost more in the join
+// than they gain (own keys in one piece need none)
+constexpr int64_t kWidePrefixKeys = 256;
+constexpr int64_t kWideOwnKeys = 512;
 // workgroups for a prompt's weights; a part has at least 256 rows or so
 constexpr int64_t kSumFill = 768;
 
@@ -1379,7 +1402,7 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
     // (beside narrow tiles of two row sets a CU takes one wide workgroup)
     const int64_t fill = !pl.p_wide ? kFill : a.S > 0 && !pl.o_wide && y.rt == 2 ? kWideFill / 2 : kWideFill;
     int64_t splits = std::max<int64_t>(1, fill / (static_cast<int64_t>(pl.p_tiles) * a.nkv));
-    splits = std::min(splits, units);
+    splits = std::min(splits, pl.p_wide ? (a.P + kWidePrefixKeys - 1) / kWidePrefixKeys : units);
     const int64_t per = (units + splits - 1) / splits;
     pl.p_keys = static_cast<int>(per * kPiece);
     pl.p_splits = static_cast<int>((units + per - 1) / per);
@@ -1389,7 +1412,7 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
     if (pl.o_wide) {
       pl.o_tiles = (pl.R + kWideRows - 1) / kWideRows;
       const int64_t fill = kWideFill / (static_cast<int64_t>(pl.o_tiles) * a.nkv * a.B);
-      pl.o_splits = static_cast<int>(std::max<int64_t>(1, std::min(fill, units)));
+      pl.o_splits = static_cast<int>(std::max<int64_t>(1, std::min(fill, a.S / kWideOwnKeys)));
     } else {
       pl.o_tiles = (pl.R + tr - 1) / tr;
       // no more pieces than units of 128 keys, and the table's room
@@ -1457,10 +1480,9 @@ hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stre
     return hipGetLastError();
   }
   hipError_t e = hipSuccess;
-  if (np) hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(np), wg, 0, stream, a, pl, pg);
-  if (np) e = hipGetLastError();
-  if (e == hipSuccess && no) {
-    hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(no), wg, 0, stream, a, pl, og);
+  if (np + no) {
+    const int first = static_cast<int>(align_up(np, 8));  // (own blocks start on the first XCD)
+    hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(first + no), wg, 0, stream, a, pl, pg, og, first);
     e = hipGetLastError();
   }
   if (e == hipSuccess && n) {
@@ -1529,13 +1551,20 @@ hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
     e = a.hd == 256 && !any ? launch_parts<F16, 256, false>(a, pl, y.rt, stream)
                             : launch_parts<F16, 256, true>(a, pl, y.rt, stream);
   if (e != hipSuccess) return e;
-  const int64_t n_join = pl.direct ? 0 : static_cast<int64_t>(a.B) * a.L * a.nh;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.L * a.nh;
+  const bool per_wave = rows > kJoinWaves;
+  const int64_t n_join = pl.direct ? 0 : per_wave ? (rows + kWaves - 1) / kWaves : rows;
   const int64_t w_tiles = pl.scores ? (a.S + kWeightKeys - 1) / kWeightKeys : 0;
   const int64_t grid = n_join + w_tiles * a.nkv * a.B;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
   if (grid > 0) {
-    hipLaunchKernelGGL(attn_join_kernel<F16>, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a, pl,
-                       static_cast<int>(n_join), static_cast<int>(w_tiles));
+    const dim3 gr(static_cast<uint32_t>(grid)), wg(kThreads);
+    if (per_wave)
+      hipLaunchKernelGGL((attn_join_kernel<F16, true>), gr, wg, 0, stream, a, pl, static_cast<int>(n_join),
+                         static_cast<int>(w_tiles));
+    else
+      hipLaunchKernelGGL((attn_join_kernel<F16, false>), gr, wg, 0, stream, a, pl, static_cast<int>(n_join),
+                         static_cast<int>(w_tiles));
     e = hipGetLastError();
   }
   if (e == hipSuccess && a.w_out && !pl.scores) e = launch_weights<F16>(a, pl, stream);
