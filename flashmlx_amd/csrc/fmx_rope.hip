@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotUnits = 2;       // units of a thread: pairs of vectors in flight
-constexpr int kRotTable = 4096;    // (cos, sin) of a workgroup: 32 KB of LDS
+constexpr int kRotTable = 2048;    // (cos, sin) of a workgroup at most: 16 KB of LDS
 constexpr double kInv2Pi = 0.15915494309189533577;
 
 template <int ES, bool F16>
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kRotThreads) void rotate_kernel(RotateArgs a, RotPl
   typedef Elem<ES, F16> E;
   typedef typename E::T T;
   typedef Vec<T, VEC> V;
-  __shared__ float2 s_cs[kRotTable];
+  extern __shared__ float2 s_cs[];  // (cos, sin) of the tokens' pairs
   const int tid = threadIdx.x;
   const int half = a.dims / 2;
   const int rows = a.B * a.L;
@@ -182,12 +182,12 @@ hipError_t rotate(const RotateArgs& a, hipStream_t stream) {
   pl.tokens = pl.parts > 1 ? 1 : std::max(1, std::min(kPer / pl.units, kRotTable / half));
   const int64_t grid = (rows + pl.tokens - 1) / pl.tokens * pl.parts;
   if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  const dim3 gr(static_cast<uint32_t>(grid)), wg(kRotThreads);
+  const size_t lds = static_cast<size_t>(pl.tokens) * half * sizeof(float2);
   if (a.interleaved)
-    hipLaunchKernelGGL((rotate_kernel<ES, F16, VEC, true>), dim3(static_cast<uint32_t>(grid)), dim3(kRotThreads), 0,
-                       stream, a, pl);
+    hipLaunchKernelGGL((rotate_kernel<ES, F16, VEC, true>), gr, wg, lds, stream, a, pl);
   else
-    hipLaunchKernelGGL((rotate_kernel<ES, F16, VEC, false>), dim3(static_cast<uint32_t>(grid)), dim3(kRotThreads), 0,
-                       stream, a, pl);
+    hipLaunchKernelGGL((rotate_kernel<ES, F16, VEC, false>), gr, wg, lds, stream, a, pl);
   return hipGetLastError();
 }
 
