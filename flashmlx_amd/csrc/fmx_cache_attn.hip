@@ -334,7 +334,7 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
       const uint16_t* p = whole ? kp0 + (kk - kk0 + 16 * x) * kts : kb + min(kk + 16 * x + i16, k1 - 1) * kts + 8 * j;
 #pragma unroll
       for (int t = 0; t < KC; ++t)
-        if (!ANY || 32 * t + 8 * j < a.hd) kw[x][t] = *reinterpret_cast<const u32x4_t*>(p + 32 * t);
+        if (!ANY || 32 * t + 8 * j < a.hd) kw[x][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 32 * t));
         else kw[x][t] = u32x4_t{0, 0, 0, 0};
     }
   };
@@ -347,14 +347,14 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
                                 : vb + min(kk + row + 4 * j, k1 - 1) * vts + (VPL == 4 ? 4 : 8) * i16;
       if constexpr (VPL == 4) {
         u32x2_t w = {0, 0};
-        if (!ANY || 4 * i16 < a.hd) w = *reinterpret_cast<const u32x2_t*>(p);
+        if (!ANY || 4 * i16 < a.hd) w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(p));
         vw[sl][0] = w[0];
         vw[sl][1] = w[1];
       } else {
 #pragma unroll
         for (int q = 0; q < VPL / 8; ++q) {
           u32x4_t w = {0, 0, 0, 0};
-          if (!ANY || 128 * q + 8 * i16 < a.hd) w = *reinterpret_cast<const u32x4_t*>(p + 128 * q);
+          if (!ANY || 128 * q + 8 * i16 < a.hd) w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 128 * q));
 #pragma unroll
           for (int i = 0; i < 4; ++i) vw[sl][4 * q + i] = w[i];
         }
