@@ -203,7 +203,9 @@ __device__ void cut_row(const EvictArgs& a, SelShared& s, const float* w, float*
 }
 
 // Bound by its chain of rounds: the weights are read once (up to 16384
-// positions: kept in registers), a round is an LDS histogram and a scan.
+// positions: kept in registers), a round is an LDS histogram and a scan. 64
+// rows of up to 1152 weights 6.7 us, 64 rows of up to 16384 16 us (32 us with
+// one copy of the histogram and every round reading them again).
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
   __shared__ SelShared s;
   const int tid = threadIdx.x;
@@ -248,8 +250,10 @@ struct Unit<2> {
   typedef uint16_t T;
 };
 
-// Bound by HBM: kept rows are read and written once. 16 bytes per lane where
-// rows and strides allow.
+// Bound by HBM: kept rows are read and written once, in kept order, so reads
+// are runs of rows. 16 bytes per lane where rows and strides allow. 16
+// sequences of 4 kv heads cut to 4000 rows of 128: 55 us for 250 MB, 4.5 TB/s
+// (4.9 is a large copy's).
 template <int VB>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, int chunks, int chunk_rows) {
   typedef typename Unit<VB>::T T;
@@ -300,7 +304,9 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
 // block of rows after the other. Row i comes from row kept[i] >= i, so what a
 // block reads lies behind all that earlier blocks wrote, and what it writes is
 // read by no later block: only a block's own reads have to end before its
-// writes begin.
+// writes begin. Bound by that chain of blocks, so rows are sliced until 512
+// workgroups run: 80 us for 16 sequences of 16384 cut to 4000
+// positions, the selection included; one of 16384 cut to 8192, 60 us.
 template <int VB>
 __global__ __launch_bounds__(kMoveThreads) void evict_shift_kernel(EvictArgs a, int slices, int slice_units) {
   typedef typename Unit<VB>::T T;
@@ -362,7 +368,7 @@ hipError_t move_rows(const EvictArgs& a, hipStream_t stream) {
     int slices = 1;
     while (slices * 2 * 64 <= a.row_bytes && heads * 2 * slices < 512 && per % (slices * 2) == 0) slices *= 2;
     // (and no longer than a block of threads)
-    while (per / slices > kMoveThreads) ++slices;
+    while ((per + slices - 1) / slices > kMoveThreads) ++slices;
     const int units = (per + slices - 1) / slices;
     slices = (per + units - 1) / units;
     const int64_t n = heads * 2 * slices;
@@ -387,7 +393,8 @@ hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   int64_t all = a.row_bytes;
-  for (int64_t s : {a.k_bs, a.k_ts, a.k_hs, a.v_bs, a.v_ts, a.v_hs, a.ko_bs, a.ko_ts, a.ko_hs, a.vo_bs, a.vo_ts, a.vo_hs})
+  for (int64_t s : {a.k_bs, a.k_ts, a.k_hs, a.v_bs, a.v_ts, a.v_hs,
+                    a.ko_bs, a.ko_ts, a.ko_hs, a.vo_bs, a.vo_ts, a.vo_hs})
     all |= s;
   for (const void* p : {static_cast<const void*>(a.k), static_cast<const void*>(a.v),
                         static_cast<const void*>(a.k_out), static_cast<const void*>(a.v_out)})

@@ -81,6 +81,14 @@ def test_evict(gpu, fmx, dt, B, nkv, S, hd, budget, sinks, recent):
     _both_ways(fmx, k, v, w, lens, budget, sinks, recent, S_out=min(budget, S) + 3)
 
 
+@pytest.mark.parametrize("hd", [511, 513, 769, 1023])
+def test_evict_odd_wide_heads(gpu, fmx, hd):
+    """Rows of an odd number of elements, longer than a workgroup."""
+    B, nkv, S, budget = 2, 2, 90, 50
+    k, v = _randn((B, nkv, S, hd), torch.bfloat16, 1), _randn((B, nkv, S, hd), torch.bfloat16, 2)
+    _both_ways(fmx, k, v, _randn((B, nkv, S), torch.float32, 3), [S, 60], budget, 2, 8)
+
+
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few", "special", "negative", "close"])
 def test_evict_ties_and_special_weights(gpu, fmx, kind):
     B, nkv, S, hd, budget = 2, 2, 2100, 16, 700
