@@ -274,7 +274,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     (lengths_out int32 [batch], kept int32 [batch, kv_heads, budget]: the kept
     positions, -1 behind the last). lengths_out may be lengths."""
     lib = _lib.load()
-    dev, pool, dt, i32, f32 = _device(k_cache, "k_cache", _SLOTS), k_cache.shape, k_cache.dtype, torch.int32, torch.float32
+    dev, pool, dt = _device(k_cache, "k_cache", _SLOTS), k_cache.shape, k_cache.dtype
+    i32, f32 = torch.int32, torch.float32
     n_slots, nkv, S, hd = pool
     if lengths.dim() != 1:
         raise ValueError(f"lengths: shape {tuple(lengths.shape)}, expected [batch]")

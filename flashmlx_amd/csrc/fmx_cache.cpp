@@ -167,6 +167,19 @@ int check_attention(const fmx_attention_shape* s, int64_t prefix_len, int64_t ma
   return FMX_OK;
 }
 
+// out against what is read after parts of it may have been written
+int check_out(const CacheAttnArgs& a, int64_t n_slots) {
+  const auto at = [&](const HeadsView& v, int64_t nb, int64_t nt, int64_t nh) {
+    const fmx_heads h{v.p, v.bs, v.ts, v.hs};
+    return v.p ? span(&h, nb, nt, nh, a.hd, 2) : Span{0, 0};
+  };
+  const Span out = at(a.out, a.B, a.L, a.nh);
+  for (const Span& i : {at(a.q, a.B, a.L, a.nh), at(a.kp, 1, a.P, a.nkv), at(a.vp, 1, a.P, a.nkv),
+                        at(a.kc, n_slots, a.S, a.nkv), at(a.vc, n_slots, a.S, a.nkv)})
+    if (overlap(out, i)) return fail(FMX_ERR_ARG, "out overlaps q, the prefix or a cache");
+  return FMX_OK;
+}
+
 CacheAttnArgs attention_args(const fmx_attention_shape* s, int64_t prefix_len, int64_t max_seq, bool weights) {
   CacheAttnArgs a{};
   a.B = static_cast<int>(s->batch);
@@ -381,6 +394,7 @@ int fmx_attention_shared_prefix(const fmx_attention_shape* shape, const fmx_head
   a.q = view(&q_v);
   a.out = view(&out_v);
   a.lse = lse;
+  FMX_RC(check_out(a, n_slots));
   Workspace ws;
   FMX_RC(ws.bind(workspace, workspace_bytes, cache_attn_workspace(a), stream));
   FMX_HIP(launch_cache_attn(a, shape->dtype == FMX_F16, ws.p, stream));
@@ -426,6 +440,7 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
   a.n_slots = n_slots;
   a.w_in = weights_in;
   a.w_out = weights_out;
+  FMX_RC(check_out(a, n_slots));
   Workspace ws;
   FMX_RC(ws.bind(workspace, workspace_bytes, cache_attn_workspace(a), stream));
   FMX_HIP(launch_cache_attn(a, shape->dtype == FMX_F16, ws.p, stream));

@@ -158,11 +158,18 @@ __device__ int find_piece(const CacheAttnArgs& a, const Plan& pl, int w, bool wr
 // wave), and pairs of keys are put together by v_perm. Nothing passes through
 // LDS and no load is narrower than a cache line's half.
 //
-// Bound by HBM: every key and value is read once, 512 bytes (heads of 128)
-// for 16 bytes of partial results per 128 keys and row. 16 sequences of up to
-// 16001 keys, 32 heads over 4, fp16, weights stored and added: 91 us, 3.0 TB/s;
-// one row per workgroup and head took 6.6 ms, the same values read for every
-// head and queried one after the other.
+// The matrix cores have time to spare, so the weights go into the value product
+// as two numbers of the inputs' type, their leading bits and the rest (2^-17
+// or 2^-22 of the weight is lost): only the output is rounded.
+//
+// Bound by HBM: every key and value is read once, past the caches (60.3 us
+// through them for the 59.4 below), 512 bytes (heads of 128) for 16 bytes of partial results per 128
+// keys and row. 16 sequences of up to 16001 keys, 32 heads over 4, fp16,
+// scores stored: 59 us for 271 MB, 4.6 TB/s (4.9 is a large copy's); one row
+// per workgroup and head took 6.6 ms, the same values read for every head and
+// queried one after the other. Short calls are bound by the chain of a
+// workgroup (a piece's address, its loads, two products): 4 sequences of up to
+// 64 keys behind 512 shared ones, 16 kv heads, 5 MB, take 6.7 us.
 template <int HD>
 struct Narrow {
   static constexpr int KC = HD / 32;            // 32-dimension steps of a score
@@ -334,8 +341,10 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
       const uint16_t* p = whole ? kp0 + (kk - kk0 + 16 * x) * kts : kb + min(kk + 16 * x + i16, k1 - 1) * kts + 8 * j;
 #pragma unroll
       for (int t = 0; t < KC; ++t)
-        if (!ANY || 32 * t + 8 * j < a.hd) kw[x][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 32 * t));
-        else kw[x][t] = u32x4_t{0, 0, 0, 0};
+        if (!ANY || 32 * t + 8 * j < a.hd)
+          kw[x][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 32 * t));
+        else
+          kw[x][t] = u32x4_t{0, 0, 0, 0};
     }
   };
   auto load_v = [&](int kk) {
@@ -354,7 +363,8 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
 #pragma unroll
         for (int q = 0; q < VPL / 8; ++q) {
           u32x4_t w = {0, 0, 0, 0};
-          if (!ANY || 128 * q + 8 * i16 < a.hd) w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 128 * q));
+          if (!ANY || 128 * q + 8 * i16 < a.hd)
+            w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 128 * q));
 #pragma unroll
           for (int i = 0; i < 4; ++i) vw[sl][4 * q + i] = w[i];
         }
@@ -486,7 +496,6 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
   }
-  constexpr int V4 = DT < 8 ? DT : 8;  // consecutive dimensions of a lane and row
   auto leave = [&](bool add) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
@@ -499,7 +508,6 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
           *p = add ? *p + v : v;
         }
   };
-  static_assert(V4 % 4 == 0, "dimensions in fours");
   if (wave < 2) leave(false);
   __syncthreads();
   if (wave >= 2) leave(true);
@@ -548,19 +556,24 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 // S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_32x32x16. Register 8u + 4v + r
 // of a lane (row c of the 32, half h) is the score of key 16u + 8v + 4h + r:
 // after exp2 the B operand of the value product over those 16 keys, if key 16u
-// + 8v + 4h + r is its slot 8h + 4v + r. Values are staged dimension by
-// dimension with the keys in slot order, so that the A operand of a dimension
-// is 16 consecutive bytes: a thread loads 16 bytes of four keys, transposes
-// them by v_perm and writes four keys of each of its eight dimensions. Rows of
-// both arrays are padded by 16 bytes: the 16 lanes that an LDS access serves
-// at a time fall on different banks. The next positions are loaded while
-// these are multiplied.
+// + 8v + 4h + r is its slot 8h + 4v + r. Its A operand is the same keys' values of
+// one dimension, which two transposing LDS reads of four keys each deliver.
+// Keys and values come to LDS past the registers, in two buffers: the next
+// positions are on their way while these are multiplied.
 //
 // The weights are rounded to the inputs' type for the value product (2^-9 or
-// 2^-12 of each, as random as the values' own rounding); their sum is formed
-// before the rounding. The maximum is only raised when a score lies more than
-// kLazy above it: the weights reach 2^kLazy times kBias' 2^8 at most, in fp16
-// 2^14 of 65504.
+// 2^-12 of each at most, as random as the values' own rounding; a second
+// product for the rest, as in narrow tiles, would be half of all the work
+// again); their sum is formed before the rounding. The maximum is only raised
+// when a score lies more than kLazy above it: the weights reach 2^kLazy times
+// kBias' 2^8 at most, in fp16 2^14 of 65504.
+//
+// Bound by the vector instructions beside the matrix ones: exp2, maxima and
+// conversions of 32 x 64 scores take a wave longer than their 32 matrix
+// instructions, and each row waits for its maximum before its weights. A step
+// of 64 keys takes 1.6 us alone on a CU and 2.4 us beside another workgroup's.
+// A prompt of 2000 tokens, 32 heads over 4: 65 us, 0.5 PFLOP/s of the causal
+// half (1.4 is a large library product's).
 constexpr int kWideRows = 32 * kWaves;
 constexpr int kCus = 256;
 constexpr float kLazy = 6.0f;

@@ -25,8 +25,9 @@ extern "C" {
 /* A strided view of rows of heads: element (b, l, h, d) is at
  * data + b * batch_stride + l * token_stride + h * head_stride + d, strides in
  * elements, not negative. For a cache, b is the slot and l the position. An
- * output's rows must not overlap one another nor, except where a call says
- * so, an input. */
+ * output's rows must not overlap one another. Nor, except where a call says
+ * so, may they lie between an input's first and last element (or an input's
+ * between theirs): such calls are refused. */
 typedef struct fmx_heads {
   void* data;
   int64_t batch_stride;
@@ -142,8 +143,9 @@ typedef struct fmx_attention_shape {
  * stride per position (batch_stride unused; may be NULL when prefix_len is
  * 0). k_cache, v_cache: slots[b] as in fmx_rope_append (need not be
  * distinct); a slot outside [0, n_slots) has no keys. max_seq 0: no own keys
- * (the caches may then be NULL). Keys and values that no query may see are
- * never used, whatever they hold. */
+ * (the caches may then be NULL). Keys and values that a query may not see
+ * do not reach its results, whatever they hold; an infinite value that it
+ * sees leaves it infinity or NaN. */
 size_t fmx_attention_shared_prefix_workspace_size(const fmx_attention_shape* shape,
                                                   int64_t prefix_len, int64_t max_seq);
 int fmx_attention_shared_prefix(const fmx_attention_shape* shape, const fmx_heads* q,

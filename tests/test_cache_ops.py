@@ -206,6 +206,24 @@ def test_attention_workspaces(lib, kw):
             assert call(lib, sh, ws=(1 << 20) + 16, ws_bytes=size, **more) == ARG
 
 
+def test_attention_limits(lib):
+    """Token strides that 64 rows' byte offsets do not hold, positions and
+    query rows beyond what one call counts, outputs among the inputs."""
+    far = Heads(ts=(1 << 24) + 8)
+    for call in (_shared, _scored):
+        assert call(lib, kc=far) == UNSUP
+        assert call(lib, vc=far) == UNSUP
+        assert call(lib, _shape(B=1 << 13), n_slots=1 << 13, S=(1 << 23) + 1) == UNSUP
+        assert call(lib, _shape(B=1 << 14, L=1 << 10, nh=128), n_slots=1 << 14) == UNSUP
+    assert _shared(lib, kp=far) == UNSUP
+    assert _shared(lib, vp=far) == UNSUP
+    at = 1 << 50
+    for call, names in ((_shared, ("q", "kc", "vc", "kp", "vp")), (_scored, ("q", "kc", "vc"))):
+        for name in names:
+            assert call(lib, **{name: Heads(data=at), "out": Heads(data=at)}) == ARG, name
+            assert call(lib, **{name: Heads(data=at), "out": Heads(data=at + 256)}) == ARG, name
+
+
 # ------------------------------------------------------------------ eviction
 
 def _evict(lib, dtype=BF16, B=2, nkv=2, hd=64, k=None, v=None, w=1 << 35, n_slots=2, S=100, lens=1 << 33, slots=None,

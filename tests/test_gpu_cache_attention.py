@@ -145,6 +145,40 @@ def test_later_keys_do_not_reach_earlier_queries(gpu, fmx, L, rep):
             assert not bool(torch.isfinite(out[:, L - 1]).any())
 
 
+@pytest.mark.parametrize("B,L,nh,nkv,hd,P,S", [
+    (300, 1, 4, 1, 64, 40, 20),       # more sequences than threads in a workgroup
+    (300, 1, 32, 4, 64, 200, 12),     # more rows than the join has waves
+    (1, 1, 2, 1, 64, 20000, 300),     # more pieces than lanes
+    (2, 1, 2, 1, 128, 0, 30000),
+    (1, 40, 4, 1, 64, 50, 2100),      # own keys of wide tiles in several pieces
+    (2, 9, 8, 2, 256, 700, 1100),
+    (36, 1, 2, 2, 256, 600, 40),      # wide prefix, narrow own keys, wide heads
+    (20, 3, 16, 2, 80, 500, 70),
+])
+def test_shared_prefix_plans(gpu, fmx, B, L, nh, nkv, hd, P, S):
+    """Both sides of every choice of tiles, pieces and joins."""
+    q, kp, vp, kc, vc, offs = _inputs(torch.float16, B, L, nh, nkv, hd, P, S, seed=80)
+    _blank(kc, vc, offs, L)
+    scale = 1 / math.sqrt(hd)
+    out, lse = fmx.attention_shared_prefix(q, kp, vp, kc, vc, offs, scale)
+    r = R.attention(q, _finite(kc), _finite(vc), offs, scale, kp=kp, vp=vp)
+    R.assert_within(out, r["out"], r["out_b"], "out")
+    R.assert_within(lse, r["lse"], r["lse_b"], "lse")
+
+
+@pytest.mark.parametrize("B,L,nh,nkv,hd,S", [
+    (300, 1, 4, 1, 64, 20), (300, 1, 32, 4, 64, 12), (2, 1, 2, 1, 128, 30000), (1, 40, 4, 1, 64, 2100),
+    (2, 9, 8, 2, 256, 1100), (2, 600, 4, 1, 64, 900)])
+def test_scored_plans(gpu, fmx, B, L, nh, nkv, hd, S):
+    q, _, _, kc, vc, offs = _inputs(torch.bfloat16, B, L, nh, nkv, hd, 0, S, seed=81)
+    _blank(kc, vc, offs, L)
+    scale = 1 / math.sqrt(hd)
+    r = R.attention(q, _finite(kc), _finite(vc), offs, scale)
+    out, w = fmx.attention_scored(q, kc, vc, offs, scale)
+    R.assert_within(out, r["out"], r["out_b"], "out")
+    R.assert_within(w, r["w"], r["w_b"], "weights")
+
+
 def test_slots_and_unused_sequences(gpu, fmx):
     B, nh, nkv, hd, S, n = 5, 8, 2, 64, 50, 7
     q = _randn((B, 1, nh, hd), torch.bfloat16, 1)
