@@ -61,6 +61,14 @@ def _cache(t: torch.Tensor, name: str, shape, dtype, dev: int):
     return _byref(FmxHeads(t.data_ptr(), s[0], s[2], s[1]))
 
 
+def _prefix(t: torch.Tensor, name: str, shape, dtype, dev: int):
+    """The view of a [head, position, element] tensor."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev or t.stride(2) != 1 and shape[2] != 1:
+        _refuse(t, name, shape, dtype, dev)
+    s = t.stride()
+    return _byref(FmxHeads(t.data_ptr(), 0, s[1], s[0]))
+
+
 def _flat(t: Optional[torch.Tensor], name: str, shape, dtype, dev: int) -> Optional[int]:
     """The address of a contiguous array, or None."""
     if t is None:
@@ -92,8 +100,9 @@ def _pool(k: torch.Tensor, hd: int) -> tuple:
     return k.shape[0], k.shape[1], k.shape[2]
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+def _stream(dev: int) -> int:
+    # (without torch's Stream object, whose making takes 2.4 us of an append's 13)
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _workspace(ws: Optional[torch.Tensor], need: int, like: torch.Tensor) -> torch.Tensor:
@@ -168,7 +177,7 @@ class Rope:
         _lib.check(self.lib.fmx_rope(
             _byref(self._c), _DT[dt], B, L, nh, hd, _heads(x, "x", shape, dt, dev),
             _flat(positions, "positions", (B, L), torch.int32, dev), int(inverse),
-            _heads(out, "out", shape, dt, dev), _stream()))
+            _heads(out, "out", shape, dt, dev), _stream(dev)))
         return out
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -189,7 +198,7 @@ class Rope:
             _heads(v, "v", new, dt, dev), _flat(positions, "positions", (B, L), i32, dev),
             _flat(offsets, "offsets", (B,), i32, dev), _flat(slots, "slots", (B,), i32, dev), n_slots, S,
             _heads(out, "out", shape, dt, dev), _cache(k_cache, "k_cache", pool, dt, dev),
-            _cache(v_cache, "v_cache", pool, dt, dev), _stream()))
+            _cache(v_cache, "v_cache", pool, dt, dev), _stream(dev)))
         return out
 
 
@@ -214,9 +223,8 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v
         raise ValueError("k_prefix and v_prefix: both or neither")
     if k_prefix is not None:
         P = k_prefix.shape[1] if k_prefix.dim() == 3 else -1
-        prefix = (1, nkv, P, hd)
-        kp = _cache(k_prefix.unsqueeze(0), "k_prefix", prefix, dt, dev)
-        vp = _cache(v_prefix.unsqueeze(0), "v_prefix", prefix, dt, dev)
+        kp = _prefix(k_prefix, "k_prefix", (nkv, P, hd), dt, dev)
+        vp = _prefix(v_prefix, "v_prefix", (nkv, P, hd), dt, dev)
     if out is None:
         out = q.new_empty(shape)
     lse = q.new_empty((B, L, nh), dtype=torch.float32)
@@ -226,7 +234,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v
         c, _heads(q, "q", shape, dt, dev), kp, vp, P, _cache(k_cache, "k_cache", pool, dt, dev),
         _cache(v_cache, "v_cache", pool, dt, dev), n_slots, S, _flat(offsets, "offsets", (B,), i32, dev),
         _flat(slots, "slots", (B,), i32, dev), _heads(out, "out", shape, dt, dev), lse.data_ptr(), ws.data_ptr(),
-        ws.numel(), _stream()))
+        ws.numel(), _stream(dev)))
     return out, lse
 
 
@@ -259,7 +267,7 @@ def attention_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         c, _heads(q, "q", shape, dt, dev), _cache(k_cache, "k_cache", pool, dt, dev),
         _cache(v_cache, "v_cache", pool, dt, dev), n_slots, S, _flat(offsets, "offsets", (B,), i32, dev),
         _flat(slots, "slots", (B,), i32, dev), w_in, _flat(weights_out, "weights_out", wsh, f32, dev),
-        _heads(out, "out", shape, dt, dev), ws.data_ptr(), ws.numel(), _stream()))
+        _heads(out, "out", shape, dt, dev), ws.data_ptr(), ws.numel(), _stream(dev)))
     return out, weights_out
 
 
@@ -297,5 +305,5 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
         _DT[dt], B, nkv, hd, _cache(k_cache, "k_cache", pool, dt, dev), _cache(v_cache, "v_cache", pool, dt, dev),
         _flat(weights, "weights", (n_slots, nkv, S), f32, dev), n_slots, S, _flat(lengths, "lengths", (B,), i32, dev),
         _flat(slots, "slots", (B,), i32, dev), budget, sinks, recent, ko, vo, wo, S_out,
-        _flat(lengths_out, "lengths_out", (B,), i32, dev), kept.data_ptr(), None, 0, _stream()))
+        _flat(lengths_out, "lengths_out", (B,), i32, dev), kept.data_ptr(), None, 0, _stream(dev)))
     return lengths_out, kept
