@@ -568,12 +568,15 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 // when a score lies more than kLazy above it: the weights reach 2^kLazy times
 // kBias' 2^8 at most, in fp16 2^14 of 65504.
 //
-// Bound by the vector instructions beside the matrix ones: exp2, maxima and
-// conversions of 32 x 64 scores take a wave longer than their 32 matrix
-// instructions, and each row waits for its maximum before its weights. A step
-// of 64 keys takes 1.6 us alone on a CU and 2.4 us beside another workgroup's.
-// A prompt of 2000 tokens, 32 heads over 4: 65 us, 0.5 PFLOP/s of the causal
-// half (1.4 is a large library product's).
+// Bound by a wave's own chain: by the cycle counter a step of 64 keys takes it
+// about 3000 cycles (issuing the next loads 500, scores 900, maximum 300,
+// weights and values 1300, of which the matrix cores work 1000), and a tile
+// some 14000 before its first and after its last step (queries from HBM,
+// outputs). The longest tile of a causal grid alone is two thirds of the
+// kernel's time; keys dealt to two halves of a workgroup, or long and short
+// tiles one after the other, gained nothing. A prompt of 2000 tokens, 32 heads
+// over 4: 59 us, 0.56 PFLOP/s of the causal half (1.4 is a large library
+// product's).
 constexpr int kWideRows = 32 * kWaves;
 constexpr int kCus = 256;
 constexpr float kLazy = 6.0f;
@@ -736,13 +739,16 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
   }
   auto dma = [&](const uint16_t* base, int64_t ts, const uint32_t (&off_b)[NL], bool keys, int kt, uint16_t* to) {
     const uint8_t* at = reinterpret_cast<const uint8_t*>(base + kt * ts);
-    const bool whole = kt + KT <= k1;
+    if (kt + KT <= k1 && (!ANY || a.hd == HD)) {
 #pragma unroll
+      for (int i = 0; i < NL; ++i) load_to_lds16(at + off_b[i], to + (wave * kWaveRows + i * kDmaRows) * HD);
+      return;
+    }
+#pragma nounroll
     for (int i = 0; i < NL; ++i) {
       const int row = wave * kWaveRows + i * kDmaRows + lr, ch = keys ? k_chunk(i) : v_chunk(i);
-      uint32_t o = off_b[i];
       // rows behind the piece's last are read as its last
-      if (!whole) o = (static_cast<uint32_t>(min(row, k1 - 1 - kt)) * static_cast<uint32_t>(ts) + 8 * ch) * 2;
+      const uint32_t o = (static_cast<uint32_t>(min(row, k1 - 1 - kt)) * static_cast<uint32_t>(ts) + 8 * ch) * 2;
       if (!ANY || 8 * ch < a.hd) load_to_lds16(at + o, to + (wave * kWaveRows + i * kDmaRows) * HD);
     }
   };
@@ -791,14 +797,24 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
   float mref = neg_inf(), lsum = 0.0f;
   const float sc = a.scale * kLog2e;
 
-  // scores of half x of the keys
-  auto scores = [&](int x, int buf) {
+  // operands from LDS: of score step t, and of dimension tile dt with 16 keys,
+  // of part x (32) of the keys
+  auto k_frag = [&](int t, int x, int buf) {
+    return *reinterpret_cast<const frag_t*>((buf ? sh.k1 : sh.k0) + ka[t] + 32 * x * HD);
+  };
+  auto v_frag = [&](int t, int dt, int x, int buf) {
+    typedef short s16x8_t __attribute__((ext_vector_type(8)));
+    const uint16_t* v = (buf ? sh.v1 : sh.v0) + va[dt] + (32 * x + 16 * t) * HD;
+    const s16x4_t lo = lds_read_tr(v), hi = lds_read_tr(v + 8 * HD);
+    const s16x8_t w = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(frag_t, w);
+  };
+  auto scores = [&](auto&& frag) {
     f32x16_t s;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-    for (int t = 0; t < KS; ++t)
-      s = mfma32(*reinterpret_cast<const frag_t*>((buf ? sh.k1 : sh.k0) + ka[t] + 32 * x * HD), qf[t], s);
+    for (int t = 0; t < KS; ++t) s = mfma32(frag(t), qf[t], s);
     return s;
   };
   // those that the row sees, and the maximum raised to them
@@ -822,7 +838,7 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
     }
   };
   // the half's weights, and the values' sums with them
-  auto values = [&](const f32x16_t& s, int x, int buf) {
+  auto values = [&](const f32x16_t& s, auto&& frag) {
     const float ms = mref == neg_inf() ? 0.0f : mref;
     float ls[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -836,19 +852,16 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
         pf[i] = static_cast<half_t>(p);
       }
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        typedef short s16x8_t __attribute__((ext_vector_type(8)));
-        const uint16_t* v = (buf ? sh.v1 : sh.v0) + va[dt] + (32 * x + 16 * t) * HD;
-        const s16x4_t lo = lds_read_tr(v), hi = lds_read_tr(v + 8 * HD);
-        const s16x8_t f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        o[dt] = mfma32(__builtin_bit_cast(frag_t, f), pf, o[dt]);
-      }
+      for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32(frag(t, dt), pf, o[dt]);
     }
     lsum += ls[0] + ls[1];
   };
-  // The keys at kt, in buffers buf. The second half's scores are formed among
-  // the first's exponentials, so that a wave's matrix and vector instructions
-  // overlap (the scheduler is told to deal them out in turn).
+  // The keys at kt, in buffers buf. With 64 of them, the second 32's scores are
+  // formed among the first's exponentials, so that a wave's matrix and vector
+  // instructions overlap (the scheduler is told to deal them out in turn), and
+  // operands are read before the branch ahead of their use (read there, a
+  // product each time waits for LDS: 65 us for a prompt of 2000 tokens, 59 so).
+  // With 32 there are no registers for that.
   auto step = [&](int kt, int buf) {
     // these keys and values have landed, and every wave is done with the
     // other buffers
@@ -861,29 +874,45 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
     }
     if (kt + KT > all) clean_v(kt, buf);
     if (kt >= w_end) return;
-    f32x16_t s0 = scores(0, buf);
-    raise(s0, kt);
     if constexpr (KT == 32) {
-      values(s0, 0, buf);
+      f32x16_t s0 = scores([&](int t) { return k_frag(t, 0, buf); });
+      raise(s0, kt);
+      values(s0, [&](int t, int dt) { return v_frag(t, dt, 0, buf); });
     } else {
-      f32x16_t s1 = scores(1, buf);
-      values(s0, 0, buf);
-      // (LDS reads run four matrix instructions ahead)
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      frag_t kf[2][KS], vf[2][2][DT];
+      auto read_k = [&](int x) {
+#pragma unroll
+        for (int t = 0; t < KS; ++t) kf[x][t] = k_frag(t, x, buf);
+      };
+      auto read_v = [&](int x) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) vf[x][t][dt] = v_frag(t, dt, x, buf);
+      };
+      read_k(0);
+      f32x16_t s0 = scores([&](int t) { return kf[0][t]; });
+      read_k(1);
+      asm volatile("" ::: "memory");  // (not to be moved behind the branch)
+      raise(s0, kt);
+      read_v(0);
+      f32x16_t s1 = scores([&](int t) { return kf[1][t]; });
+      values(s0, [&](int t, int dt) { return vf[0][t][dt]; });
+      __builtin_amdgcn_sched_group_barrier(0x100, 4 * DT, 0);  // LDS reads
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
-        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // vector ones
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // vector ones
       }
 #pragma unroll
       for (int i = 0; i < 2 * DT; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
       }
+      read_v(1);
+      asm volatile("" ::: "memory");
       raise(s1, kt + 32);
-      values(s1, 1, buf);
+      values(s1, [&](int t, int dt) { return vf[1][t][dt]; });
     }
   };
 
@@ -960,22 +989,23 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
   if (h2 == 0) (wg.prefix ? pl.p_ml : pl.o_ml)[at] = make_float2(mref, z);
 }
 
-// keys of a step: 64 where a CU has two workgroups at most (64.5 us for a prompt
-// of 2000 tokens; 73 with 32), 32 where there are enough for three
+// keys of a step: 64 (a prompt of 2000 tokens took 64.5 us so and 73 with 32),
+// beyond heads of 128 as many as registers hold operands of
 template <bool F16, int HD, bool ANY>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD > 128 ? 1 : 2)))
 void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid pg, WideGrid og, int n_prefix) {
-  FMX_WIDE_LDS(HD, 64, s);
+  constexpr int KT = HD > 128 ? 32 : 64;
+  FMX_WIDE_LDS(HD, KT, s);
   // (the prefix's blocks, then the own keys')
   const bool prefix = static_cast<int>(blockIdx.x) < n_prefix;
-  wide_item<F16, HD, 64, ANY>(a, pl, prefix ? pg : og, prefix ? blockIdx.x : blockIdx.x - n_prefix, s);
+  wide_item<F16, HD, KT, ANY>(a, pl, prefix ? pg : og, prefix ? blockIdx.x : blockIdx.x - n_prefix, s);
 }
 
 // A prefix in wide tiles and own keys in narrow ones in one grid: the former
 // keep the matrix cores busy, the latter HBM, as workgroups end at different
 // times. With 32 keys per step both fit three times on a CU (narrow tiles of
 // two row sets do not: then 64 keys, twice). 128 sequences behind 32768 shared
-// positions: 90 + 65 us as two grids, 121 us so; 140 us with 64 keys.
+// positions: 90 + 65 us as two grids, 116 us so; 140 us with 64 keys.
 template <bool F16, int HD, int RT, bool ANY>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(RT == 1 ? 3 : 2)))
 void attn_both_kernel(CacheAttnArgs a, Plan pl, WideGrid wg, int n_wide, int n_narrow) {
@@ -1185,7 +1215,7 @@ __global__ __launch_bounds__(kThreads) void attn_join_kernel(CacheAttnArgs a, Pl
 // roundings, not by a thousand). A part is every w_parts-th block of rows, so
 // that all parts of a causal triangle are equally long (parts of consecutive
 // rows left some XCDs with 2.4 times the work of others: 64 us for a prompt of
-// 2000 tokens, 32 heads over 4). The parts' sums are added by
+// 2000 tokens, 32 heads over 4, which takes 37 us so). The parts' sums are added by
 // attn_weights_sum_kernel, in order. Workgroups over one part's rows run on
 // one XCD.
 constexpr int kSumRows = 64;
@@ -1361,9 +1391,19 @@ __global__ __launch_bounds__(kThreads) void attn_weights_sum_kernel(CacheAttnArg
     // key have left a sum
     const int64_t l0 = max(j / kSumKeys * kSumKeys - off, static_cast<int64_t>(0));
     const int first = static_cast<int>(l0) * a.rep / kSumRows, last = (pl.R - 1) / kSumRows;
-    for (int p = 0; p < pl.w_parts; ++p)
-      if (last - (last - p) % pl.w_parts >= first)
-        w += pl.w_part[((static_cast<int64_t>(p) * a.B + b) * a.nkv + g) * a.S + j];
+    const float* at = pl.w_part + (static_cast<int64_t>(b) * a.nkv + g) * a.S + j;
+    const int64_t step = static_cast<int64_t>(a.B) * a.nkv * a.S;
+    constexpr int kAhead = 8;  // loads on their way
+    for (int p0 = 0; p0 < pl.w_parts; p0 += kAhead) {
+      float v[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int p = p0 + i;
+        v[i] = p < pl.w_parts && last - (last - p) % pl.w_parts >= first ? at[p * step] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) w += v[i];
+    }
   }
   const int64_t at = (slot * a.nkv + g) * a.S + j;
   if (seen || a.w_in != a.w_out) a.w_out[at] = (a.w_in ? a.w_in[at] : 0.0f) + w;
@@ -1381,8 +1421,10 @@ constexpr int64_t kJoinWaves = 8192;
 // than they gain (own keys in one piece need none)
 constexpr int64_t kWidePrefixKeys = 256;
 constexpr int64_t kWideOwnKeys = 512;
-// workgroups for a prompt's weights; a part has at least 256 rows or so
-constexpr int64_t kSumFill = 768;
+// workgroups for a prompt's weights, twice what runs at a time, as those of
+// late keys have few rows (40 us with 768 for 37); a part has at least 256 rows
+// or so
+constexpr int64_t kSumFill = 1536;
 
 struct Layout {
   Plan pl;
