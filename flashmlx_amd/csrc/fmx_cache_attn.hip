@@ -162,9 +162,9 @@ __device__ int find_piece(const CacheAttnArgs& a, const Plan& pl, int w, bool wr
 // as two numbers of the inputs' type, their leading bits and the rest (2^-17
 // or 2^-22 of the weight is lost): only the output is rounded.
 //
-// Bound by HBM: every key and value is read once, past the caches (60.3 us
-// through them for the 59.4 below), 512 bytes (heads of 128) for 16 bytes of partial results per 128
-// keys and row. 16 sequences of up to 16001 keys, 32 heads over 4, fp16,
+// Bound by HBM: every key and value is read once, 512 bytes (heads of 128) for
+// 16 bytes of partial results per 128 keys and row. 16 sequences of up to
+// 16001 keys, 32 heads over 4, fp16,
 // scores stored: 59 us for 271 MB, 4.6 TB/s (4.9 is a large copy's); one row
 // per workgroup and head took 6.6 ms, the same values read for every head and
 // queried one after the other. Short calls are bound by the chain of a
@@ -212,6 +212,12 @@ __device__ inline bool is_top(u16x2_t m) {
   return m[0] == e || m[1] == e;
 }
 
+template <bool PAST, typename T>
+__device__ inline T load(const T* p) {
+  if constexpr (PAST) return __builtin_nontemporal_load(p);
+  return *p;
+}
+
 // the halves of w that are infinite or NaN made 0
 template <bool F16>
 __device__ inline uint32_t word_finite(uint32_t w) {
@@ -233,9 +239,10 @@ __device__ __attribute__((noinline)) void add_left_out(f32x4_t& acc, const uint1
     }
 }
 
-// ANY: hd may be below HD (chunks behind it read as zeros), and the rows of a
-// tile may see different keys (several queries per sequence)
-template <bool F16, int HD, int RT, bool ANY>
+// PAST: loads go past the caches. ANY: hd may be below HD (chunks behind it
+// read as zeros), and the rows of a tile may see different keys (several
+// queries per sequence)
+template <bool F16, int HD, int RT, bool PAST, bool ANY>
 __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& a, const Plan& pl, int n_prefix,
                                                            int block, float* o0, float* o1,
                                                            NarrowLds<RT>& s) {
@@ -342,7 +349,7 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
 #pragma unroll
       for (int t = 0; t < KC; ++t)
         if (!ANY || 32 * t + 8 * j < a.hd)
-          kw[x][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 32 * t));
+          kw[x][t] = load<PAST>(reinterpret_cast<const u32x4_t*>(p + 32 * t));
         else
           kw[x][t] = u32x4_t{0, 0, 0, 0};
     }
@@ -356,7 +363,7 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
                                 : vb + min(kk + row + 4 * j, k1 - 1) * vts + (VPL == 4 ? 4 : 8) * i16;
       if constexpr (VPL == 4) {
         u32x2_t w = {0, 0};
-        if (!ANY || 4 * i16 < a.hd) w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(p));
+        if (!ANY || 4 * i16 < a.hd) w = load<PAST>(reinterpret_cast<const u32x2_t*>(p));
         vw[sl][0] = w[0];
         vw[sl][1] = w[1];
       } else {
@@ -364,7 +371,7 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
         for (int q = 0; q < VPL / 8; ++q) {
           u32x4_t w = {0, 0, 0, 0};
           if (!ANY || 128 * q + 8 * i16 < a.hd)
-            w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 128 * q));
+            w = load<PAST>(reinterpret_cast<const u32x4_t*>(p + 128 * q));
 #pragma unroll
           for (int i = 0; i < 4; ++i) vw[sl][4 * q + i] = w[i];
         }
@@ -540,12 +547,12 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
   }
 }
 
-template <bool F16, int HD, int RT, bool ANY>
+template <bool F16, int HD, int RT, bool PAST, bool ANY>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2)))
 void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
   __shared__ __attribute__((aligned(16))) float s_o[2][16 * RT * HD];
   __shared__ NarrowLds<RT> s;
-  narrow_item<F16, HD, RT, ANY>(a, pl, n_prefix, blockIdx.x, s_o[0], s_o[1], s);
+  narrow_item<F16, HD, RT, PAST, ANY>(a, pl, n_prefix, blockIdx.x, s_o[0], s_o[1], s);
 }
 
 // ------------------------------------------------------------------ wide tiles
@@ -1006,7 +1013,7 @@ void attn_wide_kernel(CacheAttnArgs a, Plan pl, WideGrid pg, WideGrid og, int n_
 // times. With 32 keys per step both fit three times on a CU (narrow tiles of
 // two row sets do not: then 64 keys, twice). 128 sequences behind 32768 shared
 // positions: 90 + 65 us as two grids, 116 us so; 140 us with 64 keys.
-template <bool F16, int HD, int RT, bool ANY>
+template <bool F16, int HD, int RT, bool PAST, bool ANY>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(RT == 1 ? 3 : 2)))
 void attn_both_kernel(CacheAttnArgs a, Plan pl, WideGrid wg, int n_wide, int n_narrow) {
   constexpr int KT = RT == 1 ? 32 : 64;
@@ -1017,7 +1024,7 @@ void attn_both_kernel(CacheAttnArgs a, Plan pl, WideGrid wg, int n_wide, int n_n
     if (static_cast<int>(blockIdx.x) < n_wide) wide_item<F16, HD, KT, ANY>(a, pl, wg, blockIdx.x, s);
   } else {
     if (static_cast<int>(blockIdx.x) - base < n_narrow)
-      narrow_item<F16, HD, RT, ANY>(a, pl, 0, blockIdx.x - base, reinterpret_cast<float*>(s.k0),
+      narrow_item<F16, HD, RT, PAST, ANY>(a, pl, 0, blockIdx.x - base, reinterpret_cast<float*>(s.k0),
                                     reinterpret_cast<float*>(s.k1), *reinterpret_cast<NarrowLds<RT>*>(s.v0));
   }
 }
@@ -1415,6 +1422,10 @@ __global__ __launch_bounds__(kThreads) void attn_weights_sum_kernel(CacheAttnArg
 constexpr int64_t kFill = 768;
 // and of wide tiles: two
 constexpr int64_t kWideFill = 512;
+// Narrow tiles load past the caches where keys and values are more than the
+// 256 MB that the last of them holds: 271 MB 69.9 us a call for 72.5 through
+// them, but 41 MB 25.2 us for 22.4.
+constexpr int64_t kPastBytes = int64_t{256} << 20;
 // rows from which a wave of the join takes one of its own: 32 waves per CU
 constexpr int64_t kJoinWaves = 8192;
 // keys of a wide tile's piece at least: shorter ones cost more in the join
@@ -1515,7 +1526,7 @@ bool wide_grid(const CacheAttnArgs& a, const Plan& pl, bool prefix, WideGrid* wg
   return padded * wg->tiles <= 0x3fffffff;
 }
 
-template <bool F16, int HD, int RT, bool ANY>
+template <bool F16, int HD, int RT, bool PAST, bool ANY>
 hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stream) {
   WideGrid pg{}, og{};
   int np = 0, no = 0;
@@ -1530,7 +1541,7 @@ hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stre
   if (HD <= 128 && pl.p_wide && n > 0) {
     const int groups = (np + 7) / 8 + static_cast<int>((n + 7) / 8);
     if constexpr (HD <= 128)
-      hipLaunchKernelGGL((attn_both_kernel<F16, HD, RT, ANY>), dim3(static_cast<uint32_t>(groups) * 8), wg, 0, stream,
+      hipLaunchKernelGGL((attn_both_kernel<F16, HD, RT, PAST, ANY>), dim3(static_cast<uint32_t>(groups) * 8), wg, 0, stream,
                          a, pl, pg, np, static_cast<int>(n));
     return hipGetLastError();
   }
@@ -1541,7 +1552,7 @@ hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stre
     e = hipGetLastError();
   }
   if (e == hipSuccess && n) {
-    hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, RT, ANY>), dim3(static_cast<uint32_t>(n)), wg, 0, stream, a, pl,
+    hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, RT, PAST, ANY>), dim3(static_cast<uint32_t>(n)), wg, 0, stream, a, pl,
                        static_cast<int>(n_prefix));
     e = hipGetLastError();
   }
@@ -1550,10 +1561,14 @@ hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stre
 
 template <bool F16, int HD, bool ANY>
 hipError_t launch_parts(const CacheAttnArgs& a, const Plan& pl, int rt, hipStream_t stream) {
+  const bool past = (a.P + static_cast<int64_t>(a.B) * a.S) * a.nkv * a.hd * 4 > kPastBytes;
   if constexpr (HD <= 128) {
-    if (rt == 2) return launch_tiles<F16, HD, 2, ANY>(a, pl, stream);
+    if (rt == 2)
+      return past ? launch_tiles<F16, HD, 2, true, ANY>(a, pl, stream)
+                  : launch_tiles<F16, HD, 2, false, ANY>(a, pl, stream);
   }
-  return launch_tiles<F16, HD, 1, ANY>(a, pl, stream);
+  return past ? launch_tiles<F16, HD, 1, true, ANY>(a, pl, stream)
+              : launch_tiles<F16, HD, 1, false, ANY>(a, pl, stream);
 }
 
 template <bool F16, int HD>
