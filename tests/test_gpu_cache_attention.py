@@ -290,6 +290,23 @@ def test_other_stream(gpu, fmx):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("B,L,P,S", [(4, 1, 300, 700), (40, 1, 700, 300), (2, 150, 60, 300)])
+def test_two_streams_at_once(gpu, fmx, B, L, P, S):
+    """Both attentions in flight on two streams over the same inputs."""
+    q, kp, vp, kc, vc, offs = _inputs(torch.bfloat16, B, L, 8, 2, 64, P, S, seed=70)
+    want = fmx.attention_shared_prefix(q, kp, vp, kc, vc, offs, 0.125)
+    want_s = fmx.attention_scored(q, kc, vc, offs, 0.125)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((fmx.attention_shared_prefix(q, kp, vp, kc, vc, offs, 0.125),
+                        fmx.attention_scored(q, kc, vc, offs, 0.125)))
+    torch.cuda.synchronize()
+    for shared, scored in got:
+        assert all(torch.equal(x, y) for x, y in zip(shared + scored, want + want_s))
+
+
 @pytest.mark.parametrize("L", [1, 70])
 def test_offsets_beyond_32_bits(gpu, fmx, L):
     """Slots and positions more than 2^32 elements apart: two heads of one
