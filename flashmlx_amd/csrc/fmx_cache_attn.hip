@@ -1541,8 +1541,8 @@ hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stre
   if (HD <= 128 && pl.p_wide && n > 0) {
     const int groups = (np + 7) / 8 + static_cast<int>((n + 7) / 8);
     if constexpr (HD <= 128)
-      hipLaunchKernelGGL((attn_both_kernel<F16, HD, RT, PAST, ANY>), dim3(static_cast<uint32_t>(groups) * 8), wg, 0, stream,
-                         a, pl, pg, np, static_cast<int>(n));
+      hipLaunchKernelGGL((attn_both_kernel<F16, HD, RT, PAST, ANY>), dim3(static_cast<uint32_t>(groups) * 8), wg, 0,
+                         stream, a, pl, pg, np, static_cast<int>(n));
     return hipGetLastError();
   }
   hipError_t e = hipSuccess;
@@ -1552,8 +1552,8 @@ hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stre
     e = hipGetLastError();
   }
   if (e == hipSuccess && n) {
-    hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, RT, PAST, ANY>), dim3(static_cast<uint32_t>(n)), wg, 0, stream, a, pl,
-                       static_cast<int>(n_prefix));
+    hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, RT, PAST, ANY>), dim3(static_cast<uint32_t>(n)), wg, 0, stream, a,
+                       pl, static_cast<int>(n_prefix));
     e = hipGetLastError();
   }
   return e;
