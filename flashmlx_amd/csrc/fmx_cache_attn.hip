@@ -158,9 +158,9 @@ __device__ int find_piece(const CacheAttnArgs& a, const Plan& pl, int w, bool wr
 // wave), and pairs of keys are put together by v_perm. Nothing passes through
 // LDS and no load is narrower than a cache line's half.
 //
-// The matrix cores have time to spare, so the weights go into the value product
-// as two numbers of the inputs' type, their leading bits and the rest (2^-17
-// or 2^-22 of the weight is lost): only the output is rounded.
+// The weights go into the value product as two numbers of the inputs' type,
+// their leading bits and the rest (2^-16 or 2^-22 of a weight is lost at most):
+// only the output is rounded. The matrix cores have time to spare here.
 //
 // Bound by HBM: every key and value is read once, 512 bytes (heads of 128) for
 // 16 bytes of partial results per 128 keys and row. 16 sequences of up to
@@ -568,22 +568,25 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 // Keys and values come to LDS past the registers, in two buffers: the next
 // positions are on their way while these are multiplied.
 //
-// The weights are rounded to the inputs' type for the value product (2^-9 or
-// 2^-12 of each at most, as random as the values' own rounding; a second
-// product for the rest, as in narrow tiles, would be half of all the work
-// again); their sum is formed before the rounding. The maximum is only raised
-// when a score lies more than kLazy above it: the weights reach 2^kLazy times
-// kBias' 2^8 at most, in fp16 2^14 of 65504.
+// The weights go into the value product as two numbers of the inputs' type, as
+// in narrow tiles, so that a row's precision does not hang on how many rows its
+// call has. That is half of all matrix work again (59 -> 70 us for the prompt
+// below, 115 -> 125 us for 128 sequences behind 32768 positions; the figures
+// given for choices further down are from before), but one number alone, off by
+// up to 2^-8 or 2^-11 of the weight, moves a row with one dominating key by a
+// step of the output. The maximum is only raised when a score lies more than
+// kLazy above it: the weights reach 2^kLazy times kBias' 2^8 at most, in fp16
+// 2^14 of 65504.
 //
-// Bound by a wave's own chain: by the cycle counter a step of 64 keys takes it
-// about 3000 cycles (issuing the next loads 500, scores 900, maximum 300,
-// weights and values 1300, of which the matrix cores work 1000), and a tile
-// some 14000 before its first and after its last step (queries from HBM,
-// outputs). The longest tile of a causal grid alone is two thirds of the
-// kernel's time; keys dealt to two halves of a workgroup, or long and short
-// tiles one after the other, gained nothing. A prompt of 2000 tokens, 32 heads
-// over 4: 59 us, 0.56 PFLOP/s of the causal half (1.4 is a large library
-// product's).
+// Bound by a wave's own chain: by the cycle counter a step of 64 keys took it
+// about 3000 cycles before the second product (issuing the next loads 500,
+// scores 900, maximum 300, weights and values 1300, of which the matrix cores
+// worked 1000), and a tile some 14000 before its first and after its last step
+// (queries from HBM, outputs). The longest tile of a causal grid alone is two
+// thirds of the kernel's time; keys dealt to two halves of a workgroup, or long
+// and short tiles one after the other, gained nothing. A prompt of 2000 tokens,
+// 32 heads over 4: 70 us, 0.47 PFLOP/s of the causal half (1.4 is a large
+// library product's).
 constexpr int kWideRows = 32 * kWaves;
 constexpr int kCus = 256;
 constexpr float kLazy = 6.0f;
@@ -850,16 +853,29 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
     float ls[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      frag_t pf;
+      frag_t ph, pw;  // their leading bits and the rest
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * t + i], sc, -ms));
         ls[i & 1] += p;
         typedef typename std::conditional<F16, _Float16, __bf16>::type half_t;
-        pf[i] = static_cast<half_t>(p);
+        const half_t hi = static_cast<half_t>(p);
+        ph[i] = hi;
+        pw[i] = static_cast<half_t>(p - static_cast<float>(hi));
       }
+      if constexpr (KT == 32) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32(frag(t, dt), pf, o[dt]);
+        for (int dt = 0; dt < DT; ++dt) {
+          const frag_t f = frag(t, dt);
+          o[dt] = mfma32(f, ph, o[dt]);
+          o[dt] = mfma32(f, pw, o[dt]);
+        }
+      } else {  // (no product waits for the one before it)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32(frag(t, dt), ph, o[dt]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32(frag(t, dt), pw, o[dt]);
+      }
     }
     lsum += ls[0] + ls[1];
   };
@@ -909,12 +925,12 @@ __device__ __attribute__((always_inline)) void wide_item(const CacheAttnArgs& a,
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
-        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // vector ones
+        __builtin_amdgcn_sched_group_barrier(0x002, 10, 0);  // vector ones
       }
 #pragma unroll
-      for (int i = 0; i < 2 * DT; ++i) {
+      for (int i = 0; i < 4 * DT; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
       }
       read_v(1);
       asm volatile("" ::: "memory");
