@@ -30,7 +30,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kStep = 32;                // keys of a wave's step
-constexpr int kPiece = kStep * kWaves;   // pieces are whole multiples of these
+constexpr int kPiece = kPieceKeys;
+static_assert(kPiece == kStep * kWaves, "a unit is one step of every wave");
 // up to so many rows of a kv head run in narrow tiles
 constexpr int kNarrowRows = 32;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -103,7 +104,7 @@ struct Plan {
 // Pieces of the own keys, found by every workgroup from the device's lengths:
 // sequence b has u_b = ceil(keys / kPiece) units and ceil(u_b / c) pieces of c
 // units, c the smallest that keeps all pieces within the grid: sum u_b / (grid
-// - B) rounded up. Lengths may differ as they like: all pieces but each
+// - B) rounded up, or all of the longest possible sequence's. Lengths may differ as they like: all pieces but each
 // sequence's last are equally long. Returns the sequence of piece w (-1:
 // none), its piece number in *k and c in *units; workgroup 0 leaves the table.
 struct PieceLds {
@@ -122,7 +123,7 @@ __device__ int find_piece(const CacheAttnArgs& a, const Plan& pl, int w, bool wr
   uint32_t total;
   block_exclusive_scan<kThreads>(mine, s.tmp, &total);
   const uint32_t room = static_cast<uint32_t>(pl.o_grid - a.B);
-  const uint32_t c = max(1u, (total + room - 1) / room);
+  const uint32_t c = max(1u, piece_units(total, room, a.S));
   if (tid == 0) s.seq = -1;
   uint32_t base = 0;
   for (int b0 = 0; b0 < a.B; b0 += kThreads) {
@@ -284,8 +285,8 @@ __device__ __attribute__((always_inline)) void narrow_item(const CacheAttnArgs& 
     seq = __builtin_amdgcn_readfirstlane(seq);
     slot = seq_slot(a.slots, a.n_slots, seq);
     off = a.offs[seq];
-    k0 = __builtin_amdgcn_readfirstlane(k * units * kPiece);
-    k1 = static_cast<int>(min(own_keys(a, slot, off, a.L - 1), static_cast<int64_t>(k0) + units * kPiece));
+    piece_keys(k, units, own_keys(a, slot, off, a.L - 1), &k0, &k1);
+    k0 = __builtin_amdgcn_readfirstlane(k0);
     k1 = __builtin_amdgcn_readfirstlane(k1);
     kb = static_cast<const uint16_t*>(a.kc.p) + slot * a.kc.bs + g * a.kc.hs;
     vb = static_cast<const uint16_t*>(a.vc.p) + slot * a.vc.bs + g * a.vc.hs;

@@ -66,6 +66,25 @@ __device__ inline int64_t own_keys(const CacheAttnArgs& a, int64_t slot, int off
   return n < 0 ? 0 : (n > a.S ? a.S : n);
 }
 
+// Own keys in pieces of whole units of kPieceKeys keys.
+constexpr int kPieceKeys = 128;
+
+// Units of a piece, the fewest that keep `total` units of all sequences within
+// `room` pieces beside one per sequence: never more than a sequence of max_seq
+// positions has, so that a piece's keys count within 32 bits.
+__host__ __device__ inline uint32_t piece_units(uint32_t total, uint32_t room, int64_t max_seq) {
+  const uint32_t c = total / room + (total % room != 0);
+  const uint32_t most = static_cast<uint32_t>((max_seq + kPieceKeys - 1) / kPieceKeys);
+  return c < most ? c : most;
+}
+
+// Keys [k0, k1) of piece k of a sequence of n keys.
+__host__ __device__ inline void piece_keys(int k, int units, int64_t n, int* k0, int* k1) {
+  *k0 = k * units * kPieceKeys;
+  const int64_t end = *k0 + static_cast<int64_t>(units) * kPieceKeys;
+  *k1 = static_cast<int>(n < end ? n : end);
+}
+
 // ------------------------------------------------------------------ eviction
 
 struct EvictArgs {
