@@ -354,7 +354,7 @@ int fmx_rope_append(const fmx_rope_angles* angles, int dtype, int64_t batch, int
 
 size_t fmx_attention_shared_prefix_workspace_size(const fmx_attention_shape* shape, int64_t prefix_len,
                                                   int64_t max_seq) {
-  if (check_attention(shape, prefix_len, max_seq) != FMX_OK) return 0;
+  if (check_attention(shape, prefix_len, max_seq) != FMX_OK || shape->batch * shape->seq_len == 0) return 0;
   return cache_attn_workspace(attention_args(shape, prefix_len, max_seq, false));
 }
 
@@ -402,7 +402,7 @@ int fmx_attention_shared_prefix(const fmx_attention_shape* shape, const fmx_head
 }
 
 size_t fmx_attention_scored_workspace_size(const fmx_attention_shape* shape, int64_t max_seq) {
-  if (check_attention(shape, 0, max_seq) != FMX_OK) return 0;
+  if (check_attention(shape, 0, max_seq) != FMX_OK || shape->batch * shape->seq_len == 0) return 0;
   return cache_attn_workspace(attention_args(shape, 0, max_seq, true));
 }
 

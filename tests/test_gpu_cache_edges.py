@@ -1,0 +1,40 @@
+"""The cache's long-context operators at the edges of their range: empty
+batches, loads past the caches, eviction without the kept positions."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _randn(shape, dt, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda", dtype=torch.float32).to(dt)
+
+
+@pytest.mark.parametrize("B,L", [(0, 1), (0, 40), (3, 0), (0, 0)])
+@pytest.mark.parametrize("P,S", [(0, 9), (20, 9), (20, 0)])
+def test_empty_batches(gpu, fmx, B, L, P, S):
+    """No sequences, or no new tokens: empty results, caches and weights as they were."""
+    nh, nkv, hd, n, dt = 8, 2, 64, 3, torch.bfloat16
+    q, k = _randn((B, L, nh, hd), dt, 1), _randn((B, L, nkv, hd), dt, 2)
+    kc, vc = _randn((n, nkv, S, hd), dt, 3), _randn((n, nkv, S, hd), dt, 4)
+    kp = vp = _randn((nkv, P, hd), dt, 5) if P else None
+    offs = torch.zeros(B, dtype=torch.int32, device="cuda")
+    pos = torch.zeros((B, L), dtype=torch.int32, device="cuda")
+    out, lse = fmx.attention_shared_prefix(q, kp, vp, kc, vc, offs, 0.1)
+    assert out.shape == q.shape and lse.shape == (B, L, nh)
+    rope = fmx.Rope(fmx.RopeConfig(dims=hd))
+    assert rope(q, pos).shape == q.shape
+    if S:
+        before = kc.clone(), vc.clone()
+        assert rope.append(q, k, k, pos, offs, kc, vc).shape == q.shape
+        w = _randn((n, nkv, S), torch.float32, 6)
+        out, w_out = fmx.attention_scored(q, kc, vc, offs, 0.1, weights=w)
+        assert out.shape == q.shape and torch.equal(w_out, w)
+        assert bool((fmx.attention_scored(q, kc, vc, offs, 0.1)[1] == 0).all())
+        if B == 0:
+            lengths, kept = fmx.cache_evict(kc, vc, w, offs, 4)
+            assert lengths.shape == (0,) and kept.shape == (0, nkv, 4)
+        assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
