@@ -415,14 +415,7 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
   if (max_seq < 1) return fail(FMX_ERR_SHAPE, "max_seq below 1");
   CacheAttnArgs a = attention_args(shape, 0, max_seq, true);
   if (!slots && n_slots < shape->batch) return fail(FMX_ERR_SHAPE, "n_slots below batch without slots");
-  if (shape->batch * shape->seq_len == 0) return ok();
-  fmx_heads q_v, out_v, kc_v, vc_v;
-  FMX_RC(check_view(q, "q", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &q_v));
-  FMX_RC(check_view(out, "out", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &out_v));
-  FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &kc_v));
-  FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &vc_v));
-  FMX_RC(check_key_stride(kc_v, vc_v, "caches"));
-  if (!offsets || !weights_out) return fail(FMX_ERR_ARG, "NULL offsets or weights_out");
+  if (shape->batch == 0) return ok();
   if (!aligned(weights_in, 4) || !aligned(weights_out, 4)) return fail(FMX_ERR_ARG, "weights not 4-byte aligned");
   if (weights_in && weights_in != weights_out) {
     const uintptr_t n = static_cast<uintptr_t>(n_slots) * static_cast<uintptr_t>(a.nkv) *
@@ -431,15 +424,26 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
     if (overlap({i, i + n}, {o, o + n})) return fail(FMX_ERR_ARG, "weights_out overlaps weights_in in part");
   }
   hipStream_t stream = static_cast<hipStream_t>(stream_);
+  a.slots = slots;
+  a.n_slots = n_slots;
+  a.w_in = weights_in;
+  a.w_out = weights_out;
+  if (shape->seq_len == 0) {  // no weights to add
+    if (weights_out && weights_out != weights_in) FMX_HIP(launch_cache_weights_kept(a, stream));
+    return ok();
+  }
+  fmx_heads q_v, out_v, kc_v, vc_v;
+  FMX_RC(check_view(q, "q", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &q_v));
+  FMX_RC(check_view(out, "out", shape->batch, shape->seq_len, shape->n_heads, 16, 8, &out_v));
+  FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &kc_v));
+  FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, shape->n_kv_heads, 16, 8, &vc_v));
+  FMX_RC(check_key_stride(kc_v, vc_v, "caches"));
+  if (!offsets || !weights_out) return fail(FMX_ERR_ARG, "NULL offsets or weights_out");
   a.q = view(&q_v);
   a.out = view(&out_v);
   a.kc = view(&kc_v);
   a.vc = view(&vc_v);
   a.offs = offsets;
-  a.slots = slots;
-  a.n_slots = n_slots;
-  a.w_in = weights_in;
-  a.w_out = weights_out;
   FMX_RC(check_out(a, n_slots));
   Workspace ws;
   FMX_RC(ws.bind(workspace, workspace_bytes, cache_attn_workspace(a), stream));

@@ -1407,9 +1407,9 @@ __global__ __launch_bounds__(kThreads) void attn_weights_sum_kernel(CacheAttnArg
   const int bg = blockIdx.x / tiles, b = bg / a.nkv, g = bg % a.nkv;
   const int64_t slot = seq_slot(a.slots, a.n_slots, b);
   if (slot < 0 || j >= a.S) return;
-  const int off = a.offs[b];
   float w = 0.0f;
-  const bool seen = j < own_keys(a, slot, off, a.L - 1);
+  const int off = a.L > 0 ? a.offs[b] : 0;
+  const bool seen = a.L > 0 && j < own_keys(a, slot, off, a.L - 1);
   if (seen) {
     // the parts with a block from the first row on that sees the tile's first
     // key have left a sum
@@ -1661,6 +1661,14 @@ hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
 }  // namespace
 
 size_t cache_attn_workspace(const CacheAttnArgs& a) { return make_plan(a, nullptr).bytes; }
+
+hipError_t launch_cache_weights_kept(const CacheAttnArgs& a, hipStream_t stream) {
+  const int64_t tiles = (a.S + kThreads - 1) / kThreads, grid = tiles * a.nkv * a.B;
+  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(attn_weights_sum_kernel, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a, Plan{},
+                     static_cast<int>(tiles));
+  return hipGetLastError();
+}
 
 hipError_t launch_cache_attn(const CacheAttnArgs& a, bool f16, void* ws, hipStream_t stream) {
   return f16 ? launch<true>(a, ws, stream) : launch<false>(a, ws, stream);

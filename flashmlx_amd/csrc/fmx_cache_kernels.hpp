@@ -58,6 +58,8 @@ struct CacheAttnArgs {
 };
 size_t cache_attn_workspace(const CacheAttnArgs& a);
 hipError_t launch_cache_attn(const CacheAttnArgs& a, bool f16, void* ws, hipStream_t stream);
+// no queries (L 0): w_out's rows of the sequences' slots from w_in, or 0
+hipError_t launch_cache_weights_kept(const CacheAttnArgs& a, hipStream_t stream);
 
 // own keys that query l of sequence b sees (slot: of that sequence, or -1)
 __device__ inline int64_t own_keys(const CacheAttnArgs& a, int64_t slot, int off, int l) {

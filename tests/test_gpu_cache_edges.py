@@ -38,3 +38,22 @@ def test_empty_batches(gpu, fmx, B, L, P, S):
             lengths, kept = fmx.cache_evict(kc, vc, w, offs, 4)
             assert lengths.shape == (0,) and kept.shape == (0, nkv, 4)
         assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+
+
+@pytest.mark.parametrize("S", [1, 300])
+@pytest.mark.parametrize("given", [False, True])
+def test_no_queries_keep_the_weights(gpu, fmx, given, S):
+    """seq_len 0 adds an empty sum: a weights array of its own gets what was
+    there (or 0) in the sequences' slots, and only there."""
+    n, nkv, hd, dt = 4, 2, 64, torch.bfloat16
+    q = torch.empty((3, 0, 8, hd), dtype=dt, device="cuda")
+    kc, vc = _randn((n, nkv, S, hd), dt, 1), _randn((n, nkv, S, hd), dt, 2)
+    w, w_out = _randn((n, nkv, S), torch.float32, 3), _randn((n, nkv, S), torch.float32, 4)
+    slots = torch.tensor([2, -1, 0], dtype=torch.int32, device="cuda")
+    offs = torch.full((3,), 5, dtype=torch.int32, device="cuda")
+    want = w_out.clone()
+    want[[2, 0]] = w[[2, 0]] if given else 0.0
+    _, got = fmx.attention_scored(q, kc, vc, offs, 0.1, weights=w if given else None, weights_out=w_out, slots=slots)
+    assert got is w_out and torch.equal(w_out, want)
+    fmx.attention_scored(q, kc, vc, offs, 0.1, weights=w_out, weights_out=w_out, slots=slots)
+    assert torch.equal(w_out, want)
