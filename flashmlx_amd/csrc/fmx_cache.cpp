@@ -77,6 +77,8 @@ constexpr int64_t kMaxHeads = 65535;
 constexpr int64_t kMaxStride = int64_t{1} << 34;
 // of the positions that attention reads: 64 rows' byte offsets within 32 bits
 constexpr int64_t kMaxKeyStride = int64_t{1} << 24;
+// (sequence, kv head) pairs of an eviction: a workgroup of 1024 threads each
+constexpr int64_t kMaxEvictRows = int64_t{1} << 22;
 
 int check_counts(int64_t batch, int64_t seq_len, int64_t n_heads, int64_t n_kv_heads) {
   if (batch < 0 || seq_len < 0 || batch > kMaxRows || seq_len > kMaxRows || batch * seq_len > kMaxRows)
@@ -178,6 +180,10 @@ int check_out(const CacheAttnArgs& a, int64_t n_slots) {
                         at(a.kc, n_slots, a.S, a.nkv), at(a.vc, n_slots, a.S, a.nkv)})
     if (overlap(out, i)) return fail(FMX_ERR_ARG, "out overlaps q, the prefix or a cache");
   return FMX_OK;
+}
+
+int check_launches(const CacheAttnArgs& a) {
+  return cache_attn_fits(a) ? FMX_OK : fail(FMX_ERR_UNSUPPORTED, "more work than launches of fewer than 2^32 threads");
 }
 
 CacheAttnArgs attention_args(const fmx_attention_shape* s, int64_t prefix_len, int64_t max_seq, bool weights) {
@@ -395,6 +401,7 @@ int fmx_attention_shared_prefix(const fmx_attention_shape* shape, const fmx_head
   a.out = view(&out_v);
   a.lse = lse;
   FMX_RC(check_out(a, n_slots));
+  FMX_RC(check_launches(a));
   Workspace ws;
   FMX_RC(ws.bind(workspace, workspace_bytes, cache_attn_workspace(a), stream));
   FMX_HIP(launch_cache_attn(a, shape->dtype == FMX_F16, ws.p, stream));
@@ -445,6 +452,7 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
   a.vc = view(&vc_v);
   a.offs = offsets;
   FMX_RC(check_out(a, n_slots));
+  FMX_RC(check_launches(a));
   Workspace ws;
   FMX_RC(ws.bind(workspace, workspace_bytes, cache_attn_workspace(a), stream));
   FMX_HIP(launch_cache_attn(a, shape->dtype == FMX_F16, ws.p, stream));
@@ -453,7 +461,7 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
 
 size_t fmx_cache_evict_workspace_size(int64_t batch, int64_t n_kv_heads, int64_t budget) {
   if (batch < 0 || batch > kMaxRows || n_kv_heads < 1 || n_kv_heads > kMaxHeads || budget < 1 || budget > kMaxRows ||
-      batch * n_kv_heads > (int64_t{1} << 30))
+      batch * n_kv_heads >= kMaxEvictRows)
     return 0;
   return static_cast<size_t>(align_up(batch * n_kv_heads * budget * 4, 256));
 }
@@ -466,7 +474,7 @@ int fmx_cache_evict(int dtype, int64_t batch, int64_t n_kv_heads, int64_t head_d
                     fmx_stream stream_) {
   if (dtype != FMX_BF16 && dtype != FMX_F16) return fail(FMX_ERR_DTYPE, "dtype %d (bf16 or float16)", dtype);
   FMX_RC(check_counts(batch, 1, 1, n_kv_heads));
-  if (batch * n_kv_heads > (int64_t{1} << 30)) return fail(FMX_ERR_UNSUPPORTED, "more than 2^30 rows of weights");
+  if (batch * n_kv_heads >= kMaxEvictRows) return fail(FMX_ERR_UNSUPPORTED, "2^22 rows of weights or more");
   FMX_RC(check_pool(n_slots, max_seq));
   if (max_seq < 1) return fail(FMX_ERR_SHAPE, "max_seq below 1");
   if (head_dim < 1 || head_dim > kRopeMaxHd)
@@ -540,6 +548,7 @@ int fmx_cache_evict(int dtype, int64_t batch, int64_t n_kv_heads, int64_t head_d
   a.recent = recent;
   a.lens_out = lengths_out;
   a.in_place = in_place;
+  if (!evict_fits(a)) return fail(FMX_ERR_UNSUPPORTED, "more rows than launches of fewer than 2^32 threads move");
   Workspace ws;
   if (!kept) {
     FMX_RC(ws.bind(workspace, workspace_bytes, fmx_cache_evict_workspace_size(batch, n_kv_heads, budget), stream));

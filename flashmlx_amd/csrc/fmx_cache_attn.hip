@@ -1531,7 +1531,8 @@ Layout make_plan(const CacheAttnArgs& a, char* ws) {
   return y;
 }
 
-bool wide_grid(const CacheAttnArgs& a, const Plan& pl, bool prefix, WideGrid* wg, int* blocks) {
+// blocks of a launch over wide tiles
+int64_t wide_grid(const CacheAttnArgs& a, const Plan& pl, bool prefix, WideGrid* wg) {
   wg->prefix = prefix;
   wg->splits = prefix ? pl.p_splits : pl.o_splits;
   wg->tiles = prefix ? pl.p_tiles : pl.o_tiles;
@@ -1539,86 +1540,105 @@ bool wide_grid(const CacheAttnArgs& a, const Plan& pl, bool prefix, WideGrid* wg
   const int64_t padded = pairs <= 8 ? pairs : align_up(pairs, 8);
   wg->pairs = static_cast<int>(pairs);
   wg->padded = static_cast<int>(padded);
-  *blocks = static_cast<int>(padded * wg->tiles);
-  return padded * wg->tiles <= 0x3fffffff;
+  return padded * wg->tiles;
+}
+
+// A call's launches, in blocks of kThreads.
+struct Grids {
+  WideGrid pg, og;           // over wide tiles of the prefix and of own keys,
+  int64_t p_wide, o_wide;    // their blocks,
+  int64_t p_narrow, narrow;  // those over narrow tiles of the prefix, and of both
+  bool per_wave;             // the join: rows, then weights from stored scores
+  int64_t join, w_tiles, join_all;
+  int64_t w_pairs, w_padded, w_grid, w_sum_tiles, w_sum;  // weights of many rows
+  bool fits;
+};
+
+Grids make_grids(const CacheAttnArgs& a, const Plan& pl) {
+  Grids gr{};
+  if (pl.p_wide) gr.p_wide = wide_grid(a, pl, true, &gr.pg);
+  if (pl.o_wide) gr.o_wide = wide_grid(a, pl, false, &gr.og);
+  gr.p_narrow = pl.p_wide ? 0 : static_cast<int64_t>(pl.p_splits) * a.nkv * pl.p_tiles;
+  gr.narrow = gr.p_narrow + (pl.o_wide ? 0 : static_cast<int64_t>(pl.o_grid) * a.nkv * pl.o_tiles);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.L * a.nh, bg = static_cast<int64_t>(a.B) * a.nkv;
+  gr.per_wave = rows > kJoinWaves;
+  gr.join = pl.direct ? 0 : gr.per_wave ? (rows + kWaves - 1) / kWaves : rows;
+  gr.w_tiles = a.w_out && !pl.o_wide ? (a.S + kWeightKeys - 1) / kWeightKeys : 0;
+  gr.join_all = gr.join + gr.w_tiles * bg;
+  if (a.w_out && pl.o_wide) {
+    gr.w_pairs = pl.w_parts * bg;
+    gr.w_padded = gr.w_pairs <= 8 ? gr.w_pairs : align_up(gr.w_pairs, 8);
+    gr.w_grid = (a.S + kSumKeys - 1) / kSumKeys * gr.w_padded;
+    gr.w_sum_tiles = (a.S + kThreads - 1) / kThreads;
+    gr.w_sum = gr.w_sum_tiles * bg;
+  }
+  // (wide and narrow ones may share a launch)
+  const int64_t most = max_blocks(kThreads);
+  gr.fits = gr.p_wide + gr.o_wide + gr.narrow + 16 <= most && gr.join_all <= most && gr.w_grid <= most && gr.w_sum <= most;
+  return gr;
 }
 
 template <bool F16, int HD, int RT, bool PAST, bool ANY>
-hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, hipStream_t stream) {
-  WideGrid pg{}, og{};
-  int np = 0, no = 0;
-  if (pl.p_wide && !wide_grid(a, pl, true, &pg, &np)) return hipErrorInvalidValue;
-  if (pl.o_wide && !wide_grid(a, pl, false, &og, &no)) return hipErrorInvalidValue;
-  const int64_t n_prefix = pl.p_wide ? 0 : static_cast<int64_t>(pl.p_splits) * a.nkv * pl.p_tiles;
-  const int64_t n = n_prefix + (pl.o_wide ? 0 : static_cast<int64_t>(pl.o_grid) * a.nkv * pl.o_tiles);
-  if (n > 0x3fffffff) return hipErrorInvalidValue;
+hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, const Grids& gr, hipStream_t stream) {
+  const int np = static_cast<int>(gr.p_wide), no = static_cast<int>(gr.o_wide), n = static_cast<int>(gr.narrow);
   const dim3 wg(kThreads);
   // (heads beyond 128: a wide workgroup fills a CU's LDS, and so would narrow
   // ones in its grid)
   if (HD <= 128 && pl.p_wide && n > 0) {
-    const int groups = (np + 7) / 8 + static_cast<int>((n + 7) / 8);
+    const int groups = (np + 7) / 8 + (n + 7) / 8;
     if constexpr (HD <= 128)
       hipLaunchKernelGGL((attn_both_kernel<F16, HD, RT, PAST, ANY>), dim3(static_cast<uint32_t>(groups) * 8), wg, 0,
-                         stream, a, pl, pg, np, static_cast<int>(n));
+                         stream, a, pl, gr.pg, np, n);
     return hipGetLastError();
   }
   hipError_t e = hipSuccess;
   if (np + no) {
     const int first = static_cast<int>(align_up(np, 8));  // (own blocks start on the first XCD)
-    hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(first + no), wg, 0, stream, a, pl, pg, og, first);
+    hipLaunchKernelGGL((attn_wide_kernel<F16, HD, ANY>), dim3(first + no), wg, 0, stream, a, pl, gr.pg, gr.og, first);
     e = hipGetLastError();
   }
   if (e == hipSuccess && n) {
     hipLaunchKernelGGL((attn_narrow_kernel<F16, HD, RT, PAST, ANY>), dim3(static_cast<uint32_t>(n)), wg, 0, stream, a,
-                       pl, static_cast<int>(n_prefix));
+                       pl, static_cast<int>(gr.p_narrow));
     e = hipGetLastError();
   }
   return e;
 }
 
 template <bool F16, int HD, bool ANY>
-hipError_t launch_parts(const CacheAttnArgs& a, const Plan& pl, int rt, hipStream_t stream) {
+hipError_t launch_parts(const CacheAttnArgs& a, const Plan& pl, const Grids& gr, int rt, hipStream_t stream) {
   const bool past = (a.P + static_cast<int64_t>(a.B) * a.S) * a.nkv * a.hd * 4 > kPastBytes;
   if constexpr (HD <= 128) {
     if (rt == 2)
-      return past ? launch_tiles<F16, HD, 2, true, ANY>(a, pl, stream)
-                  : launch_tiles<F16, HD, 2, false, ANY>(a, pl, stream);
+      return past ? launch_tiles<F16, HD, 2, true, ANY>(a, pl, gr, stream)
+                  : launch_tiles<F16, HD, 2, false, ANY>(a, pl, gr, stream);
   }
-  return past ? launch_tiles<F16, HD, 1, true, ANY>(a, pl, stream)
-              : launch_tiles<F16, HD, 1, false, ANY>(a, pl, stream);
+  return past ? launch_tiles<F16, HD, 1, true, ANY>(a, pl, gr, stream)
+              : launch_tiles<F16, HD, 1, false, ANY>(a, pl, gr, stream);
 }
 
 template <bool F16, int HD>
-void launch_weight_parts(const CacheAttnArgs& a, const Plan& pl, uint32_t grid, int pairs, int padded,
-                         hipStream_t stream) {
+void launch_weight_parts(const CacheAttnArgs& a, const Plan& pl, const Grids& gr, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(gr.w_grid)), wg(kThreads);
+  const int pairs = static_cast<int>(gr.w_pairs), padded = static_cast<int>(gr.w_padded);
   if (a.hd == HD)
-    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, false>), dim3(grid), dim3(kThreads), 0, stream, a, pl, pairs,
-                       padded);
+    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, false>), grid, wg, 0, stream, a, pl, pairs, padded);
   else
-    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, true>), dim3(grid), dim3(kThreads), 0, stream, a, pl, pairs,
-                       padded);
+    hipLaunchKernelGGL((attn_weights_kernel<F16, HD, true>), grid, wg, 0, stream, a, pl, pairs, padded);
 }
 
 template <bool F16>
-hipError_t launch_weights(const CacheAttnArgs& a, const Plan& pl, hipStream_t stream) {
-  const int64_t tiles = (a.S + kSumKeys - 1) / kSumKeys;
-  const int64_t pairs = static_cast<int64_t>(pl.w_parts) * a.nkv * a.B;
-  const int64_t padded = pairs <= 8 ? pairs : align_up(pairs, 8);
-  const int64_t grid = tiles * padded;
-  const int64_t sum_tiles = (a.S + kThreads - 1) / kThreads;
-  if (grid > 0x7fffffff || sum_tiles * a.nkv * a.B > 0x7fffffff) return hipErrorInvalidValue;
-  const uint32_t n = static_cast<uint32_t>(grid);
-  const int np = static_cast<int>(pairs), npad = static_cast<int>(padded);
+hipError_t launch_weights(const CacheAttnArgs& a, const Plan& pl, const Grids& gr, hipStream_t stream) {
   if (a.hd <= 64)
-    launch_weight_parts<F16, 64>(a, pl, n, np, npad, stream);
+    launch_weight_parts<F16, 64>(a, pl, gr, stream);
   else if (a.hd <= 128)
-    launch_weight_parts<F16, 128>(a, pl, n, np, npad, stream);
+    launch_weight_parts<F16, 128>(a, pl, gr, stream);
   else
-    launch_weight_parts<F16, 256>(a, pl, n, np, npad, stream);
+    launch_weight_parts<F16, 256>(a, pl, gr, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(attn_weights_sum_kernel, dim3(static_cast<uint32_t>(sum_tiles * a.nkv * a.B)), dim3(kThreads), 0,
-                     stream, a, pl, static_cast<int>(sum_tiles));
+  hipLaunchKernelGGL(attn_weights_sum_kernel, dim3(static_cast<uint32_t>(gr.w_sum)), dim3(kThreads), 0, stream, a, pl,
+                     static_cast<int>(gr.w_sum_tiles));
   return hipGetLastError();
 }
 
@@ -1626,35 +1646,29 @@ template <bool F16>
 hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
   const Layout y = make_plan(a, static_cast<char*>(ws));
   const Plan& pl = y.pl;
+  const Grids gr = make_grids(a, pl);
   hipError_t e;
   const bool any = a.L > 1;
   if (a.hd <= 64)
-    e = a.hd == 64 && !any ? launch_parts<F16, 64, false>(a, pl, y.rt, stream)
-                           : launch_parts<F16, 64, true>(a, pl, y.rt, stream);
+    e = a.hd == 64 && !any ? launch_parts<F16, 64, false>(a, pl, gr, y.rt, stream)
+                           : launch_parts<F16, 64, true>(a, pl, gr, y.rt, stream);
   else if (a.hd <= 128)
-    e = a.hd == 128 && !any ? launch_parts<F16, 128, false>(a, pl, y.rt, stream)
-                            : launch_parts<F16, 128, true>(a, pl, y.rt, stream);
+    e = a.hd == 128 && !any ? launch_parts<F16, 128, false>(a, pl, gr, y.rt, stream)
+                            : launch_parts<F16, 128, true>(a, pl, gr, y.rt, stream);
   else
-    e = a.hd == 256 && !any ? launch_parts<F16, 256, false>(a, pl, y.rt, stream)
-                            : launch_parts<F16, 256, true>(a, pl, y.rt, stream);
+    e = a.hd == 256 && !any ? launch_parts<F16, 256, false>(a, pl, gr, y.rt, stream)
+                            : launch_parts<F16, 256, true>(a, pl, gr, y.rt, stream);
   if (e != hipSuccess) return e;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.L * a.nh;
-  const bool per_wave = rows > kJoinWaves;
-  const int64_t n_join = pl.direct ? 0 : per_wave ? (rows + kWaves - 1) / kWaves : rows;
-  const int64_t w_tiles = pl.scores ? (a.S + kWeightKeys - 1) / kWeightKeys : 0;
-  const int64_t grid = n_join + w_tiles * a.nkv * a.B;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  if (grid > 0) {
-    const dim3 gr(static_cast<uint32_t>(grid)), wg(kThreads);
-    if (per_wave)
-      hipLaunchKernelGGL((attn_join_kernel<F16, true>), gr, wg, 0, stream, a, pl, static_cast<int>(n_join),
-                         static_cast<int>(w_tiles));
+  if (gr.join_all > 0) {
+    const dim3 grid(static_cast<uint32_t>(gr.join_all)), wg(kThreads);
+    const int join = static_cast<int>(gr.join), w_tiles = static_cast<int>(gr.w_tiles);
+    if (gr.per_wave)
+      hipLaunchKernelGGL((attn_join_kernel<F16, true>), grid, wg, 0, stream, a, pl, join, w_tiles);
     else
-      hipLaunchKernelGGL((attn_join_kernel<F16, false>), gr, wg, 0, stream, a, pl, static_cast<int>(n_join),
-                         static_cast<int>(w_tiles));
+      hipLaunchKernelGGL((attn_join_kernel<F16, false>), grid, wg, 0, stream, a, pl, join, w_tiles);
     e = hipGetLastError();
   }
-  if (e == hipSuccess && a.w_out && !pl.scores) e = launch_weights<F16>(a, pl, stream);
+  if (e == hipSuccess && a.w_out && pl.o_wide) e = launch_weights<F16>(a, pl, gr, stream);
   return e;
 }
 
@@ -1662,9 +1676,11 @@ hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
 
 size_t cache_attn_workspace(const CacheAttnArgs& a) { return make_plan(a, nullptr).bytes; }
 
+bool cache_attn_fits(const CacheAttnArgs& a) { return make_grids(a, make_plan(a, nullptr).pl).fits; }
+
 hipError_t launch_cache_weights_kept(const CacheAttnArgs& a, hipStream_t stream) {
   const int64_t tiles = (a.S + kThreads - 1) / kThreads, grid = tiles * a.nkv * a.B;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
+  if (grid > max_blocks(kThreads)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(attn_weights_sum_kernel, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a, Plan{},
                      static_cast<int>(tiles));
   return hipGetLastError();

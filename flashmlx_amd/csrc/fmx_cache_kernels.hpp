@@ -7,6 +7,9 @@
 
 namespace fmx {
 
+// workgroups of a launch: HIP takes fewer than 2^32 threads
+constexpr int64_t max_blocks(int threads) { return ((int64_t{1} << 32) - 1) / threads; }
+
 // strided rows of heads, as fmx_heads
 struct HeadsView {
   void* p;
@@ -57,6 +60,8 @@ struct CacheAttnArgs {
   float* w_out;           // or null: no weights
 };
 size_t cache_attn_workspace(const CacheAttnArgs& a);
+// whether all of its launches are within max_blocks
+bool cache_attn_fits(const CacheAttnArgs& a);
 hipError_t launch_cache_attn(const CacheAttnArgs& a, bool f16, void* ws, hipStream_t stream);
 // no queries (L 0): w_out's rows of the sequences' slots from w_in, or 0
 hipError_t launch_cache_weights_kept(const CacheAttnArgs& a, hipStream_t stream);
@@ -108,6 +113,8 @@ struct EvictArgs {
   int32_t* kept;          // [B, nkv, budget]
   bool in_place;
 };
+// whether both of its launches are within max_blocks
+bool evict_fits(const EvictArgs& a);
 hipError_t launch_evict(const EvictArgs& a, hipStream_t stream);
 
 }  // namespace fmx

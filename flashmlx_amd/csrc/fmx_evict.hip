@@ -358,40 +358,16 @@ __global__ __launch_bounds__(kMoveThreads) void evict_shift_kernel(EvictArgs a, 
   }
 }
 
-template <int VB>
-hipError_t move_rows(const EvictArgs& a, hipStream_t stream) {
-  const int64_t heads = static_cast<int64_t>(a.B) * a.nkv;
-  const int per = static_cast<int>(a.row_bytes / VB);
-  const dim3 wg(kMoveThreads);
-  if (a.in_place) {
-    // slices of a row, each at least 64 bytes, until 512 workgroups are busy
-    int slices = 1;
-    while (slices * 2 * 64 <= a.row_bytes && heads * 2 * slices < 512 && per % (slices * 2) == 0) slices *= 2;
-    // (and no longer than a block of threads)
-    while ((per + slices - 1) / slices > kMoveThreads) ++slices;
-    const int units = (per + slices - 1) / slices;
-    slices = (per + units - 1) / units;
-    const int64_t n = heads * 2 * slices;
-    if (n > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(evict_shift_kernel<VB>, dim3(static_cast<uint32_t>(n)), wg, 0, stream, a, slices, units);
-    return hipGetLastError();
-  }
-  // rows of a workgroup: about two rounds of its threads
-  const int rows = std::max(1, 2 * kMoveThreads * kMoveUnits / per);
-  const int64_t chunks = (a.budget + rows - 1) / rows;
-  if (chunks * heads > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(evict_move_kernel<VB>, dim3(static_cast<uint32_t>(chunks * heads)), wg, 0, stream, a,
-                     static_cast<int>(chunks), rows);
-  return hipGetLastError();
-}
+// the second launch
+struct MoveGrid {
+  int vb;             // bytes of a unit
+  int slices, units;  // in place: slices of a row, units of a slice
+  int64_t chunks;     // else: chunks of `rows` kept positions per (sequence, kv head)
+  int rows;
+  int64_t blocks;
+};
 
-}  // namespace
-
-hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
-  const uint32_t heads = static_cast<uint32_t>(a.B) * static_cast<uint32_t>(a.nkv);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(heads), dim3(kSelThreads), 0, stream, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
+MoveGrid move_grid(const EvictArgs& a) {
   int64_t all = a.row_bytes;
   for (int64_t s : {a.k_bs, a.k_ts, a.k_hs, a.v_bs, a.v_ts, a.v_hs,
                     a.ko_bs, a.ko_ts, a.ko_hs, a.vo_bs, a.vo_ts, a.vo_hs})
@@ -399,7 +375,51 @@ hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
   for (const void* p : {static_cast<const void*>(a.k), static_cast<const void*>(a.v),
                         static_cast<const void*>(a.k_out), static_cast<const void*>(a.v_out)})
     all |= static_cast<int64_t>(reinterpret_cast<uintptr_t>(p) & 15);
-  return all % 16 == 0 ? move_rows<16>(a, stream) : move_rows<2>(a, stream);
+  MoveGrid m{};
+  m.vb = all % 16 == 0 ? 16 : 2;
+  const int64_t heads = static_cast<int64_t>(a.B) * a.nkv;
+  const int per = static_cast<int>(a.row_bytes / m.vb);
+  if (a.in_place) {
+    // slices of a row, each at least 64 bytes, until 512 workgroups are busy
+    int slices = 1;
+    while (slices * 2 * 64 <= a.row_bytes && heads * 2 * slices < 512 && per % (slices * 2) == 0) slices *= 2;
+    // (and no longer than a block of threads)
+    while ((per + slices - 1) / slices > kMoveThreads) ++slices;
+    m.units = (per + slices - 1) / slices;
+    m.slices = (per + m.units - 1) / m.units;
+    m.blocks = heads * 2 * m.slices;
+  } else {
+    // rows of a workgroup: about two rounds of its threads
+    m.rows = std::max(1, 2 * kMoveThreads * kMoveUnits / per);
+    m.chunks = (std::min(a.budget, a.S) + m.rows - 1) / m.rows;
+    m.blocks = m.chunks * heads;
+  }
+  return m;
+}
+
+template <int VB>
+hipError_t move_rows(const EvictArgs& a, const MoveGrid& m, hipStream_t stream) {
+  const dim3 gr(static_cast<uint32_t>(m.blocks)), wg(kMoveThreads);
+  if (a.in_place)
+    hipLaunchKernelGGL(evict_shift_kernel<VB>, gr, wg, 0, stream, a, m.slices, m.units);
+  else
+    hipLaunchKernelGGL(evict_move_kernel<VB>, gr, wg, 0, stream, a, static_cast<int>(m.chunks), m.rows);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+bool evict_fits(const EvictArgs& a) {
+  return static_cast<int64_t>(a.B) * a.nkv <= max_blocks(kSelThreads) && move_grid(a).blocks <= max_blocks(kMoveThreads);
+}
+
+hipError_t launch_evict(const EvictArgs& a, hipStream_t stream) {
+  const uint32_t heads = static_cast<uint32_t>(a.B) * static_cast<uint32_t>(a.nkv);
+  hipLaunchKernelGGL(evict_select_kernel, dim3(heads), dim3(kSelThreads), 0, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const MoveGrid m = move_grid(a);
+  return m.vb == 16 ? move_rows<16>(a, m, stream) : move_rows<2>(a, m, stream);
 }
 
 }  // namespace fmx

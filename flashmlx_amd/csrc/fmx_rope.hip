@@ -60,6 +60,7 @@ struct RotPlan {
   int units_turn;
   int units_copy;  // of a v head
   int units;       // of a token
+  int first;       // the launch's first token
 };
 
 // VEC elements per load; a turned unit is a pair of vectors (half layout), a
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(kRotThreads) void rotate_kernel(RotateArgs a, RotPl
   const int tid = threadIdx.x;
   const int half = a.dims / 2;
   const int rows = a.B * a.L;
-  const int t0 = static_cast<int>(blockIdx.x / pl.parts) * pl.tokens;
+  const int t0 = pl.first + static_cast<int>(blockIdx.x / pl.parts) * pl.tokens;
   const int part = static_cast<int>(blockIdx.x % pl.parts);
   const int nt = min(pl.tokens, rows - t0);
 
@@ -186,15 +187,21 @@ hipError_t rotate(const RotateArgs& a, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.B) * a.L;
   pl.parts = (pl.units + kPer - 1) / kPer;
   pl.tokens = pl.parts > 1 ? 1 : std::max(1, std::min(kPer / pl.units, kRotTable / half));
-  const int64_t grid = (rows + pl.tokens - 1) / pl.tokens * pl.parts;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  const dim3 gr(static_cast<uint32_t>(grid)), wg(kRotThreads);
+  const dim3 wg(kRotThreads);
   const size_t lds = static_cast<size_t>(pl.tokens) * half * sizeof(float2);
-  if (a.interleaved)
-    hipLaunchKernelGGL((rotate_kernel<ES, F16, VEC, true>), gr, wg, lds, stream, a, pl);
-  else
-    hipLaunchKernelGGL((rotate_kernel<ES, F16, VEC, false>), gr, wg, lds, stream, a, pl);
-  return hipGetLastError();
+  const int64_t per = max_blocks(kRotThreads) / pl.parts * pl.tokens;  // tokens of a launch
+  for (int64_t first = 0; first < rows; first += per) {
+    pl.first = static_cast<int>(first);
+    const int64_t grid = (std::min(per, rows - first) + pl.tokens - 1) / pl.tokens * pl.parts;
+    const dim3 gr(static_cast<uint32_t>(grid));
+    if (a.interleaved)
+      hipLaunchKernelGGL((rotate_kernel<ES, F16, VEC, true>), gr, wg, lds, stream, a, pl);
+    else
+      hipLaunchKernelGGL((rotate_kernel<ES, F16, VEC, false>), gr, wg, lds, stream, a, pl);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 bool vec_view(const HeadsView& v, int es, int vec) {

@@ -120,7 +120,9 @@ int fmx_rope_append(const fmx_rope_angles* angles, int dtype, int64_t batch, int
  * h / (n_heads / n_kv_heads)); head_dim a multiple of 8, at most 256; scale
  * finite and positive. q, out, keys and values are FMX_BF16 or FMX_F16;
  * their data 16-byte aligned, strides multiples of 8, and the token strides
- * of keys and values at most 2^24. */
+ * of keys and values at most 2^24. Calls whose work takes a launch of 2^32
+ * threads or more are refused (FMX_ERR_UNSUPPORTED): those of 2^26 query rows
+ * (batch * seq_len * n_heads) and of about 2^24 pairs of sequence and kv head. */
 typedef struct fmx_attention_shape {
   int32_t dtype;
   int64_t batch;
@@ -195,7 +197,8 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q,
  * k_out, v_out, weights_out: caches of out_max_seq >= min(budget, max_seq)
  * positions, weights [n_slots, n_kv_heads, out_max_seq], that overlap none
  * of the inputs; or all three NULL (out_max_seq ignored): in place. dtype:
- * FMX_BF16 or FMX_F16. head_dim at most 1024. */
+ * FMX_BF16 or FMX_F16. head_dim at most 1024. batch * n_kv_heads below 2^22,
+ * and no launch of 2^32 threads or more (FMX_ERR_UNSUPPORTED). */
 size_t fmx_cache_evict_workspace_size(int64_t batch, int64_t n_kv_heads, int64_t budget);
 int fmx_cache_evict(int dtype, int64_t batch, int64_t n_kv_heads, int64_t head_dim,
                     const fmx_heads* k_cache, const fmx_heads* v_cache, float* weights,

@@ -41,3 +41,53 @@ def test_empty_calls_need_no_workspace(lib, kw):
         if S:
             assert lib.fmx_attention_scored_workspace_size(_shape(**kw), S) == 0
         assert lib.fmx_attention_shared_prefix_workspace_size(_shape(**kw), P, S) == 0
+
+
+class Heads:
+    """Distinct fake arrays: never read, the calls are refused first."""
+    next = 1 << 40
+
+    def __new__(cls, bs=1 << 13, ts=1 << 10, hs=1 << 7, data=None):
+        if data is None:
+            cls.next += 1 << 39
+            data = cls.next
+        return C.byref(_lib.FmxHeads(data, bs, ts, hs))
+
+
+def _shared(lib, shape, P=5, n_slots=2, S=8, slots=None, lse=None, **at):
+    h = {n: at.get(n) or Heads() for n in ("q", "kp", "vp", "kc", "vc", "out")}
+    return lib.fmx_attention_shared_prefix(shape, h["q"], h["kp"], h["vp"], P, h["kc"], h["vc"], n_slots, S, 1 << 35,
+                                           slots, h["out"], lse, None, 0, None)
+
+
+def _scored(lib, shape, n_slots=2, S=8, slots=None, w_in=None, w_out=1 << 36, **at):
+    h = {n: at.get(n) or Heads() for n in ("q", "kc", "vc", "out")}
+    return lib.fmx_attention_scored(shape, h["q"], h["kc"], h["vc"], n_slots, S, 1 << 35, slots, w_in, w_out, h["out"],
+                                    None, 0, None)
+
+
+def _evict(lib, B=2, nkv=2, hd=64, w=1 << 36, n_slots=2, S=100, lens=1 << 33, slots=None, budget=50, out=None,
+           S_out=0, lens_out=1 << 34, kept=1 << 37, **at):
+    h = {n: at.get(n) or Heads() for n in ("k", "v")}
+    ko, vo, wo = out or (None, None, None)
+    return lib.fmx_cache_evict(_lib.FMX_BF16, B, nkv, hd, h["k"], h["v"], w, n_slots, S, lens, slots, budget, 0, 0, ko,
+                               vo, wo, S_out, lens_out, kept, None, 0, None)
+
+
+def test_launches_beyond_the_device(lib):
+    """HIP takes launches of fewer than 2^32 threads: work that needs more is
+    refused before anything runs (an in-place eviction had moved the weights
+    before its second launch failed)."""
+    unsup, one = _lib.FMX_ERR_UNSUPPORTED, 1 << 30
+    for kw in (dict(B=1 << 20, nh=16, nkv=16), dict(B=1 << 17, nh=128, nkv=128), dict(B=1 << 19, nh=128, nkv=8, hd=8)):
+        assert _shared(lib, _shape(**kw), n_slots=1, slots=one) == unsup, kw
+        assert _scored(lib, _shape(**kw), n_slots=1, slots=one) == unsup, kw
+    # the weights of a prompt in a cache far longer than it
+    assert _scored(lib, _shape(B=1 << 10, L=64, nh=16, nkv=16, hd=8), n_slots=1, S=1 << 24, slots=one) == unsup
+    assert _evict(lib, B=1 << 22, nkv=1, n_slots=1, slots=one) == unsup
+    assert _evict(lib, B=1 << 20, nkv=4, n_slots=1, slots=one, out=(Heads(), Heads(), 1 << 38), S_out=60) == unsup
+    assert lib.fmx_cache_evict_workspace_size(1 << 21, 2, 50) == 0
+    # rows of an odd number of elements in four slices; many chunks of rows
+    assert _evict(lib, B=1 << 21, nkv=1, hd=1023, n_slots=1, slots=one) == unsup
+    far = dict(S=1 << 23, budget=1 << 23, S_out=1 << 23, out=(Heads(ts=64), Heads(ts=64), 1 << 38))
+    assert _evict(lib, B=1 << 12, nkv=1, n_slots=1, slots=one, k=Heads(ts=64), v=Heads(ts=64), **far) == unsup

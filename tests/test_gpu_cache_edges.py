@@ -57,3 +57,18 @@ def test_no_queries_keep_the_weights(gpu, fmx, given, S):
     assert got is w_out and torch.equal(w_out, want)
     fmx.attention_scored(q, kc, vc, offs, 0.1, weights=w_out, weights_out=w_out, slots=slots)
     assert torch.equal(w_out, want)
+
+
+def test_rope_of_the_most_rows(gpu, fmx):
+    """2^24 rows of a workgroup each are more threads than one launch takes."""
+    B, L, hd = 1 << 12, 1 << 12, 514  # (an odd number of 16-byte vectors: one pair per thread)
+    x = _randn((1, 1, 1, hd), torch.bfloat16, 1)
+    pos = torch.arange(B * L, dtype=torch.int32, device="cuda").view(B, L)
+    rope = fmx.Rope(fmx.RopeConfig(dims=hd))
+    out = rope(x.expand(B, L, 1, hd), pos)
+    for b, l in ((0, 0), (B // 2, 7), (B - 1, L - 2), (B - 1, L - 1)):
+        assert torch.equal(out[b, l], rope(x, pos[b:b + 1, l:l + 1].contiguous())[0, 0]), (b, l)
+    # (every row but position 0's turns some element)
+    assert int((out[:, :, 0, 0] == 0).sum()) == int((x[..., 0] == 0).sum()) * B * L
+    del out
+    torch.cuda.empty_cache()
