@@ -131,6 +131,27 @@ Span span(const fmx_heads* v, int64_t nb, int64_t nt, int64_t nh, int64_t hd, in
                                            (nh - 1) * v->head_stride + hd) * es)};
 }
 bool overlap(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+Span flat(const void* p, int64_t n) {  // n elements of 4 bytes
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+  return {lo, p ? lo + static_cast<uintptr_t>(n) * 4 : lo};
+}
+
+// A written view's rows of hd elements: two that are one row (a broadcast axis).
+int check_written(const fmx_heads& v, const char* name, int64_t nb, int64_t nt, int64_t nh) {
+  if ((nb > 1 && v.batch_stride == 0) || (nt > 1 && v.token_stride == 0) || (nh > 1 && v.head_stride == 0))
+    return fail(FMX_ERR_ARG, "%s: written, with a stride of 0", name);
+  return FMX_OK;
+}
+
+// Keys and values, both written: rows that overlap where the layouts are alike
+// (they may well lie among each other, as in [slot, position, 2, head, element]).
+int check_apart(const fmx_heads& k, const fmx_heads& v, const char* name, int64_t hd, int es) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(k.data), b = reinterpret_cast<uintptr_t>(v.data);
+  const bool alike = k.batch_stride == v.batch_stride && k.token_stride == v.token_stride && k.head_stride == v.head_stride;
+  if (a == b || (alike && (a < b ? b - a : a - b) < static_cast<uintptr_t>(hd * es)))
+    return fail(FMX_ERR_ARG, "%s: keys and values overlap", name);
+  return FMX_OK;
+}
 
 int elem_size(int dtype) { return dtype == FMX_F32 ? 4 : 2; }
 
@@ -169,17 +190,26 @@ int check_attention(const fmx_attention_shape* s, int64_t prefix_len, int64_t ma
   return FMX_OK;
 }
 
-// out against what is read after parts of it may have been written
-int check_out(const CacheAttnArgs& a, int64_t n_slots) {
+// what is written against what is read after parts of it may have been
+// written, and against each other
+int check_out(const CacheAttnArgs& a) {
   const auto at = [&](const HeadsView& v, int64_t nb, int64_t nt, int64_t nh) {
     const fmx_heads h{v.p, v.bs, v.ts, v.hs};
     return v.p ? span(&h, nb, nt, nh, a.hd, 2) : Span{0, 0};
   };
   const Span out = at(a.out, a.B, a.L, a.nh);
+  const Span lse = flat(a.lse, static_cast<int64_t>(a.B) * a.L * a.nh);
+  const Span w = flat(a.w_out, a.n_slots * a.nkv * a.S);
   for (const Span& i : {at(a.q, a.B, a.L, a.nh), at(a.kp, 1, a.P, a.nkv), at(a.vp, 1, a.P, a.nkv),
-                        at(a.kc, n_slots, a.S, a.nkv), at(a.vc, n_slots, a.S, a.nkv)})
+                        at(a.kc, a.n_slots, a.S, a.nkv), at(a.vc, a.n_slots, a.S, a.nkv)}) {
     if (overlap(out, i)) return fail(FMX_ERR_ARG, "out overlaps q, the prefix or a cache");
-  return FMX_OK;
+    if (overlap(lse, i)) return fail(FMX_ERR_ARG, "lse overlaps q, the prefix or a cache");
+    if (overlap(w, i)) return fail(FMX_ERR_ARG, "weights_out overlaps q or a cache");
+  }
+  if (overlap(out, lse) || overlap(out, w)) return fail(FMX_ERR_ARG, "out overlaps lse or weights_out");
+  if (overlap(out, flat(a.w_in, a.n_slots * a.nkv * a.S))) return fail(FMX_ERR_ARG, "out overlaps weights_in");
+  const fmx_heads o{a.out.p, a.out.bs, a.out.ts, a.out.hs};
+  return check_written(o, "out", a.B, a.L, a.nh);
 }
 
 int check_launches(const CacheAttnArgs& a) {
@@ -272,6 +302,7 @@ int fmx_rope(const fmx_rope_angles* angles, int dtype, int64_t batch, int64_t se
   fmx_heads x_v, out_v;
   FMX_RC(check_view(x, "x", batch, seq_len, n_heads, es, 1, &x_v));
   FMX_RC(check_view(out, "out", batch, seq_len, n_heads, es, 1, &out_v));
+  FMX_RC(check_written(out_v, "out", batch, seq_len, n_heads));
   x = &x_v;
   out = &out_v;
   if (!same(x, out) && overlap(span(x, batch, seq_len, n_heads, head_dim, es),
@@ -315,6 +346,10 @@ int fmx_rope_append(const fmx_rope_angles* angles, int dtype, int64_t batch, int
   FMX_RC(check_view(q_out, "q_out", batch, seq_len, n_heads, es, 1, &qo_v));
   FMX_RC(check_view(k_cache, "k_cache", n_slots, max_seq, n_kv_heads, es, 1, &kc_v));
   FMX_RC(check_view(v_cache, "v_cache", n_slots, max_seq, n_kv_heads, es, 1, &vc_v));
+  FMX_RC(check_written(qo_v, "q_out", batch, seq_len, n_heads));
+  FMX_RC(check_written(kc_v, "k_cache", n_slots, max_seq, n_kv_heads));
+  FMX_RC(check_written(vc_v, "v_cache", n_slots, max_seq, n_kv_heads));
+  FMX_RC(check_apart(kc_v, vc_v, "caches", head_dim, es));
   q = &q_v;
   k = &k_v;
   v = &v_v;
@@ -396,11 +431,12 @@ int fmx_attention_shared_prefix(const fmx_attention_shape* shape, const fmx_head
     a.n_slots = n_slots;
     if (!offsets) return fail(FMX_ERR_ARG, "offsets is NULL");
   }
+  if (!aligned(lse, 4)) return fail(FMX_ERR_ARG, "lse not 4-byte aligned");
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   a.q = view(&q_v);
   a.out = view(&out_v);
   a.lse = lse;
-  FMX_RC(check_out(a, n_slots));
+  FMX_RC(check_out(a));
   FMX_RC(check_launches(a));
   Workspace ws;
   FMX_RC(ws.bind(workspace, workspace_bytes, cache_attn_workspace(a), stream));
@@ -451,7 +487,7 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
   a.kc = view(&kc_v);
   a.vc = view(&vc_v);
   a.offs = offsets;
-  FMX_RC(check_out(a, n_slots));
+  FMX_RC(check_out(a));
   FMX_RC(check_launches(a));
   Workspace ws;
   FMX_RC(ws.bind(workspace, workspace_bytes, cache_attn_workspace(a), stream));
@@ -501,25 +537,41 @@ int fmx_cache_evict(int dtype, int64_t batch, int64_t n_kv_heads, int64_t head_d
     FMX_RC(check_view(v_out, "v_out", n_slots, out_max_seq, n_kv_heads, 2, 1, &vo_v));
     k_out = &ko_v;
     v_out = &vo_v;
-    const uintptr_t w = reinterpret_cast<uintptr_t>(weights), wo = reinterpret_cast<uintptr_t>(weights_out);
-    const uintptr_t rows = static_cast<uintptr_t>(n_slots) * static_cast<uintptr_t>(n_kv_heads) * 4;
-    const Span ins[3] = {span(k_cache, n_slots, max_seq, n_kv_heads, head_dim, 2),
-                         span(v_cache, n_slots, max_seq, n_kv_heads, head_dim, 2),
-                         {w, w + rows * static_cast<uintptr_t>(max_seq)}};
-    const Span outs[3] = {span(k_out, n_slots, out_max_seq, n_kv_heads, head_dim, 2),
-                          span(v_out, n_slots, out_max_seq, n_kv_heads, head_dim, 2),
-                          {wo, wo + rows * static_cast<uintptr_t>(out_max_seq)}};
+  } else {
+    k_out = k_cache;
+    v_out = v_cache;
+    weights_out = weights;
+    out_max_seq = max_seq;
+  }
+  FMX_RC(check_written(*k_out, "keys", n_slots, out_max_seq, n_kv_heads));
+  FMX_RC(check_written(*v_out, "values", n_slots, out_max_seq, n_kv_heads));
+  FMX_RC(check_apart(*k_out, *v_out, in_place ? "caches" : "outputs", head_dim, 2));
+  const Span ins[3] = {span(k_cache, n_slots, max_seq, n_kv_heads, head_dim, 2),
+                       span(v_cache, n_slots, max_seq, n_kv_heads, head_dim, 2),
+                       flat(weights, n_slots * n_kv_heads * max_seq)};
+  const Span outs[3] = {span(k_out, n_slots, out_max_seq, n_kv_heads, head_dim, 2),
+                        span(v_out, n_slots, out_max_seq, n_kv_heads, head_dim, 2),
+                        flat(weights_out, n_slots * n_kv_heads * out_max_seq)};
+  if (!in_place)
     for (const Span& o : outs)
       for (const Span& i : ins)
         if (overlap(o, i)) return fail(FMX_ERR_ARG, "an output overlaps an input");
+  if (overlap(outs[2], outs[0]) || overlap(outs[2], outs[1])) return fail(FMX_ERR_ARG, "weights overlap a cache");
+  // kept and lengths_out, against everything but lengths_out that is lengths
+  const Span kept_s = flat(kept, batch * n_kv_heads * budget), lens_s = flat(lengths, batch);
+  const Span lens_out_s = flat(lengths_out, batch), slots_s = flat(slots, slots ? batch : 0);
+  for (const Span& o : {kept_s, lens_out_s}) {
+    for (const Span& i : {ins[0], ins[1], ins[2], outs[0], outs[1], outs[2], slots_s})
+      if (overlap(o, i)) return fail(FMX_ERR_ARG, "kept or lengths_out overlaps another array");
+    if (overlap(o, lens_s) && lengths_out != lengths) return fail(FMX_ERR_ARG, "kept or lengths_out overlaps lengths");
   }
+  if (overlap(kept_s, lens_s) || overlap(kept_s, lens_out_s))
+    return fail(FMX_ERR_ARG, "kept overlaps lengths or lengths_out");
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   EvictArgs a{};
   a.B = static_cast<int>(batch);
   a.nkv = static_cast<int>(n_kv_heads);
   a.row_bytes = head_dim * 2;
-  const fmx_heads* ko = in_place ? k_cache : k_out;
-  const fmx_heads* vo = in_place ? v_cache : v_out;
   a.k = static_cast<const uint8_t*>(k_cache->data);
   a.v = static_cast<const uint8_t*>(v_cache->data);
   a.k_bs = 2 * k_cache->batch_stride;
@@ -528,19 +580,19 @@ int fmx_cache_evict(int dtype, int64_t batch, int64_t n_kv_heads, int64_t head_d
   a.v_bs = 2 * v_cache->batch_stride;
   a.v_ts = 2 * v_cache->token_stride;
   a.v_hs = 2 * v_cache->head_stride;
-  a.k_out = static_cast<uint8_t*>(ko->data);
-  a.v_out = static_cast<uint8_t*>(vo->data);
-  a.ko_bs = 2 * ko->batch_stride;
-  a.ko_ts = 2 * ko->token_stride;
-  a.ko_hs = 2 * ko->head_stride;
-  a.vo_bs = 2 * vo->batch_stride;
-  a.vo_ts = 2 * vo->token_stride;
-  a.vo_hs = 2 * vo->head_stride;
+  a.k_out = static_cast<uint8_t*>(k_out->data);
+  a.v_out = static_cast<uint8_t*>(v_out->data);
+  a.ko_bs = 2 * k_out->batch_stride;
+  a.ko_ts = 2 * k_out->token_stride;
+  a.ko_hs = 2 * k_out->head_stride;
+  a.vo_bs = 2 * v_out->batch_stride;
+  a.vo_ts = 2 * v_out->token_stride;
+  a.vo_hs = 2 * v_out->head_stride;
   a.w = weights;
-  a.w_out = in_place ? weights : weights_out;
+  a.w_out = weights_out;
   a.n_slots = n_slots;
   a.S = max_seq;
-  a.S_out = in_place ? max_seq : out_max_seq;
+  a.S_out = out_max_seq;
   a.lens = lengths;
   a.slots = slots;
   a.budget = budget;

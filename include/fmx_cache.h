@@ -25,9 +25,10 @@ extern "C" {
 /* A strided view of rows of heads: element (b, l, h, d) is at
  * data + b * batch_stride + l * token_stride + h * head_stride + d, strides in
  * elements, not negative. For a cache, b is the slot and l the position. An
- * output's rows must not overlap one another. Nor, except where a call says
- * so, may they lie between an input's first and last element (or an input's
- * between theirs): such calls are refused. */
+ * output's rows must not overlap one another (strides of 0 are refused). Nor,
+ * except where a call says so, may they lie between an input's first and last
+ * element (or an input's between theirs), or between those of another output:
+ * such calls are refused. Keys and values alone may lie among each other. */
 typedef struct fmx_heads {
   void* data;
   int64_t batch_stride;

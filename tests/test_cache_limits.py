@@ -91,3 +91,57 @@ def test_launches_beyond_the_device(lib):
     assert _evict(lib, B=1 << 21, nkv=1, hd=1023, n_slots=1, slots=one) == unsup
     far = dict(S=1 << 23, budget=1 << 23, S_out=1 << 23, out=(Heads(ts=64), Heads(ts=64), 1 << 38))
     assert _evict(lib, B=1 << 12, nkv=1, n_slots=1, slots=one, k=Heads(ts=64), v=Heads(ts=64), **far) == unsup
+
+
+def _rope(lib, x=None, out=None, B=2, L=3, nh=4, hd=128):
+    angles = C.byref(_lib.FmxRopeAngles(1 << 33, 64, 1.0, 0))
+    return lib.fmx_rope(angles, _lib.FMX_BF16, B, L, nh, hd, x or Heads(), 1 << 34, 0, out or Heads(), None)
+
+
+def _append(lib, q_out=None, kc=None, vc=None):
+    angles = C.byref(_lib.FmxRopeAngles(1 << 33, 64, 1.0, 0))
+    return lib.fmx_rope_append(angles, _lib.FMX_BF16, 2, 3, 4, 4, 128, Heads(), Heads(), Heads(), 1 << 34, 1 << 35, None, 2,
+                               8, q_out or Heads(), kc or Heads(), vc or Heads(), None)
+
+
+def test_outputs_that_overlap(lib):
+    """Arrays that are written may lie over no other array of the call."""
+    arg, at = _lib.FMX_ERR_ARG, 1 << 52
+    # rows that are one row (a broadcast axis)
+    for flat in (dict(bs=0), dict(ts=0), dict(hs=0)):
+        for data in (None, at):
+            v = Heads(data=data, **flat)
+            assert _rope(lib, x=v, out=v) == arg
+            assert _append(lib, q_out=v) == arg
+            assert _append(lib, kc=v) == arg
+            assert _append(lib, vc=v) == arg
+            assert _shared(lib, _shape(L=2), out=v) == arg
+            assert _scored(lib, _shape(L=2), out=v) == arg
+            assert _evict(lib, k=v) == arg
+            assert _evict(lib, out=(v, Heads(), 1 << 50), S_out=60) == arg
+            assert _evict(lib, out=(Heads(), v, 1 << 50), S_out=60) == arg
+    # keys over values
+    for d in (0, 64):
+        assert _append(lib, kc=Heads(data=at), vc=Heads(data=at + d)) == arg
+        assert _evict(lib, k=Heads(data=at), v=Heads(data=at + d)) == arg
+        assert _evict(lib, out=(Heads(data=at), Heads(data=at + d), 1 << 50), S_out=60) == arg
+    # lse and weights
+    for name in ("q", "kp", "vp", "kc", "vc", "out"):
+        assert _shared(lib, _shape(), lse=at + 256, **{name: Heads(data=at)}) == arg, name
+    assert _shared(lib, _shape(), lse=2) == arg
+    for name in ("q", "kc", "vc", "out"):
+        assert _scored(lib, _shape(), w_out=at + 256, **{name: Heads(data=at)}) == arg, name
+    assert _scored(lib, _shape(), w_in=at + 256, out=Heads(data=at)) == arg
+    # eviction's weights, positions and lengths
+    for kw in (dict(k=Heads(data=at)), dict(v=Heads(data=at)), dict(out=(Heads(data=at), Heads(), 1 << 50), S_out=60),
+               dict(out=(Heads(), Heads(data=at), 1 << 50), S_out=60)):
+        assert _evict(lib, kept=at + 256, **kw) == arg, kw
+        assert _evict(lib, lens_out=at + 256, **kw) == arg, kw
+    assert _evict(lib, k=Heads(data=at), w=at + 256) == arg
+    assert _evict(lib, out=(Heads(data=at), Heads(), at + 256), S_out=60) == arg
+    assert _evict(lib, kept=1 << 36) == arg            # over the weights
+    assert _evict(lib, lens_out=(1 << 36) + 8) == arg
+    assert _evict(lib, kept=1 << 33) == arg            # over the lengths
+    assert _evict(lib, kept=1 << 34) == arg            # over lengths_out
+    assert _evict(lib, lens_out=(1 << 33) + 4) == arg  # over the lengths in part
+    assert _evict(lib, n_slots=2, slots=at, kept=at) == arg
