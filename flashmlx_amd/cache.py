@@ -31,10 +31,13 @@ _TURNS = {"parts": (1.0, 4.0), "yarn": (1.0, 32.0)}
 _byref = C.byref
 
 
-def _refuse(t, name: str, shape: tuple, dtype, dev: int) -> None:
-    """Says which of an argument's shape, dtype, device or layout is wrong."""
+def _tensor(t, name: str) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: a tensor expected, got {type(t).__name__}")
+
+
+def _refuse(t, name: str, shape: tuple, dtype, dev: int) -> None:
+    """Says which of an argument's shape, dtype, device or layout is wrong."""
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
@@ -47,6 +50,7 @@ def _refuse(t, name: str, shape: tuple, dtype, dev: int) -> None:
 
 def _heads(t: torch.Tensor, name: str, shape, dtype, dev: int):
     """The view of a [batch, token, head, element] tensor."""
+    _tensor(t, name)
     s = t.stride()
     if t.shape != shape or t.dtype != dtype or t.get_device() != dev or s[3] != 1 and shape[3] != 1:
         _refuse(t, name, shape, dtype, dev)
@@ -55,6 +59,7 @@ def _heads(t: torch.Tensor, name: str, shape, dtype, dev: int):
 
 def _cache(t: torch.Tensor, name: str, shape, dtype, dev: int):
     """The view of a [slot, head, position, element] tensor."""
+    _tensor(t, name)
     s = t.stride()
     if t.shape != shape or t.dtype != dtype or t.get_device() != dev or s[3] != 1 and shape[3] != 1:
         _refuse(t, name, shape, dtype, dev)
@@ -63,6 +68,7 @@ def _cache(t: torch.Tensor, name: str, shape, dtype, dev: int):
 
 def _prefix(t: torch.Tensor, name: str, shape, dtype, dev: int):
     """The view of a [head, position, element] tensor."""
+    _tensor(t, name)
     if t.shape != shape or t.dtype != dtype or t.get_device() != dev or t.stride(2) != 1 and shape[2] != 1:
         _refuse(t, name, shape, dtype, dev)
     s = t.stride()
@@ -73,6 +79,7 @@ def _flat(t: Optional[torch.Tensor], name: str, shape, dtype, dev: int) -> Optio
     """The address of a contiguous array, or None."""
     if t is None:
         return None
+    _tensor(t, name)
     if t.shape != shape or t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
         _refuse(t, name, shape, dtype, dev)
     return t.data_ptr()
@@ -80,6 +87,7 @@ def _flat(t: Optional[torch.Tensor], name: str, shape, dtype, dev: int) -> Optio
 
 def _device(t: torch.Tensor, name: str, dims: str) -> int:
     """The index of the current device, on which t, of four axes, has to be."""
+    _tensor(t, name)
     if t.dim() != 4:
         raise ValueError(f"{name}: [{dims}] expected, got {tuple(t.shape)}")
     if t.dtype not in _DT:
@@ -95,6 +103,7 @@ _ROWS, _SLOTS = "batch, seq_len, heads, head_dim", "slots, kv_heads, positions, 
 
 def _pool(k: torch.Tensor, hd: int) -> tuple:
     """(slots, kv heads, positions) of the caches."""
+    _tensor(k, "k_cache")
     if k.dim() != 4 or k.shape[3] != hd:
         raise ValueError(f"k_cache: shape {tuple(k.shape)}, expected [slots, kv_heads, positions, {hd}]")
     return k.shape[0], k.shape[1], k.shape[2]
@@ -108,6 +117,7 @@ def _stream(dev: int) -> int:
 def _workspace(ws: Optional[torch.Tensor], need: int, like: torch.Tensor) -> torch.Tensor:
     if ws is None:
         return like.new_empty(max(need, 1), dtype=torch.uint8)
+    _tensor(ws, "workspace")
     if ws.get_device() != like.get_device() or not ws.is_contiguous() or ws.dtype != torch.uint8:
         raise ValueError(f"workspace: a contiguous uint8 tensor on {like.device} expected")
     return ws
@@ -222,6 +232,7 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: Optional[torch.Tensor], v
     if (k_prefix is None) != (v_prefix is None):
         raise ValueError("k_prefix and v_prefix: both or neither")
     if k_prefix is not None:
+        _tensor(k_prefix, "k_prefix")
         P = k_prefix.shape[1] if k_prefix.dim() == 3 else -1
         kp = _prefix(k_prefix, "k_prefix", (nkv, P, hd), dt, dev)
         vp = _prefix(v_prefix, "v_prefix", (nkv, P, hd), dt, dev)
@@ -285,6 +296,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     dev, pool, dt = _device(k_cache, "k_cache", _SLOTS), k_cache.shape, k_cache.dtype
     i32, f32 = torch.int32, torch.float32
     n_slots, nkv, S, hd = pool
+    _tensor(lengths, "lengths")
     if lengths.dim() != 1:
         raise ValueError(f"lengths: shape {tuple(lengths.shape)}, expected [batch]")
     if budget < 1:
@@ -294,6 +306,7 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     S_out = 0
     if out is not None:
         k_out, v_out, w_out = out
+        _tensor(k_out, "out[0]")
         S_out = k_out.shape[2] if k_out.dim() == 4 else -1
         to = (n_slots, nkv, S_out, hd)
         ko, vo = _cache(k_out, "out[0]", to, dt, dev), _cache(v_out, "out[1]", to, dt, dev)

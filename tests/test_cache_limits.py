@@ -145,3 +145,27 @@ def test_outputs_that_overlap(lib):
     assert _evict(lib, kept=1 << 34) == arg            # over lengths_out
     assert _evict(lib, lens_out=(1 << 33) + 4) == arg  # over the lengths in part
     assert _evict(lib, n_slots=2, slots=at, kept=at) == arg
+
+
+@pytest.mark.parametrize("bad", [None, [1, 2], 3.0, "numpy"], ids=str)
+def test_python_arguments_that_are_no_tensors(fmx, bad):
+    """A TypeError that names the argument."""
+    import numpy as np
+    import torch
+    from flashmlx_amd import cache as M
+    if bad == "numpy":
+        bad = np.zeros((2, 1, 8, 64), dtype=np.float32)
+    q = torch.zeros(2, 1, 8, 64, dtype=torch.bfloat16)
+    for f in (M._heads, M._cache, M._prefix):
+        with pytest.raises(TypeError, match="some_array: a tensor expected"):
+            f(bad, "some_array", (2, 1, 8, 64), torch.bfloat16, -1)
+    if bad is not None:
+        with pytest.raises(TypeError, match="some_array: a tensor expected"):
+            M._flat(bad, "some_array", (2,), torch.int32, -1)
+        with pytest.raises(TypeError, match="workspace: a tensor expected"):
+            M._workspace(bad, 5, q)
+    for call, name in ((lambda: fmx.attention_scored(bad, q, q, q, 0.1), "q"),
+                       (lambda: fmx.attention_shared_prefix(bad, None, None, q, q, q, 0.1), "q"),
+                       (lambda: fmx.cache_evict(bad, q, q, q, 4), "k_cache"), (lambda: M._pool(bad, 64), "k_cache")):
+        with pytest.raises(TypeError, match=f"^{name}: a tensor expected"):
+            call()
