@@ -2,8 +2,13 @@
 batches, loads past the caches, eviction without the kept positions."""
 from __future__ import annotations
 
+import ctypes as C
+import math
+
 import pytest
 import torch
+
+import cache_oracle as R
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +77,86 @@ def test_rope_of_the_most_rows(gpu, fmx):
     assert int((out[:, :, 0, 0] == 0).sum()) == int((x[..., 0] == 0).sum()) * B * L
     del out
     torch.cuda.empty_cache()
+
+
+def _long_cache(B, L, nh, nkv, hd, P, S, seen, dt, seed):
+    """Caches of S positions of which sequences use up to `seen`; the rest are
+    NaN keys and infinite values."""
+    q = _randn((B, L, nh, hd), dt, seed)
+    kc = torch.full((B, nkv, S, hd), math.nan, dtype=dt, device="cuda")
+    vc = torch.full((B, nkv, S, hd), math.inf, dtype=dt, device="cuda")
+    marks = [seen, 0, 1, seen - 1, seen // 2, 17, 130, 33]
+    lens = [min(marks[b % len(marks)], seen) for b in range(B)]
+    for b, n in enumerate(lens):
+        kc[b, :, :n], vc[b, :, :n] = _randn((nkv, n, hd), dt, seed + 10 + b), _randn((nkv, n, hd), dt, seed + 500 + b)
+    offs = torch.tensor([n - L for n in lens], dtype=torch.int32, device="cuda")
+    kp, vp = (_randn((nkv, P, hd), dt, seed + 1), _randn((nkv, P, hd), dt, seed + 2)) if P else (None, None)
+    small = [torch.nan_to_num(t[:, :, :seen], nan=0.0, posinf=0.0) for t in (kc, vc)]
+    return q, kp, vp, kc, vc, small, offs
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("B,L,nh,nkv,hd,P,S,seen", [
+    # narrow tiles alone: one row set, one query (heads of a template and others) and several
+    (3, 1, 16, 4, 128, 0, 50000, 700), (4, 1, 4, 4, 64, 70, 70000, 500), (2, 1, 8, 2, 256, 33, 70000, 400),
+    (2, 1, 8, 2, 80, 0, 220000, 300), (2, 3, 8, 2, 64, 40, 270000, 333), (2, 2, 6, 3, 96, 515, 120000, 290),
+    (2, 2, 8, 2, 256, 20, 70000, 260),
+    # two row sets
+    (2, 5, 8, 2, 128, 0, 140000, 700), (2, 5, 8, 2, 72, 0, 240000, 300), (3, 1, 24, 1, 64, 0, 360000, 400),
+    # beside a prefix in wide tiles
+    (40, 1, 8, 2, 128, 300, 7000, 600), (36, 1, 4, 4, 64, 200, 8000, 260), (40, 2, 8, 4, 80, 150, 6000, 200),
+    (10, 5, 8, 2, 64, 400, 60000, 300), (10, 5, 8, 2, 128, 150, 30000, 280), (36, 1, 2, 2, 256, 100, 4000, 150)])
+def test_caches_beyond_256_mb(gpu, fmx, dt, B, L, nh, nkv, hd, P, S, seen):
+    """From 256 MB of prefix and caches on, narrow tiles load past the caches."""
+    assert (P + B * S) * nkv * hd * 4 > 256 << 20
+    q, kp, vp, kc, vc, small, offs = _long_cache(B, L, nh, nkv, hd, P, S, seen, dt, hd + B)
+    scale = hd ** -0.5
+    out, lse = fmx.attention_shared_prefix(q, kp, vp, kc, vc, offs, scale)
+    r = R.attention(q, *small, offs, scale, kp=kp, vp=vp)
+    R.assert_within(out, r["out"], r["out_b"], "out")
+    R.assert_within(lse, r["lse"], r["lse_b"], "lse")
+    if P:
+        r = R.attention(q, *small, offs, scale)
+    out, w = fmx.attention_scored(q, kc, vc, offs, scale)
+    R.assert_within(out, r["out"], r["out_b"], "out of the scored call")
+    R.assert_within(w[:, :, :seen], r["w"], r["w_b"], "weights")
+    assert bool((w[:, :, seen:] == 0).all())
+
+
+@pytest.mark.parametrize("own_workspace", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_without_kept_positions(gpu, fmx, in_place, own_workspace):
+    """kept NULL: the positions stay in the workspace, the caller's or the call's own."""
+    from flashmlx_amd import _lib
+    from flashmlx_amd._lib import FmxHeads
+    lib = _lib.load()
+    B, nkv, S, hd, budget = 3, 2, 700, 64, 300
+    k, v = _randn((B, nkv, S, hd), torch.bfloat16, 1), _randn((B, nkv, S, hd), torch.bfloat16, 2)
+    w = _randn((B, nkv, S), torch.float32, 3)
+    lens = torch.tensor([700, 250, 301], dtype=torch.int32, device="cuda")
+
+    def outputs():
+        if in_place:
+            return k.clone(), v.clone(), w.clone()
+        return tuple(torch.zeros((B, nkv, budget) + t, dtype=d, device="cuda")
+                     for t, d in (((hd,), k.dtype), ((hd,), k.dtype), ((), w.dtype)))
+
+    want = outputs()
+    src = want if in_place else (k, v, w)
+    lens_want, _ = fmx.cache_evict(*src, lens, budget, sinks=4, recent=20, out=None if in_place else want)
+    got = outputs()
+    src = got if in_place else (k, v, w)
+
+    def heads(t):
+        return C.byref(FmxHeads(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1)))
+
+    need = lib.fmx_cache_evict_workspace_size(B, nkv, budget)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    lens_got = torch.empty_like(lens)
+    to = (None, None, None, 0) if in_place else (heads(got[0]), heads(got[1]), got[2].data_ptr(), budget)
+    _lib.check(lib.fmx_cache_evict(
+        _lib.FMX_BF16, B, nkv, hd, heads(src[0]), heads(src[1]), src[2].data_ptr(), B, S, lens.data_ptr(), None, budget, 4,
+        20, *to, lens_got.data_ptr(), None, ws.data_ptr() if own_workspace else None, need if own_workspace else 0,
+        torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert torch.equal(lens_got, lens_want) and all(torch.equal(a, b) for a, b in zip(got, want))
