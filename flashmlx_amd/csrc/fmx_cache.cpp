@@ -212,6 +212,16 @@ int check_out(const CacheAttnArgs& a) {
   return check_written(o, "out", a.B, a.L, a.nh);
 }
 
+// Rows of q turned in place, and new keys or values that are among them (they
+// may well lie between them, as in a fused row of q, k and v).
+int check_not_among(const fmx_heads& k, const fmx_heads& q, const char* name, int64_t n_heads, int64_t hd, int es) {
+  if (k.batch_stride != q.batch_stride || k.token_stride != q.token_stride) return FMX_OK;
+  const int64_t d = (static_cast<const uint8_t*>(k.data) - static_cast<const uint8_t*>(q.data)) / es;
+  const int64_t hs = q.head_stride;
+  const bool among = (d < 0 ? -d : d) < hd || (hs > 0 && d > 0 && d % hs == 0 && d / hs < n_heads);
+  return among ? fail(FMX_ERR_ARG, "q_out overlaps %s", name) : FMX_OK;
+}
+
 int check_launches(const CacheAttnArgs& a) {
   return cache_attn_fits(a) ? FMX_OK : fail(FMX_ERR_UNSUPPORTED, "more work than launches of fewer than 2^32 threads");
 }
@@ -365,9 +375,13 @@ int fmx_rope_append(const fmx_rope_angles* angles, int dtype, int64_t batch, int
   for (int c = 1; c < 3; ++c)  // caches against the inputs and q_out
     for (const Span& i : {ins[0], ins[1], ins[2], outs[0]})
       if (overlap(outs[c], i)) return fail(FMX_ERR_ARG, "a cache overlaps q, k, v or q_out");
-  if (!same(q, q_out))
+  if (same(q, q_out)) {
+    FMX_RC(check_not_among(*k, *q, "k", n_heads, head_dim, es));
+    FMX_RC(check_not_among(*v, *q, "v", n_heads, head_dim, es));
+  } else {
     for (const Span& i : ins)
       if (overlap(outs[0], i)) return fail(FMX_ERR_ARG, "q_out overlaps q, k or v and is not q itself");
+  }
   RotateArgs a{};
   a.freqs = angles->freqs;
   a.dims = static_cast<int>(angles->dims);

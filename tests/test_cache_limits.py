@@ -169,3 +169,22 @@ def test_python_arguments_that_are_no_tensors(fmx, bad):
                        (lambda: fmx.cache_evict(bad, q, q, q, 4), "k_cache"), (lambda: M._pool(bad, 64), "k_cache")):
         with pytest.raises(TypeError, match=f"^{name}: a tensor expected"):
             call()
+
+
+def test_keys_among_queries_in_place(lib):
+    """Queries turned in place, new keys or values among their heads: a
+    workgroup could read a key that another has turned already. Beside them in
+    a fused row they are taken (that call ends at a later check here)."""
+    angles = C.byref(_lib.FmxRopeAngles(1 << 33, 64, 1.0, 0))
+    arg, at, row = _lib.FMX_ERR_ARG, 1 << 52, dict(bs=3 * 12 * 128, ts=12 * 128, hs=128)
+
+    def call(k, v, cache=None):
+        q = Heads(data=at, **row)
+        caches = Heads(), cache or Heads()
+        return lib.fmx_rope_append(angles, _lib.FMX_BF16, 2, 3, 4, 4, 128, q, Heads(data=at + 2 * k, **row),
+                                   Heads(data=at + 2 * v, **row), 1 << 34, 1 << 35, None, 2, 8, q, *caches, None)
+
+    for h in (0, 64, 128, 3 * 128):
+        assert call(h, 8 * 128) == arg and b"overlaps k" in lib.fmx_last_error(), h
+        assert call(4 * 128, h) == arg and b"overlaps v" in lib.fmx_last_error(), h
+    assert call(4 * 128, 8 * 128, Heads(data=at)) == arg and b"a cache overlaps" in lib.fmx_last_error()
