@@ -38,6 +38,7 @@ def _tensor(t, name: str) -> None:
 
 def _refuse(t, name: str, shape: tuple, dtype, dev: int) -> None:
     """Says which of an argument's shape, dtype, device or layout is wrong."""
+    _tensor(t, name)
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
@@ -50,8 +51,11 @@ def _refuse(t, name: str, shape: tuple, dtype, dev: int) -> None:
 
 def _heads(t: torch.Tensor, name: str, shape, dtype, dev: int):
     """The view of a [batch, token, head, element] tensor."""
-    _tensor(t, name)
-    s = t.stride()
+    try:
+        s = t.stride()
+    except AttributeError:
+        _tensor(t, name)
+        raise
     if t.shape != shape or t.dtype != dtype or t.get_device() != dev or s[3] != 1 and shape[3] != 1:
         _refuse(t, name, shape, dtype, dev)
     return _byref(FmxHeads(t.data_ptr(), s[0], s[1], s[2]))
@@ -59,8 +63,11 @@ def _heads(t: torch.Tensor, name: str, shape, dtype, dev: int):
 
 def _cache(t: torch.Tensor, name: str, shape, dtype, dev: int):
     """The view of a [slot, head, position, element] tensor."""
-    _tensor(t, name)
-    s = t.stride()
+    try:
+        s = t.stride()
+    except AttributeError:
+        _tensor(t, name)
+        raise
     if t.shape != shape or t.dtype != dtype or t.get_device() != dev or s[3] != 1 and shape[3] != 1:
         _refuse(t, name, shape, dtype, dev)
     return _byref(FmxHeads(t.data_ptr(), s[0], s[2], s[1]))
@@ -68,10 +75,13 @@ def _cache(t: torch.Tensor, name: str, shape, dtype, dev: int):
 
 def _prefix(t: torch.Tensor, name: str, shape, dtype, dev: int):
     """The view of a [head, position, element] tensor."""
-    _tensor(t, name)
-    if t.shape != shape or t.dtype != dtype or t.get_device() != dev or t.stride(2) != 1 and shape[2] != 1:
+    try:
+        s = t.stride()
+    except AttributeError:
+        _tensor(t, name)
+        raise
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev or s[2] != 1 and shape[2] != 1:
         _refuse(t, name, shape, dtype, dev)
-    s = t.stride()
     return _byref(FmxHeads(t.data_ptr(), 0, s[1], s[0]))
 
 
@@ -79,16 +89,23 @@ def _flat(t: Optional[torch.Tensor], name: str, shape, dtype, dev: int) -> Optio
     """The address of a contiguous array, or None."""
     if t is None:
         return None
-    _tensor(t, name)
-    if t.shape != shape or t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
+    try:
+        wrong = t.shape != shape or t.dtype != dtype or t.get_device() != dev or not t.is_contiguous()
+    except AttributeError:
+        wrong = True
+    if wrong:
         _refuse(t, name, shape, dtype, dev)
     return t.data_ptr()
 
 
 def _device(t: torch.Tensor, name: str, dims: str) -> int:
     """The index of the current device, on which t, of four axes, has to be."""
-    _tensor(t, name)
-    if t.dim() != 4:
+    try:
+        dims_there = t.dim()
+    except AttributeError:
+        _tensor(t, name)
+        raise
+    if dims_there != 4:
         raise ValueError(f"{name}: [{dims}] expected, got {tuple(t.shape)}")
     if t.dtype not in _DT:
         raise TypeError(f"{name}: {t.dtype} (bfloat16, float16 or float32)")
@@ -103,8 +120,12 @@ _ROWS, _SLOTS = "batch, seq_len, heads, head_dim", "slots, kv_heads, positions, 
 
 def _pool(k: torch.Tensor, hd: int) -> tuple:
     """(slots, kv heads, positions) of the caches."""
-    _tensor(k, "k_cache")
-    if k.dim() != 4 or k.shape[3] != hd:
+    try:
+        wrong = k.dim() != 4 or k.shape[3] != hd
+    except AttributeError:
+        _tensor(k, "k_cache")
+        raise
+    if wrong:
         raise ValueError(f"k_cache: shape {tuple(k.shape)}, expected [slots, kv_heads, positions, {hd}]")
     return k.shape[0], k.shape[1], k.shape[2]
 
