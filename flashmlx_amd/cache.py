@@ -8,7 +8,8 @@ Arrays: queries and new keys [batch, seq_len, heads, head_dim], caches
 weights fp32 [slots, kv_heads, max_seq]. Any strides with the head's elements
 contiguous will do (16-byte steps for attention); weights, positions, offsets,
 lengths and slots are contiguous. torch tensors only carry device memory and
-the current stream into the C-ABI.
+the current stream into the C-ABI: no call is recorded for autograd, and a
+result never requires a gradient, whatever its inputs do.
 """
 from __future__ import annotations
 

@@ -166,7 +166,7 @@ __device__ int find_piece(const CacheAttnArgs& a, const Plan& pl, int w, bool wr
 // Bound by HBM: every key and value is read once, 512 bytes (heads of 128) for
 // 16 bytes of partial results per 128 keys and row. 16 sequences of up to
 // 16001 keys, 32 heads over 4, fp16,
-// scores stored: 59 us for 271 MB, 4.6 TB/s (4.9 is a large copy's); one row
+// scores stored: 59 us for 271 MB, 4.6 TB/s (6.2 is a large read's); one row
 // per workgroup and head took 6.6 ms, the same values read for every head and
 // queried one after the other. Short calls are bound by the chain of a
 // workgroup (a piece's address, its loads, two products): 4 sequences of up to
@@ -571,9 +571,9 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 //
 // The weights go into the value product as two numbers of the inputs' type, as
 // in narrow tiles, so that a row's precision does not hang on how many rows its
-// call has. That is half of all matrix work again (59 -> 70 us for the prompt
-// below, 115 -> 125 us for 128 sequences behind 32768 positions; the figures
-// given for choices further down are from before), but one number alone, off by
+// call has. That is half of all matrix work again (59 -> 71 us for the prompt
+// below, 126 -> 145 us a call of 128 sequences behind 32768 positions; the
+// figures given for choices further down are from before), but one number alone, off by
 // up to 2^-8 or 2^-11 of the weight, moves a row with one dominating key by a
 // step of the output. The maximum is only raised when a score lies more than
 // kLazy above it: the weights reach 2^kLazy times kBias' 2^8 at most, in fp16
@@ -586,7 +586,7 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 // (queries from HBM, outputs). The longest tile of a causal grid alone is two
 // thirds of the kernel's time; keys dealt to two halves of a workgroup, or long
 // and short tiles one after the other, gained nothing. A prompt of 2000 tokens,
-// 32 heads over 4: 70 us, 0.47 PFLOP/s of the causal half (1.4 is a large
+// 32 heads over 4: 71 us, 0.46 PFLOP/s of the causal half (1.4 is a large
 // library product's).
 constexpr int kWideRows = 32 * kWaves;
 constexpr int kCus = 256;
@@ -1439,14 +1439,21 @@ __global__ __launch_bounds__(kThreads) void attn_weights_sum_kernel(CacheAttnArg
 constexpr int64_t kFill = 768;
 // and of wide tiles: two
 constexpr int64_t kWideFill = 512;
-// Narrow tiles load past the caches where keys and values are more than the
-// 256 MB that the last of them holds: 271 MB 69.9 us a call for 72.5 through
-// them, but 41 MB 25.2 us for 22.4.
+// Narrow tiles load past the caches where prefix and cache slots are more than
+// the 256 MB that the last of them holds. The rule goes by room (lengths are on
+// the device): it gains where much of the room is in use, and loses where
+// little is, so that what calls in turn read would have stayed. A call through
+// them and past them, two sets of caches in turn: 16 sequences, 4 kv heads of
+// 128, 16384 positions: 16000 each 99.8 and 89.1 us, 1000 16.7 and 15.1; 64
+// sequences, 8 kv heads, 4096 positions: 2000 each 107.7 and 104.6 us, 500
+// 32.6 and 37.9, 100 17.1 and 16.5.
 constexpr int64_t kPastBytes = int64_t{256} << 20;
 // rows from which a wave of the join takes one of its own: 32 waves per CU
 constexpr int64_t kJoinWaves = 8192;
 // keys of a wide tile's piece at least: shorter ones cost more in the join
-// than they gain (own keys in one piece need none)
+// than they gain (own keys in one piece need none). Own pieces go by room too:
+// 40 queries of 32 heads over 4 after 160 keys take 14.5 us in a cache of 512
+// positions and 25 in one of 16384, after 3960 keys 26.8 in 4096 and 27.9.
 constexpr int64_t kWidePrefixKeys = 256;
 constexpr int64_t kWideOwnKeys = 512;
 // workgroups for a prompt's weights, twice what runs at a time, as those of
@@ -1582,8 +1589,8 @@ template <bool F16, int HD, int RT, bool PAST, bool ANY>
 hipError_t launch_tiles(const CacheAttnArgs& a, const Plan& pl, const Grids& gr, hipStream_t stream) {
   const int np = static_cast<int>(gr.p_wide), no = static_cast<int>(gr.o_wide), n = static_cast<int>(gr.narrow);
   const dim3 wg(kThreads);
-  // (heads beyond 128: a wide workgroup fills a CU's LDS, and so would narrow
-  // ones in its grid)
+  // (heads beyond 128: a wide workgroup takes all registers of a CU, and so
+  // would narrow ones in its grid)
   if (HD <= 128 && pl.p_wide && n > 0) {
     const int groups = (np + 7) / 8 + (n + 7) / 8;
     if constexpr (HD <= 128)

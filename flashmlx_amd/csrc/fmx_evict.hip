@@ -305,8 +305,9 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
 // block reads lies behind all that earlier blocks wrote, and what it writes is
 // read by no later block: only a block's own reads have to end before its
 // writes begin. Bound by that chain of blocks, so rows are sliced until 512
-// workgroups run: 80 us for 16 sequences of 16384 cut to 4000
-// positions, the selection included; one of 16384 cut to 8192, 60 us.
+// workgroups run: 79 us for 16 sequences of up to 16384 cut to
+// 4000 positions, the selection included; one of 16384 cut to 8192, 57 us, 32
+// workgroups for what a copy moves in 7.
 template <int VB>
 __global__ __launch_bounds__(kMoveThreads) void evict_shift_kernel(EvictArgs a, int slices, int slice_units) {
   typedef typename Unit<VB>::T T;

@@ -13,12 +13,11 @@
 // the rows of one or a few tokens (or a part of one token's), its loads are
 // issued first, then its threads form the tokens' cosines and sines once for
 // all heads in LDS while the loads are in flight; only as much LDS as those
-// take (16 KB for every workgroup: 18.1 us for the 15.4 below). 4099 tokens of
-// 32 heads of 128, half of each turned, fp16: 15.4 us for 67 MB, 4.4 TB/s (4.9
-// is a large copy's); 2 x 777 tokens of
-// 16 heads in fp32: 7.7 us for 25 MB. Eight decoded
-// tokens take 4.3 us, a launch and one chain of loads, fp64 products and
-// stores.
+// take (16 KB for every workgroup: 18.1 us for the 15.5 below). 4099 tokens of
+// 32 heads of 128, half of each turned, fp16: 15.5 us alone for 67 MB, 4.3
+// TB/s, and 14.1 a call among others, 4.8 (4.9 is a large copy's); 2 x 777
+// tokens of 16 heads in fp32: 7.6 us for 25 MB. Eight decoded tokens take 4.6
+// us, a launch and one chain of loads, fp64 products and stores.
 #include <algorithm>
 
 #include "fmx_cache_kernels.hpp"

@@ -105,7 +105,9 @@ int fmx_rope(const fmx_rope_angles* angles, int dtype, int64_t batch, int64_t se
  * slots[b] (device int32 [batch], distinct; NULL: slot b). A row whose slot
  * is outside [0, n_slots) or whose position is outside [0, max_seq) is not
  * written. positions as in fmx_rope: a key's cache position and its rotary
- * position need not agree. q_out may be q itself, with the same strides. */
+ * position need not agree. q_out may be q itself, with the same strides, if no
+ * new key or value is among its rows. (FMX_F32 caches: the attentions and the
+ * eviction below take 16-bit ones.) */
 int fmx_rope_append(const fmx_rope_angles* angles, int dtype, int64_t batch, int64_t seq_len,
                     int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const fmx_heads* q,
                     const fmx_heads* k, const fmx_heads* v, const int32_t* positions,
@@ -123,7 +125,9 @@ int fmx_rope_append(const fmx_rope_angles* angles, int dtype, int64_t batch, int
  * their data 16-byte aligned, strides multiples of 8, and the token strides
  * of keys and values at most 2^24. Calls whose work takes a launch of 2^32
  * threads or more are refused (FMX_ERR_UNSUPPORTED): those of 2^26 query rows
- * (batch * seq_len * n_heads) and of about 2^24 pairs of sequence and kv head. */
+ * (batch * seq_len * n_heads) and of about 2^24 pairs of sequence and kv head.
+ * Scores, weights and sums are fp32; in the products with the values a weight
+ * has 16 bits (bf16) or 22 (float16), whatever the number of rows. */
 typedef struct fmx_attention_shape {
   int32_t dtype;
   int64_t batch;
@@ -167,7 +171,9 @@ int fmx_attention_shared_prefix(const fmx_attention_shape* shape, const fmx_head
  * (the weights that fmx_cache_evict goes by). weights fp32
  * [n_slots, n_kv_heads, max_seq], contiguous; weights_in NULL: 0;
  * weights_out may be weights_in. Positions that no query sees keep
- * weights_in's value; slots of no sequence are not written. slots distinct.
+ * weights_in's value (all do with seq_len 0); slots of no sequence are not
+ * written. slots distinct. A slot's row starts from 0 when another sequence
+ * takes it: the caller clears it.
  * The sums are in a fixed order: equal calls give equal bits. */
 size_t fmx_attention_scored_workspace_size(const fmx_attention_shape* shape, int64_t max_seq);
 int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q,
