@@ -486,7 +486,9 @@ int fmx_attention_scored(const fmx_attention_shape* shape, const fmx_heads* q, c
   a.w_in = weights_in;
   a.w_out = weights_out;
   if (shape->seq_len == 0) {  // no weights to add
-    if (weights_out && weights_out != weights_in) FMX_HIP(launch_cache_weights_kept(a, stream));
+    if (!weights_out || weights_out == weights_in) return ok();
+    FMX_RC(check_launches(a));
+    FMX_HIP(launch_cache_weights_kept(a, stream));
     return ok();
   }
   fmx_heads q_v, out_v, kc_v, vc_v;

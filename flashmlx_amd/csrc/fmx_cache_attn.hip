@@ -1683,13 +1683,18 @@ hipError_t launch(const CacheAttnArgs& a, void* ws, hipStream_t stream) {
 
 size_t cache_attn_workspace(const CacheAttnArgs& a) { return make_plan(a, nullptr).bytes; }
 
-bool cache_attn_fits(const CacheAttnArgs& a) { return make_grids(a, make_plan(a, nullptr).pl).fits; }
+// no queries: one launch over the weights' rows
+static int64_t kept_tiles(const CacheAttnArgs& a) { return (a.S + kThreads - 1) / kThreads; }
+
+bool cache_attn_fits(const CacheAttnArgs& a) {
+  if (a.L == 0) return kept_tiles(a) * a.nkv * a.B <= max_blocks(kThreads);
+  return make_grids(a, make_plan(a, nullptr).pl).fits;
+}
 
 hipError_t launch_cache_weights_kept(const CacheAttnArgs& a, hipStream_t stream) {
-  const int64_t tiles = (a.S + kThreads - 1) / kThreads, grid = tiles * a.nkv * a.B;
-  if (grid > max_blocks(kThreads)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(attn_weights_sum_kernel, dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a, Plan{},
-                     static_cast<int>(tiles));
+  const dim3 grid(static_cast<uint32_t>(kept_tiles(a) * a.nkv * a.B));
+  hipLaunchKernelGGL(attn_weights_sum_kernel, grid, dim3(kThreads), 0, stream, a, Plan{},
+                     static_cast<int>(kept_tiles(a)));
   return hipGetLastError();
 }
 

@@ -82,6 +82,7 @@ def test_launches_beyond_the_device(lib):
     for kw in (dict(B=1 << 20, nh=16, nkv=16), dict(B=1 << 17, nh=128, nkv=128), dict(B=1 << 19, nh=128, nkv=8, hd=8)):
         assert _shared(lib, _shape(**kw), n_slots=1, slots=one) == unsup, kw
         assert _scored(lib, _shape(**kw), n_slots=1, slots=one) == unsup, kw
+    assert _scored(lib, _shape(B=1 << 10, L=0, nh=16, nkv=16), n_slots=1, S=1 << 24, slots=one) == unsup
     # the weights of a prompt in a cache far longer than it
     assert _scored(lib, _shape(B=1 << 10, L=64, nh=16, nkv=16, hd=8), n_slots=1, S=1 << 24, slots=one) == unsup
     assert _evict(lib, B=1 << 22, nkv=1, n_slots=1, slots=one) == unsup
