@@ -321,8 +321,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     _tensor(lengths, "lengths")
     if lengths.dim() != 1:
         raise ValueError(f"lengths: shape {tuple(lengths.shape)}, expected [batch]")
-    if budget < 1:
-        raise ValueError(f"budget {budget}")
+    if not 1 <= budget <= 1 << 24:  # (before `kept` of so many positions is made)
+        raise ValueError(f"budget {budget} (1 .. 2^24)")
     B = lengths.shape[0]
     ko = vo = wo = None
     S_out = 0

@@ -160,3 +160,14 @@ def test_evict_without_kept_positions(gpu, fmx, in_place, own_workspace):
         torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert torch.equal(lens_got, lens_want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("budget", [0, -1, (1 << 24) + 1, 1 << 40])
+def test_evict_refuses_a_budget_before_memory_is_taken(gpu, fmx, budget):
+    kc = torch.zeros((2, 2, 9, 8), dtype=torch.bfloat16, device="cuda")
+    w, lens = torch.zeros((2, 2, 9), device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.max_memory_allocated()
+    with pytest.raises(ValueError, match="budget"):
+        fmx.cache_evict(kc, kc.clone(), w, lens, budget)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
