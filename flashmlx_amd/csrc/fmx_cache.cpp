@@ -147,7 +147,8 @@ int check_written(const fmx_heads& v, const char* name, int64_t nb, int64_t nt, 
 // (they may well lie among each other, as in [slot, position, 2, head, element]).
 int check_apart(const fmx_heads& k, const fmx_heads& v, const char* name, int64_t hd, int es) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(k.data), b = reinterpret_cast<uintptr_t>(v.data);
-  const bool alike = k.batch_stride == v.batch_stride && k.token_stride == v.token_stride && k.head_stride == v.head_stride;
+  const bool alike =
+      k.batch_stride == v.batch_stride && k.token_stride == v.token_stride && k.head_stride == v.head_stride;
   if (a == b || (alike && (a < b ? b - a : a - b) < static_cast<uintptr_t>(hd * es)))
     return fail(FMX_ERR_ARG, "%s: keys and values overlap", name);
   return FMX_OK;

@@ -104,9 +104,10 @@ struct Plan {
 // Pieces of the own keys, found by every workgroup from the device's lengths:
 // sequence b has u_b = ceil(keys / kPiece) units and ceil(u_b / c) pieces of c
 // units, c the smallest that keeps all pieces within the grid: sum u_b / (grid
-// - B) rounded up, or all of the longest possible sequence's. Lengths may differ as they like: all pieces but each
-// sequence's last are equally long. Returns the sequence of piece w (-1:
-// none), its piece number in *k and c in *units; workgroup 0 leaves the table.
+// - B) rounded up, or all of the longest possible sequence's. Lengths may
+// differ as they like: all pieces but each sequence's last are equally long.
+// Returns the sequence of piece w (-1: none), its piece number in *k and c in
+// *units; workgroup 0 leaves the table.
 struct PieceLds {
   uint32_t tmp[kWaves + 1];
   int seq, k;
@@ -573,11 +574,11 @@ void attn_narrow_kernel(CacheAttnArgs a, Plan pl, int n_prefix) {
 // in narrow tiles, so that a row's precision does not hang on how many rows its
 // call has. That is half of all matrix work again (59 -> 71 us for the prompt
 // below, 126 -> 145 us a call of 128 sequences behind 32768 positions; the
-// figures given for choices further down are from before), but one number alone, off by
-// up to 2^-8 or 2^-11 of the weight, moves a row with one dominating key by a
-// step of the output. The maximum is only raised when a score lies more than
-// kLazy above it: the weights reach 2^kLazy times kBias' 2^8 at most, in fp16
-// 2^14 of 65504.
+// figures given for choices further down are from before), but one number
+// alone, off by up to 2^-8 or 2^-11 of the weight, moves a row with one
+// dominating key by a step of the output. The maximum is only raised when a
+// score lies more than kLazy above it: the weights reach 2^kLazy times kBias'
+// 2^8 at most, in fp16 2^14 of 65504.
 //
 // Bound by a wave's own chain: by the cycle counter a step of 64 keys took it
 // about 3000 cycles before the second product (issuing the next loads 500,
@@ -1581,7 +1582,8 @@ Grids make_grids(const CacheAttnArgs& a, const Plan& pl) {
   }
   // (wide and narrow ones may share a launch)
   const int64_t most = max_blocks(kThreads);
-  gr.fits = gr.p_wide + gr.o_wide + gr.narrow + 16 <= most && gr.join_all <= most && gr.w_grid <= most && gr.w_sum <= most;
+  gr.fits = gr.p_wide + gr.o_wide + gr.narrow + 16 <= most && gr.join_all <= most && gr.w_grid <= most &&
+            gr.w_sum <= most;
   return gr;
 }
 

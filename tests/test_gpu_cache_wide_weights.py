@@ -37,9 +37,11 @@ def _setup(dt, B, L, nh, nkv, hd, P, S, late):
 
 
 SHAPES = [
-    # B, L, nh, nkv, hd, P, S: own keys in one piece, in several
+    # B, L, nh, nkv, hd, P, S: many rows, own keys in one piece, in several
     (1, 40, 4, 1, 128, 0, 300), (2, 40, 4, 2, 64, 0, 300), (1, 40, 4, 1, 256, 0, 300), (1, 40, 4, 1, 72, 0, 300),
     (1, 40, 4, 1, 64, 0, 1030), (1, 1, 48, 1, 128, 0, 300),
+    # few rows, which run in narrow tiles
+    (1, 1, 4, 1, 128, 0, 300), (7, 1, 4, 1, 128, 200, 40), (8, 1, 4, 1, 64, 200, 40), (2, 5, 6, 2, 256, 200, 40),
     # a prefix with own keys in narrow tiles of one and two row sets, in wide ones, with none
     (40, 1, 4, 1, 128, 200, 40), (10, 5, 4, 1, 128, 200, 40), (3, 40, 4, 1, 64, 200, 60), (40, 1, 4, 1, 128, 200, 0),
     (40, 1, 4, 1, 256, 600, 40), (20, 2, 6, 3, 80, 300, 33),
