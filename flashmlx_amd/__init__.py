@@ -23,6 +23,12 @@ from .moe import (  # noqa: F401
     synth_normal_bf16,
     synth_normal_bf16_device,
 )
+from .ssm import (  # noqa: F401
+    SsmLayer,
+    causal_conv,
+    gated_norm,
+    ssm_scan,
+)
 
 __all__ = [
     "FmxError",
@@ -32,16 +38,20 @@ __all__ = [
     "QWeight",
     "Rope",
     "RopeConfig",
+    "SsmLayer",
     "attention_scored",
     "attention_shared_prefix",
     "cache_evict",
+    "causal_conv",
     "dequantize",
+    "gated_norm",
     "gather_qmm",
     "load",
     "moe_sort",
     "quantize",
     "quantized_matmul",
     "router_topk",
+    "ssm_scan",
     "synth_normal_bf16",
     "synth_normal_bf16_device",
 ]

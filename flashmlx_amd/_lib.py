@@ -178,6 +178,45 @@ class FmxAttentionShape(C.Structure):
     ]
 
 
+class FmxSsmShape(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("batch", C.c_int64),
+        ("seq_len", C.c_int64),
+        ("n_heads", C.c_int64),
+        ("head_dim", C.c_int64),
+        ("n_groups", C.c_int64),
+        ("state_dim", C.c_int64),
+        ("dt_softplus", C.c_int32),
+        ("dt_min", C.c_float),
+        ("dt_max", C.c_float),
+    ]
+
+
+class FmxSsmLayer(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("n_heads", C.c_int64),
+        ("head_dim", C.c_int64),
+        ("n_groups", C.c_int64),
+        ("state_dim", C.c_int64),
+        ("taps", C.c_int64),
+        ("activation", C.c_int32),
+        ("conv_weight", C.c_void_p),
+        ("conv_bias", C.c_void_p),
+        ("a", C.c_void_p),
+        ("d", C.c_void_p),
+        ("dt_bias", C.c_void_p),
+        ("dt_softplus", C.c_int32),
+        ("dt_min", C.c_float),
+        ("dt_max", C.c_float),
+        ("norm_weight", C.c_void_p),
+        ("norm_groups", C.c_int64),
+        ("eps", C.c_float),
+        ("gate_first", C.c_int32),
+    ]
+
+
 class FmxError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"{STATUS_NAMES.get(status, status)}: {message}")
@@ -364,6 +403,24 @@ _SIGS = {
         C.c_int,
         [C.c_int] + [C.c_int64] * 3 + [_H, _H, C.c_void_p] + [C.c_int64] * 2 + [C.c_void_p] * 2 + [C.c_int64] * 3 +
         [_H, _H, C.c_void_p, C.c_int64] + [C.c_void_p] * 3 + [C.c_size_t, C.c_void_p]),
+    # the state space layer's operators (include/fmx_ssm.h)
+    "fmx_causal_conv": (
+        C.c_int,
+        [C.c_int] + [C.c_int64] * 4 + [C.c_int, _H] + [C.c_void_p] * 4 + [C.c_int64] + [C.c_void_p] * 2 +
+        [_H, C.c_void_p]),
+    "fmx_ssm_scan_workspace_size": (C.c_size_t, [P(FmxSsmShape)]),
+    "fmx_ssm_scan": (
+        C.c_int,
+        [P(FmxSsmShape), _H, _H, C.c_void_p, _H, _H] + [C.c_void_p] * 4 + [C.c_int64] + [C.c_void_p] * 2 +
+        [_H, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fmx_gated_norm": (
+        C.c_int,
+        [C.c_int] + [C.c_int64] * 4 + [C.c_float, C.c_int, _H, _H] + [C.c_void_p] * 2 + [_H, C.c_void_p]),
+    "fmx_ssm_step_workspace_size": (C.c_size_t, [P(FmxSsmLayer), C.c_int64]),
+    "fmx_ssm_step": (
+        C.c_int,
+        [P(FmxSsmLayer), C.c_int64, _H, _H, _H, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, _H, C.c_void_p,
+         C.c_size_t, C.c_void_p]),
 }
 
 FMX_STATUS_WAIT_TIMEOUT = 1

@@ -37,6 +37,11 @@ SOURCES = [
     "csrc/fmx_cache_attn.hip",
     "csrc/fmx_evict.hip",
     "csrc/fmx_cache.cpp",
+    "csrc/fmx_ssm_conv.hip",
+    "csrc/fmx_ssm_scan.hip",
+    "csrc/fmx_ssm_step.hip",
+    "csrc/fmx_ssm_norm.hip",
+    "csrc/fmx_ssm.cpp",
 ]
 
 ARCH = os.environ.get("FMX_OFFLOAD_ARCH", "gfx950")

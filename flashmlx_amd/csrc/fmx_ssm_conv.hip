@@ -1,0 +1,127 @@
+// fmx_ssm_conv.hip -- the short causal convolution of the state space layer
+// (the mixer's conv1d, server/src/nemotron_h.cpp):
+//   out[t] = act(bias + sum over k of w[k] x[t - taps + 1 + k])  per channel
+//
+// Bound by HBM: every element is read and written once. A thread takes one
+// vector of channels over a run of tokens, whose taps - 1 rows before it it
+// reads again (from the caches); neighbouring threads take neighbouring
+// channels. The thread of a sequence's first run also keeps the state, so that
+// state_out may be state_in: nobody else reads it.
+#include "fmx_ssm_kernels.hpp"
+
+namespace fmx {
+
+namespace {
+
+constexpr int kConvThreads = 256;
+// tokens of a run: at least taps - 1, so that only a sequence's first run
+// reaches into the state
+constexpr int kConvRun = 8;
+static_assert(kConvRun >= kMaxTaps - 1, "a run's rows before it are one run's");
+
+template <int DT, int VEC, int K>
+__global__ __launch_bounds__(kConvThreads) void conv_kernel(ConvArgs a, uint32_t per_seq, uint32_t total) {
+  typedef typename El<DT>::T T;
+  typedef Pack<T, VEC> V;
+  const uint32_t id = blockIdx.x * kConvThreads + threadIdx.x;
+  if (id >= total) return;
+  const uint32_t cvs = static_cast<uint32_t>(a.C) / VEC;
+  const int b = static_cast<int>(id / per_seq);
+  const uint32_t rest = id - b * per_seq;
+  const int t0 = static_cast<int>(rest / cvs) * kConvRun;
+  const int ch = static_cast<int>(rest % cvs) * VEC;
+  const int len = seq_length(a.lens, a.L, b);
+  if (t0 >= len && t0 > 0) return;
+  const int64_t slot = K > 1 ? seq_slot(a.slots, a.n_slots, b) : -1;
+  const T* x = static_cast<const T*>(a.x.p) + b * a.x.bs + ch;
+  T* out = static_cast<T*>(a.out.p) + b * a.out.bs + ch;
+  const int64_t state0 = slot * (K - 1) * a.C + ch;
+  const T* s_in = slot >= 0 && a.s_in ? static_cast<const T*>(a.s_in) + state0 : nullptr;
+  V zero{};
+
+  V rows[kConvRun + K - 1];
+#pragma unroll
+  for (int i = 0; i < kConvRun + K - 1; ++i) {
+    const int t = t0 - (K - 1) + i;
+    rows[i] = zero;
+    if (t < 0) {
+      if (s_in) rows[i] = *reinterpret_cast<const V*>(s_in + static_cast<int64_t>(i) * a.C);
+    } else if (t < len) {
+      rows[i] = *reinterpret_cast<const V*>(x + t * a.x.ts);
+    }
+  }
+  V w[K], bias = zero;  // [channel][tap], in a row
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    w[k] = *reinterpret_cast<const V*>(static_cast<const T*>(a.w) + static_cast<int64_t>(ch) * K + k * VEC);
+  if (a.bias) bias = *reinterpret_cast<const V*>(static_cast<const T*>(a.bias) + ch);
+
+#pragma unroll
+  for (int r = 0; r < kConvRun; ++r) {
+    if (t0 + r >= len) break;
+    V y;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float acc = El<DT>::ld(bias.e[e]);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        acc = __builtin_fmaf(El<DT>::ld(w[(e * K + k) / VEC].e[(e * K + k) % VEC]), El<DT>::ld(rows[r + k].e[e]), acc);
+      y.e[e] = El<DT>::st(a.silu ? silu_f32(acc) : acc);
+    }
+    *reinterpret_cast<V*>(out + (t0 + r) * a.out.ts) = y;
+  }
+
+  if (K > 1 && t0 == 0 && slot >= 0 && a.s_out) {
+    T* s_out = static_cast<T*>(a.s_out) + state0;
+    // rows of the old state move to lower places only: in order, none is lost
+    for (int j = 0; j < K - 1; ++j) {
+      const int t = len - (K - 1) + j;
+      V v = zero;
+      if (t >= 0)
+        v = *reinterpret_cast<const V*>(x + t * a.x.ts);
+      else if (s_in)
+        v = *reinterpret_cast<const V*>(s_in + static_cast<int64_t>(t + K - 1) * a.C);
+      *reinterpret_cast<V*>(s_out + static_cast<int64_t>(j) * a.C) = v;
+    }
+  }
+}
+
+int64_t conv_threads(const ConvArgs& a, int vec) {
+  const int64_t runs = std::max<int64_t>(1, (static_cast<int64_t>(a.L) + kConvRun - 1) / kConvRun);
+  return a.B * runs * (a.C / vec);
+}
+
+template <int DT, int VEC>
+hipError_t conv(const ConvArgs& a, hipStream_t stream) {
+  const int64_t total = conv_threads(a, VEC);
+  if (total == 0) return hipSuccess;
+  const dim3 grid(static_cast<uint32_t>((total + kConvThreads - 1) / kConvThreads)), wg(kConvThreads);
+  const uint32_t per_seq = static_cast<uint32_t>(total / a.B), n = static_cast<uint32_t>(total);
+  switch (a.taps) {
+#define FMX_CONV(K) \
+  case K: hipLaunchKernelGGL((conv_kernel<DT, VEC, K>), grid, wg, 0, stream, a, per_seq, n); break;
+    FMX_CONV(1) FMX_CONV(2) FMX_CONV(3) FMX_CONV(4) FMX_CONV(5) FMX_CONV(6) FMX_CONV(7) FMX_CONV(8)
+#undef FMX_CONV
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+bool conv_fits(const ConvArgs& a) {
+  return conv_threads(a, 1) <= max_blocks(kConvThreads) * kConvThreads;
+}
+
+hipError_t launch_conv(const ConvArgs& a, int dt, hipStream_t stream) {
+  // 16-byte vectors where every array falls on them, single elements otherwise
+  const int es = dt == kElF32 ? 4 : 2, vec = 16 / es;
+  bool wide = a.C % vec == 0 && on_vectors(a.x, es, vec) && on_vectors(a.out, es, vec);
+  for (const void* p : {a.w, a.bias, a.s_in, static_cast<const void*>(a.s_out)})
+    wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  if (dt == kElF32) return wide ? conv<kElF32, 4>(a, stream) : conv<kElF32, 1>(a, stream);
+  if (dt == kElF16) return wide ? conv<kElF16, 8>(a, stream) : conv<kElF16, 1>(a, stream);
+  return wide ? conv<kElBf16, 8>(a, stream) : conv<kElBf16, 1>(a, stream);
+}
+
+}  // namespace fmx

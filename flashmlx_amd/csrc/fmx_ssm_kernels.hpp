@@ -1,0 +1,151 @@
+// fmx_ssm_kernels.hpp -- argument blocks, launchers and shared device code of
+// the state space layer's operators (fmx_ssm_conv.hip, fmx_ssm_scan.hip,
+// fmx_ssm_step.hip, fmx_ssm_norm.hip; library-internal).
+#pragma once
+
+#include "fmx_cache_kernels.hpp"
+#include "fmx_dev.hpp"
+
+namespace fmx {
+
+enum { kElBf16 = 0, kElF16 = 1, kElF32 = 2 };
+
+// an element type's loads and stores
+template <int DT>
+struct El {
+  typedef uint16_t T;
+  static __device__ inline float ld(T v) { return Act<DT == kElF16>::ld(v); }
+  static __device__ inline T st(float f) { return Act<DT == kElF16>::st(f); }
+};
+template <>
+struct El<kElF32> {
+  typedef float T;
+  static __device__ inline float ld(T v) { return v; }
+  static __device__ inline T st(float f) { return f; }
+};
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T e[N];
+};
+
+// v sigmoid(v): hardware exponential and reciprocal, a few steps of 2^-24
+__device__ inline float silu_f32(float v) {
+  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * 1.4426950408889634f));
+}
+
+// whether a view's rows start on vectors of vec elements of es bytes
+inline bool on_vectors(const HeadsView& v, int es, int vec) {
+  return !v.p || (reinterpret_cast<uintptr_t>(v.p) % (es * vec) == 0 && v.bs % vec == 0 && v.ts % vec == 0);
+}
+
+__device__ inline int seq_length(const int32_t* lens, int L, int b) {
+  return lens ? min(max(lens[b], 0), L) : L;
+}
+
+// ------------------------------------------------------------------ convolution
+
+constexpr int kMaxTaps = 8;
+
+struct ConvArgs {
+  int B, L, C, taps, silu;
+  HeadsView x, out;
+  const void* w;
+  const void* bias;
+  const void* s_in;
+  void* s_out;
+  int64_t n_slots;
+  const int32_t* lens;
+  const int32_t* slots;
+};
+bool conv_fits(const ConvArgs& a);
+hipError_t launch_conv(const ConvArgs& a, int dt, hipStream_t stream);
+
+// ------------------------------------------------------------------ scan
+
+constexpr int kScanMaxDim = 256;  // of a head, and of its state
+
+struct ScanArgs {
+  int B, L, nh, hd, groups, N, rep;
+  HeadsView x, dt, b, c, out;
+  const float* a;
+  const float* d;
+  const float* dt_bias;
+  int softplus;
+  float dt_min, dt_max;
+  const float* s_in;
+  float* s_out;
+  int64_t n_slots;
+  const int32_t* lens;
+  const int32_t* slots;
+};
+size_t scan_workspace(const ScanArgs& a);
+bool scan_fits(const ScanArgs& a);
+hipError_t launch_scan(const ScanArgs& a, bool f16, void* ws, hipStream_t stream);
+
+// the time step: ln(1 + e^v) = max(v, 0) + ln(1 + e^-|v|), which loses nothing
+// where e^v is small; comparisons that leave a NaN one
+__device__ inline float time_step(float raw, const float* bias, int h, int softplus, float lo, float hi) {
+  float v = bias ? raw + bias[h] : raw;
+  if (softplus) v = (v > 0.0f ? v : v == v ? 0.0f : v) + log1pf(expf(-fabsf(v)));
+  return v < lo ? lo : v > hi ? hi : v;
+}
+
+// ------------------------------------------------------------------ one token
+
+struct StepArgs {
+  int B, nh, hd, groups, N, rep, taps, silu, C;
+  HeadsView xbc, dt, z, out;
+  const void* conv_w;
+  const void* conv_b;
+  const float* a;
+  const float* d;
+  const float* dt_bias;
+  int softplus;
+  float dt_min, dt_max;
+  const void* norm_w;
+  int norm_groups;
+  float eps;
+  int gate_first;
+  void* conv_state;
+  float* state;
+  int64_t n_slots;
+  const int32_t* slots;
+};
+size_t step_workspace(const StepArgs& a);
+bool step_fits(const StepArgs& a);
+hipError_t launch_step(const StepArgs& a, bool f16, void* ws, hipStream_t stream);
+
+// ------------------------------------------------------------------ norm
+
+struct GatedNormArgs {
+  int B, L, C, groups;
+  float eps;
+  int gate_first;
+  HeadsView x, z, out;
+  const void* w;
+  const int32_t* lens;
+};
+bool gated_norm_fits(const GatedNormArgs& a);
+hipError_t launch_gated_norm(const GatedNormArgs& a, int dt, hipStream_t stream);
+
+// ------------------------------------------------------------------ a state's rows
+
+// Rows of a head's state in registers: lane j of LN neighbouring ones holds
+// columns 4 j .. 4 j + 3 of RP rows. One token:
+//   s = decay s + u b;  y = sum over the columns of c s, in the lanes' last one
+template <int LN, int RP>
+struct StateRows {
+  f32x4_t s[RP];
+
+  __device__ inline void step(float decay, const float* u, f32x4_t b, f32x4_t c, float* y) {
+#pragma unroll
+    for (int i = 0; i < RP; ++i) {
+      s[i] = s[i] * decay + u[i] * b;
+      const f32x4_t p = s[i] * c;
+      y[i] = tree_to_last<LN>((p[0] + p[1]) + (p[2] + p[3]), 0.0f, [](float a, float b) { return a + b; });
+    }
+  }
+};
+
+}  // namespace fmx
