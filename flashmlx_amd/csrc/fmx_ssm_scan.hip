@@ -17,6 +17,7 @@
 // each segment's state from 0, a second starts each segment from the sum of
 // those before it.
 #include <algorithm>
+#include <cstddef>
 
 #include "fmx_ssm_kernels.hpp"
 
@@ -188,12 +189,21 @@ __device__ inline int chunk_at(int row, int c) {
 
 // two floats as bf16, rounded, in one word
 __device__ inline uint32_t pack_bf16(float a, float b) {
-  return static_cast<uint32_t>(f32_to_bf16(a)) | static_cast<uint32_t>(f32_to_bf16(b)) << 16;
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
 __device__ inline float lo_bf16(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ inline float hi_bf16(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// Values as a sum of PARTS numbers of bf16 (8 bits each), in order
+template <bool F16>
+__device__ inline uint32_t pack_in(float a, float b) {
+  return F16 ? __builtin_bit_cast(uint32_t, f16x2_t{static_cast<_Float16>(a), static_cast<_Float16>(b)}) : pack_bf16(a, b);
+}
+
+// Values as a sum of PARTS numbers of bf16, in order: the first ones cut to 8
+// bits (an AND, which is the float as well as what is packed; a conversion and
+// its way back take 14 cycles a pair for 12), the last rounded. Three are exact.
 template <int PARTS>
 __device__ inline void split_bf16(const float* v, s16x8_t* part) {
   float rest[8];
@@ -204,10 +214,15 @@ __device__ inline void split_bf16(const float* v, s16x8_t* part) {
     u32x4_t w;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      w[j] = pack_bf16(rest[2 * j], rest[2 * j + 1]);
-      if (k + 1 < PARTS) {
-        rest[2 * j] -= lo_bf16(w[j]);
-        rest[2 * j + 1] -= hi_bf16(w[j]);
+      if (k + 1 == PARTS && PARTS < 3) {
+        w[j] = pack_bf16(rest[2 * j], rest[2 * j + 1]);
+      } else {
+        const uint32_t lo = __float_as_uint(rest[2 * j]), hi = __float_as_uint(rest[2 * j + 1]);
+        w[j] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+        if (k + 1 < PARTS) {
+          rest[2 * j] -= __uint_as_float(lo & 0xffff0000u);
+          rest[2 * j + 1] -= __uint_as_float(hi & 0xffff0000u);
+        }
       }
     }
     part[k] = __builtin_bit_cast(s16x8_t, w);
@@ -249,27 +264,57 @@ struct ChunkPlan {
   int keep_first;   // state_in is copied (state_out is the same array)
 };
 
-// What a chunk's tokens need, per slot and buffer. Sums of log2 e dt a from the
-// chunk's start as two floats: their differences are exact to 2^-24 of
-// themselves, however far the sums have run.
+// 16 bytes of each lane, at base + offset, to LDS, lane i's at byte `to` + 16 i;
+// masked lanes' stay.
+// (The builtin makes every later read of LDS wait for all loads in flight,
+// also of the buffer that no load writes: here the wait is the caller's. The
+// compiler sets m0 right before the instructions that it uses it for.)
+__device__ inline void to_lds16(const void* base, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
+               : "memory");
+}
+// a value that the compiler takes to be another one here, so that what is
+// formed from it is formed again rather than kept through a loop
+__device__ inline int afresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+// keeps what is read from LDS above it above it
+__device__ inline void read_first() { asm volatile("" ::: "memory"); }
+
+// What a chunk's tokens need, per slot. Sums of log2 e dt a are formed in 64
+// bits; from the chunk's start as two floats, whose differences are exact to
+// 2^-24 of themselves however far the sums have run.
+template <bool STATES>
 struct ChunkSteps {
-  float sum[kChunk], rest[kChunk], dt[kChunk];
-  float in[kChunk];    // dt times the decay from the token to the chunk's end
-  float out[kChunk];   // the decay from the chunk's start to the token
-  float decay;         // of the whole chunk
-  float pad[3];
+  float in[kChunk];         // dt times the decay from the token to the chunk's end
+  float decay, pad[3];      // of the whole chunk
+  float dt[kChunk];
+  float sum[kChunk], rest[kChunk];
+  float out[kChunk];        // the decay from the chunk's start to the token
+  float near[kChunk];       // the decay from the token before its 16 to the token
+  float far[16 + 32 + 48];  // dt times the decay from the token to the end of the 16 before 16 k: k = 1, 2, 3
 };
+template <>
+struct ChunkSteps<true> {
+  float in[kChunk];
+  float decay, pad[3];
+};
+__device__ inline int far_at(int k) { return 8 * k * (k - 1); }
+
+constexpr int kRound = 4;  // chunks whose steps are formed together, one by each wave of a slot
 
 template <int NK, int SLOTS, bool STATES>
 struct ChunkLds {
   static constexpr int kRow = NK * 64;  // bytes of a token's b or c
-  __attribute__((aligned(16))) uint8_t b[kChunk * kRow];
-  __attribute__((aligned(16))) uint8_t c[STATES ? 16 : kChunk * kRow];
-  __attribute__((aligned(16))) uint8_t x[SLOTS][kChunk * kTileRows * 2];
+  static constexpr int kBufs = NK > 4 && !STATES ? 1 : 2;
+  __attribute__((aligned(16))) uint8_t b[kBufs][kChunk * kRow];
+  __attribute__((aligned(16))) uint8_t x[kBufs][SLOTS][kChunk * kTileRows * 2];
+  __attribute__((aligned(16))) uint8_t c[STATES ? 1 : kBufs][STATES ? 16 : kChunk * kRow];
   // weights of the tokens s for token t, in two parts: rows t < 32 of 32
   // tokens, the others of 64
   __attribute__((aligned(16))) uint8_t m[STATES ? 1 : SLOTS][STATES ? 1 : 2][STATES ? 16 : 32 * 64 + 32 * 128];
-  ChunkSteps steps[2][SLOTS];
+  ChunkSteps<STATES> steps[2][kRound][SLOTS];
 };
 
 __device__ inline int weight_at(int t, int chunk) {
@@ -279,9 +324,11 @@ __device__ inline int weight_at(int t, int chunk) {
 // NK: 32-column steps of a state row. STATES: the first pass over segments,
 // which forms their states alone.
 template <bool F16, int NK, int SLOTS, bool STATES>
-__global__ __launch_bounds__(kSlotThreads* SLOTS, NK > 4 ? 2 : 4) void scan_chunk_kernel(ScanArgs a, ChunkPlan pl, float* seg_states, float* seg_decays) {
+__global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(ScanArgs a, ChunkPlan pl, float* seg_states,
+                                                                         float* seg_decays) {
   typedef ChunkLds<NK, SLOTS, STATES> Lds;
-  constexpr int kThreads = kSlotThreads * SLOTS;
+  constexpr int kThreads = kSlotThreads * SLOTS, kWaves = 4 * SLOTS;
+  constexpr int kBufs = Lds::kBufs;
   constexpr int CH = NK * 4;
   constexpr int NT = 2 * NK;  // 16-column tiles of a state row
   __shared__ Lds lds;
@@ -312,117 +359,133 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, NK > 4 ? 2 : 4) void scan_chun
   const int h = grp * a.rep + item / pl.tiles, row0 = item % pl.tiles * kTileRows;
   const int64_t pool = seq_slot(a.slots, a.n_slots, b);
 
-  // ---- loads of a chunk to registers, and from there to LDS
-  constexpr int kBc = NK > SLOTS ? NK / SLOTS : 1;  // vectors of a thread, of b and c each
-  constexpr int kBcVecs = kChunk * CH;
-  u32x4_t vb[kBc], vc[kBc], vx[2];
-  uint16_t vdt = 0;
+  // ---- a chunk's rows straight to LDS, each wave a few KB of each (a wave's
+  // loads of an array are kStep rows apart; their columns differ by what that
+  // changes in the swizzle)
+  constexpr int kBi = NK * 4 > kWaves ? NK * 4 / kWaves : 1;
+  constexpr int kStep = kWaves * 64 / CH;
+  static_assert(kBi == 1 || kStep % 8 == 0, "rows of a wave's loads");
+  const int b_row = (wave * 64 + lane) / CH, b_col = (lane % CH ^ swizzle<CH>(b_row)) * 8;
+  const int x_row = w4 * 16 + lane / 8, x_col = (lane % 8 ^ swizzle<8>(x_row)) * 8;
   const uint16_t* bp = static_cast<const uint16_t*>(a.b.p) + b * a.b.bs + grp * a.b.hs;
   const uint16_t* cp = STATES ? nullptr : static_cast<const uint16_t*>(a.c.p) + b * a.c.bs + grp * a.c.hs;
   const uint16_t* xp = static_cast<const uint16_t*>(a.x.p) + b * a.x.bs + h * a.x.hs + row0;
+  uint16_t* op = STATES ? nullptr : static_cast<uint16_t*>(a.out.p) + b * a.out.bs + h * a.out.hs + row0;
+  const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) Lds*)&lds));
+  bp += t_first * a.b.ts;
+  if (!STATES) cp += t_first * a.c.ts;
+  xp += t_first * a.x.ts;
+  if (!STATES) op += t_first * a.out.ts;
+  const uint32_t b_off = static_cast<uint32_t>(b_row * static_cast<int>(a.b.ts)) * 2;
+  const uint32_t c_off = STATES ? 0 : static_cast<uint32_t>(b_row * static_cast<int>(a.c.ts)) * 2;
+  const uint32_t x_off = static_cast<uint32_t>(x_row * static_cast<int>(a.x.ts)) * 2;
+  // (pointers go on by a chunk with each load)
+  auto load_rows = [&](const uint16_t*& from, uint32_t off, int64_t ts, int t0, uint32_t to) {  // of b or c
+#pragma unroll
+    for (int k = 0; k < kBi; ++k) {
+      const int col = b_col ^ (k * kStep / 4 % 4 * 8);
+      if ((NK * 4 >= kWaves || wave < NK * 4) && t0 + b_row + k * kStep < t_end && col < a.N)
+        to_lds16(from + k * kStep * ts, off + col * 2, to + (wave + k * kWaves) * 1024);
+    }
+    from += kChunk * ts;
+  };
+  auto load = [&](int t0, int buf) {
+    load_rows(bp, b_off, a.b.ts, t0, lds_at + offsetof(Lds, b) + buf * sizeof(lds.b[0]));
+    if (!STATES) load_rows(cp, c_off, a.c.ts, t0, lds_at + offsetof(Lds, c) + buf * sizeof(lds.c[0]));
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int col = x_col ^ (k * 16);
+      if (live && t0 + x_row + k * 8 < t_end && row0 + col < a.hd)
+        to_lds16(xp + k * 8 * a.x.ts, x_off + col * 2,
+                 lds_at + offsetof(Lds, x) + (buf * SLOTS + slot) * sizeof(lds.x[0][0]) + (w4 * 2 + k) * 1024);
+    }
+    xp += kChunk * a.x.ts;
+  };
+
+  // ---- the tokens' steps
+  const float rate = a.a[h], bias = a.dt_bias ? a.dt_bias[h] : 0.0f;
+  const float skip = !STATES && a.d ? a.d[h] : 0.0f;
   const uint16_t* dtp = static_cast<const uint16_t*>(a.dt.p) + b * a.dt.bs + h * a.dt.hs;
-  const u32x4_t zero{0, 0, 0, 0};
-  const bool steps_wave = live && w4 == 3;
-  auto load = [&](int t0) {
-#pragma unroll
-    for (int k = 0; k < kBc; ++k) {
-      const int v = tid + k * kThreads, row = v / CH, col = v % CH * 8;
-      vb[k] = zero;
-      vc[k] = zero;
-      if (v < kBcVecs && t0 + row < t_end && col < a.N) {
-        vb[k] = *reinterpret_cast<const u32x4_t*>(bp + (t0 + row) * a.b.ts + col);
-        if (!STATES) vc[k] = *reinterpret_cast<const u32x4_t*>(cp + (t0 + row) * a.c.ts + col);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int v = (tid & 255) + k * kSlotThreads, row = v / 8, col = v % 8 * 8;
-      vx[k] = zero;
-      if (live && t0 + row < t_end && row0 + col < a.hd)
-        vx[k] = *reinterpret_cast<const u32x4_t*>(xp + (t0 + row) * a.x.ts + col);
-    }
-    if (steps_wave) vdt = t0 + lane < t_end ? dtp[(t0 + lane) * a.dt.ts] : 0;
+  uint16_t vdt = 0;
+  auto load_dt = [&](int ck) {
+    const int t = t_first + ck * kChunk + lane;
+    vdt = t < t_end ? dtp[t * a.dt.ts] : 0;
   };
-  auto stage = [&]() {
-#pragma unroll
-    for (int k = 0; k < kBc; ++k) {
-      // columns 8 m .. 8 m + 7 of a 32-column step in the order in which an
-      // accumulator's rows come: 4 g + i beside 16 + 4 g + i
-      const int v = tid + k * kThreads, row = v / CH, m = v % 4, step = v % CH / 4;
-      if (v >= kBcVecs) continue;
-      const int half = (m >> 1) * 8;
-      const int at0 = chunk_at<CH>(row, step * 4 + 2 * (m & 1)) + half;
-      const int at1 = chunk_at<CH>(row, step * 4 + 2 * (m & 1) + 1) + half;
-      *reinterpret_cast<u32x2_t*>(lds.b + at0) = u32x2_t{vb[k][0], vb[k][1]};
-      *reinterpret_cast<u32x2_t*>(lds.b + at1) = u32x2_t{vb[k][2], vb[k][3]};
-      if (!STATES) {
-        *reinterpret_cast<u32x2_t*>(lds.c + at0) = u32x2_t{vc[k][0], vc[k][1]};
-        *reinterpret_cast<u32x2_t*>(lds.c + at1) = u32x2_t{vc[k][2], vc[k][3]};
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int v = (tid & 255) + k * kSlotThreads;
-      *reinterpret_cast<u32x4_t*>(lds.x[slot] + chunk_at<8>(v / 8, v % 8)) = vx[k];
-    }
-  };
-
-  // ---- the tokens' steps, formed by one wave of a slot: sums and their
-  // differences in 64 bits
-  const float rate = a.a[h], skip = a.d ? a.d[h] : 0.0f;
-  double seg_sum = 0.0;
-  auto steps = [&](int t0, int buf) {
-    const bool in = t0 + lane < t_end;
-    const float dt = in ? time_step(Act<F16>::ld(vdt), a.dt_bias, h, a.softplus, a.dt_min, a.dt_max) : 0.0f;
-    double sum = in ? static_cast<double>(dt) * static_cast<double>(rate) * 1.4426950408889634074 : 0.0;
-    sum = tree_to_last<64>(sum, 0.0, [](double x, double y) { return x + y; });
+  auto steps = [&](int ck) {
+    const bool in = t_first + ck * kChunk + lane < t_end;
+    const float dt = in ? time_step(Act<F16>::ld(vdt) + bias, nullptr, 0, a.softplus, a.dt_min, a.dt_max) : 0.0f;
+    const double own = in ? static_cast<double>(dt) * static_cast<double>(rate) * 1.4426950408889634074 : 0.0;
+    const double sum = tree_to_last<64>(own, 0.0, [](double x, double y) { return x + y; });  // (an inclusive scan)
     const double all = readlane_f64(sum, 63);
-    ChunkSteps& s = lds.steps[buf][slot];
-    const float lead = static_cast<float>(sum);
-    s.sum[lane] = lead;
-    s.rest[lane] = static_cast<float>(sum - static_cast<double>(lead));
-    s.dt[lane] = dt;
-    s.in[lane] = in ? dt * __builtin_amdgcn_exp2f(static_cast<float>(all - sum)) : 0.0f;
-    s.out[lane] = __builtin_amdgcn_exp2f(lead);
-    if (lane == 0) s.decay = __builtin_amdgcn_exp2f(static_cast<float>(all));
-    seg_sum += all;
+    auto power = [](double e) { return __builtin_amdgcn_exp2f(static_cast<float>(e)); };
+    ChunkSteps<STATES>& s = lds.steps[ck / kRound & 1][ck % kRound][slot];
+    s.in[lane] = in ? dt * power(all - sum) : 0.0f;
+    if (lane == 0) s.decay = power(all);
+    if constexpr (!STATES) {
+      const double at[3] = {readlane_f64(sum, 15), readlane_f64(sum, 31), readlane_f64(sum, 47)};
+      const float lead = static_cast<float>(sum);
+      s.dt[lane] = dt;
+      s.sum[lane] = lead;
+      s.rest[lane] = static_cast<float>(sum - static_cast<double>(lead));
+      s.out[lane] = __builtin_amdgcn_exp2f(lead);
+      s.near[lane] = power(lane < 16 ? sum : sum - at[max(g4, 1) - 1]);
+#pragma unroll
+      for (int k = 1; k < 4; ++k)
+        if (lane < 16 * k) s.far[far_at(k) + lane] = dt * power(at[k - 1] - sum);
+    }
   };
+  const u32x4_t zero{0, 0, 0, 0};
+  // What no load writes is 0, or of earlier tokens of the sequence: finite, or
+  // of a row that is NaN by now.
+  if (t_end - t_first < kBufs * kChunk || a.N < 32 * NK || a.hd % kTileRows != 0) {
+    for (int i = tid; i < static_cast<int>(sizeof(lds.b) / 16); i += kThreads) reinterpret_cast<u32x4_t*>(lds.b)[i] = zero;
+    for (int i = tid; i < static_cast<int>(sizeof(lds.x) / 16); i += kThreads) reinterpret_cast<u32x4_t*>(lds.x)[i] = zero;
+    if (!STATES)
+      for (int i = tid; i < static_cast<int>(sizeof(lds.c) / 16); i += kThreads) reinterpret_cast<u32x4_t*>(lds.c)[i] = zero;
+  }
+  if (!STATES) {  // tokens behind t in a step that t's own are in
+    for (int v = tid; v < SLOTS * 2 * 16 * 2; v += kThreads) {
+      const int c = v % 2, t = v / 2 % 16, part = v / 32 % 2, q = v / 64;
+      *reinterpret_cast<u32x4_t*>(lds.m[q][part] + weight_at(t, 2 + c)) = zero;
+      *reinterpret_cast<u32x4_t*>(lds.m[q][part] + weight_at(32 + t, 6 + c)) = zero;
+    }
+  }
+  lds_barrier();
+  if (chunks > 0) {
+    load(t_first, 0);
+    if (live && w4 < chunks) load_dt(w4);
+  }
 
-  // ---- the state: lane i16 has row i16 of its wave's 16, of the 16-column
-  // tile nt columns 16 nt + 4 g4 .. + 3
+  // ---- the state: lane i16 has row i16 of its wave's 16; of tile nt columns
+  // 32 (nt / 2) + 8 g4 + 4 (nt % 2) .. + 3, so that two tiles are 8 columns in
+  // a row, as an operand takes them
   f32x4_t S[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   const int p_row = row0 + 16 * w4 + i16;
-  const int64_t state0 = ((pool * a.nh + h) * a.hd + p_row) * a.N + 4 * g4;
+  const int64_t state0 = ((pool * a.nh + h) * a.hd + p_row) * a.N;
+  auto column = [&](int nt) { return 32 * (nt >> 1) + 8 * g4 + 4 * (nt & 1); };
   const int64_t head = (static_cast<int64_t>(b) * a.nh + h) * pl.tiles + item % pl.tiles;
   constexpr int kBlock = kTileRows * NK * 32;
   auto seg_state = [&](int s, int nt) {
     return reinterpret_cast<f32x4_t*>(seg_states + (head * pl.segs + s) * kBlock + ((nt * 4 + w4) * 64 + lane) * 4);
   };
-  bool begun = false;  // whether the state may be other than 0
   if (live) {
     if (seg == 0) {
-      const bool copied = !STATES && pl.keep_first && pl.segs > 1;
-      if (copied ? t_first + seg_len < len : false) {
-        // (written by the first pass; the array itself may have moved on)
+      if (!STATES && pl.keep_first && t_first + seg_len < len) {
+        // (copied by the first pass; the array itself may have moved on)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) S[nt] = *seg_state(pl.segs - 1, nt);
-        begun = true;
-      } else if (a.s_in && pool >= 0) {
-        begun = true;
-        if (p_row < a.hd) {
+      } else if (a.s_in && pool >= 0 && p_row < a.hd) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            if (16 * nt + 4 * g4 < a.N) S[nt] = *reinterpret_cast<const f32x4_t*>(a.s_in + state0 + 16 * nt);
-        }
+        for (int nt = 0; nt < NT; ++nt)
+          if (column(nt) < a.N) S[nt] = *reinterpret_cast<const f32x4_t*>(a.s_in + state0 + column(nt));
       }
       if (STATES && pl.keep_first) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) *seg_state(pl.segs - 1, nt) = S[nt];
       }
     } else if (!STATES) {
-      begun = true;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) S[nt] = *seg_state(0, nt);
       for (int s = 1; s < seg; ++s) {
@@ -432,125 +495,131 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, NK > 4 ? 2 : 4) void scan_chun
       }
     }
   }
+  if (live && w4 < chunks) steps(w4);
+  float seg_decay = 1.0f;
 
-  // ---- operands' places in LDS
-  int row_at[NK];  // 16 rows, one each lane: chunk 4 step + g4
-#pragma unroll
-  for (int kk = 0; kk < NK; ++kk) row_at[kk] = chunk_at<CH>(i16, 4 * kk + g4);
+  // ---- operands' places in LDS, from a buffer's start; a few registers, of
+  // which the others differ by a constant, added or (columns, swizzled) exclusive
   const int e4 = i16 >> 2, c4 = i16 & 3;
-  int col_at[NK][2];  // columns of 4 rows by 4: rows 8 g4 + e4, and 4 behind them
-#pragma unroll
-  for (int kk = 0; kk < NK; ++kk)
-#pragma unroll
-    for (int u = 0; u < 2; ++u) col_at[kk][u] = chunk_at<CH>(8 * g4 + 4 * u + e4, 4 * kk + c4);
-  int x_at[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-    x_at[u] = chunk_at<8>(8 * g4 + 4 * u + e4, 2 * w4 + (c4 >> 1)) + (c4 & 1) * 8;
-  const uint8_t* xs = lds.x[slot];
+  const int row_base = chunk_at<CH>(i16, g4);               // 16 rows, one each lane: columns 8 g4 .. + 7
+  const int col_base0 = chunk_at<CH>(8 * g4 + e4, c4);      // columns 8 c4 .. + 3 of row 8 g4 + e4
+  const int col_base1 = chunk_at<CH>(8 * g4 + 4 + e4, c4);  // and of the row 4 behind it
+  const int x_base0 = chunk_at<8>(8 * g4 + e4, 2 * w4 + (c4 >> 1)) + (c4 & 1) * 8;
+  const int x_base1 = chunk_at<8>(8 * g4 + 4 + e4, 2 * w4 + (c4 >> 1)) + (c4 & 1) * 8;
+  const int own_base = chunk_at<8>(i16, 2 * w4 + (g4 >> 1)) + (g4 & 1) * 8;  // rows 4 g4 .. + 3 of token i16
+  const int m_base0 = weight_at(i16, g4), m_base1 = weight_at(32 + i16, g4);
 
   // weights' tiles (tokens s, token t) of this wave, rows of t from the longest on
   const int tile0 = SLOTS == 2 ? (wave < 2 ? 2 * wave : wave + 2) : (wave < 2 ? 2 * wave : 3 * wave - 2);
   const int tile1 = SLOTS == 2 ? (wave < 2 ? tile0 + 2 : tile0 + 1) : (wave < 2 ? tile0 + 2 : tile0 + 3);
 
-  if (!STATES) {  // tokens behind t in a step that t's own are in
-    for (int v = tid; v < SLOTS * 2 * 16 * 2; v += kThreads) {
-      const int c = v % 2, t = v / 2 % 16, part = v / 32 % 2, q = v / 64;
-      *reinterpret_cast<u32x4_t*>(lds.m[q][part] + weight_at(t, 2 + c)) = zero;
-      *reinterpret_cast<u32x4_t*>(lds.m[q][part] + weight_at(32 + t, 6 + c)) = zero;
-    }
-  }
-
-  if (chunks > 0) {
-    load(t_first);
-    if (steps_wave) steps(t_first, 0);
-    stage();
-  }
-  lds_barrier();
-
+  wait_vmcnt0();
   for (int ck = 0; ck < chunks; ++ck) {
     const int t0 = t_first + ck * kChunk, nt_live = min(kChunk, t_end - t0);
+    const int buf = kBufs == 2 ? ck & 1 : 0;
     const bool more = ck + 1 < chunks;
-    const ChunkSteps& st = lds.steps[ck & 1][slot];
-    if (more) load(t0 + kChunk);
+    lds_barrier();  // the chunk's rows have landed, and every wave is done with the one before it
+    const int next = ck - ck % kRound + kRound + w4;  // of the next round, this wave's
+    if (live && ck % kRound == 0 && next < chunks) load_dt(next);
+    if (kBufs == 2 && more) load(t0 + kChunk, buf ^ 1);
+    const uint8_t* bs = lds.b[buf];
+    const uint8_t* xs = lds.x[buf][slot];
+    const ChunkSteps<STATES>* round = lds.steps[ck / kRound & 1][ck % kRound];
+    const ChunkSteps<STATES>& st = round[slot];
     f32x4_t y[4];
-    float most_s = 0.0f;  // of the state's magnitudes (float16)
-    if (F16 && live && begun) {
+    float most_s = 0.0f;  // of the state's magnitudes (float16), NaN aside
+    if (F16 && live) {
+      auto largest = [&]() {
+        most_s = 0.0f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) most_s = fmaxf(most_s, fabsf(S[nt][i]));
-      most_s = wave_max_f32(most_s);
+          for (int i = 0; i < 4; ++i) most_s = fmaxf(most_s, fabsf(S[nt][i]));
+        most_s = wave_max_f32(most_s);
+      };
+      largest();
+      if (__float_as_uint(most_s) >= 0x7f800000u) {  // (infinities would be every row's scale)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) S[nt] += S[nt] * 0.0f;
+        largest();
+      }
     }
-    bool slow = F16 && __float_as_uint(most_s) >= 0x7f800000u;
 
     if constexpr (!STATES) {
-      // ---- weights of the chunk's tokens: (c . b) times decay and step
-      for (int k = tile0; k < tile1; ++k) {
-        const int tt = k < 4 ? 3 : k < 7 ? 2 : k < 9 ? 1 : 0;
-        const int ss = k < 4 ? k : k < 7 ? k - 4 : k < 9 ? k - 7 : 0;
-        if (16 * tt >= nt_live) continue;
-        f32x4_t dot{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-          const s16x8_t fb = *reinterpret_cast<const s16x8_t*>(lds.b + row_at[kk] + ss * 16 * Lds::kRow);
-          const s16x8_t fc = *reinterpret_cast<const s16x8_t*>(lds.c + row_at[kk] + tt * 16 * Lds::kRow);
-          dot = mfma_in<F16>(fb, fc, dot);
-        }
-        const int t = 16 * tt + i16, s = 16 * ss + 4 * g4;
-#pragma unroll
-        for (int q = 0; q < SLOTS; ++q) {
-          if (q >= n_slots) break;
-          const ChunkSteps& sq = lds.steps[ck & 1][q];
-          const f32x4_t sum = *reinterpret_cast<const f32x4_t*>(sq.sum + s);
-          const f32x4_t rest = *reinterpret_cast<const f32x4_t*>(sq.rest + s);
-          const f32x4_t dt = *reinterpret_cast<const f32x4_t*>(sq.dt + s);
-          const float sum_t = sq.sum[t], rest_t = sq.rest[t];
-          float m[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float f = __builtin_amdgcn_exp2f((sum_t - sum[i]) + (rest_t - rest[i]));
-            m[i] = s + i <= t ? dot[i] * (f * dt[i]) : 0.0f;
-          }
-          const uint32_t h0 = pack_bf16(m[0], m[1]), h1 = pack_bf16(m[2], m[3]);
-          const uint32_t l0 = pack_bf16(m[0] - lo_bf16(h0), m[1] - hi_bf16(h0));
-          const uint32_t l1 = pack_bf16(m[2] - lo_bf16(h1), m[3] - hi_bf16(h1));
-          const int at = weight_at(t, 2 * ss + (g4 >> 1)) + (g4 & 1) * 8;
-          *reinterpret_cast<u32x2_t*>(lds.m[q][0] + at) = u32x2_t{h0, h1};
-          *reinterpret_cast<u32x2_t*>(lds.m[q][1] + at) = u32x2_t{l0, l1};
-        }
-      }
+      const uint8_t* cs = lds.c[buf];
+      const int row_at = afresh(row_base);
       // ---- what the state before the chunk gives: rows p, columns t
+      if (live) {
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) y[tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-      if (live && begun) {
+        for (int tt = 0; tt < 4; ++tt) y[tt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         float back = 1.0f;
         const float scale = F16 ? scale_of(most_s, &back) : 1.0f;
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
+          s16x8_t fc[4];
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt)
+            fc[tt] = *reinterpret_cast<const s16x8_t*>(cs + (row_at ^ 64 * kk) + tt * 16 * Lds::kRow);
           float v[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[i] = F16 ? S[2 * kk][i] * scale : S[2 * kk][i];
-            v[4 + i] = F16 ? S[2 * kk + 1][i] * scale : S[2 * kk + 1][i];
-          }
+          for (int i = 0; i < 8; ++i) v[i] = F16 ? S[2 * kk + i / 4][i % 4] * scale : S[2 * kk + i / 4][i % 4];
           s16x8_t part[2];
           if (F16)
             split_f16(v, part);
           else
             split_bf16<2>(v, part);
+          read_first();
 #pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
-            if (16 * tt >= nt_live) break;
-            const s16x8_t fc = *reinterpret_cast<const s16x8_t*>(lds.c + row_at[kk] + tt * 16 * Lds::kRow);
-            y[tt] = mfma_in<F16>(part[0], fc, y[tt]);
-            y[tt] = mfma_in<F16>(part[1], fc, y[tt]);
-          }
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) y[tt] = mfma_in<F16>(part[k], fc[tt], y[tt]);
         }
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          const float f = st.out[16 * tt + i16];
-          y[tt] *= F16 ? f * back : f;
+        for (int tt = 0; tt < 4; ++tt) y[tt] *= F16 ? st.out[16 * tt + i16] * back : st.out[16 * tt + i16];
+      }
+      // ---- weights of the chunk's tokens: (c . b) times decay and step
+      for (int k = tile0; k < tile1; ++k) {
+        const int tt = k < 4 ? 3 : k < 7 ? 2 : k < 9 ? 1 : 0;
+        const int ss = k < 4 ? k : k < 7 ? k - 4 : k < 9 ? k - 7 : 0;
+        f32x4_t dot{0.0f, 0.0f, 0.0f, 0.0f};
+        s16x8_t fb[NK], fc[NK];
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          fb[kk] = *reinterpret_cast<const s16x8_t*>(bs + (row_at ^ 64 * kk) + ss * 16 * Lds::kRow);
+          fc[kk] = *reinterpret_cast<const s16x8_t*>(cs + (row_at ^ 64 * kk) + tt * 16 * Lds::kRow);
+        }
+        read_first();
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) dot = mfma_in<F16>(fb[kk], fc[kk], dot);
+        const int t = 16 * tt + i16, s = 16 * ss + 4 * g4;
+#pragma unroll
+        for (int q = 0; q < SLOTS; ++q) {
+          if (q >= n_slots) break;
+          const ChunkSteps<STATES>& sq = round[q];
+          float m[4];
+          if (ss < tt) {
+            const f32x4_t far = *reinterpret_cast<const f32x4_t*>(sq.far + far_at(tt) + s);
+            const float near = sq.near[t];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = dot[i] * (far[i] * near);
+          } else {
+            const f32x4_t sum = *reinterpret_cast<const f32x4_t*>(sq.sum + s);
+            const f32x4_t rest = *reinterpret_cast<const f32x4_t*>(sq.rest + s);
+            const f32x4_t dt = *reinterpret_cast<const f32x4_t*>(sq.dt + s);
+            const float sum_t = sq.sum[t], rest_t = sq.rest[t];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float f = __builtin_amdgcn_exp2f((sum_t - sum[i]) + (rest_t - rest[i]));
+              // (by its bits: tokens behind t may hold anything)
+              m[i] = __uint_as_float(__float_as_uint(dot[i] * (f * dt[i])) & (s + i <= t ? 0xffffffffu : 0u));
+            }
+          }
+          const uint32_t h0 = __builtin_amdgcn_perm(__float_as_uint(m[1]), __float_as_uint(m[0]), 0x07060302u);
+          const uint32_t h1 = __builtin_amdgcn_perm(__float_as_uint(m[3]), __float_as_uint(m[2]), 0x07060302u);
+          auto low = [](float v) { return v - hi_bf16(__float_as_uint(v)); };
+          const int at = weight_at(t, 2 * ss + (g4 >> 1)) + (g4 & 1) * 8;
+          *reinterpret_cast<u32x2_t*>(lds.m[q][0] + at) = u32x2_t{h0, h1};
+          *reinterpret_cast<u32x2_t*>(lds.m[q][1] + at) = u32x2_t{pack_bf16(low(m[0]), low(m[1])), pack_bf16(low(m[2]), low(m[3]))};
         }
       }
       lds_barrier();  // the weights are in LDS
@@ -558,20 +627,47 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, NK > 4 ? 2 : 4) void scan_chun
 
     if (live) {
       // ---- the chunk's rows of x: lane i16 has row p, tokens 32 ks + 8 g4 + j
+      const int x_at0 = afresh(x_base0), x_at1 = afresh(x_base1);
       s16x8_t fx[2];
-      uint32_t odd = 0;  // values that are not finite
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        const s16x4_t lo = read_tr(xs + x_at[0] + ks * 32 * 128), hi = read_tr(xs + x_at[1] + ks * 32 * 128);
+        const s16x4_t lo = read_tr(xs + x_at0 + ks * 32 * 128), hi = read_tr(xs + x_at1 + ks * 32 * 128);
         fx[ks] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        const u32x4_t w = __builtin_bit_cast(u32x4_t, fx[ks]);
-        const uint32_t unit = F16 ? 0x04000400u : 0x00800080u;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) odd |= (w[j] & 0x7fff7fffu) + unit;
       }
-      slow = slow || ((!STATES || F16) && __any((odd & 0x80008000u) != 0));
-      float u[2][8];
-      float most_u = 0.0f;
+      uint32_t odd = 0;
+      constexpr uint32_t kUnit = F16 ? 0x04000400u : 0x00800080u;  // carries an exponent of ones into the sign
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const u32x4_t w = __builtin_bit_cast(u32x4_t, fx[ks]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) odd |= (w[j] & 0x7fff7fffu) + kUnit;
+      }
+      int from = kChunk;  // the token from which row i16 is NaN
+      const bool spoiled = __any((odd & 0x80008000u) != 0);
+      if (spoiled) {
+        // Values that are not finite, which the products would carry to the
+        // tokens before theirs as 0 times infinity: taken out, and their row
+        // NaN from their token on.
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          u32x4_t w = __builtin_bit_cast(u32x4_t, fx[ks]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t is = ((w[j] & 0x7fff7fffu) + kUnit) >> 15 & 0x00010001u;
+            w[j] &= ~((is << 16) - is);
+            const int t = 32 * ks + 8 * g4 + 2 * j;
+            from = min(from, t + kChunk - kChunk * static_cast<int>(is & 1));
+            from = min(from, t + 1 + kChunk - kChunk * static_cast<int>(is >> 16));
+          }
+          fx[ks] = __builtin_bit_cast(s16x8_t, w);
+        }
+        from = min(from, __shfl_xor(from, 16));
+        from = min(from, __shfl_xor(from, 32));
+        const float nan = from < kChunk ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) S[nt] += nan;
+      }
+      float u[8];  // what tokens 32 ks + 8 g4 + j bring
       auto incoming = [&](int ks) {
         const f32x4_t in0 = *reinterpret_cast<const f32x4_t*>(st.in + 32 * ks + 8 * g4);
         const f32x4_t in1 = *reinterpret_cast<const f32x4_t*>(st.in + 32 * ks + 8 * g4 + 4);
@@ -579,153 +675,126 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, NK > 4 ? 2 : 4) void scan_chun
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float x = j % 2 ? Act<F16>::hi(w[j / 2]) : Act<F16>::lo(w[j / 2]);
-          u[ks][j] = (j < 4 ? in0[j] : in1[j - 4]) * x;
+          u[j] = (j < 4 ? in0[j] : in1[j - 4]) * x;
         }
       };
       float unscale = 1.0f, scale = 1.0f;
       if constexpr (F16) {
+        float most = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
           incoming(ks);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) most_u = fmaxf(most_u, fabsf(u[ks][j]));
+          for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(u[j]));
         }
-        most_u = wave_max_f32(most_u);
-        const float most = fmaxf(most_u, most_s * st.decay);
-        slow = slow || __float_as_uint(most) >= 0x7f800000u;
-        scale = scale_of(most, &unscale);
+        most = wave_max_f32(most);
+        if (__float_as_uint(most) >= 0x7f800000u) {  // steps without end: every row's state
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4_t{most, most, most, most} * 0.0f;
+          most = 0.0f;
+        }
+        scale = scale_of(fmaxf(most, most_s * st.decay), &unscale);
       }
-      if (!slow) {
-        if constexpr (!STATES) {
-          // ---- what the chunk's own tokens give
-          s16x8_t xh[2], xl[2];
-          if (F16) {
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-              const u32x4_t w = __builtin_bit_cast(u32x4_t, fx[ks]);
-              float v[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = j % 2 ? Act<F16>::hi(w[j / 2]) : Act<F16>::lo(w[j / 2]);
-              s16x8_t part[2];
-              split_bf16<2>(v, part);
-              xh[ks] = part[0];
-              xl[ks] = part[1];
-            }
-          } else {
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) xh[ks] = fx[ks];
-          }
-#pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
-            if (16 * tt >= nt_live) break;
-#pragma unroll
-            for (int ks = 0; ks <= tt / 2; ++ks) {
-              const int at = weight_at(16 * tt + i16, 4 * ks + g4);
-              const s16x8_t mh = *reinterpret_cast<const s16x8_t*>(lds.m[slot][0] + at);
-              const s16x8_t ml = *reinterpret_cast<const s16x8_t*>(lds.m[slot][1] + at);
-              y[tt] = mfma_bf16(xh[ks], mh, y[tt]);
-              y[tt] = mfma_bf16(xh[ks], ml, y[tt]);
-              if (F16) y[tt] = mfma_bf16(xl[ks], mh, y[tt]);
-            }
-          }
-          // ---- the skip, and out: lane i16 has token t, rows 4 g4 .. + 3
-          const int p = 16 * w4 + 4 * g4;
-#pragma unroll
-          for (int tt = 0; tt < 4; ++tt) {
-            const int t = 16 * tt + i16;
-            const u32x2_t w = *reinterpret_cast<const u32x2_t*>(xs + chunk_at<8>(t, 2 * w4 + (g4 >> 1)) + (g4 & 1) * 8);
-            float v[4] = {y[tt][0], y[tt][1], y[tt][2], y[tt][3]};
-            if (a.d) {
-              v[0] = __builtin_fmaf(skip, Act<F16>::lo(w[0]), v[0]);
-              v[1] = __builtin_fmaf(skip, Act<F16>::hi(w[0]), v[1]);
-              v[2] = __builtin_fmaf(skip, Act<F16>::lo(w[1]), v[2]);
-              v[3] = __builtin_fmaf(skip, Act<F16>::hi(w[1]), v[3]);
-            }
-            if (t < nt_live && row0 + p < a.hd) {
-              uint16_t* to = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + (t0 + t) * a.out.ts + h * a.out.hs + row0 + p;
-              *reinterpret_cast<u32x2_t*>(to) =
-                  u32x2_t{static_cast<uint32_t>(Act<F16>::st(v[0])) | static_cast<uint32_t>(Act<F16>::st(v[1])) << 16,
-                          static_cast<uint32_t>(Act<F16>::st(v[2])) | static_cast<uint32_t>(Act<F16>::st(v[3])) << 16};
-            }
-          }
-        }
-        // ---- the state behind the chunk
-        const float f = F16 ? st.decay * scale : st.decay;
-        if (begun) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) S[nt] *= f;
-        }
+      if constexpr (!STATES) {
+        // ---- what the chunk's own tokens give
+        const int m_at0 = afresh(m_base0), m_at1 = afresh(m_base1);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          if (32 * ks >= nt_live) break;
-          s16x8_t part[3];
-          if constexpr (F16) {
+          s16x8_t fm[4][2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) u[ks][j] *= scale;
-            split_f16(u[ks], part);
-          } else {
-            incoming(ks);
-            split_bf16<3>(u[ks], part);
+          for (int tt = 2 * ks; tt < 4; ++tt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              fm[tt][k] = *reinterpret_cast<const s16x8_t*>(
+                  lds.m[slot][k] + (tt < 2 ? m_at0 + tt * 1024 : (m_at1 ^ 64 * ks) + (tt - 2) * 2048));
+          read_first();
+          s16x8_t xq[2] = {fx[ks], fx[ks]};
+          if (F16) {
+            const u32x4_t w = __builtin_bit_cast(u32x4_t, fx[ks]);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j % 2 ? Act<F16>::hi(w[j / 2]) : Act<F16>::lo(w[j / 2]);
+            split_bf16<2>(v, xq);
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint8_t* at = lds.b + ks * 32 * Lds::kRow + (nt & 1) * 8;
-            const s16x4_t lo = read_tr(at + col_at[nt >> 1][0]), hi = read_tr(at + col_at[nt >> 1][1]);
-            const s16x8_t fb = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            S[nt] = mfma_in<F16>(fb, part[0], S[nt]);
-            S[nt] = mfma_in<F16>(fb, part[1], S[nt]);
-            if (!F16) S[nt] = mfma_in<F16>(fb, part[2], S[nt]);
+          for (int k = 0; k < (F16 ? 3 : 2); ++k)
+#pragma unroll
+            for (int tt = 2 * ks; tt < 4; ++tt) y[tt] = mfma_bf16(xq[k == 2], fm[tt][k % 2], y[tt]);
+        }
+      }
+      // ---- the state behind the chunk
+      {
+        const int col_at0 = afresh(col_base0), col_at1 = afresh(col_base1);
+        const float f = F16 ? st.decay * scale : st.decay;
+        if (STATES) seg_decay *= st.decay;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) S[nt] *= f;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          constexpr int kParts = F16 ? 2 : 3, kAhead = NT < 4 ? NT : 4;
+          s16x8_t part[kParts];
+          incoming(ks);
+          if constexpr (F16) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u[j] *= scale;
+            split_f16(u, part);
+          } else {
+            split_bf16<3>(u, part);
+          }
+#pragma unroll
+          for (int first = 0; first < NT; first += kAhead) {
+            s16x8_t fb[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+              const uint8_t* at = bs + ks * 32 * Lds::kRow;
+              const int nt = first + k, flip = 64 * (nt >> 1), half = 8 * (nt & 1);
+              const s16x4_t lo = read_tr(at + (col_at0 ^ flip) + half), hi = read_tr(at + (col_at1 ^ flip) + half);
+              fb[k] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            read_first();
+#pragma unroll
+            for (int k = 0; k < kParts; ++k)
+#pragma unroll
+              for (int j = 0; j < kAhead; ++j) S[first + j] = mfma_in<F16>(fb[j], part[k], S[first + j]);
           }
         }
         if (F16) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) S[nt] *= unscale;
         }
-      } else {
-        // ---- values that are not finite: token by token, so that they reach
-        // no other row and no earlier token
-        for (int t = 0; t < nt_live; ++t) {
-          const float s1 = st.sum[t], r1 = st.rest[t];
-          const float f = __builtin_amdgcn_exp2f(t ? (s1 - st.sum[t - 1]) + (r1 - st.rest[t - 1]) : s1 + r1);
-          const int pl_row = 16 * w4 + i16;
-          const float x = Act<F16>::ld(
-              *reinterpret_cast<const uint16_t*>(xs + chunk_at<8>(t, pl_row >> 3) + (pl_row & 7) * 2));
-          const float ux = st.dt[t] * x;
-          float sum = 0.0f;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int at = chunk_at<CH>(t, (nt >> 1) * 4 + g4) + (nt & 1) * 8;
-            const u32x2_t wb = *reinterpret_cast<const u32x2_t*>(lds.b + at);
-            const float vb4[4] = {Act<F16>::lo(wb[0]), Act<F16>::hi(wb[0]), Act<F16>::lo(wb[1]), Act<F16>::hi(wb[1])};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S[nt][i] = S[nt][i] * f + ux * vb4[i];
-            if constexpr (!STATES) {
-              const u32x2_t wc = *reinterpret_cast<const u32x2_t*>(lds.c + at);
-              const float vc4[4] = {Act<F16>::lo(wc[0]), Act<F16>::hi(wc[0]), Act<F16>::lo(wc[1]), Act<F16>::hi(wc[1])};
-              // (columns behind the state's end would make 0 times infinity)
-              if (16 * nt + 4 * g4 < a.N) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(S[nt][i], vc4[i], sum);
-              }
-            }
-          }
-          if constexpr (!STATES) {
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (a.d) sum = __builtin_fmaf(skip, x, sum);
-            if (g4 == 0 && row0 + pl_row < a.hd)
-              (static_cast<uint16_t*>(a.out.p) + b * a.out.bs + (t0 + t) * a.out.ts + h * a.out.hs)[row0 + pl_row] =
-                  Act<F16>::st(sum);
-          }
-        }
       }
-      begun = true;
+      // ---- the skip, and out: lane i16 has token t, rows 4 g4 .. + 3
+      if constexpr (!STATES) {
+        const int own_at = afresh(own_base);
+        u32x2_t v[4];
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(xs + own_at + tt * 2048);
+          v[tt][0] = pack_in<F16>(__builtin_fmaf(skip, Act<F16>::lo(w[0]), y[tt][0]),
+                                  __builtin_fmaf(skip, Act<F16>::hi(w[0]), y[tt][1]));
+          v[tt][1] = pack_in<F16>(__builtin_fmaf(skip, Act<F16>::lo(w[1]), y[tt][2]),
+                                  __builtin_fmaf(skip, Act<F16>::hi(w[1]), y[tt][3]));
+        }
+        if (kBufs == 2) wait_vmcnt0();  // (before the stores, which nobody waits for)
+        const uint32_t to = static_cast<uint32_t>(i16 * static_cast<int>(a.out.ts) + 16 * w4 + 4 * g4);
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+          if (16 * tt + i16 < nt_live && row0 + 16 * w4 + 4 * g4 < a.hd)
+            *reinterpret_cast<u32x2_t*>(op + 16 * tt * a.out.ts + to) = v[tt];
+        if (spoiled) {
+          wait_vmcnt0();
+          for (int t = from + g4; t < nt_live; t += 4)
+            if (p_row < a.hd) op[t * a.out.ts + 16 * w4 + i16] = F16 ? 0x7e00u : 0x7fc0u;
+        }
+        op += kChunk * a.out.ts;
+      }
     }
-    if (more) {
-      if (steps_wave) steps(t0 + kChunk, (ck + 1) & 1);
-      lds_barrier();  // every wave is done with this chunk
-      stage();
+    if (live && ck % kRound == kRound / 2 && next < chunks) steps(next);
+    if (kBufs == 2 && (STATES || !live)) wait_vmcnt0();
+    if (kBufs == 1 && more) {
       lds_barrier();
+      load(t0 + kChunk, 0);
+      wait_vmcnt0();
     }
   }
 
@@ -733,11 +802,11 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, NK > 4 ? 2 : 4) void scan_chun
   if (STATES) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) *seg_state(seg, nt) = S[nt];
-    if (steps_wave && lane == 0) seg_decays[head * pl.segs + seg] = __builtin_amdgcn_exp2f(static_cast<float>(seg_sum));
+    if (w4 == 0 && lane == 0) seg_decays[head * pl.segs + seg] = seg_decay;
   } else if (a.s_out && pool >= 0 && p_row < a.hd && seg == (len > 0 ? (len - 1) / seg_len : 0)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
-      if (16 * nt + 4 * g4 < a.N) *reinterpret_cast<f32x4_t*>(a.s_out + state0 + 16 * nt) = S[nt];
+      if (column(nt) < a.N) *reinterpret_cast<f32x4_t*>(a.s_out + state0 + column(nt)) = S[nt];
   }
 }
 
@@ -746,7 +815,7 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, NK > 4 ? 2 : 4) void scan_chun
 int chunk_steps(int N) { return N <= 32 ? 1 : N <= 64 ? 2 : N <= 128 ? 4 : 8; }
 
 constexpr int kFewMost = 16;      // tokens that the walk takes
-constexpr int kFullGrid = 512;    // workgroups that fill the CUs
+constexpr int kFullGrid = 256;    // workgroups that fill the CUs (one each, by its LDS)
 
 struct ScanPlan {
   ChunkPlan ck;
@@ -812,7 +881,11 @@ hipError_t scan_chunks(const ScanArgs& a, float* ws, hipStream_t stream) {
 #undef FMX_CHUNKS
 }
 
-bool scan_in_chunks(const ScanArgs& a) { return a.L > kFewMost; }
+// (the chunks' lanes address 64 rows by 32-bit offsets)
+bool scan_in_chunks(const ScanArgs& a) {
+  constexpr int64_t kMost = int64_t{1} << 24;
+  return a.L > kFewMost && a.x.ts < kMost && a.b.ts < kMost && a.c.ts < kMost && a.out.ts < kMost;
+}
 
 }  // namespace
 
