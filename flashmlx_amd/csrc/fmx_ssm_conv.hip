@@ -14,12 +14,16 @@ namespace fmx {
 namespace {
 
 constexpr int kConvThreads = 256;
-// tokens of a run: at least taps - 1, so that only a sequence's first run
-// reaches into the state
-constexpr int kConvRun = 8;
+// Tokens of a run: at least taps - 1, so that only a sequence's first run
+// reaches into the state. 8, or 4 where 8 make fewer threads than kConvFew: 7
+// ragged sequences of up to 777 tokens of 1792 channels take 12.7 us in a graph
+// for 15.0, 2048 of 6144 17.8 for 17.0, 8191 of 6144 in fp32 87.5 for 81.4 (16
+// tokens: 18.6, 20.8, 83.3).
+constexpr int kConvRun = 8, kConvShort = 4;
 static_assert(kConvRun >= kMaxTaps - 1, "a run's rows before it are one run's");
+constexpr int64_t kConvFew = 160 * 1024;
 
-template <int DT, int VEC, int K>
+template <int DT, int VEC, int K, int R>
 __global__ __launch_bounds__(kConvThreads) void conv_kernel(ConvArgs a, uint32_t per_seq, uint32_t total) {
   typedef typename El<DT>::T T;
   typedef Pack<T, VEC> V;
@@ -28,7 +32,7 @@ __global__ __launch_bounds__(kConvThreads) void conv_kernel(ConvArgs a, uint32_t
   const uint32_t cvs = static_cast<uint32_t>(a.C) / VEC;
   const int b = static_cast<int>(id / per_seq);
   const uint32_t rest = id - b * per_seq;
-  const int t0 = static_cast<int>(rest / cvs) * kConvRun;
+  const int t0 = static_cast<int>(rest / cvs) * R;
   const int ch = static_cast<int>(rest % cvs) * VEC;
   const int len = seq_length(a.lens, a.L, b);
   if (t0 >= len && t0 > 0) return;
@@ -39,9 +43,9 @@ __global__ __launch_bounds__(kConvThreads) void conv_kernel(ConvArgs a, uint32_t
   const T* s_in = slot >= 0 && a.s_in ? static_cast<const T*>(a.s_in) + state0 : nullptr;
   V zero{};
 
-  V rows[kConvRun + K - 1];
+  V rows[R + K - 1];
 #pragma unroll
-  for (int i = 0; i < kConvRun + K - 1; ++i) {
+  for (int i = 0; i < R + K - 1; ++i) {
     const int t = t0 - (K - 1) + i;
     rows[i] = zero;
     if (t < 0) {
@@ -57,7 +61,7 @@ __global__ __launch_bounds__(kConvThreads) void conv_kernel(ConvArgs a, uint32_t
   if (a.bias) bias = *reinterpret_cast<const V*>(static_cast<const T*>(a.bias) + ch);
 
 #pragma unroll
-  for (int r = 0; r < kConvRun; ++r) {
+  for (int r = 0; r < R; ++r) {
     if (t0 + r >= len) break;
     V y;
 #pragma unroll
@@ -86,31 +90,47 @@ __global__ __launch_bounds__(kConvThreads) void conv_kernel(ConvArgs a, uint32_t
   }
 }
 
-int64_t conv_threads(const ConvArgs& a, int vec) {
-  const int64_t runs = std::max<int64_t>(1, (static_cast<int64_t>(a.L) + kConvRun - 1) / kConvRun);
+int64_t conv_threads(const ConvArgs& a, int vec, int run) {
+  const int64_t runs = std::max<int64_t>(1, (static_cast<int64_t>(a.L) + run - 1) / run);
   return a.B * runs * (a.C / vec);
+}
+
+template <int DT, int VEC, int R>
+hipError_t conv(const ConvArgs& a, hipStream_t stream) {
+  const int64_t total = conv_threads(a, VEC, R);
+  if (total == 0) return hipSuccess;
+  const dim3 grid(static_cast<uint32_t>((total + kConvThreads - 1) / kConvThreads)), wg(kConvThreads);
+  const uint32_t per_seq = static_cast<uint32_t>(total / a.B), n = static_cast<uint32_t>(total);
+#define FMX_CONV(K) hipLaunchKernelGGL((conv_kernel<DT, VEC, K, R>), grid, wg, 0, stream, a, per_seq, n)
+  switch (a.taps) {
+    case 1: FMX_CONV(1); break;
+    case 2: FMX_CONV(2); break;
+    case 3: FMX_CONV(3); break;
+    case 4: FMX_CONV(4); break;
+    case 5: FMX_CONV(5); break;
+    default:
+      if constexpr (R == kConvRun) {
+        if (a.taps == 6) FMX_CONV(6);
+        if (a.taps == 7) FMX_CONV(7);
+        if (a.taps == 8) FMX_CONV(8);
+        break;
+      }
+      return hipErrorInvalidValue;
+  }
+#undef FMX_CONV
+  return hipGetLastError();
 }
 
 template <int DT, int VEC>
 hipError_t conv(const ConvArgs& a, hipStream_t stream) {
-  const int64_t total = conv_threads(a, VEC);
-  if (total == 0) return hipSuccess;
-  const dim3 grid(static_cast<uint32_t>((total + kConvThreads - 1) / kConvThreads)), wg(kConvThreads);
-  const uint32_t per_seq = static_cast<uint32_t>(total / a.B), n = static_cast<uint32_t>(total);
-  switch (a.taps) {
-#define FMX_CONV(K) \
-  case K: hipLaunchKernelGGL((conv_kernel<DT, VEC, K>), grid, wg, 0, stream, a, per_seq, n); break;
-    FMX_CONV(1) FMX_CONV(2) FMX_CONV(3) FMX_CONV(4) FMX_CONV(5) FMX_CONV(6) FMX_CONV(7) FMX_CONV(8)
-#undef FMX_CONV
-    default: return hipErrorInvalidValue;
-  }
-  return hipGetLastError();
+  const bool few = a.taps - 1 <= kConvShort && conv_threads(a, VEC, kConvRun) < kConvFew;
+  return few ? conv<DT, VEC, kConvShort>(a, stream) : conv<DT, VEC, kConvRun>(a, stream);
 }
 
 }  // namespace
 
 bool conv_fits(const ConvArgs& a) {
-  return conv_threads(a, 1) <= max_blocks(kConvThreads) * kConvThreads;
+  return conv_threads(a, 1, kConvShort) <= max_blocks(kConvThreads) * kConvThreads;
 }
 
 hipError_t launch_conv(const ConvArgs& a, int dt, hipStream_t stream) {

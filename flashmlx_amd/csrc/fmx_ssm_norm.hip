@@ -28,34 +28,41 @@ __device__ inline Pack<typename El<DT>::T, VEC> norm_load(const void* p, int64_t
 }
 
 // LN lanes per group (a workgroup for 256), NV vectors per lane kept (0: read
-// again)
-template <int DT, int VEC, int LN, int NV>
+// again), GR groups one after the other whose loads are all in flight
+template <int DT, int VEC, int LN, int NV, int GR>
 __global__ __launch_bounds__(kGateThreads) void gated_norm_kernel(GatedNormArgs a, NormPlan pl) {
   typedef typename El<DT>::T T;
   typedef Pack<T, VEC> V;
+  static_assert(GR == 1 || (NV && LN < kGateThreads), "several groups: kept, within a wave");
   __shared__ float s_sum[kGateThreads / kWave];
-  constexpr int kPer = kGateThreads / LN;  // groups of a workgroup
-  const uint32_t item = blockIdx.x * kPer + threadIdx.x / LN;
-  const int j = threadIdx.x % LN;
-  const uint32_t row = item / static_cast<uint32_t>(a.groups);
-  const int g = static_cast<int>(item - row * a.groups);
-  const int b = static_cast<int>(row / a.L), l = static_cast<int>(row % a.L);
-  const bool live = item < pl.items && l < seq_length(a.lens, a.L, min(b, a.B - 1));
-  if (LN == kGateThreads && !live) return;  // (a workgroup's threads agree)
-  const int size = a.C / a.groups;
-  const int64_t xo = b * a.x.bs + l * a.x.ts + static_cast<int64_t>(g) * size;
-  const int64_t zo = b * a.z.bs + l * a.z.ts + static_cast<int64_t>(g) * size;
-  const int64_t oo = b * a.out.bs + l * a.out.ts + static_cast<int64_t>(g) * size;
+  constexpr int kPer = kGateThreads / LN;  // groups of a workgroup at once
+  const int j = threadIdx.x % LN, size = a.C / a.groups;
   const bool gate = a.z.p != nullptr;
 
   auto value = [&](const V& x, const V& z, int e) {
     const float v = El<DT>::ld(x.e[e]);
     return gate && a.gate_first ? v * silu_f32(El<DT>::ld(z.e[e])) : v;
   };
-  auto store = [&](int i, const float* u, const V& z, float f) {
+  int64_t xo[GR], zo[GR], oo[GR], wo[GR];
+  bool live[GR];
+#pragma unroll
+  for (int r = 0; r < GR; ++r) {
+    const uint32_t item = (blockIdx.x * GR + r) * kPer + threadIdx.x / LN;
+    const uint32_t row = item / static_cast<uint32_t>(a.groups);
+    const int g = static_cast<int>(item - row * a.groups);
+    const int b = static_cast<int>(row / a.L), l = static_cast<int>(row % a.L);
+    live[r] = item < pl.items && l < seq_length(a.lens, a.L, min(b, a.B - 1));
+    wo[r] = static_cast<int64_t>(g) * size;
+    xo[r] = b * a.x.bs + l * a.x.ts + wo[r];
+    zo[r] = b * a.z.bs + l * a.z.ts + wo[r];
+    oo[r] = b * a.out.bs + l * a.out.ts + wo[r];
+  }
+  if (LN == kGateThreads && !live[0]) return;  // (a workgroup's threads agree)
+
+  auto store = [&](int r, int i, const float* u, const V& z, float f) {
     V y;
     V w{};
-    if (a.w) w = norm_load<DT, VEC>(a.w, static_cast<int64_t>(g) * size + i * VEC);
+    if (a.w) w = norm_load<DT, VEC>(a.w, wo[r] + i * VEC);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       float v = u[e] * f;
@@ -63,67 +70,72 @@ __global__ __launch_bounds__(kGateThreads) void gated_norm_kernel(GatedNormArgs 
       if (gate && !a.gate_first) v *= silu_f32(El<DT>::ld(z.e[e]));
       y.e[e] = El<DT>::st(v);
     }
-    *reinterpret_cast<V*>(static_cast<T*>(a.out.p) + oo + i * VEC) = y;
+    *reinterpret_cast<V*>(static_cast<T*>(a.out.p) + oo[r] + i * VEC) = y;
   };
 
   constexpr int kKeep = NV ? NV : 1;
-  V x[kKeep], z[kKeep];
-  float sum = 0.0f;
+  V x[GR][kKeep], z[GR][kKeep];
   if (NV) {
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
-      x[i] = V{};
-      z[i] = V{};
-      if (live && j + i * LN < pl.vecs) {
-        x[i] = norm_load<DT, VEC>(a.x.p, xo + (j + i * LN) * VEC);
-        if (gate) z[i] = norm_load<DT, VEC>(a.z.p, zo + (j + i * LN) * VEC);
+    for (int r = 0; r < GR; ++r)
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i) {
+        x[r][i] = V{};
+        z[r][i] = V{};
+        if (live[r] && j + i * LN < pl.vecs) {
+          x[r][i] = norm_load<DT, VEC>(a.x.p, xo[r] + (j + i * LN) * VEC);
+          if (gate) z[r][i] = norm_load<DT, VEC>(a.z.p, zo[r] + (j + i * LN) * VEC);
+        }
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < GR; ++r) {
+    float u[kKeep][VEC];
+    float sum = 0.0f;
+    auto add = [&](const V& x, const V& z, float* u) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        u[e] = value(x, z, e);
+        sum = __builtin_fmaf(u[e], u[e], sum);
+      }
+    };
+    if (NV) {
+#pragma unroll
+      for (int i = 0; i < kKeep; ++i)
+        if (j + i * LN < pl.vecs) add(x[r][i], z[r][i], u[i]);
+    } else {
+      for (int i = j; i < pl.vecs; i += LN) {
+        const V xv = norm_load<DT, VEC>(a.x.p, xo[r] + static_cast<int64_t>(i) * VEC);
+        const V zv = gate ? norm_load<DT, VEC>(a.z.p, zo[r] + static_cast<int64_t>(i) * VEC) : V{};
+        add(xv, zv, u[0]);
       }
     }
-  }
-  float u[kKeep][VEC];
-  auto add = [&](const V& x, const V& z, float* u) {
+    if (LN == kGateThreads) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      u[e] = value(x, z, e);
-      sum = __builtin_fmaf(u[e], u[e], sum);
+      for (int m = 1; m < kWave; m *= 2) sum += __shfl_xor(sum, m);
+      if (threadIdx.x % kWave == 0) s_sum[threadIdx.x / kWave] = sum;
+      __syncthreads();
+      sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kGateThreads / kWave; ++i) sum += s_sum[i];
+    } else {
+#pragma unroll
+      for (int m = 1; m < LN; m *= 2) sum += __shfl_xor(sum, m);
     }
-  };
-  if (NV) {
+    if (!live[r]) continue;
+    const float f = 1.0f / sqrtf(sum / static_cast<float>(size) + a.eps);
+    if (NV) {
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i)
-      if (j + i * LN < pl.vecs) add(x[i], z[i], u[i]);
-  } else if (live) {
-    for (int i = j; i < pl.vecs; i += LN) {
-      const V xv = norm_load<DT, VEC>(a.x.p, xo + static_cast<int64_t>(i) * VEC);
-      const V zv = gate ? norm_load<DT, VEC>(a.z.p, zo + static_cast<int64_t>(i) * VEC) : V{};
-      add(xv, zv, u[0]);
-    }
-  }
-  if (LN == kGateThreads) {
+      for (int i = 0; i < kKeep; ++i)
+        if (j + i * LN < pl.vecs) store(r, j + i * LN, u[i], z[r][i], f);
+    } else {
+      for (int i = j; i < pl.vecs; i += LN) {
+        const V xv = norm_load<DT, VEC>(a.x.p, xo[r] + static_cast<int64_t>(i) * VEC);
+        const V zv = gate ? norm_load<DT, VEC>(a.z.p, zo[r] + static_cast<int64_t>(i) * VEC) : V{};
 #pragma unroll
-    for (int m = 1; m < kWave; m *= 2) sum += __shfl_xor(sum, m);
-    if (threadIdx.x % kWave == 0) s_sum[threadIdx.x / kWave] = sum;
-    __syncthreads();
-    sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kGateThreads / kWave; ++i) sum += s_sum[i];
-  } else {
-#pragma unroll
-    for (int m = 1; m < LN; m *= 2) sum += __shfl_xor(sum, m);
-  }
-  if (!live) return;
-  const float f = 1.0f / sqrtf(sum / static_cast<float>(size) + a.eps);
-  if (NV) {
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i)
-      if (j + i * LN < pl.vecs) store(j + i * LN, u[i], z[i], f);
-  } else {
-    for (int i = j; i < pl.vecs; i += LN) {
-      const V xv = norm_load<DT, VEC>(a.x.p, xo + static_cast<int64_t>(i) * VEC);
-      const V zv = gate ? norm_load<DT, VEC>(a.z.p, zo + static_cast<int64_t>(i) * VEC) : V{};
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) u[0][e] = value(xv, zv, e);
-      store(i, u[0], zv, f);
+        for (int e = 0; e < VEC; ++e) u[0][e] = value(xv, zv, e);
+        store(r, i, u[0], zv, f);
+      }
     }
   }
 }
@@ -144,16 +156,28 @@ hipError_t gated_norm(const GatedNormArgs& a, hipStream_t stream) {
   if (items == 0) return hipSuccess;
   NormPlan pl{static_cast<uint32_t>(items), a.C / a.groups / VEC};
   const int ln = norm_lanes(pl.vecs), per = kGateThreads / ln;
-  const dim3 grid(static_cast<uint32_t>((items + per - 1) / per)), wg(kGateThreads);
-#define FMX_NORM(LN, NV) hipLaunchKernelGGL((gated_norm_kernel<DT, VEC, LN, NV>), grid, wg, 0, stream, a, pl)
-  if (ln == 4) FMX_NORM(4, 1);
-  else if (ln == 16) FMX_NORM(16, 1);
-  else if (ln == 64 && pl.vecs <= 64) FMX_NORM(64, 1);
-  else if (ln == 64) FMX_NORM(64, 2);
-  else if (pl.vecs <= 256) FMX_NORM(256, 1);
-  else if (pl.vecs <= 512) FMX_NORM(256, 2);
-  else if (pl.vecs <= 1024) FMX_NORM(256, 4);
-  else FMX_NORM(256, 0);
+  // Two groups' loads in flight where there are enough for it: 8192 rows of 8
+  // groups of 512 50.4 us (4.0 TB/s) in a graph, one 52.3, four 60.6.
+  constexpr int kRounds = VEC > 1 ? 2 : 1;
+  const int rounds = ln < kGateThreads && items >= int64_t{4096} * per ? kRounds : 1;
+  const dim3 grid(static_cast<uint32_t>((items + per * rounds - 1) / (per * rounds))), wg(kGateThreads);
+#define FMX_NORM(LN, NV, GR) hipLaunchKernelGGL((gated_norm_kernel<DT, VEC, LN, NV, GR>), grid, wg, 0, stream, a, pl)
+#define FMX_NORM_FEW(LN, NV)                        \
+  do {                                              \
+    if (rounds > 1)                                 \
+      FMX_NORM(LN, NV, kRounds);                    \
+    else                                            \
+      FMX_NORM(LN, NV, 1);                          \
+  } while (0)
+  if (ln == 4) FMX_NORM_FEW(4, 1);
+  else if (ln == 16) FMX_NORM_FEW(16, 1);
+  else if (ln == 64 && pl.vecs <= 64) FMX_NORM_FEW(64, 1);
+  else if (ln == 64) FMX_NORM_FEW(64, 2);
+  else if (pl.vecs <= 256) FMX_NORM(256, 1, 1);
+  else if (pl.vecs <= 512) FMX_NORM(256, 2, 1);
+  else if (pl.vecs <= 1024) FMX_NORM(256, 4, 1);
+  else FMX_NORM(256, 0, 1);
+#undef FMX_NORM_FEW
 #undef FMX_NORM
   return hipGetLastError();
 }

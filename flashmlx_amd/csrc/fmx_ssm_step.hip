@@ -20,19 +20,35 @@ namespace {
 
 constexpr int kStepThreads = 256;
 
-// channel ch of the convolution of sequence b, before anything is rounded
-template <bool F16>
+// Channel ch of the convolution of sequence b, before anything is rounded. K:
+// the taps, whose loads are then all in flight at once; 0: a.taps of them.
+template <bool F16, int K>
 __device__ inline float step_conv(const StepArgs& a, int b, int64_t slot, int ch) {
-  const uint16_t* w = static_cast<const uint16_t*>(a.conv_w) + static_cast<int64_t>(ch) * a.taps;
-  const uint16_t* s = static_cast<const uint16_t*>(a.conv_state) + slot * (a.taps - 1) * a.C + ch;
+  const int taps = K ? K : a.taps;
+  const uint16_t* w = static_cast<const uint16_t*>(a.conv_w) + static_cast<int64_t>(ch) * taps;
+  const uint16_t* s = static_cast<const uint16_t*>(a.conv_state) + slot * (taps - 1) * a.C + ch;
+  const uint16_t x = (static_cast<const uint16_t*>(a.xbc.p) + b * a.xbc.bs)[ch];
   float v = a.conv_b ? Act<F16>::ld(static_cast<const uint16_t*>(a.conv_b)[ch]) : 0.0f;
-  if (slot >= 0)
-    for (int k = 0; k < a.taps - 1; ++k) v = __builtin_fmaf(Act<F16>::ld(w[k]), Act<F16>::ld(s[static_cast<int64_t>(k) * a.C]), v);
-  v = __builtin_fmaf(Act<F16>::ld(w[a.taps - 1]), Act<F16>::ld((static_cast<const uint16_t*>(a.xbc.p) + b * a.xbc.bs)[ch]), v);
+  if (slot >= 0) {
+    if (K) {
+      uint16_t wk[K ? K : 1], sk[K ? K : 1];
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k) {
+        wk[k] = w[k];
+        sk[k] = s[static_cast<int64_t>(k) * a.C];
+      }
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k) v = __builtin_fmaf(Act<F16>::ld(wk[k]), Act<F16>::ld(sk[k]), v);
+    } else {
+      for (int k = 0; k < taps - 1; ++k)
+        v = __builtin_fmaf(Act<F16>::ld(w[k]), Act<F16>::ld(s[static_cast<int64_t>(k) * a.C]), v);
+    }
+  }
+  v = __builtin_fmaf(Act<F16>::ld(w[taps - 1]), Act<F16>::ld(x), v);
   return a.silu ? silu_f32(v) : v;
 }
 
-template <bool F16, int LN, int RP>
+template <bool F16, int LN, int RP, int K>
 __global__ __launch_bounds__(kStepThreads) void step_kernel(StepArgs a, int parts, float* y_out) {
   constexpr int kRows = kStepThreads / LN * RP;
   constexpr int kCols = 4 * LN;
@@ -59,11 +75,11 @@ __global__ __launch_bounds__(kStepThreads) void step_kernel(StepArgs a, int part
   const int d = a.nh * a.hd, n = a.groups * a.N;
   for (int i = tid; i < kRows + 2 * kCols; i += kStepThreads) {
     if (i < kRows) {
-      s_x[i] = i < rows ? step_conv<F16>(a, b, slot, h * a.hd + row0 + i) : 0.0f;
+      s_x[i] = i < rows ? step_conv<F16, K>(a, b, slot, h * a.hd + row0 + i) : 0.0f;
     } else {
       const bool second = i >= kRows + kCols;
       const int j = i - kRows - (second ? kCols : 0);
-      const float v = j < a.N ? step_conv<F16>(a, b, slot, d + (second ? n : 0) + g * a.N + j) : 0.0f;
+      const float v = j < a.N ? step_conv<F16, K>(a, b, slot, d + (second ? n : 0) + g * a.N + j) : 0.0f;
       reinterpret_cast<float*>(second ? s_c : s_b)[j] = v;
     }
   }
@@ -87,32 +103,78 @@ __global__ __launch_bounds__(kStepThreads) void step_kernel(StepArgs a, int part
   }
 }
 
-// workgroups [0, norms): a sequence's group each; the others: channels' states
-template <bool F16>
+// Workgroups [0, norms): a sequence's group each, its products kept in
+// registers (NV vectors of VEC a thread; 0: formed again); the others:
+// vectors of channels' states.
+template <bool F16, int VEC, int NV>
 __global__ __launch_bounds__(kStepThreads) void step_norm_kernel(StepArgs a, uint32_t norms, const float* y_in) {
+  typedef Pack<uint16_t, VEC> V;
+  typedef Pack<float, VEC> Y;
   __shared__ float s_sum[kStepThreads / kWave];
   const int tid = threadIdx.x;
   if (blockIdx.x >= norms) {
-    const uint32_t per = (a.C + kStepThreads - 1) / kStepThreads, id = blockIdx.x - norms;
-    const int b = static_cast<int>(id / per), ch = static_cast<int>(id % per) * kStepThreads + tid;
+    const uint32_t vecs = a.C / VEC, per = (vecs + kStepThreads - 1) / kStepThreads, id = blockIdx.x - norms;
+    const int b = static_cast<int>(id / per), v = static_cast<int>(id % per) * kStepThreads + tid;
     const int64_t slot = seq_slot(a.slots, a.n_slots, b);
-    if (slot < 0 || ch >= a.C) return;
-    uint16_t* s = static_cast<uint16_t*>(a.conv_state) + slot * (a.taps - 1) * a.C + ch;
-    for (int k = 0; k < a.taps - 2; ++k) s[static_cast<int64_t>(k) * a.C] = s[static_cast<int64_t>(k + 1) * a.C];
-    s[static_cast<int64_t>(a.taps - 2) * a.C] = (static_cast<const uint16_t*>(a.xbc.p) + b * a.xbc.bs)[ch];
+    if (slot < 0 || v >= static_cast<int>(vecs)) return;
+    uint16_t* s = static_cast<uint16_t*>(a.conv_state) + slot * (a.taps - 1) * a.C + v * VEC;
+    V rows[kMaxTaps - 1];
+#pragma unroll
+    for (int k = 1; k < kMaxTaps; ++k) {
+      if (k < a.taps - 1) rows[k - 1] = *reinterpret_cast<const V*>(s + static_cast<int64_t>(k) * a.C);
+      if (k == a.taps - 1) rows[k - 1] = *reinterpret_cast<const V*>(static_cast<const uint16_t*>(a.xbc.p) + b * a.xbc.bs + v * VEC);
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxTaps - 1; ++k)
+      if (k < a.taps - 1) *reinterpret_cast<V*>(s + static_cast<int64_t>(k) * a.C) = rows[k];
     return;
   }
-  const int d = a.nh * a.hd, size = d / a.norm_groups;
+  const int d = a.nh * a.hd, size = d / a.norm_groups, vecs = size / VEC;
   const int b = static_cast<int>(blockIdx.x / a.norm_groups), at = static_cast<int>(blockIdx.x % a.norm_groups) * size;
   const float* y = y_in + static_cast<int64_t>(b) * d + at;
   const uint16_t* z = a.z.p ? static_cast<const uint16_t*>(a.z.p) + b * a.z.bs + at : nullptr;
+  const uint16_t* w = a.norm_w ? static_cast<const uint16_t*>(a.norm_w) + at : nullptr;
   uint16_t* out = static_cast<uint16_t*>(a.out.p) + b * a.out.bs + at;
   const bool first = z && a.gate_first;
-  auto value = [&](int i) { return first ? y[i] * silu_f32(Act<F16>::ld(z[i])) : y[i]; };
+  constexpr int kKeep = NV ? NV : 1;
+  Y yv[kKeep];
+  V zv[kKeep], wv[kKeep];
+  auto read = [&](int k, int i) {
+    yv[k] = *reinterpret_cast<const Y*>(y + i * VEC);
+    zv[k] = z ? *reinterpret_cast<const V*>(z + i * VEC) : V{};
+    wv[k] = w ? *reinterpret_cast<const V*>(w + i * VEC) : V{};
+  };
   float sum = 0.0f;
-  for (int i = tid; i < size; i += kStepThreads) {
-    const float v = value(i);
-    sum = __builtin_fmaf(v, v, sum);
+  auto form = [&](int k) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (first) yv[k].e[e] *= silu_f32(Act<F16>::ld(zv[k].e[e]));
+      sum = __builtin_fmaf(yv[k].e[e], yv[k].e[e], sum);
+    }
+  };
+  auto store = [&](int k, int i, float f) {
+    V o;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float v = yv[k].e[e] * f;
+      if (w) v *= Act<F16>::ld(wv[k].e[e]);
+      if (z && !first) v *= silu_f32(Act<F16>::ld(zv[k].e[e]));
+      o.e[e] = Act<F16>::st(v);
+    }
+    *reinterpret_cast<V*>(out + i * VEC) = o;
+  };
+  if (NV) {
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      if (tid + k * kStepThreads < vecs) read(k, tid + k * kStepThreads);
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      if (tid + k * kStepThreads < vecs) form(k);
+  } else {
+    for (int i = tid; i < vecs; i += kStepThreads) {
+      read(0, i);
+      form(0);
+    }
   }
 #pragma unroll
   for (int m = 1; m < kWave; m *= 2) sum += __shfl_xor(sum, m);
@@ -122,11 +184,16 @@ __global__ __launch_bounds__(kStepThreads) void step_norm_kernel(StepArgs a, uin
 #pragma unroll
   for (int i = 0; i < kStepThreads / kWave; ++i) sum += s_sum[i];
   const float f = 1.0f / sqrtf(sum / static_cast<float>(size) + a.eps);
-  for (int i = tid; i < size; i += kStepThreads) {
-    float v = value(i) * f;
-    if (a.norm_w) v *= Act<F16>::ld(static_cast<const uint16_t*>(a.norm_w)[at + i]);
-    if (z && !first) v *= silu_f32(Act<F16>::ld(z[i]));
-    out[i] = Act<F16>::st(v);
+  if (NV) {
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      if (tid + k * kStepThreads < vecs) store(k, tid + k * kStepThreads, f);
+  } else {
+    for (int i = tid; i < vecs; i += kStepThreads) {
+      read(0, i);
+      form(0);
+      store(0, i, f);
+    }
   }
 }
 
@@ -135,18 +202,20 @@ int step_lanes(int N) {
   while (4 * n < N) n *= 2;
   return n;
 }
+// Rows per lane: as many as a head has, up to 8. (One sequence's 64 heads in
+// 64 to 512 workgroups: 12.4 us and 13 to 14.)
 int step_rows(int hd, int ln) {
   int r = 1;
   while (r < 8 && kStepThreads / ln * r < hd) r *= 2;
   return r;
 }
 
-template <bool F16, int LN>
+template <bool F16, int LN, int K>
 hipError_t step_scan(const StepArgs& a, float* y, hipStream_t stream) {
   const int rp = step_rows(a.hd, LN), rows = kStepThreads / LN * rp;
   const int parts = (a.hd + rows - 1) / rows;
   const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.nh * parts)), wg(kStepThreads);
-#define FMX_STEP(RP) hipLaunchKernelGGL((step_kernel<F16, LN, RP>), grid, wg, 0, stream, a, parts, y)
+#define FMX_STEP(RP) hipLaunchKernelGGL((step_kernel<F16, LN, RP, K>), grid, wg, 0, stream, a, parts, y)
   if (rp == 1) FMX_STEP(1);
   else if (rp == 2) FMX_STEP(2);
   else if (rp == 4) FMX_STEP(4);
@@ -154,8 +223,28 @@ hipError_t step_scan(const StepArgs& a, float* y, hipStream_t stream) {
 #undef FMX_STEP
   return hipGetLastError();
 }
+template <bool F16, int LN>
+hipError_t step_scan(const StepArgs& a, float* y, hipStream_t stream) {
+  return a.taps == 4 ? step_scan<F16, LN, 4>(a, y, stream) : step_scan<F16, LN, 0>(a, y, stream);
+}
 
-int64_t step_shifts(const StepArgs& a) { return static_cast<int64_t>(a.B) * ((a.C + kStepThreads - 1) / kStepThreads); }
+int64_t step_shifts(const StepArgs& a, int vec) {
+  return static_cast<int64_t>(a.B) * ((a.C / vec + kStepThreads - 1) / kStepThreads);
+}
+
+template <bool F16, int VEC>
+hipError_t step_norm(const StepArgs& a, float* y, hipStream_t stream) {
+  const uint32_t norms = static_cast<uint32_t>(a.B * a.norm_groups);
+  const dim3 grid(norms + static_cast<uint32_t>(step_shifts(a, VEC))), wg(kStepThreads);
+  const int vecs = a.nh * a.hd / a.norm_groups / VEC;
+  if (vecs <= kStepThreads)
+    hipLaunchKernelGGL((step_norm_kernel<F16, VEC, 1>), grid, wg, 0, stream, a, norms, y);
+  else if (vecs <= 4 * kStepThreads)
+    hipLaunchKernelGGL((step_norm_kernel<F16, VEC, 4>), grid, wg, 0, stream, a, norms, y);
+  else
+    hipLaunchKernelGGL((step_norm_kernel<F16, VEC, 0>), grid, wg, 0, stream, a, norms, y);
+  return hipGetLastError();
+}
 
 template <bool F16>
 hipError_t step(const StepArgs& a, float* y, hipStream_t stream) {
@@ -169,10 +258,11 @@ hipError_t step(const StepArgs& a, float* y, hipStream_t stream) {
     default: e = step_scan<F16, 64>(a, y, stream); break;
   }
   if (e != hipSuccess) return e;
-  const uint32_t norms = static_cast<uint32_t>(a.B * a.norm_groups);
-  const dim3 grid(norms + static_cast<uint32_t>(step_shifts(a))), wg(kStepThreads);
-  hipLaunchKernelGGL((step_norm_kernel<F16>), grid, wg, 0, stream, a, norms, y);
-  return hipGetLastError();
+  // vectors of 8 where every row falls on them
+  const int size = a.nh * a.hd / a.norm_groups;
+  bool wide = a.C % 8 == 0 && size % 8 == 0 && reinterpret_cast<uintptr_t>(a.norm_w) % 16 == 0;
+  for (const HeadsView* v : {&a.xbc, &a.z, &a.out}) wide = wide && on_vectors(*v, 2, 8);
+  return wide ? step_norm<F16, 8>(a, y, stream) : step_norm<F16, 1>(a, y, stream);
 }
 
 }  // namespace
@@ -181,7 +271,7 @@ size_t step_workspace(const StepArgs& a) { return static_cast<size_t>(a.B) * a.n
 
 bool step_fits(const StepArgs& a) {
   return static_cast<int64_t>(a.B) * a.nh * ((a.hd + 3) / 4) <= max_blocks(kStepThreads) &&
-         static_cast<int64_t>(a.B) * a.norm_groups + step_shifts(a) <= max_blocks(kStepThreads);
+         static_cast<int64_t>(a.B) * a.norm_groups + step_shifts(a, 1) <= max_blocks(kStepThreads);
 }
 
 hipError_t launch_step(const StepArgs& a, bool f16, void* ws, hipStream_t stream) {

@@ -204,6 +204,7 @@ class SsmLayer:
             _flat(a, "a", (heads,), _F32, dev), _flat(d, "d", (heads,), _F32, dev),
             _flat(dt_bias, "dt_bias", (heads,), _F32, dev), int(softplus), dt_limits[0], dt_limits[1],
             _flat(norm_weight, "norm_weight", (inner,), dt, dev), self.norm_groups, eps, int(gate_first))
+        self._ref, self._bytes = _byref(self._c), {}  # (of the struct; workspace bytes by batch)
 
     def new_states(self, slots: int) -> tuple:
         """(conv_state, state) of a pool of so many slots, zeros."""
@@ -237,13 +238,16 @@ class SsmLayer:
         dev, ty = _device(xbc, "xbc", "batch, channels", 2), self.dtype
         if dev != self._dev:
             raise ValueError(f"the weights are on cuda:{self._dev}, the rows on cuda:{dev}")
-        B, inner = xbc.shape[0], (xbc.shape[0], self.inner)
+        B = xbc.shape[0]
+        inner = (B, self.inner)
         _tensor(state, "state")
         n_slots = state.shape[0] if state.dim() == 4 else -1
         if out is None:
             out = xbc.new_empty(inner)
-        c = _byref(self._c)
-        ws = _workspace(workspace, self.lib.fmx_ssm_step_workspace_size(c, B), xbc)
+        need, c = self._bytes.get(B), self._ref
+        if need is None:
+            need = self._bytes[B] = self.lib.fmx_ssm_step_workspace_size(c, B)
+        ws = _workspace(workspace, need, xbc)
         _lib.check(self.lib.fmx_ssm_step(
             c, B, _row(xbc, "xbc", (B, self.channels), ty, dev), _steps(dt, "dt", (B, self.heads), ty, dev),
             None if z is None else _row(z, "z", inner, ty, dev),
