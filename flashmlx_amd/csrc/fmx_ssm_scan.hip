@@ -228,7 +228,8 @@ __device__ inline void split_bf16(const float* v, s16x8_t* part) {
     part[k] = __builtin_bit_cast(s16x8_t, w);
   }
 }
-// as a sum of two of float16 (22 bits), of values within 2^15
+// as a sum of two of float16 (22 bits, or to 2^-25 where they are small), of
+// values within 2^15
 __device__ inline void split_f16(const float* v, s16x8_t* part) {
   u32x4_t h, l;
 #pragma unroll
@@ -527,7 +528,13 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
     const ChunkSteps<STATES>* round = lds.steps[ck / kRound & 1][ck % kRound];
     const ChunkSteps<STATES>& st = round[slot];
     f32x4_t y[4];
-    float most_s = 0.0f;  // of the state's magnitudes (float16), NaN aside
+    // float16's operands are scaled, each row by its own power of two: a row
+    // much smaller than its neighbours keeps its bits
+    auto row_max = [](float v) {
+      v = fmaxf(v, __shfl_xor(v, 16));
+      return fmaxf(v, __shfl_xor(v, 32));
+    };
+    float most_s = 0.0f;  // of the row's magnitudes, NaN aside
     if (F16 && live) {
       auto largest = [&]() {
         most_s = 0.0f;
@@ -535,10 +542,10 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) most_s = fmaxf(most_s, fabsf(S[nt][i]));
-        most_s = wave_max_f32(most_s);
+        most_s = row_max(most_s);
       };
       largest();
-      if (__float_as_uint(most_s) >= 0x7f800000u) {  // (infinities would be every row's scale)
+      if (__any(__float_as_uint(most_s) >= 0x7f800000u)) {  // (no scale takes an infinity)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) S[nt] += S[nt] * 0.0f;
         largest();
@@ -574,8 +581,16 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) y[tt] = mfma_in<F16>(part[k], fc[tt], y[tt]);
         }
+        f32x4_t backs{1.0f, 1.0f, 1.0f, 1.0f};  // of the rows that the products are in
+        if (F16) {
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) y[tt] *= F16 ? st.out[16 * tt + i16] * back : st.out[16 * tt + i16];
+          for (int i = 0; i < 4; ++i) backs[i] = __shfl(back, 4 * g4 + i);
+        }
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          y[tt] *= st.out[16 * tt + i16];
+          if (F16) y[tt] *= backs;
+        }
       }
       // ---- weights of the chunk's tokens: (c . b) times decay and step
       for (int k = tile0; k < tile1; ++k) {
@@ -687,8 +702,8 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
 #pragma unroll
           for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(u[j]));
         }
-        most = wave_max_f32(most);
-        if (__float_as_uint(most) >= 0x7f800000u) {  // steps without end: every row's state
+        most = row_max(most);
+        if (__float_as_uint(most) >= 0x7f800000u) {  // a step without end
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) S[nt] = f32x4_t{most, most, most, most} * 0.0f;
           most = 0.0f;

@@ -92,6 +92,23 @@ def test_conv_in_chunks_is_the_whole(gpu, fmx):
     assert torch.equal(state, x[:, -3:])
 
 
+@pytest.mark.parametrize("dtype,B,L,C,taps", [
+    (BF16, 20, 65, 8192, 4), (F16, 1, 1301, 1023, 3), (F32, 20, 61, 4096, 2), (BF16, 16, 70, 8192, 8)])
+def test_conv_of_many(gpu, fmx, dtype, B, L, C, taps):
+    """Enough work for runs of 8 tokens, vectors and single elements."""
+    g = _gen(C)
+    x = _randn(g, B, L, C, dtype=dtype).cuda()
+    w, bias = _randn(g, C, taps, dtype=dtype).cuda(), _randn(g, C, dtype=dtype).cuda()
+    lengths = [L - 3 * (b % 3) for b in range(B)]
+    want, bound, after = O.conv(x, w, bias, True, None, B, lengths)
+    state = torch.full((B, taps - 1, C), 3.0, dtype=dtype, device="cuda")
+    print("conv", dtype, B, L, C, taps, flush=True)
+    out = fmx.causal_conv(x, w, bias, None, state, _lens(lengths))
+    for b, n in enumerate(lengths):
+        O.assert_within(out[b, :n], want[b, :n], bound[b, :n], f"row {b}")
+    assert torch.equal(state.double().cpu(), after)
+
+
 # ------------------------------------------------------------------ scan
 
 def _scan_inputs(seed, dtype, B, L, nh, hd, groups, N, slots=6):
@@ -174,6 +191,147 @@ def test_scan_options(gpu, fmx, dtype, L):
     _check_scan(fmx, p)
 
 
+@pytest.mark.parametrize("dtype,nh,hd,groups,N", [
+    (BF16, 4, 64, 2, 128), (F16, 4, 64, 2, 128), (F16, 2, 64, 2, 64), (BF16, 3, 64, 1, 32), (F16, 2, 128, 1, 256),
+    (BF16, 1, 40, 1, 120), (BF16, 2, 32, 2, 256)])
+@pytest.mark.parametrize("lengths,slots,keep", [
+    (None, None, "out"), ([700, 385], [4, 2], "in place"), ([0, 513], None, "in place"), ([640, 64], [-1, 5], "out")])
+def test_scan_segments(gpu, fmx, dtype, nh, hd, groups, N, lengths, slots, keep):
+    """Long sequences of few heads: cut, with a state to start from."""
+    _check_scan(fmx, _scan_inputs(N + nh, dtype, 2, 700, nh, hd, groups, N), lengths, slots, True, keep)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("L", [9, 300])
+def test_scan_rows_of_all_sizes(gpu, fmx, dtype, L):
+    """A head's rows from 2^-12 to 2^8: each keeps its own bits."""
+    p = _scan_inputs(6, dtype, 1, L, 2, 64, 1, 128)
+    by = 2.0 ** (torch.randperm(128, generator=_gen(1)) % 21 - 12).float().cuda().view(2, 64)
+    p["x"] = (p["x"].float() * by).to(dtype)
+    p["state"] *= by[..., None]
+    _check_scan(fmx, p)
+
+
+@pytest.mark.parametrize("L", [5, 130])
+def test_scan_views(gpu, fmx, L):
+    """b shared by the groups, c by the sequences, tokens in another order than
+    memory's, a token's dt 17 elements apart."""
+    p = _scan_inputs(7, BF16, 2, L, 4, 64, 2, 64)
+    p["b"] = p["b"][:, :, :1].expand(2, L, 2, 64)
+    p["c"] = p["c"][:1].expand(2, L, 2, 64)
+    p["x"] = p["x"].permute(1, 2, 0, 3).contiguous().permute(2, 0, 1, 3)
+    p["dt"] = torch.randn(2, 4, L, 17, generator=_gen(2)).to(BF16).cuda()[..., 5].permute(0, 2, 1)
+    _check_scan(fmx, p)
+
+
+@pytest.mark.parametrize("L", [12, 20])
+def test_scan_of_far_tokens(gpu, fmx, L):
+    """Tokens 2^24 elements apart, more than the chunks' lanes address."""
+    p = _scan_inputs(8, BF16, 1, L, 2, 16, 1, 16)
+    x = torch.empty(L * 2 ** 24, dtype=BF16, device="cuda").as_strided((1, L, 2, 16), (8, 2 ** 24, 16, 1))
+    x.copy_(p["x"])
+    p["x"] = x
+    _check_scan(fmx, p, begun=False)
+
+
+def test_scan_slots_beyond_32_bits(gpu, fmx):
+    p = _scan_inputs(10, F16, 2, 70, 64, 64, 1, 128, slots=2)
+    slots = [8200, 3]
+    pool = torch.empty(8201, 64, 64, 128, device="cuda")  # 2^32 elements before the last slot
+    assert slots[0] * pool.stride(0) > 2 ** 32
+    pool[8200], pool[3] = p["state"][0], p["state"][1]
+    sl = torch.tensor(slots, dtype=torch.int32, device="cuda")
+    for L in (70, 4):
+        q = {k: v[:, :L] if k in "xbc" or k == "dt" else v for k, v in p.items()}
+        want_state = p["state"].clone()
+        args = (q["x"], q["dt"], q["a"], q["b"], q["c"], q["d"], q["dt_bias"])
+        want = fmx.ssm_scan(*args, want_state, want_state, dt_limits=LIMITS)
+        got = fmx.ssm_scan(*args, pool, pool, slots=sl, dt_limits=LIMITS)
+        assert torch.equal(got, want) and torch.equal(pool[8200], want_state[0]) and torch.equal(pool[3], want_state[1])
+        p["state"] = want_state
+
+
+def test_rows_beyond_32_bits(gpu, fmx):
+    """The second sequence's rows 2^32 elements behind the first one's."""
+    g, C, L = _gen(15), 64, 21
+    far = [torch.empty(2 ** 32 + 2 * L * C, dtype=BF16, device="cuda").as_strided((2, L, C), (2 ** 32 + C, C, 1))
+           for _ in range(2)]
+    x, w = _randn(g, 2, L, C, dtype=BF16).cuda(), _randn(g, C, 4, dtype=BF16).cuda()
+    far[0].copy_(x)
+    assert torch.equal(fmx.causal_conv(far[0], w, out=far[1]), fmx.causal_conv(x, w))
+    assert torch.equal(fmx.gated_norm(far[0], None, far[0], groups=4, out=far[1]), fmx.gated_norm(x, None, x, groups=4))
+    p = _scan_inputs(16, BF16, 2, L, 1, 64, 1, 8)
+    far[0].copy_(p["x"].flatten(2))
+    args = (p["dt"], p["a"], p["b"], p["c"], p["d"], p["dt_bias"])
+    for n in (L, 3):
+        cut = tuple(t[:, :n] if t.dim() > 1 else t for t in args)
+        got = fmx.ssm_scan(far[0].unflatten(2, (1, 64))[:, :n], *cut, out=far[1].unflatten(2, (1, 64))[:, :n])
+        assert torch.equal(got, fmx.ssm_scan(p["x"][:, :n], *cut))
+
+
+def test_nothing_to_do(gpu, fmx):
+    """No sequences, no tokens: outputs of that shape; without tokens states are carried over."""
+    p = _scan_inputs(17, BF16, 2, 3, 2, 16, 1, 16, slots=2)
+    for B, L in ((0, 3), (2, 0)):
+        q = {k: v[:B, :L] if k in "xbc" or k == "dt" else v for k, v in p.items()}
+        s_out = torch.full_like(p["state"], 3.0)
+        y = fmx.ssm_scan(q["x"], q["dt"], q["a"], q["b"], q["c"], q["d"], q["dt_bias"], p["state"], s_out)
+        assert y.shape == (B, L, 2, 16)
+        assert torch.equal(s_out, p["state"] if B else torch.full_like(s_out, 3.0))
+        x, w = torch.randn(B, L, 16, device="cuda"), torch.randn(16, 4, device="cuda")
+        c_in, c_out = torch.randn(2, 3, 16, device="cuda"), torch.full((2, 3, 16), 3.0, device="cuda")
+        assert fmx.causal_conv(x, w, None, c_in, c_out).shape == x.shape
+        assert torch.equal(c_out, c_in if B else torch.full_like(c_out, 3.0))
+        assert fmx.gated_norm(x).shape == x.shape
+    none = torch.empty(0, 2, 16, 16, device="cuda")  # a pool of no slots: from 0, nothing kept
+    args = (p["x"], p["dt"], p["a"], p["b"], p["c"])
+    assert torch.equal(fmx.ssm_scan(*args, state=none, state_out=none), fmx.ssm_scan(*args))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("L", [4, 100])
+def test_scan_from_a_state_with_infinities(gpu, fmx, dtype, L):
+    """They stay in their rows."""
+    p = _scan_inputs(18, dtype, 1, L, 2, 64, 1, 128, slots=1)
+    args = (p["x"], p["dt"], p["a"], p["b"], p["c"], p["d"], p["dt_bias"])
+    after, after_bad = torch.empty_like(p["state"]), torch.empty_like(p["state"])
+    clean = fmx.ssm_scan(*args, p["state"], after, dt_limits=LIMITS)
+    bad = p["state"].clone()
+    bad[0, 1, 5, 7], bad[0, 0, 63, 0] = math.inf, math.nan
+    y = fmx.ssm_scan(*args, bad, after_bad, dt_limits=LIMITS)
+    for h, r in ((1, 5), (0, 63)):
+        assert not torch.isfinite(y[0, :, h, r]).any() and not torch.isfinite(after_bad[0, h, r]).all()
+        y[0, :, h, r], after_bad[0, h, r] = clean[0, :, h, r], after[0, h, r]
+    assert torch.equal(y, clean) and torch.equal(after_bad, after)
+
+
+def test_scan_graphs_share_a_workspace(gpu, fmx):
+    """Two captured scans of several segments with one workspace, replayed in
+    turn on one stream, with eager ones between."""
+    ps = [_scan_inputs(19 + i, BF16, 1, 700 - 60 * i, 2, 64, 1, 128, slots=1) for i in range(2)]
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    run = [lambda p=p, out=torch.zeros_like(p["x"], memory_format=torch.contiguous_format): fmx.ssm_scan(
+        p["x"], p["dt"], p["a"], p["b"], p["c"], p["d"], p["dt_bias"], p["state"], p["state"], dt_limits=LIMITS, out=out,
+        workspace=ws) for p in ps]
+    first = [p["state"].clone() for p in ps]
+    want = []
+    for i in range(2):
+        want.append([(run[i]().clone(), ps[i]["state"].clone()) for _ in range(3)])
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = run[i]()
+        graphs.append((g, y))
+        ps[i]["state"].copy_(first[i])
+    for k in range(3):
+        for i in range(2):
+            graphs[i][0].replay()
+            fmx.ssm_scan(ps[i]["x"], ps[i]["dt"], ps[i]["a"], ps[i]["b"], ps[i]["c"], workspace=ws)
+            torch.cuda.synchronize()
+            assert torch.equal(graphs[i][1], want[i][k][0]) and torch.equal(ps[i]["state"], want[i][k][1])
+
+
 def test_scan_infinities_come_late(gpu, fmx):
     """What is not finite in a token reaches it and later tokens, none before."""
     for at in (0, 5, 66, 127):
@@ -221,6 +379,28 @@ def test_gated_norm(gpu, fmx, dtype, B, L, C, groups, lengths, pad, gate):
         assert torch.equal(x[b, :live[b]], out[b, :live[b]])
 
 
+@pytest.mark.parametrize("dtype,B,L,C,groups", [
+    (BF16, 1, 262145, 32, 1), (F16, 3, 2731, 1024, 8), (BF16, 2, 1025, 4096, 8), (F16, 1, 2051, 8192, 8),
+    (F32, 3, 5462, 64, 4), (BF16, 1, 16400, 36, 1)])
+@pytest.mark.parametrize("gate_first", [True, False])
+def test_gated_norm_of_many(gpu, fmx, dtype, B, L, C, groups, gate_first):
+    """Enough groups for two at a time, and the last ones left over."""
+    g = _gen(C)
+    x, z = _randn(g, B, L, C, dtype=dtype).cuda(), _randn(g, B, L, C, dtype=dtype).cuda()
+    w = (1 + 0.1 * _randn(g, C)).to(dtype).cuda()
+    want, bound = O.gated_norm(x, w, z, 1e-5, groups, gate_first, dtype)
+    lengths = [L - 5 * b for b in range(B)]
+    out = torch.full((B, L, C), 7.0, dtype=dtype, device="cuda")
+    print("norm", dtype, B, L, C, groups, flush=True)
+    fmx.gated_norm(x, w, z, groups=groups, gate_first=gate_first, lengths=_lens(lengths), out=out)
+    _untouched(out, lengths)
+    for b, n in enumerate(lengths):
+        O.assert_within(out[b, :n], want[b, :n], bound[b, :n], f"row {b}")
+    fmx.gated_norm(x, w, z, groups=groups, gate_first=gate_first, out=z)  # in place of the gate: the same bits
+    for b, n in enumerate(lengths):
+        assert torch.equal(z[b, :n], out[b, :n])
+
+
 def test_gated_norm_of_zeros(gpu, fmx):
     x = torch.zeros(1, 2, 64, dtype=BF16, device="cuda")
     assert (fmx.gated_norm(x, None, eps=1e-6) == 0).all()
@@ -249,10 +429,14 @@ def _project(seed, dtype, shape, layer):
 @pytest.mark.parametrize("dtype,B,nh,hd,groups,N,taps,kw", [
     (BF16, 1, 4, 64, 2, 128, 4, {}), (F16, 5, 3, 80, 1, 48, 3, dict(norm_groups=1)),
     (BF16, 3, 2, 128, 1, 64, 2, dict(gate_first=False)), (F16, 2, 6, 24, 3, 256, 8, dict(activation=None, eps=1e-3)),
-    (BF16, 2, 1, 8, 1, 8, 4, dict(softplus=True))])
-def test_step(gpu, fmx, dtype, B, nh, hd, groups, N, taps, kw):
+    (BF16, 2, 1, 8, 1, 8, 4, dict(softplus=True)), (BF16, 2, 64, 64, 8, 16, 4, dict(norm_groups=1)),
+    (F16, 2, 160, 64, 1, 8, 4, {}), (BF16, 1, 4, 200, 4, 32, 5, dict(norm_groups=2))])
+@pytest.mark.parametrize("odd", [False, True])
+def test_step(gpu, fmx, dtype, B, nh, hd, groups, N, taps, kw, odd):
     layer = _layer(fmx, 3, dtype, nh, hd, groups, N, taps, **kw)
     xbc, dt, z = _project(4, dtype, (B,), layer)
+    if odd:  # rows on no vector
+        xbc, z = _cut(xbc.cpu(), 3, dtype), _cut(z.cpu(), 5, dtype)
     conv_state, state = (torch.randn(*t.shape, generator=_gen(5)).to(t.dtype).cuda() for t in layer.new_states(7))
     slots = [6, 0, 9, 3, -1][:B]
     n = groups * N
@@ -366,3 +550,60 @@ def test_prompt_captured_and_on_two_streams(gpu, fmx):
         torch.cuda.synchronize()
         for b, n in enumerate((300, 131)):
             assert torch.equal(out[b, :n], want[i][b, :n])
+
+
+def test_step_slots_beyond_32_bits(gpu, fmx):
+    layer = _layer(fmx, 21, BF16, 64, 64, 1, 128, 4)
+    xbc, dt, z = _project(22, BF16, (2,), layer)
+    conv_small, small = (torch.randn(*t.shape, generator=_gen(5)).to(t.dtype).cuda() for t in layer.new_states(2))
+    pool, slots = torch.empty(8201, 64, 64, 128, device="cuda"), [8200, 3]
+    conv_pool = torch.empty(8201, 3, layer.channels, dtype=BF16, device="cuda")
+    for i, s in enumerate(slots):
+        pool[s], conv_pool[s] = small[i], conv_small[i]
+    sl = torch.tensor(slots, dtype=torch.int32, device="cuda")
+    got = layer.step(xbc, dt, z, conv_pool, pool, sl)
+    want = layer.step(xbc, dt, z, conv_small, small)
+    assert torch.equal(got, want)
+    for i, s in enumerate(slots):
+        assert torch.equal(pool[s], small[i]) and torch.equal(conv_pool[s], conv_small[i])
+
+
+def test_step_graphs_share_a_workspace(gpu, fmx):
+    """Two layers' steps captured with one workspace, replayed in turn."""
+    layers = [_layer(fmx, 23 + i, BF16, 4, 64, 2, 64, 4) for i in range(2)]
+    ins = [_project(25 + i, BF16, (5,), m) for i, m in enumerate(layers)]
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    states, refs = [m.new_states(5) for m in layers], [m.new_states(5) for m in layers]
+    graphs = []
+    for m, p, st in zip(layers, ins, states):
+        m.step(*p, *st, workspace=ws)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = m.step(*p, *st, workspace=ws)
+        graphs.append((g, y))
+        for t in st:
+            t.zero_()
+    for _ in range(4):
+        for m, p, st, ref, (g, y) in zip(layers, ins, states, refs, graphs):
+            g.replay()
+            want = m.step(*p, *ref)
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and all(torch.equal(s, r) for s, r in zip(st, ref))
+
+
+def test_a_nan_stays_in_its_sequence(gpu, fmx):
+    """A padded batch with one bad sequence: the others' bits are the same."""
+    layer = _layer(fmx, 27, BF16, 4, 64, 2, 128, 4)
+    xbc, dt, z = (t.clone() for t in _project(28, BF16, (3, 150), layer))
+    lens = _lens([150, 90, 20])
+    for t in (xbc, dt, z):
+        t[2, 20:] = math.nan
+    states, bad_states = layer.new_states(3), layer.new_states(3)
+    clean = layer.prompt(xbc, dt, z, *states, lens)
+    xbc[1, 30:40] = math.inf
+    bad = layer.prompt(xbc, dt, z, *bad_states, lens)
+    for b, n in ((0, 150), (2, 20)):
+        assert torch.equal(bad[b, :n], clean[b, :n])
+        assert all(torch.equal(s[b], t[b]) for s, t in zip(states, bad_states))
+    # the tokens before it sum the same numbers in an order that depends on none of their values
+    assert torch.equal(bad[1, :30], clean[1, :30]) and not torch.isfinite(bad[1, 34:90]).any()
