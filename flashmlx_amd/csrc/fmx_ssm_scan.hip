@@ -829,8 +829,16 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
 
 int chunk_steps(int N) { return N <= 32 ? 1 : N <= 64 ? 2 : N <= 128 ? 4 : 8; }
 
-constexpr int kFewMost = 16;      // tokens that the walk takes
+// Tokens that the walk takes. One sequence of 64 heads of 64 rows and 128
+// columns: 8 tokens 12.3 us, 12 15.3, 16 18.1, a chunk 13.0; 16 of them 26, 33,
+// 38 and 33; 16 of 24 heads 18, 22, 26 and 18.
+constexpr int kFewMost = 8;
 constexpr int kFullGrid = 256;    // workgroups that fill the CUs (one each, by its LDS)
+// Chunks of a segment up to which a workgroup takes one item rather than two
+// (which halve the reads of b and c and half hide each other's latencies): 64
+// heads of 200 tokens 25 us for 27, of 768 (3 chunks, 2 by two) 34 for 38, of
+// 1024 (4, 2) 39 for 38; 4 sequences of 200 (4, 2) 28 for 34.
+constexpr int kAloneChunks = 4;
 
 struct ScanPlan {
   ChunkPlan ck;
@@ -839,14 +847,17 @@ struct ScanPlan {
   size_t bytes;
 };
 
-ScanPlan scan_plan(const ScanArgs& a) {
+// Workgroups of `slots` items; as many segments as leave no CU without one and
+// none with two (16 ragged sequences of 24 heads, 192 workgroups: 129 us, in 2
+// segments 158, in 4 137; 8192 tokens of 64 heads in 6 155, in 8 127, in 16
+// 141), of 2 chunks at least.
+ScanPlan scan_plan(const ScanArgs& a, int slots) {
   ScanPlan p{};
   ChunkPlan& c = p.ck;
   c.tiles = (a.hd + kTileRows - 1) / kTileRows;
-  const int items = a.rep * c.tiles;
-  p.slots = items > 1 ? 2 : 1;
+  p.slots = slots;
   p.nk = chunk_steps(a.N);
-  c.pairs = (items + p.slots - 1) / p.slots;
+  c.pairs = (a.rep * c.tiles + slots - 1) / slots;
   const int64_t base = static_cast<int64_t>(a.B) * a.groups * c.pairs;
   const int chunks = (a.L + kChunk - 1) / kChunk;
   const int want = static_cast<int>(std::min<int64_t>(kFullGrid / std::max<int64_t>(base, 1), 32));
@@ -859,6 +870,11 @@ ScanPlan scan_plan(const ScanArgs& a) {
     p.bytes = (p.states + heads) * sizeof(float);
   }
   return p;
+}
+ScanPlan scan_plan(const ScanArgs& a) {
+  const ScanPlan p = scan_plan(a, 1);
+  const bool alone = static_cast<int64_t>(a.B) * a.groups * p.ck.pairs <= kFullGrid && p.ck.seg_chunks <= kAloneChunks;
+  return alone || a.rep * p.ck.tiles == 1 ? p : scan_plan(a, 2);
 }
 
 template <bool F16, int NK, int SLOTS>

@@ -201,6 +201,15 @@ def test_scan_segments(gpu, fmx, dtype, nh, hd, groups, N, lengths, slots, keep)
     _check_scan(fmx, _scan_inputs(N + nh, dtype, 2, 700, nh, hd, groups, N), lengths, slots, True, keep)
 
 
+@pytest.mark.parametrize("dtype,nh,hd,groups,N,L,lengths,keep", [
+    (BF16, 258, 8, 2, 128, 100, None, "out"), (F16, 258, 8, 2, 64, 130, None, "in place"), (BF16, 300, 16, 3, 256, 70, None, "no"),
+    (F16, 260, 64, 4, 16, 65, [33], "out"), (F16, 128, 64, 1, 32, 660, [651], "in place"),
+    (BF16, 127, 8, 1, 128, 700, None, "in place"), (F16, 126, 8, 2, 256, 660, [640], "out"), (BF16, 66, 72, 2, 64, 645, None, "out")])
+def test_scan_of_many_heads(gpu, fmx, dtype, nh, hd, groups, N, L, lengths, keep):
+    """Enough items for two to a workgroup, an odd one alone in its group among them."""
+    _check_scan(fmx, _scan_inputs(nh + N, dtype, 1, L, nh, hd, groups, N, slots=2), lengths, [1], True, keep)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("L", [9, 300])
 def test_scan_rows_of_all_sizes(gpu, fmx, dtype, L):
