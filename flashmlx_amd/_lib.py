@@ -1,5 +1,6 @@
 """ctypes binding of libfmx.so (the C-ABI declared in include/fmx.h,
-include/fmx_model.h, include/fmx_nemotron.h and include/fmx_cache.h).
+include/fmx_model.h, include/fmx_nemotron.h, include/fmx_cache.h and
+include/fmx_ssm.h).
 
 This module only loads the library and declares its signatures. It raises
 ImportError when libfmx.so is missing: there is no fallback path.

@@ -90,9 +90,11 @@ typedef struct fmx_ssm_shape {
  * state [n_slots, n_heads, head_dim, state_dim] fp32, contiguous, 16-byte
  * aligned: state_in NULL: 0; state_out receives S behind the last token, may
  * be state_in; NULL: not kept.
- * S, sums and decays are fp32 or more, out is rounded once. What is infinite
- * or NaN in a token's rows reaches that token and later ones of its sequence,
- * none before it. */
+ * S, sums and decays are fp32 or more, out is rounded once. (float16 with more
+ * than 8 tokens: to 2^-37 of the largest value in a row of a head's state, and
+ * of those that 64 tokens bring to it.) What is infinite or NaN in a token's
+ * rows reaches that token and later ones of its sequence, as either, and none
+ * before it; of a state's row, that row. */
 size_t fmx_ssm_scan_workspace_size(const fmx_ssm_shape* shape);
 int fmx_ssm_scan(const fmx_ssm_shape* shape, const fmx_heads* x, const fmx_heads* dt,
                  const float* a, const fmx_heads* b, const fmx_heads* c, const float* d,

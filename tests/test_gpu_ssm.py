@@ -221,6 +221,30 @@ def test_scan_rows_of_all_sizes(gpu, fmx, dtype, L):
     _check_scan(fmx, p)
 
 
+@pytest.mark.parametrize("L", [40, 100])
+def test_scan_f16_tokens_of_all_sizes(gpu, fmx, L):
+    """A token 2^24 times the others, alone in its column of the state. What
+    tokens bring is scaled to its largest and taken as two numbers of float16,
+    2^13 .. 2^14 at most and cut at 2^-24: off by 2^-37 of the largest, as the
+    state is where it goes into outputs."""
+    p = _scan_inputs(13, F16, 1, L, 1, 64, 1, 32, slots=1)
+    p["x"][:, 1:] *= 2.0 ** -13
+    p["x"][:, 0] *= 2.0 ** 11
+    p["b"][:, 0, :, 1:] = 0
+    p["b"][:, 1:, :, 0] = 0
+    steps, rel = O.time_step(p["dt"], p["dt_bias"], True, *LIMITS)
+    want, bound, after, after_b = O.scan(p["x"], steps, rel, p["a"], p["b"], p["c"], p["d"], None, 1, rounded=F16)
+    most = (steps[0, :, :, None] * p["x"][0].double().cpu().abs()).sum(0)[..., None]  # [1, 64, 1], of what tokens bring
+    b, c = p["b"][0, :, 0].double().cpu().abs(), p["c"][0, :, 0].double().cpu().abs()
+    lost = 2.0 ** -37 * most * b.sum(0)
+    s_out = torch.empty(1, 1, 64, 32, device="cuda")
+    y = fmx.ssm_scan(p["x"], p["dt"], p["a"], p["b"], p["c"], p["d"], p["dt_bias"], None, s_out, dt_limits=LIMITS)
+    O.assert_within(s_out[0], after[0], after_b[0] + lost, "state")
+    more = (lost[None] * c[:, None, None]).sum(-1) + 2.0 ** -37 * (most * b.max())[None, ..., 0] * c.sum(-1)[:, None, None]
+    O.assert_within(y[0], want[0], bound[0] + more, "out")
+    assert (lost[0, :, 1:] < 2.0 ** -9 * after[0, 0, :, 1:].abs().max()).all()  # (far from what a missing second number would lose)
+
+
 @pytest.mark.parametrize("L", [5, 130])
 def test_scan_views(gpu, fmx, L):
     """b shared by the groups, c by the sequences, tokens in another order than

@@ -159,3 +159,26 @@ def test_python_refusals():
             call()
     with pytest.raises(TypeError):
         F.gated_norm(x.int())
+
+
+def test_scan_workspaces(lib):
+    """Segments' states: none for few tokens or few chunks, a bounded number for
+    long sequences; one too small, or on no 256 bytes, is refused."""
+    size = lambda **kw: lib.fmx_ssm_scan_workspace_size(_shape(**kw))  # noqa: E731
+    assert size(B=1, L=5) == 0 and size(B=1, L=64) == 0 and size(B=256, L=4096, nh=64, g=8) == 0
+    need = size(B=1, L=8192, nh=64, g=8)
+    assert 0 < need <= 33 * 64 * (64 * 128 + 1) * 4 and size(B=1, L=1 << 24, nh=64, g=8) <= 33 * 64 * (64 * 128 + 1) * 4
+    long = dict(B=1, L=8192, nh=64, g=8)
+    views = lambda: {k: Heads(1 << 34, 1 << 14, data=1 << at)  # noqa: E731
+                     for k, at in (("x", 50), ("b", 51), ("c", 52), ("dt", 53), ("out", 54))}
+    assert _scan(lib, _shape(**long), s_in=None, s_out=None, ws=AT, ws_bytes=need - 1, **views()) == WS
+    assert _scan(lib, _shape(**long), s_in=None, s_out=None, ws=AT + 16, ws_bytes=need, **views()) == ARG
+
+
+def test_header_is_c(tmp_path):
+    import pathlib
+    import subprocess
+    include = pathlib.Path(__file__).parent.parent / "include"
+    src = tmp_path / "h.c"
+    src.write_text('#include "fmx_ssm.h"\nint main(void) { fmx_ssm_shape s = {FMX_BF16}; return s.dtype != FMX_BF16; }\n')
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-fsyntax-only", f"-I{include}", str(src)], check=True)
