@@ -395,25 +395,34 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
   const uint32_t c_off = STATES ? 0 : static_cast<uint32_t>(b_row * static_cast<int>(a.c.ts)) * 2;
   const uint32_t x_off = static_cast<uint32_t>(x_row * static_cast<int>(a.x.ts)) * 2;
   // (pointers go on by a chunk with each load)
-  auto load_rows = [&](const uint16_t*& from, uint32_t off, int64_t ts, int t0, uint32_t to) {  // of b or c
+  auto load_rows = [&](const uint16_t* from, uint32_t off, int64_t ts, int t0, uint32_t to, auto whole) {  // of b or c
 #pragma unroll
     for (int k = 0; k < kBi; ++k) {
       const int col = b_col ^ (k * kStep / 4 % 4 * 8);
-      if ((NK * 4 >= kWaves || wave < NK * 4) && t0 + b_row + k * kStep < t_end && col < a.N)
+      if ((NK * 4 >= kWaves || wave < NK * 4) && (whole() || (t0 + b_row + k * kStep < t_end && col < a.N)))
         to_lds16(from + k * kStep * ts, off + col * 2, to + (wave + k * kWaves) * 1024);
     }
-    from += kChunk * ts;
   };
-  auto load = [&](int t0, int buf) {
-    load_rows(bp, b_off, a.b.ts, t0, lds_at + offsetof(Lds, b) + buf * sizeof(lds.b[0]));
-    if (!STATES) load_rows(cp, c_off, a.c.ts, t0, lds_at + offsetof(Lds, c) + buf * sizeof(lds.c[0]));
+  auto load_all = [&](int t0, int buf, auto whole) {
+    load_rows(bp, b_off, a.b.ts, t0, lds_at + offsetof(Lds, b) + buf * sizeof(lds.b[0]), whole);
+    if (!STATES) load_rows(cp, c_off, a.c.ts, t0, lds_at + offsetof(Lds, c) + buf * sizeof(lds.c[0]), whole);
+    if (!live) return;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int col = x_col ^ (k * 16);
-      if (live && t0 + x_row + k * 8 < t_end && row0 + col < a.hd)
+      if (whole() || (t0 + x_row + k * 8 < t_end && row0 + col < a.hd))
         to_lds16(xp + k * 8 * a.x.ts, x_off + col * 2,
                  lds_at + offsetof(Lds, x) + (buf * SLOTS + slot) * sizeof(lds.x[0][0]) + (w4 * 2 + k) * 1024);
     }
+  };
+  const bool wide = a.N == 32 * NK && a.hd % kTileRows == 0;
+  auto load = [&](int t0, int buf) {
+    if (wide && t0 + kChunk <= t_end)
+      load_all(t0, buf, [] { return true; });  // (no lane masked: 40 instructions fewer)
+    else
+      load_all(t0, buf, [] { return false; });
+    bp += kChunk * a.b.ts;
+    if (!STATES) cp += kChunk * a.c.ts;
     xp += kChunk * a.x.ts;
   };
 
@@ -449,6 +458,7 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
         if (lane < 16 * k) s.far[far_at(k) + lane] = dt * power(at[k - 1] - sum);
     }
   };
+  if (live && w4 < chunks) load_dt(w4);
   const u32x4_t zero{0, 0, 0, 0};
   // What no load writes is 0, or of earlier tokens of the sequence: finite, or
   // of a row that is NaN by now.
@@ -466,10 +476,8 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
     }
   }
   lds_barrier();
-  if (chunks > 0) {
-    load(t_first, 0);
-    if (live && w4 < chunks) load_dt(w4);
-  }
+  asm volatile("" : "+v"(vdt));  // (waited for here, so that the steps need not wait for the rows)
+  if (chunks > 0) load(t_first, 0);
 
   // ---- the state: lane i16 has row i16 of its wave's 16; of tile nt columns
   // 32 (nt / 2) + 8 g4 + 4 (nt % 2) .. + 3, so that two tiles are 8 columns in
@@ -524,9 +532,11 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
   const int own_base = chunk_at<8>(i16, 2 * w4 + (g4 >> 1)) + (g4 & 1) * 8;  // rows 4 g4 .. + 3 of token i16
   const int m_base0 = weight_at(i16, g4), m_base1 = weight_at(32 + i16, g4);
 
-  // weights' tiles (tokens s, token t) of this wave, rows of t from the longest on
-  const int tile0 = SLOTS == 2 ? (wave < 2 ? 2 * wave : wave + 2) : (wave < 2 ? 2 * wave : 3 * wave - 2);
-  const int tile1 = SLOTS == 2 ? (wave < 2 ? tile0 + 2 : tile0 + 1) : (wave < 2 ? tile0 + 2 : tile0 + 3);
+  // The weights' 10 tiles of 16 tokens s and 16 tokens t: six below the diagonal
+  // and the diagonal's four, which take longer, two to three a wave, or one for
+  // both slots and, for four waves, another for one slot
+  constexpr uint32_t kTileT = 0x6e4bf, kTileS = 0x1e424;  // two bits each
+  constexpr int kTiles = 10, kTurns = SLOTS == 2 ? 2 : 3;
 
   wait_vmcnt0();
   for (int ck = 0; ck < chunks; ++ck) {
@@ -607,9 +617,11 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
         }
       }
       // ---- weights of the chunk's tokens: (c . b) times decay and step
-      for (int k = tile0; k < tile1; ++k) {
-        const int tt = k < 4 ? 3 : k < 7 ? 2 : k < 9 ? 1 : 0;
-        const int ss = k < 4 ? k : k < 7 ? k - 4 : k < 9 ? k - 7 : 0;
+      for (int turn = 0; turn < kTurns; ++turn) {
+        const bool both = SLOTS == 1 || turn == 0;
+        const int k = both ? wave + 4 * turn : 8 + (wave >> 1);
+        if (k >= kTiles) break;
+        const int tt = kTileT >> 2 * k & 3, ss = kTileS >> 2 * k & 3;
         f32x4_t dot{0.0f, 0.0f, 0.0f, 0.0f};
         s16x8_t fb[NK], fc[NK];
 #pragma unroll
@@ -623,7 +635,7 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
         const int t = 16 * tt + i16, s = 16 * ss + 4 * g4;
 #pragma unroll
         for (int q = 0; q < SLOTS; ++q) {
-          if (q >= n_slots) break;
+          if (q >= n_slots || (!both && q != (wave & 1))) continue;
           const ChunkSteps<STATES>& sq = round[q];
           float m[4];
           if (ss < tt) {
