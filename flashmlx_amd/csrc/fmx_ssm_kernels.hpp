@@ -83,11 +83,29 @@ size_t scan_workspace(const ScanArgs& a);
 bool scan_fits(const ScanArgs& a);
 hipError_t launch_scan(const ScanArgs& a, bool f16, void* ws, hipStream_t stream);
 
+// ln(1 + e^-t), t >= 0, to 8 steps of 2^-24: e = e^-t with the product's rest,
+// ln(1 + e) = 2 atanh(e / (2 + e)) by its series, whose argument is at most 1/3
+// (the ninth term 2^-29)
+__device__ inline float log1p_exp_minus(float t) {
+  t = fminf(t, 126.0f);
+  const float p = t * -1.44269504f, rest = __builtin_fmaf(t, -1.44269504f, -p) + t * -1.925963e-8f;
+  float e = __builtin_amdgcn_exp2f(p);
+  e = __builtin_fmaf(e, rest * 0.6931472f, e);
+  const float d = 2.0f + e;
+  float r = __builtin_amdgcn_rcpf(d);
+  r = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
+  const float s = e * r, q = s * s;
+  float f = 1.0f / 15;
+#pragma unroll
+  for (int k = 13; k > 0; k -= 2) f = __builtin_fmaf(f, q, 1.0f / k);
+  return 2.0f * s * f;
+}
+
 // the time step: ln(1 + e^v) = max(v, 0) + ln(1 + e^-|v|), which loses nothing
 // where e^v is small; comparisons that leave a NaN one
 __device__ inline float time_step(float raw, const float* bias, int h, int softplus, float lo, float hi) {
   float v = bias ? raw + bias[h] : raw;
-  if (softplus) v = (v > 0.0f ? v : v == v ? 0.0f : v) + log1pf(expf(-fabsf(v)));
+  if (softplus) v = (v > 0.0f ? v : v == v ? 0.0f : v) + log1p_exp_minus(fabsf(v));
   return v < lo ? lo : v > hi ? hi : v;
 }
 
