@@ -4,7 +4,7 @@
 //
 // scan_few_kernel walks the tokens one by one with the state in registers: the
 // state is read and written once, and that is its time while tokens are few (32
-// sequences of 5 tokens, 32 heads of 128 rows and 64 columns: 20.8 us in a
+// sequences of 5 tokens, 32 heads of 128 rows and 64 columns: 20.7 us in a
 // graph, 4.93 TB/s of a copy would be 14.2; each further token 0.75 us of
 // staging, a chain of adds across lanes and a barrier).
 //
@@ -20,7 +20,7 @@
 // to 8 or 11 bits. Long sequences are cut into segments: a first launch forms
 // each segment's state from 0, a second starts each segment from the sum of
 // those before it.
-// 8192 tokens of 64 heads of 64 rows, 128 columns, 8 groups: 122 us (39 and 96
+// 8192 tokens of 64 heads of 64 rows, 128 columns, 8 groups: 118 us (38 and 93
 // traced alone; a walk of the tokens 7888). A workgroup's chunk takes 12 to 14
 // thousand cycles, of which by count a SIMD's matrix instructions fill 3 (two and three
 // times those of operands rounded once), LDS 4, and vector instructions (splits,
@@ -874,9 +874,9 @@ struct ScanPlan {
 };
 
 // Workgroups of `slots` items; as many segments as leave no CU without one and
-// none with two (16 ragged sequences of 24 heads, 192 workgroups: 129 us, in 2
-// segments 158, in 4 137; 8192 tokens of 64 heads in 6 155, in 8 127, in 16
-// 141), of 2 chunks at least.
+// none with two, of 2 chunks at least. (By one build: 16 ragged sequences of 24
+// heads, 192 workgroups, 129 us, in 2 segments 158, in 4 137; 8192 tokens of 64
+// heads in 6 155, in 8 127, in 16 141.)
 ScanPlan scan_plan(const ScanArgs& a, int slots) {
   ScanPlan p{};
   ChunkPlan& c = p.ck;
