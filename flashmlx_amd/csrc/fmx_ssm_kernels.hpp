@@ -24,8 +24,10 @@ struct El<kElF32> {
   static __device__ inline T st(float f) { return f; }
 };
 
+// N elements that one instruction moves: on whole words, which is all that the
+// memory instructions of up to four words ask for
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
+struct alignas(sizeof(T) * N < 4 ? sizeof(T) * N : 4) Pack {
   T e[N];
 };
 
@@ -34,9 +36,10 @@ __device__ inline float silu_f32(float v) {
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * 1.4426950408889634f));
 }
 
-// whether a view's rows start on vectors of vec elements of es bytes
-inline bool on_vectors(const HeadsView& v, int es, int vec) {
-  return !v.p || (reinterpret_cast<uintptr_t>(v.p) % (es * vec) == 0 && v.bs % vec == 0 && v.ts % vec == 0);
+// whether an array, or a view's rows, of elements of es bytes start on words
+inline bool on_words(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+inline bool on_words(const HeadsView& v, int es) {
+  return !v.p || (on_words(v.p) && v.bs * es % 4 == 0 && v.ts * es % 4 == 0);
 }
 
 __device__ inline int seq_length(const int32_t* lens, int L, int b) {

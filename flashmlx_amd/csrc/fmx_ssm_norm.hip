@@ -140,11 +140,13 @@ __global__ __launch_bounds__(kGateThreads) void gated_norm_kernel(GatedNormArgs 
   }
 }
 
-// lanes of a group of so many vectors
+// Lanes of a group of so many vectors: up to three vectors a lane rather than
+// more lanes with some idle (8192 rows of 16 groups of 256 in bf16: 16 lanes 45
+// us, 64 72; of 8 groups of 512, four a lane: 53, 64 lanes 49).
 int norm_lanes(int vecs) {
   if (vecs > 128) return kGateThreads;
   int n = 4;
-  while (n < vecs && n < kWave) n *= 4;
+  while (3 * n < vecs && n < kWave) n *= 4;
   return n;
 }
 
@@ -159,7 +161,7 @@ hipError_t gated_norm(const GatedNormArgs& a, hipStream_t stream) {
   // Two groups' loads in flight where there are enough for it: 8192 rows of 8
   // groups of 512 50.4 us (4.0 TB/s) in a graph, one 52.3, four 60.6.
   constexpr int kRounds = VEC > 1 ? 2 : 1;
-  const int rounds = ln < kGateThreads && items >= int64_t{4096} * per ? kRounds : 1;
+  const int rounds = ln < kGateThreads && (pl.vecs <= ln || ln == kWave) && items >= int64_t{4096} * per ? kRounds : 1;
   const dim3 grid(static_cast<uint32_t>((items + per * rounds - 1) / (per * rounds))), wg(kGateThreads);
 #define FMX_NORM(LN, NV, GR) hipLaunchKernelGGL((gated_norm_kernel<DT, VEC, LN, NV, GR>), grid, wg, 0, stream, a, pl)
 #define FMX_NORM_FEW(LN, NV)                        \
@@ -169,8 +171,12 @@ hipError_t gated_norm(const GatedNormArgs& a, hipStream_t stream) {
     else                                            \
       FMX_NORM(LN, NV, 1);                          \
   } while (0)
-  if (ln == 4) FMX_NORM_FEW(4, 1);
-  else if (ln == 16) FMX_NORM_FEW(16, 1);
+  if (ln == 4 && pl.vecs <= 4) FMX_NORM_FEW(4, 1);
+  else if (ln == 4 && pl.vecs <= 8) FMX_NORM(4, 2, 1);
+  else if (ln == 4) FMX_NORM(4, 3, 1);
+  else if (ln == 16 && pl.vecs <= 16) FMX_NORM_FEW(16, 1);
+  else if (ln == 16 && pl.vecs <= 32) FMX_NORM(16, 2, 1);
+  else if (ln == 16) FMX_NORM(16, 3, 1);
   else if (ln == 64 && pl.vecs <= 64) FMX_NORM_FEW(64, 1);
   else if (ln == 64) FMX_NORM_FEW(64, 2);
   else if (pl.vecs <= 256) FMX_NORM(256, 1, 1);
@@ -187,10 +193,12 @@ hipError_t gated_norm(const GatedNormArgs& a, hipStream_t stream) {
 bool gated_norm_fits(const GatedNormArgs& a) { return norm_items(a) <= max_blocks(kGateThreads); }
 
 hipError_t launch_gated_norm(const GatedNormArgs& a, int dt, hipStream_t stream) {
-  // 16-byte vectors where every row and group falls on them, single elements otherwise
+  // 16 bytes at once where every row starts on a word and groups are whole
+  // vectors (19143 rows of 3 groups of 320 in f16, the gate's 4440 bytes apart:
+  // 35 us, by elements 102), single elements otherwise
   const int es = dt == kElF32 ? 4 : 2, vec = 16 / es;
-  bool wide = a.C / a.groups % vec == 0 && reinterpret_cast<uintptr_t>(a.w) % 16 == 0;
-  for (const HeadsView* v : {&a.x, &a.z, &a.out}) wide = wide && on_vectors(*v, es, vec);
+  bool wide = a.C / a.groups % vec == 0 && on_words(a.w);
+  for (const HeadsView* v : {&a.x, &a.z, &a.out}) wide = wide && on_words(*v, es);
   if (dt == kElF32) return wide ? gated_norm<kElF32, 4>(a, stream) : gated_norm<kElF32, 1>(a, stream);
   if (dt == kElF16) return wide ? gated_norm<kElF16, 8>(a, stream) : gated_norm<kElF16, 1>(a, stream);
   return wide ? gated_norm<kElBf16, 8>(a, stream) : gated_norm<kElBf16, 1>(a, stream);

@@ -261,10 +261,10 @@ hipError_t step(const StepArgs& a, float* y, hipStream_t stream) {
     default: e = step_scan<F16, 64>(a, y, stream); break;
   }
   if (e != hipSuccess) return e;
-  // vectors of 8 where every row falls on them
+  // vectors of 8 where every row starts on a word
   const int size = a.nh * a.hd / a.norm_groups;
-  bool wide = a.C % 8 == 0 && size % 8 == 0 && reinterpret_cast<uintptr_t>(a.norm_w) % 16 == 0;
-  for (const HeadsView* v : {&a.xbc, &a.z, &a.out}) wide = wide && on_vectors(*v, 2, 8);
+  bool wide = a.C % 8 == 0 && size % 8 == 0 && on_words(a.norm_w);
+  for (const HeadsView* v : {&a.xbc, &a.z, &a.out}) wide = wide && on_words(*v, 2);
   return wide ? step_norm<F16, 8>(a, y, stream) : step_norm<F16, 1>(a, y, stream);
 }
 

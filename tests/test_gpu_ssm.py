@@ -47,7 +47,8 @@ def _untouched(out, lengths):
     (F16, 2, 17, 40, 3, True, [2, 16], [4, -1], 8), (F32, 2, 9, 12, 2, False, [1, 9], None, 4),
     (BF16, 2, 13, 37, 4, True, [13, 2], None, 3), (F16, 1, 8, 8, 1, True, None, None, 0),
     (F32, 2, 21, 20, 8, True, [3, 21], [1, 0], 1), (BF16, 2, 1, 264, 8, True, None, [0, 9], 0),
-    (F16, 4, 5, 7, 5, False, [0, 1, 4, 5], [3, 2, 1, 0], 2)])
+    (F16, 4, 5, 7, 5, False, [0, 1, 4, 5], [3, 2, 1, 0], 2), (BF16, 2, 19, 96, 4, True, [19, 6], None, 2),
+    (F16, 2, 10, 8, 7, True, None, None, 6)])
 @pytest.mark.parametrize("begun,keep", [(False, "out"), (True, "in place"), (True, "no")])
 def test_conv(gpu, fmx, dtype, B, L, C, taps, silu, lengths, slots, pad, begun, keep):
     g = _gen(L * C + taps)
@@ -391,7 +392,8 @@ def test_scan_infinities_come_late(gpu, fmx):
     (BF16, 1, 1, 4096, 8, None, 8), (F16, 2, 5, 960, 3, [5, 0], 8), (F32, 2, 3, 512, 1, [1, 3], 4),
     (BF16, 1, 4, 4096, 1, None, 0), (F16, 1, 2, 37, 1, None, 3), (F32, 3, 2, 66, 2, None, 1), (BF16, 2, 3, 24, 3, None, 8),
     (BF16, 1, 2, 20000, 1, None, 0), (F32, 1, 2, 9000, 1, None, 0), (BF16, 1, 3, 128, 8, None, 16),
-    (F16, 1, 3, 1536, 1, None, 0), (F32, 1, 1, 1, 1, None, 0)])
+    (F16, 1, 3, 1536, 1, None, 0), (F32, 1, 1, 1, 1, None, 0), (BF16, 2, 5, 768, 4, [4, 5], 2), (F16, 1, 7, 768, 2, None, 6),
+    (BF16, 2, 3, 320, 5, [3, 1], 2), (F32, 1, 9, 320, 10, None, 1), (F16, 3, 11, 640, 8, None, 2), (BF16, 1, 5, 4104, 1, None, 2)])
 @pytest.mark.parametrize("gate", ["first", "last", "none"])
 def test_gated_norm(gpu, fmx, dtype, B, L, C, groups, lengths, pad, gate):
     g = _gen(C + L)
@@ -464,12 +466,12 @@ def _project(seed, dtype, shape, layer):
     (BF16, 3, 2, 128, 1, 64, 2, dict(gate_first=False)), (F16, 2, 6, 24, 3, 256, 8, dict(activation=None, eps=1e-3)),
     (BF16, 2, 1, 8, 1, 8, 4, dict(softplus=True)), (BF16, 2, 64, 64, 8, 16, 4, dict(norm_groups=1)),
     (F16, 2, 160, 64, 1, 8, 4, {}), (BF16, 1, 4, 200, 4, 32, 5, dict(norm_groups=2))])
-@pytest.mark.parametrize("odd", [False, True])
-def test_step(gpu, fmx, dtype, B, nh, hd, groups, N, taps, kw, odd):
+@pytest.mark.parametrize("pad", [0, 3, 2])
+def test_step(gpu, fmx, dtype, B, nh, hd, groups, N, taps, kw, pad):
     layer = _layer(fmx, 3, dtype, nh, hd, groups, N, taps, **kw)
     xbc, dt, z = _project(4, dtype, (B,), layer)
-    if odd:  # rows on no vector
-        xbc, z = _cut(xbc.cpu(), 3, dtype), _cut(z.cpu(), 5, dtype)
+    if pad:  # rows on no word, or on words only
+        xbc, z = _cut(xbc.cpu(), pad, dtype), _cut(z.cpu(), pad + 2, dtype)
     conv_state, state = (torch.randn(*t.shape, generator=_gen(5)).to(t.dtype).cuda() for t in layer.new_states(7))
     slots = [6, 0, 9, 3, -1][:B]
     n = groups * N
