@@ -3,9 +3,10 @@
 //   gate first: u = x silu(z), u / rms(u) w;  otherwise x / rms(x) w silu(z)
 //
 // Bound by HBM: x and z are read and the result is written once. A group is
-// taken whole by 2 to 64 neighbouring lanes or by a workgroup, which keep its
-// products in registers between the sum and the division; longer groups are
-// read a second time.
+// taken whole by 4 to 64 neighbouring lanes or by a workgroup, which keep its
+// products in registers between the sum and the division; groups of more than
+// 1024 vectors are read a second time. 8192 rows of 8 groups of 512 in bf16: 48
+// us in a graph, 4.1 TB/s.
 #include <algorithm>
 
 #include "fmx_ssm_kernels.hpp"
@@ -159,7 +160,8 @@ hipError_t gated_norm(const GatedNormArgs& a, hipStream_t stream) {
   NormPlan pl{static_cast<uint32_t>(items), a.C / a.groups / VEC};
   const int ln = norm_lanes(pl.vecs), per = kGateThreads / ln;
   // Two groups' loads in flight where there are enough for it: 8192 rows of 8
-  // groups of 512 50.4 us (4.0 TB/s) in a graph, one 52.3, four 60.6.
+  // groups of 512 50.4 us in a graph, one 52.3, four 60.6. (Of several vectors
+  // a lane one group's are enough: 16 groups of 256 45, two at once 51.)
   constexpr int kRounds = VEC > 1 ? 2 : 1;
   const int rounds = ln < kGateThreads && (pl.vecs <= ln || ln == kWave) && items >= int64_t{4096} * per ? kRounds : 1;
   const dim3 grid(static_cast<uint32_t>((items + per * rounds - 1) / (per * rounds))), wg(kGateThreads);
