@@ -20,7 +20,7 @@
 // to 8 or 11 bits. Long sequences are cut into segments: a first launch forms
 // each segment's state from 0, a second starts each segment from the sum of
 // those before it.
-// 8192 tokens of 64 heads of 64 rows, 128 columns, 8 groups: 118 us (38 and 93
+// 8192 tokens of 64 heads of 64 rows, 128 columns, 8 groups: 117 us (36 and 90
 // traced alone; a walk of the tokens 7888). A workgroup's chunk takes 12 to 14
 // thousand cycles, of which by count a SIMD's matrix instructions fill 3 (two and three
 // times those of operands rounded once), LDS 4, and vector instructions (splits,
@@ -684,6 +684,7 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
         for (int j = 0; j < 4; ++j) odd |= (w[j] & 0x7fff7fffu) + kUnit;
       }
       int from = kChunk;  // the token from which row i16 is NaN
+      float poison = 0.0f;  // added to its state's decay (a branch that changes the state costs a copy of it)
       const bool spoiled = __any((odd & 0x80008000u) != 0);
       if (spoiled) {
         // Values that are not finite, which the products would carry to the
@@ -704,9 +705,7 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
         }
         from = min(from, __shfl_xor(from, 16));
         from = min(from, __shfl_xor(from, 32));
-        const float nan = from < kChunk ? __builtin_nanf("") : 0.0f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) S[nt] += nan;
+        poison = from < kChunk ? __builtin_nanf("") : 0.0f;
       }
       float u[8];  // what tokens 32 ks + 8 g4 + j bring
       auto incoming = [&](int ks) {
@@ -766,7 +765,7 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
       // ---- the state behind the chunk
       {
         const int col_at0 = afresh(col_base0), col_at1 = afresh(col_base1);
-        const float f = F16 ? st.decay * scale : st.decay;
+        const float f = F16 ? (st.decay + poison) * scale : st.decay + poison;
         if (STATES) seg_decay *= st.decay;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) S[nt] *= f;

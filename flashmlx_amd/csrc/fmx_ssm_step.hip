@@ -11,7 +11,7 @@
 //
 // Bound by HBM: the state is read and written once (256 sequences of 64 heads of
 // 64 rows, 128 columns: 241 us, 4.6 TB/s, of which the second launch, in whose
-// place nothing else runs, takes 17; one sequence 9.7, two launches of one chain
+// place nothing else runs, takes 17; one sequence 9.8, two launches of one chain
 // of loads each).
 #include <algorithm>
 
