@@ -15,21 +15,20 @@
 // three products of matrices and one for the dots, which the heads of a group
 // share. A wave has 16 rows of a head's state in accumulators, whose layout is
 // an operand's as it is; only the weights of x cross waves, through LDS. fp32
-// operands go in as sums of numbers of 8 (bf16) or 11 bits: three of them (24
-// bits) where the state takes them in, two where outputs do, which are rounded
-// to 8 or 11 bits. Long sequences are cut into segments: a first launch forms
-// each segment's state from 0, a second starts each segment from the sum of
-// those before it.
-// 8192 tokens of 64 heads of 64 rows, 128 columns, 8 groups: 117 us (36 and 90
-// traced alone; a walk of the tokens 7888). A workgroup's chunk takes 12 to 14
-// thousand cycles, of which by count a SIMD's matrix instructions fill 3 (two and three
-// times those of operands rounded once), LDS 4, and vector instructions (splits,
-// scales, weights) 4: two waves per SIMD, which is what LDS holds, overlap little
-// of them. Measured and no faster: four waves per SIMD with one
-// buffer, 32 rows per wave without weights through LDS (157 us for 140 then),
-// steps in a launch of their own, the SIMD's two waves in opposite phases (104
-// for 96), one item to a workgroup and two of those to a CU (142 in a graph for
-// 134), groups of instructions interleaved by hand.
+// operands go in as sums of three numbers of bf16, all of their 24 bits; those
+// of float16 that meet b and c as sums of two of float16, scaled, to 2^-23.
+// (With weights, and bf16's state in outputs, in two bf16 numbers, 16 bits, 8192
+// tokens took 116 us for 124, but where terms cancelled outputs were off by
+// hundreds of what a walk of the same tokens is.) Long sequences are cut into
+// segments: a first launch forms each segment's state from 0, a second starts
+// each segment from the sum of those before it.
+// 8192 tokens of 64 heads of 64 rows, 128 columns, 8 groups: 124 us (a walk of
+// the tokens 7888).
+// Measured and no faster, before the weights had a third part: four waves per
+// SIMD with one buffer, 32 rows per wave without weights through LDS (157 us for
+// 140 then), steps in a launch of their own, the SIMD's two waves in opposite
+// phases (104 for 96), one item to a workgroup and two of those to a CU (142 in
+// a graph for 134), groups of instructions interleaved by hand.
 #include <algorithm>
 #include <cstddef>
 
@@ -207,7 +206,6 @@ __device__ inline uint32_t pack_bf16(float a, float b) {
   typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
-__device__ inline float lo_bf16(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ inline float hi_bf16(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
 template <bool F16>
@@ -217,7 +215,8 @@ __device__ inline uint32_t pack_in(float a, float b) {
 
 // Values as a sum of PARTS numbers of bf16, in order: the first ones cut to 8
 // bits (an AND, which is the float as well as what is packed; a conversion and
-// its way back take 14 cycles a pair for 12), the last rounded. Three are exact.
+// its way back take 14 cycles a pair for 12), the last of two rounded. Three
+// are exact, and so are two of a float16.
 template <int PARTS>
 __device__ inline void split_bf16(const float* v, s16x8_t* part) {
   float rest[8];
@@ -242,14 +241,16 @@ __device__ inline void split_bf16(const float* v, s16x8_t* part) {
     part[k] = __builtin_bit_cast(s16x8_t, w);
   }
 }
-// as a sum of two of float16 (22 bits, or to 2^-25 where they are small), of
-// values within 2^15
+// as a sum of two of float16, each rounded: off by 2^-23 of the value or by
+// 2^-25, whichever is more, of values within 2^15
 __device__ inline void split_f16(const float* v, s16x8_t* part) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
   u32x4_t h, l;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const auto a = __builtin_amdgcn_cvt_pkrtz(v[2 * j], v[2 * j + 1]);
-    const auto b = __builtin_amdgcn_cvt_pkrtz(v[2 * j] - static_cast<float>(a[0]), v[2 * j + 1] - static_cast<float>(a[1]));
+    const f16x2_t a = __builtin_convertvector((f32x2_t{v[2 * j], v[2 * j + 1]}), f16x2_t);
+    const f16x2_t b = __builtin_convertvector(
+        (f32x2_t{v[2 * j] - static_cast<float>(a[0]), v[2 * j + 1] - static_cast<float>(a[1])}), f16x2_t);
     h[j] = __builtin_bit_cast(uint32_t, a);
     l[j] = __builtin_bit_cast(uint32_t, b);
   }
@@ -318,6 +319,10 @@ struct ChunkSteps<true> {
 __device__ inline int far_at(int k) { return 8 * k * (k - 1); }
 
 constexpr int kRound = 4;  // chunks whose steps are formed together, one by each wave of a slot
+// Places for them: a round is formed in the middle of the one before it, of
+// which the second half is still needed.
+constexpr int kRing = kRound + kRound / 2;
+constexpr int kWeightParts = 3;  // of bf16: all of the weights' 24 bits
 
 template <int NK, int SLOTS, bool STATES>
 struct ChunkLds {
@@ -326,10 +331,10 @@ struct ChunkLds {
   __attribute__((aligned(16))) uint8_t b[kBufs][kChunk * kRow];
   __attribute__((aligned(16))) uint8_t x[kBufs][SLOTS][kChunk * kTileRows * 2];
   __attribute__((aligned(16))) uint8_t c[STATES ? 1 : kBufs][STATES ? 16 : kChunk * kRow];
-  // weights of the tokens s for token t, in two parts: rows t < 32 of 32
-  // tokens, the others of 64
-  __attribute__((aligned(16))) uint8_t m[STATES ? 1 : SLOTS][STATES ? 1 : 2][STATES ? 16 : 32 * 64 + 32 * 128];
-  ChunkSteps<STATES> steps[2][kRound][SLOTS];
+  // weights of the tokens s for token t, in parts: rows t < 32 of 32 tokens,
+  // the others of 64
+  __attribute__((aligned(16))) uint8_t m[STATES ? 1 : SLOTS][STATES ? 1 : kWeightParts][STATES ? 16 : 32 * 64 + 32 * 128];
+  ChunkSteps<STATES> steps[kRing][SLOTS];
 };
 
 __device__ inline int weight_at(int t, int chunk) {
@@ -442,7 +447,7 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
     const double sum = tree_to_last<64>(own, 0.0, [](double x, double y) { return x + y; });  // (an inclusive scan)
     const double all = readlane_f64(sum, 63);
     auto power = [](double e) { return __builtin_amdgcn_exp2f(static_cast<float>(e)); };
-    ChunkSteps<STATES>& s = lds.steps[ck / kRound & 1][ck % kRound][slot];
+    ChunkSteps<STATES>& s = lds.steps[ck % kRing][slot];
     s.in[lane] = in ? dt * power(all - sum) : 0.0f;
     if (lane == 0) s.decay = power(all);
     if constexpr (!STATES) {
@@ -469,8 +474,8 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
       for (int i = tid; i < static_cast<int>(sizeof(lds.c) / 16); i += kThreads) reinterpret_cast<u32x4_t*>(lds.c)[i] = zero;
   }
   if (!STATES) {  // tokens behind t in a step that t's own are in
-    for (int v = tid; v < SLOTS * 2 * 16 * 2; v += kThreads) {
-      const int c = v % 2, t = v / 2 % 16, part = v / 32 % 2, q = v / 64;
+    for (int v = tid; v < SLOTS * kWeightParts * 16 * 2; v += kThreads) {
+      const int c = v % 2, t = v / 2 % 16, part = v / 32 % kWeightParts, q = v / 32 / kWeightParts;
       *reinterpret_cast<u32x4_t*>(lds.m[q][part] + weight_at(t, 2 + c)) = zero;
       *reinterpret_cast<u32x4_t*>(lds.m[q][part] + weight_at(32 + t, 6 + c)) = zero;
     }
@@ -549,7 +554,7 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
     if (kBufs == 2 && more) load(t0 + kChunk, buf ^ 1);
     const uint8_t* bs = lds.b[buf];
     const uint8_t* xs = lds.x[buf][slot];
-    const ChunkSteps<STATES>* round = lds.steps[ck / kRound & 1][ck % kRound];
+    const ChunkSteps<STATES>* round = lds.steps[ck % kRing];
     const ChunkSteps<STATES>& st = round[slot];
     f32x4_t y[4];
     // float16's operands are scaled, each row by its own power of two: a row
@@ -594,14 +599,15 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
           float v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = F16 ? S[2 * kk + i / 4][i % 4] * scale : S[2 * kk + i / 4][i % 4];
-          s16x8_t part[2];
-          if (F16)
+          constexpr int kParts = F16 ? 2 : 3;
+          s16x8_t part[kParts];
+          if constexpr (F16)
             split_f16(v, part);
           else
-            split_bf16<2>(v, part);
+            split_bf16<3>(v, part);
           read_first();
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
+          for (int k = 0; k < kParts; ++k)
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) y[tt] = mfma_in<F16>(part[k], fc[tt], y[tt]);
         }
@@ -655,12 +661,15 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
               m[i] = __uint_as_float(__float_as_uint(dot[i] * (f * dt[i])) & (s + i <= t ? 0xffffffffu : 0u));
             }
           }
-          const uint32_t h0 = __builtin_amdgcn_perm(__float_as_uint(m[1]), __float_as_uint(m[0]), 0x07060302u);
-          const uint32_t h1 = __builtin_amdgcn_perm(__float_as_uint(m[3]), __float_as_uint(m[2]), 0x07060302u);
-          auto low = [](float v) { return v - hi_bf16(__float_as_uint(v)); };
           const int at = weight_at(t, 2 * ss + (g4 >> 1)) + (g4 & 1) * 8;
-          *reinterpret_cast<u32x2_t*>(lds.m[q][0] + at) = u32x2_t{h0, h1};
-          *reinterpret_cast<u32x2_t*>(lds.m[q][1] + at) = u32x2_t{pack_bf16(low(m[0]), low(m[1])), pack_bf16(low(m[2]), low(m[3]))};
+#pragma unroll
+          for (int k = 0; k < kWeightParts; ++k) {  // cut to 8 bits each
+            *reinterpret_cast<u32x2_t*>(lds.m[q][k] + at) =
+                u32x2_t{__builtin_amdgcn_perm(__float_as_uint(m[1]), __float_as_uint(m[0]), 0x07060302u),
+                        __builtin_amdgcn_perm(__float_as_uint(m[3]), __float_as_uint(m[2]), 0x07060302u)};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] -= hi_bf16(__float_as_uint(m[i]));
+          }
         }
       }
       lds_barrier();  // the weights are in LDS
@@ -740,11 +749,11 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
         const int m_at0 = afresh(m_base0), m_at1 = afresh(m_base1);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          s16x8_t fm[4][2];
+          s16x8_t fm[4][kWeightParts];
 #pragma unroll
           for (int tt = 2 * ks; tt < 4; ++tt)
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < kWeightParts; ++k)
               fm[tt][k] = *reinterpret_cast<const s16x8_t*>(
                   lds.m[slot][k] + (tt < 2 ? m_at0 + tt * 1024 : (m_at1 ^ 64 * ks) + (tt - 2) * 2048));
           read_first();
@@ -757,9 +766,10 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
             split_bf16<2>(v, xq);
           }
 #pragma unroll
-          for (int k = 0; k < (F16 ? 3 : 2); ++k)
+          for (int k = 0; k < (F16 ? 2 : 1) * kWeightParts; ++k)
 #pragma unroll
-            for (int tt = 2 * ks; tt < 4; ++tt) y[tt] = mfma_bf16(xq[k == 2], fm[tt][k % 2], y[tt]);
+            for (int tt = 2 * ks; tt < 4; ++tt)
+              y[tt] = mfma_bf16(xq[k / kWeightParts], fm[tt][k % kWeightParts], y[tt]);
         }
       }
       // ---- the state behind the chunk

@@ -91,8 +91,10 @@ typedef struct fmx_ssm_shape {
  * aligned: state_in NULL: 0; state_out receives S behind the last token, may
  * be state_in; NULL: not kept.
  * S, sums and decays are fp32 or more, out is rounded once. (float16 with more
- * than 8 tokens: to 2^-37 of the largest value in a row of a head's state, and
- * of those that 64 tokens bring to it.) What is infinite or NaN in a token's
+ * than 8 tokens: S, where c takes it into out, is off by 2^-23 of itself and
+ * 2^-37 of its row's largest; dt x with its decay, where b takes it into S, by
+ * 2^-23 of itself and 2^-37 of the row's largest, be it S's or what up to 64
+ * tokens bring.) What is infinite or NaN in a token's
  * rows reaches that token and later ones of its sequence, as either, and none
  * before it; of a state's row, that row. */
 size_t fmx_ssm_scan_workspace_size(const fmx_ssm_shape* shape);
