@@ -152,8 +152,9 @@ int fmx_causal_conv(int dtype, int64_t batch, int64_t seq_len, int64_t channels,
   if (batch == 0 || (seq_len == 0 && (!state_out || state_out == state_in))) return ok();
   const int es = elem_size(dtype);
   fmx_heads x_v{}, out_v{};
+  // (the kernel reads the weights whatever the lengths are)
+  if (!weight) return fail(FMX_ERR_ARG, "weight is NULL");
   if (seq_len > 0) {
-    if (!weight) return fail(FMX_ERR_ARG, "weight is NULL");
     FMX_RC(check_view(x, "x", batch, seq_len, 1, es, 1, &x_v));
     FMX_RC(check_view(out, "out", batch, seq_len, 1, es, 1, &out_v));
     FMX_RC(check_written(out_v, "out", batch, seq_len, 1));

@@ -61,6 +61,16 @@ def test_conv_refusals(lib):
     assert _conv(lib, L=0, x=Heads(data=0), out=Heads(data=0), w=None, s_out=1 << 35) == OK
 
 
+def test_conv_without_tokens_needs_its_weight(lib):
+    """A call without tokens that carries states over runs the kernel, which
+    reads the weights: none is refused, rather than read at address 0."""
+    none = dict(L=0, x=Heads(data=0), out=Heads(data=0), w=None)
+    assert _conv(lib, **none) == ARG  # state_out another array than state_in
+    assert _conv(lib, s_in=None, **none) == ARG
+    assert _conv(lib, s_in=None, s_out=None, **none) == OK  # (nothing runs)
+    assert _conv(lib, taps=1, **none) == OK  # (one tap keeps no state)
+
+
 def _shape(dtype=BF16, B=2, L=3, nh=4, hd=64, g=2, N=128, lo=0.0, hi=math.inf):
     return C.byref(_lib.FmxSsmShape(dtype, B, L, nh, hd, g, N, 1, lo, hi))
 
