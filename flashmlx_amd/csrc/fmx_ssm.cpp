@@ -134,22 +134,20 @@ StepArgs step_args(const fmx_ssm_layer* l, int64_t batch) {
 
 int too_much() { return fail(FMX_ERR_UNSUPPORTED, "more work than launches of fewer than 2^32 threads"); }
 
-}  // namespace
-
-extern "C" {
-
-int fmx_causal_conv(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64_t taps, int activation,
-                    const fmx_heads* x, const void* weight, const void* bias, const void* state_in, void* state_out,
-                    int64_t n_slots, const int32_t* lengths, const int32_t* slots, const fmx_heads* out,
-                    fmx_stream stream) {
-  const int el = element(dtype, true);
-  if (el < 0) return fail(FMX_ERR_DTYPE, "dtype %d (bf16, float16 or float32)", dtype);
+// Each call's checks: what its kernels are handed, and whether there is
+// anything to run. Nothing is launched or allocated.
+int plan_conv(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64_t taps, int activation,
+              const fmx_heads* x, const void* weight, const void* bias, const void* state_in, void* state_out,
+              int64_t n_slots, const int32_t* lengths, const int32_t* slots, const fmx_heads* out, ConvArgs* plan,
+              bool* run) {
+  *run = false;
+  if (element(dtype, true) < 0) return fail(FMX_ERR_DTYPE, "dtype %d (bf16, float16 or float32)", dtype);
   FMX_RC(check_rows(batch, seq_len, n_slots));
   if (channels < 1 || channels > kMaxChannels) return fail(FMX_ERR_SHAPE, "channels %lld (1 .. 2^20)", (long long)channels);
   if (taps < 1 || taps > kMaxTaps) return fail(FMX_ERR_SHAPE, "taps %lld (1 .. %d)", (long long)taps, kMaxTaps);
   if (activation != FMX_ACT_NONE && activation != FMX_ACT_SILU) return fail(FMX_ERR_ARG, "activation %d", activation);
   if (taps == 1) state_in = state_out = nullptr;
-  if (batch == 0 || (seq_len == 0 && (!state_out || state_out == state_in))) return ok();
+  if (batch == 0 || (seq_len == 0 && (!state_out || state_out == state_in))) return FMX_OK;
   const int es = elem_size(dtype);
   fmx_heads x_v{}, out_v{};
   // (the kernel reads the weights whatever the lengths are)
@@ -171,7 +169,8 @@ int fmx_causal_conv(int dtype, int64_t batch, int64_t seq_len, int64_t channels,
   FMX_RC(check_clear(o, {xs, ws, bs, si, so, ls, ss}));
   FMX_RC(check_clear(so, {xs, ws, bs, ls, ss}));
   if (state_out != state_in) FMX_RC(check_clear(so, {si}));
-  ConvArgs a{};
+  ConvArgs& a = *plan;
+  a = ConvArgs{};
   a.B = static_cast<int>(batch);
   a.L = static_cast<int>(seq_len);
   a.C = static_cast<int>(channels);
@@ -187,24 +186,21 @@ int fmx_causal_conv(int dtype, int64_t batch, int64_t seq_len, int64_t channels,
   a.lens = lengths;
   a.slots = slots;
   if (!conv_fits(a)) return too_much();
-  FMX_HIP(launch_conv(a, el, static_cast<hipStream_t>(stream)));
-  return ok();
+  *run = true;
+  return FMX_OK;
 }
 
-size_t fmx_ssm_scan_workspace_size(const fmx_ssm_shape* shape) {
-  if (check_scan_shape(shape, 0) || shape->batch == 0) return 0;
-  return scan_workspace(scan_args(shape));
-}
-
-int fmx_ssm_scan(const fmx_ssm_shape* shape, const fmx_heads* x, const fmx_heads* dt, const float* a,
-                 const fmx_heads* b, const fmx_heads* c, const float* d, const float* dt_bias, const float* state_in,
-                 float* state_out, int64_t n_slots, const int32_t* lengths, const int32_t* slots, const fmx_heads* out,
-                 void* workspace, size_t workspace_bytes, fmx_stream stream) {
+int plan_scan(const fmx_ssm_shape* shape, const fmx_heads* x, const fmx_heads* dt, const float* a, const fmx_heads* b,
+              const fmx_heads* c, const float* d, const float* dt_bias, const float* state_in, float* state_out,
+              int64_t n_slots, const int32_t* lengths, const int32_t* slots, const fmx_heads* out, ScanArgs* plan,
+              bool* run) {
+  *run = false;
   FMX_RC(check_scan_shape(shape, n_slots));
   const int64_t B = shape->batch, L = shape->seq_len, nh = shape->n_heads, hd = shape->head_dim;
   const int64_t G = shape->n_groups, N = shape->state_dim;
-  if (B == 0 || (L == 0 && (!state_out || state_out == state_in))) return ok();
-  ScanArgs s = scan_args(shape);
+  if (B == 0 || (L == 0 && (!state_out || state_out == state_in))) return FMX_OK;
+  ScanArgs& s = *plan;
+  s = scan_args(shape);
   fmx_heads x_v{}, dt_v{}, b_v{}, c_v{}, out_v{};
   if (!a) return fail(FMX_ERR_ARG, "a is NULL");
   if (L > 0) {
@@ -242,23 +238,20 @@ int fmx_ssm_scan(const fmx_ssm_shape* shape, const fmx_heads* x, const fmx_heads
   s.lens = lengths;
   s.slots = slots;
   if (!scan_fits(s)) return too_much();
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  Workspace ws;
-  FMX_RC(ws.bind(workspace, workspace_bytes, scan_workspace(s), st));
-  FMX_HIP(launch_scan(s, shape->dtype == FMX_F16, ws.p, st));
-  return ok();
+  *run = true;
+  return FMX_OK;
 }
 
-int fmx_gated_norm(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64_t n_groups, float eps,
-                   int gate_first, const fmx_heads* x, const fmx_heads* z, const void* weight, const int32_t* lengths,
-                   const fmx_heads* out, fmx_stream stream) {
-  const int el = element(dtype, true);
-  if (el < 0) return fail(FMX_ERR_DTYPE, "dtype %d (bf16, float16 or float32)", dtype);
+int plan_norm(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64_t n_groups, float eps, int gate_first,
+              const fmx_heads* x, const fmx_heads* z, const void* weight, const int32_t* lengths, const fmx_heads* out,
+              GatedNormArgs* plan, bool* run) {
+  *run = false;
+  if (element(dtype, true) < 0) return fail(FMX_ERR_DTYPE, "dtype %d (bf16, float16 or float32)", dtype);
   FMX_RC(check_rows(batch, seq_len, 0));
   if (channels < 1 || channels > kMaxChannels || n_groups < 1 || channels % n_groups)
     return fail(FMX_ERR_SHAPE, "channels %lld (1 .. 2^20) in %lld groups", (long long)channels, (long long)n_groups);
   if (!std::isfinite(eps) || !(eps > 0.0f)) return fail(FMX_ERR_ARG, "eps must be finite and positive");
-  if (batch * seq_len == 0) return ok();
+  if (batch * seq_len == 0) return FMX_OK;
   const int es = elem_size(dtype);
   fmx_heads x_v{}, z_v{}, out_v{};
   FMX_RC(check_view(x, "x", batch, seq_len, 1, es, 1, &x_v));
@@ -270,7 +263,8 @@ int fmx_gated_norm(int dtype, int64_t batch, int64_t seq_len, int64_t channels, 
   if (!same(&out_v, &x_v)) FMX_RC(check_clear(o, {{"x", span(&x_v, batch, seq_len, 1, channels, es)}}));
   if (z && !same(&out_v, &z_v)) FMX_RC(check_clear(o, {{"z", span(&z_v, batch, seq_len, 1, channels, es)}}));
   FMX_RC(check_clear(o, {{"weight", bytes(weight, channels * es)}, {"lengths", flat(lengths, batch)}}));
-  GatedNormArgs a{};
+  GatedNormArgs& a = *plan;
+  a = GatedNormArgs{};
   a.B = static_cast<int>(batch);
   a.L = static_cast<int>(seq_len);
   a.C = static_cast<int>(channels);
@@ -283,7 +277,97 @@ int fmx_gated_norm(int dtype, int64_t batch, int64_t seq_len, int64_t channels, 
   a.w = weight;
   a.lens = lengths;
   if (!gated_norm_fits(a)) return too_much();
-  FMX_HIP(launch_gated_norm(a, el, static_cast<hipStream_t>(stream)));
+  *run = true;
+  return FMX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fmx_causal_conv(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64_t taps, int activation,
+                    const fmx_heads* x, const void* weight, const void* bias, const void* state_in, void* state_out,
+                    int64_t n_slots, const int32_t* lengths, const int32_t* slots, const fmx_heads* out,
+                    fmx_stream stream) {
+  ConvArgs a;
+  bool run;
+  FMX_RC(plan_conv(dtype, batch, seq_len, channels, taps, activation, x, weight, bias, state_in, state_out, n_slots,
+                   lengths, slots, out, &a, &run));
+  if (run) FMX_HIP(launch_conv(a, element(dtype, true), static_cast<hipStream_t>(stream)));
+  return ok();
+}
+
+size_t fmx_ssm_scan_workspace_size(const fmx_ssm_shape* shape) {
+  if (check_scan_shape(shape, 0) || shape->batch == 0) return 0;
+  return scan_workspace(scan_args(shape));
+}
+
+int fmx_ssm_scan(const fmx_ssm_shape* shape, const fmx_heads* x, const fmx_heads* dt, const float* a,
+                 const fmx_heads* b, const fmx_heads* c, const float* d, const float* dt_bias, const float* state_in,
+                 float* state_out, int64_t n_slots, const int32_t* lengths, const int32_t* slots, const fmx_heads* out,
+                 void* workspace, size_t workspace_bytes, fmx_stream stream) {
+  ScanArgs s;
+  bool run;
+  FMX_RC(plan_scan(shape, x, dt, a, b, c, d, dt_bias, state_in, state_out, n_slots, lengths, slots, out, &s, &run));
+  if (!run) return ok();
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  Workspace ws;
+  FMX_RC(ws.bind(workspace, workspace_bytes, scan_workspace(s), st));
+  FMX_HIP(launch_scan(s, shape->dtype == FMX_F16, ws.p, st));
+  return ok();
+}
+
+int fmx_gated_norm(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64_t n_groups, float eps,
+                   int gate_first, const fmx_heads* x, const fmx_heads* z, const void* weight, const int32_t* lengths,
+                   const fmx_heads* out, fmx_stream stream) {
+  GatedNormArgs a;
+  bool run;
+  FMX_RC(plan_norm(dtype, batch, seq_len, channels, n_groups, eps, gate_first, x, z, weight, lengths, out, &a, &run));
+  if (run) FMX_HIP(launch_gated_norm(a, element(dtype, true), static_cast<hipStream_t>(stream)));
+  return ok();
+}
+
+int fmx_ssm_prompt_check(const fmx_ssm_layer* layer, int64_t batch, int64_t seq_len, const fmx_heads* xbc,
+                         const fmx_heads* dt, const fmx_heads* z, void* conv_rows, void* scan_rows, void* conv_state,
+                         float* state, int64_t n_slots, const int32_t* lengths, const int32_t* slots,
+                         const fmx_heads* out) {
+  if (!layer) return fail(FMX_ERR_ARG, "layer is NULL");
+  const fmx_ssm_layer& l = *layer;
+  const fmx_ssm_shape shape{l.dtype, batch, seq_len, l.n_heads, l.head_dim, l.n_groups, l.state_dim, l.dt_softplus,
+                            l.dt_min, l.dt_max};
+  FMX_RC(check_scan_shape(&shape, n_slots));
+  const int64_t d = l.n_heads * l.head_dim, n = l.n_groups * l.state_dim, C = d + 2 * n;
+  uint16_t* v = static_cast<uint16_t*>(conv_rows);
+  const fmx_heads v_rows{v, seq_len * C, C, 0}, y_rows{scan_rows, seq_len * d, d, 0};
+  const fmx_heads x{v, seq_len * C, C, l.head_dim}, b{v ? v + d : v, seq_len * C, C, l.state_dim},
+      c{v ? v + d + n : v, seq_len * C, C, l.state_dim}, y{scan_rows, seq_len * d, d, l.head_dim};
+  ConvArgs conv;
+  ScanArgs scan;
+  GatedNormArgs norm;
+  bool run;
+  FMX_RC(plan_conv(l.dtype, batch, seq_len, C, l.taps, l.activation, xbc, l.conv_weight, l.conv_bias, conv_state,
+                   conv_state, n_slots, lengths, slots, &v_rows, &conv, &run));
+  FMX_RC(plan_scan(&shape, &x, dt, l.a, &b, &c, l.d, l.dt_bias, state, state, n_slots, lengths, slots, &y, &scan, &run));
+  FMX_RC(plan_norm(l.dtype, batch, seq_len, d, l.norm_groups, l.eps, l.gate_first, &y_rows, z, l.norm_weight, lengths,
+                   out, &norm, &run));
+  if (!run) return ok();
+  // each call has looked at its own arrays: here one's outputs against those of the others
+  const int64_t rows = batch * seq_len;
+  const Named cs{"conv_state", bytes(l.taps > 1 ? conv_state : nullptr, n_slots * (l.taps - 1) * C * 2)};
+  const Named ss{"state", flat(state, n_slots * d * l.state_dim)};
+  const Named vs{"conv_rows", bytes(v, rows * C * 2)}, ys{"scan_rows", bytes(scan_rows, rows * d * 2)};
+  const fmx_heads dt_v{scan.dt.p, scan.dt.bs, scan.dt.ts, scan.dt.hs}, z_v{norm.z.p, norm.z.bs, norm.z.ts, 0};
+  const fmx_heads out_v{norm.out.p, norm.out.bs, norm.out.ts, 0};
+  const Named ds{"dt", span(&dt_v, batch, seq_len, l.n_heads, 1, 2)};
+  const Named zs{"z", z ? span(&z_v, batch, seq_len, 1, d, 2) : Span{0, 0}};
+  const Named as{"a", flat(l.a, l.n_heads)}, dd{"d", flat(l.d, l.n_heads)}, db{"dt_bias", flat(l.dt_bias, l.n_heads)};
+  const Named nw{"norm_weight", bytes(l.norm_weight, 2 * d)}, ls{"lengths", flat(lengths, batch)};
+  const Named cw{"conv_weight", bytes(l.conv_weight, 2 * C * l.taps)}, cb{"conv_bias", bytes(l.conv_bias, 2 * C)};
+  FMX_RC(check_clear(cs, {ss, vs, ys, ds, zs, as, dd, db, nw}));
+  FMX_RC(check_clear(ss, {vs, ys, zs, nw, cw, cb}));
+  FMX_RC(check_clear(vs, {ys, ds, zs, as, dd, db, nw}));
+  FMX_RC(check_clear(ys, {zs, nw, cw, cb, ls}));
+  FMX_RC(check_clear(Named{"out", span(&out_v, batch, seq_len, 1, d, 2)}, {cs, ss, cw, cb, as, dd, db}));
   return ok();
 }
 

@@ -212,22 +212,55 @@ class SsmLayer:
         return (torch.zeros((slots, self.taps - 1, self.channels), dtype=self.dtype, device=dev),
                 torch.zeros((slots, self.heads, self.head_dim, self.state_dim), dtype=_F32, device=dev))
 
+    def _here(self, dev: int) -> None:
+        if dev != self._dev:
+            raise ValueError(f"the weights are on cuda:{self._dev}, the rows on cuda:{dev}")
+
     def prompt(self, xbc: torch.Tensor, dt: torch.Tensor, z: Optional[torch.Tensor], conv_state: torch.Tensor,
                state: torch.Tensor, lengths: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Rows xbc [batch, seq_len, channels], dt [batch, seq_len, heads] and
         z [batch, seq_len, heads * head_dim] through causal_conv, ssm_scan and
-        gated_norm, from the slots' states and with them moved on."""
-        _device(xbc, "xbc", "batch, seq_len, channels", 3)
+        gated_norm, from the slots' states and with them moved on. A call that
+        is refused has moved neither."""
+        lib, ty = self.lib, self.dtype
+        dev = _device(xbc, "xbc", "batch, seq_len, channels", 3)
+        self._here(dev)
         B, L, _ = xbc.shape
+        nh, hd, ch, inner = self.heads, self.head_dim, self.channels, self.inner
         n = self.groups * self.state_dim
-        v = causal_conv(xbc, self.conv_weight, self.conv_bias, conv_state, conv_state, lengths, slots, self.activation)
-        y = ssm_scan(v[..., :self.inner].view(B, L, self.heads, self.head_dim), dt, self.a,
-                     v[..., self.inner:self.inner + n].view(B, L, self.groups, self.state_dim),
-                     v[..., self.inner + n:].view(B, L, self.groups, self.state_dim), self.d, self.dt_bias, state, state,
-                     lengths, slots, self.softplus, self.dt_limits)
-        return gated_norm(y.view(B, L, self.inner), self.norm_weight, z, self.eps, self.norm_groups, self.gate_first,
-                          lengths, out)
+        xbc_v, dt_v = _rows(xbc, "xbc", (B, L, ch), ty, dev), _steps(dt, "dt", (B, L, nh), ty, dev)
+        z_v = None if z is None else _rows(z, "z", (B, L, inner), ty, dev)
+        some = conv_state if state is None else state
+        n_slots = 0
+        if some is not None:
+            _tensor(some, "state")
+            n_slots = some.shape[0] if some.dim() > 0 else -1
+        cs = _flat(conv_state, "conv_state", (n_slots, self.taps - 1, ch), ty, dev)
+        st = _flat(state, "state", (n_slots, nh, hd, self.state_dim), _F32, dev)
+        lens, at = _flat(lengths, "lengths", (B,), _I32, dev), _flat(slots, "slots", (B,), _I32, dev)
+        if out is None:
+            out = xbc.new_empty((B, L, inner))
+        out_v = _rows(out, "out", (B, L, inner), ty, dev)
+        # between the calls: the convolution's rows and the scan's
+        v, y = xbc.new_empty((B, L, ch)), xbc.new_empty((B, L, inner))
+        vp, yp = v.data_ptr(), y.data_ptr()
+        _lib.check(lib.fmx_ssm_prompt_check(self._ref, B, L, xbc_v, dt_v, z_v, vp, yp, cs, st, n_slots, lens, at, out_v))
+        c = self._c
+        shape = _byref(FmxSsmShape(c.dtype, B, L, nh, hd, self.groups, self.state_dim, c.dt_softplus, c.dt_min, c.dt_max))
+        ws = _workspace(None, lib.fmx_ssm_scan_workspace_size(shape), xbc)
+        es, stream = xbc.element_size(), _stream(dev)
+        _lib.check(lib.fmx_causal_conv(
+            c.dtype, B, L, ch, self.taps, c.activation, xbc_v, c.conv_weight, c.conv_bias, cs, cs, n_slots, lens, at,
+            _byref(FmxHeads(vp, L * ch, ch, 0)), stream))
+        part = lambda first, size: _byref(FmxHeads(vp and vp + first * es, L * ch, ch, size))  # noqa: E731
+        _lib.check(lib.fmx_ssm_scan(
+            shape, part(0, hd), dt_v, c.a, part(inner, self.state_dim), part(inner + n, self.state_dim), c.d, c.dt_bias, st,
+            st, n_slots, lens, at, _byref(FmxHeads(yp, L * inner, inner, hd)), ws.data_ptr(), ws.numel(), stream))
+        _lib.check(lib.fmx_gated_norm(
+            c.dtype, B, L, inner, c.norm_groups, c.eps, c.gate_first, _byref(FmxHeads(yp, L * inner, inner, 0)), z_v,
+            c.norm_weight, lens, out_v, stream))
+        return out
 
     def step(self, xbc: torch.Tensor, dt: torch.Tensor, z: Optional[torch.Tensor], conv_state: torch.Tensor,
              state: torch.Tensor, slots: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -236,8 +269,7 @@ class SsmLayer:
         [batch, heads] and z [batch, heads * head_dim] (None: no gate), the
         slots' states moved on in place."""
         dev, ty = _device(xbc, "xbc", "batch, channels", 2), self.dtype
-        if dev != self._dev:
-            raise ValueError(f"the weights are on cuda:{self._dev}, the rows on cuda:{dev}")
+        self._here(dev)
         B = xbc.shape[0]
         inner = (B, self.inner)
         _tensor(state, "state")

@@ -157,6 +157,92 @@ def test_step_refusals(lib):
     assert lib.fmx_ssm_step_workspace_size(_layer(), 0) == 0 and lib.fmx_ssm_step_workspace_size(_layer(hd=4), 1) == 0
 
 
+def _prompt(lib, layer=None, B=2, L=3, xbc=None, dt=None, z=None, v=1 << 48, y=1 << 49, cs=1 << 35, st=1 << 36, n_slots=4,
+            lens=None, slots=None, out=None):
+    return lib.fmx_ssm_prompt_check(layer or _layer(), B, L, xbc or Heads(), dt or Heads(hs=1), z, v, y, cs, st, n_slots,
+                                    lens, slots, out or Heads())
+
+
+def test_prompt_refusals(lib):
+    """What any of a prompt's calls refuses, and outputs of one over another's
+    arrays; nothing is launched either way."""
+    assert _prompt(lib) == OK and _prompt(lib, z=Heads()) == OK and _prompt(lib, _layer(taps=1)) == OK
+    assert _prompt(lib, cs=None, st=None, n_slots=0) == OK
+    for empty in (dict(B=0), dict(L=0)):
+        assert _prompt(lib, xbc=Heads(data=0), dt=Heads(data=0), v=None, y=None, out=Heads(data=0), **empty) == OK
+    assert _prompt(lib, _layer(dtype=F32)) == DTYPE and _prompt(lib, _layer(dtype=_lib.FMX_U32)) == DTYPE
+    for bad in (_layer(nh=0), _layer(g=3), _layer(taps=0), _layer(taps=9), _layer(ng=0), _layer(ng=3),
+                _layer(nh=60000, g=1, hd=256)):
+        assert _prompt(lib, bad) == SHAPE
+    for bad in (_layer(hd=12), _layer(N=512)):
+        assert _prompt(lib, bad) == UNSUP
+    for bad in (_layer(act=5), _layer(eps=-1.0), _layer(w=None), _layer(a=None), _layer(lo=2.0, hi=1.0)):
+        assert _prompt(lib, bad) == ARG
+    assert lib.fmx_ssm_prompt_check(None, 1, 1, *[None] * 7, 0, None, None, None) == ARG
+    for bad in (dict(B=-1), dict(L=1 << 25), dict(n_slots=1 << 25), dict(dt=Heads(ts=-1)), dict(out=Heads(bs=-1))):
+        assert _prompt(lib, **bad) == SHAPE, bad
+    for bad in (dict(xbc=Heads(data=0)), dict(dt=Heads(data=0)), dict(z=Heads(data=0)), dict(out=Heads(data=0)), dict(v=None),
+                dict(y=None), dict(v=(1 << 48) + 2), dict(y=(1 << 49) + 8), dict(st=(1 << 36) + 4), dict(cs=(1 << 35) + 1),
+                dict(out=Heads(ts=0)), dict(z=Heads(data=AT), out=Heads(data=AT + 2)),
+                # one call's outputs over another's arrays
+                dict(cs=1 << 36), dict(st=(1 << 35) + 16), dict(z=Heads(data=1 << 35)), dict(z=Heads(data=1 << 36)),
+                dict(dt=Heads(data=1 << 35)), dict(dt=Heads(data=1 << 36)), dict(out=Heads(data=1 << 35)),
+                dict(out=Heads(data=1 << 36)), dict(cs=1 << 34), dict(st=1 << 33), dict(v=1 << 36), dict(y=1 << 35),
+                dict(v=1 << 49), dict(out=Heads(data=1 << 33)), dict(out=Heads(data=1 << 34)), dict(lens=1 << 49)):
+        assert _prompt(lib, **bad) == ARG, bad
+
+
+class _Recorder:
+    """The library's checks and sizes, and the names of what would be launched."""
+
+    def __init__(self, lib):
+        self.lib, self.launched = lib, []
+
+    def __getattr__(self, name):
+        if name not in ("fmx_causal_conv", "fmx_ssm_scan", "fmx_gated_norm", "fmx_ssm_step"):
+            return getattr(self.lib, name)
+        return lambda *args: self.launched.append(name) or OK
+
+
+def test_a_refused_prompt_has_run_nothing(lib, monkeypatch):
+    """On host arrays, with launches recorded instead of made: all three, or none."""
+    import flashmlx_amd.ssm as S
+    rec = _Recorder(lib)
+    monkeypatch.setattr(_lib, "load", lambda: rec)
+    monkeypatch.setattr(S, "_device", lambda t, *_: t.get_device())
+    monkeypatch.setattr(S, "_stream", lambda dev: None)
+    bf, f = torch.bfloat16, torch.float32
+    make = lambda dtype=bf, **kw: S.SsmLayer(  # noqa: E731
+        torch.zeros(48, 4, dtype=dtype), torch.zeros(2), None, **{**dict(head_dim=8, groups=1, state_dim=16), **kw})
+    layer = make()
+    good = dict(xbc=torch.zeros(2, 5, 48, dtype=bf), dt=torch.zeros(2, 5, 2, dtype=bf), z=torch.zeros(2, 5, 16, dtype=bf),
+                conv_state=torch.zeros(3, 3, 48, dtype=bf), state=torch.zeros(3, 2, 8, 16))
+    assert layer.prompt(**good).shape == (2, 5, 16)
+    assert rec.launched == ["fmx_causal_conv", "fmx_ssm_scan", "fmx_gated_norm"]
+    rec.launched.clear()
+    wrong = [dict(dt=good["dt"][:, :4]), dict(dt=good["dt"].to(f)), dict(z=good["z"][..., :8]), dict(z=good["z"].half()),
+             dict(conv_state=good["conv_state"][:2]), dict(conv_state=good["conv_state"].half()),
+             dict(state=good["state"][:, :1]), dict(state=good["state"].double()),
+             dict(state=torch.zeros(3 * 256 + 1)[1:].view(3, 2, 8, 16)), dict(state=good["state"].transpose(2, 3)),
+             dict(out=torch.zeros(2, 5, 8, dtype=bf)), dict(out=torch.zeros(2, 5, 16)),
+             dict(out=torch.zeros(2, 1, 16, dtype=bf).expand(2, 5, 16)), dict(lengths=torch.zeros(2)),
+             dict(slots=torch.zeros(3, dtype=torch.int32)), dict(dt=None), dict(z=3)]
+    shared = torch.zeros(1 << 14, dtype=torch.uint8)  # (the state at its start and what else the call writes there)
+    at = shared[-shared.data_ptr() % 256:]
+    over = at[:3072].view(f).view(3, 2, 8, 16)
+    wrong += [dict(state=over, out=at[:320].view(bf).view(2, 5, 16)), dict(state=over, z=at[:320].view(bf).view(2, 5, 16)),
+              dict(state=over, conv_state=at[:864].view(bf).view(3, 3, 48))]
+    for bad in wrong:
+        with pytest.raises((ValueError, TypeError, _lib.FmxError)):
+            layer.prompt(**{**good, **bad})
+        assert rec.launched == [], bad
+    for other, kw in ((make(eps=0.0), {}), (make(norm_groups=3), {}), (make(dt_limits=(1.0, 0.5)), {}),
+                      (make(f), {k: good[k].to(f) for k in ("xbc", "dt", "z", "conv_state")})):
+        with pytest.raises(_lib.FmxError):
+            other.prompt(**{**good, **kw})
+        assert rec.launched == []
+
+
 def test_python_refusals():
     x = torch.zeros(1, 2, 8)
     for call in (lambda: F.causal_conv(None, x), lambda: F.gated_norm(3), lambda: F.ssm_scan([], *[None] * 4),
