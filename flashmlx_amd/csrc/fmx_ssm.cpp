@@ -185,7 +185,7 @@ int plan_conv(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64
   a.n_slots = n_slots;
   a.lens = lengths;
   a.slots = slots;
-  if (!conv_fits(a)) return too_much();
+  if (!conv_fits(a, element(dtype, true))) return too_much();
   *run = true;
   return FMX_OK;
 }
@@ -276,7 +276,7 @@ int plan_norm(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64
   a.out = view(&out_v);
   a.w = weight;
   a.lens = lengths;
-  if (!gated_norm_fits(a)) return too_much();
+  if (!gated_norm_fits(a, element(dtype, true))) return too_much();
   *run = true;
   return FMX_OK;
 }

@@ -123,26 +123,35 @@ hipError_t conv(const ConvArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+int conv_run(const ConvArgs& a, int vec) {
+  return a.taps - 1 <= kConvShort && conv_threads(a, vec, kConvRun) < kConvFew ? kConvShort : kConvRun;
+}
+
 template <int DT, int VEC>
 hipError_t conv(const ConvArgs& a, hipStream_t stream) {
-  const bool few = a.taps - 1 <= kConvShort && conv_threads(a, VEC, kConvRun) < kConvFew;
-  return few ? conv<DT, VEC, kConvShort>(a, stream) : conv<DT, VEC, kConvRun>(a, stream);
+  return conv_run(a, VEC) == kConvShort ? conv<DT, VEC, kConvShort>(a, stream) : conv<DT, VEC, kConvRun>(a, stream);
 }
 
-}  // namespace
-
-bool conv_fits(const ConvArgs& a) {
-  return conv_threads(a, 1, kConvShort) <= max_blocks(kConvThreads) * kConvThreads;
-}
-
-hipError_t launch_conv(const ConvArgs& a, int dt, hipStream_t stream) {
-  // 16 bytes at once where every row starts on a word (9 sequences of 2127 rows
-  // of 1248 channels, 4440 bytes apart, 33 us, by elements 36), single elements
-  // otherwise
+// 16 bytes at once where every row starts on a word (9 sequences of 2127 rows
+// of 1248 channels, 4440 bytes apart, 33 us, by elements 36), single elements
+// otherwise
+bool conv_wide(const ConvArgs& a, int dt) {
   const int es = dt == kElF32 ? 4 : 2, vec = 16 / es;
   bool wide = a.C % vec == 0 && on_words(a.x, es) && on_words(a.out, es);
   for (const void* p : {a.w, a.bias, a.s_in, static_cast<const void*>(a.s_out)})
     wide = wide && on_words(p);
+  return wide;
+}
+
+}  // namespace
+
+bool conv_fits(const ConvArgs& a, int dt) {
+  const int vec = conv_wide(a, dt) ? (dt == kElF32 ? 4 : 8) : 1;
+  return conv_threads(a, vec, conv_run(a, vec)) <= max_blocks(kConvThreads) * kConvThreads;
+}
+
+hipError_t launch_conv(const ConvArgs& a, int dt, hipStream_t stream) {
+  const bool wide = conv_wide(a, dt);
   if (dt == kElF32) return wide ? conv<kElF32, 4>(a, stream) : conv<kElF32, 1>(a, stream);
   if (dt == kElF16) return wide ? conv<kElF16, 8>(a, stream) : conv<kElF16, 1>(a, stream);
   return wide ? conv<kElBf16, 8>(a, stream) : conv<kElBf16, 1>(a, stream);

@@ -61,7 +61,8 @@ struct ConvArgs {
   const int32_t* lens;
   const int32_t* slots;
 };
-bool conv_fits(const ConvArgs& a);
+// (of all of these: whether the launches that a call makes are within max_blocks)
+bool conv_fits(const ConvArgs& a, int dt);
 hipError_t launch_conv(const ConvArgs& a, int dt, hipStream_t stream);
 
 // ------------------------------------------------------------------ scan
@@ -147,7 +148,7 @@ struct GatedNormArgs {
   const void* w;
   const int32_t* lens;
 };
-bool gated_norm_fits(const GatedNormArgs& a);
+bool gated_norm_fits(const GatedNormArgs& a, int dt);
 hipError_t launch_gated_norm(const GatedNormArgs& a, int dt, hipStream_t stream);
 
 // ------------------------------------------------------------------ a state's rows

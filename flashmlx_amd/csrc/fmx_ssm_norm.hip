@@ -153,18 +153,28 @@ int norm_lanes(int vecs) {
 
 int64_t norm_items(const GatedNormArgs& a) { return static_cast<int64_t>(a.B) * a.L * a.groups; }
 
+// Two groups' loads in flight where there are enough for it: 8192 rows of 8
+// groups of 512 50.4 us in a graph, one 52.3, four 60.6. (Of several vectors
+// a lane one group's are enough: 16 groups of 256 45, two at once 51.)
+constexpr int norm_most_rounds(int vec) { return vec > 1 ? 2 : 1; }
+int norm_rounds(const GatedNormArgs& a, int vec) {
+  const int vecs = a.C / a.groups / vec, ln = norm_lanes(vecs);
+  const bool enough = norm_items(a) >= int64_t{4096} * (kGateThreads / ln);
+  return ln < kGateThreads && (vecs <= ln || ln == kWave) && enough ? norm_most_rounds(vec) : 1;
+}
+int64_t norm_blocks(const GatedNormArgs& a, int vec) {
+  const int at_once = kGateThreads / norm_lanes(a.C / a.groups / vec) * norm_rounds(a, vec);
+  return (norm_items(a) + at_once - 1) / at_once;
+}
+
 template <int DT, int VEC>
 hipError_t gated_norm(const GatedNormArgs& a, hipStream_t stream) {
   const int64_t items = norm_items(a);
   if (items == 0) return hipSuccess;
   NormPlan pl{static_cast<uint32_t>(items), a.C / a.groups / VEC};
-  const int ln = norm_lanes(pl.vecs), per = kGateThreads / ln;
-  // Two groups' loads in flight where there are enough for it: 8192 rows of 8
-  // groups of 512 50.4 us in a graph, one 52.3, four 60.6. (Of several vectors
-  // a lane one group's are enough: 16 groups of 256 45, two at once 51.)
-  constexpr int kRounds = VEC > 1 ? 2 : 1;
-  const int rounds = ln < kGateThreads && (pl.vecs <= ln || ln == kWave) && items >= int64_t{4096} * per ? kRounds : 1;
-  const dim3 grid(static_cast<uint32_t>((items + per * rounds - 1) / (per * rounds))), wg(kGateThreads);
+  constexpr int kRounds = norm_most_rounds(VEC);
+  const int ln = norm_lanes(pl.vecs), rounds = norm_rounds(a, VEC);
+  const dim3 grid(static_cast<uint32_t>(norm_blocks(a, VEC))), wg(kGateThreads);
 #define FMX_NORM(LN, NV, GR) hipLaunchKernelGGL((gated_norm_kernel<DT, VEC, LN, NV, GR>), grid, wg, 0, stream, a, pl)
 #define FMX_NORM_FEW(LN, NV)                        \
   do {                                              \
@@ -190,17 +200,25 @@ hipError_t gated_norm(const GatedNormArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-}  // namespace
-
-bool gated_norm_fits(const GatedNormArgs& a) { return norm_items(a) <= max_blocks(kGateThreads); }
-
-hipError_t launch_gated_norm(const GatedNormArgs& a, int dt, hipStream_t stream) {
-  // 16 bytes at once where every row starts on a word and groups are whole
-  // vectors (19143 rows of 3 groups of 320 in f16, the gate's 4440 bytes apart:
-  // 35 us, by elements 102), single elements otherwise
+// 16 bytes at once where every row starts on a word and groups are whole
+// vectors (19143 rows of 3 groups of 320 in f16, the gate's 4440 bytes apart:
+// 35 us, by elements 102), single elements otherwise
+bool norm_wide(const GatedNormArgs& a, int dt) {
   const int es = dt == kElF32 ? 4 : 2, vec = 16 / es;
   bool wide = a.C / a.groups % vec == 0 && on_words(a.w);
   for (const HeadsView* v : {&a.x, &a.z, &a.out}) wide = wide && on_words(*v, es);
+  return wide;
+}
+
+}  // namespace
+
+// (max_blocks of up to 64 groups twice are fewer than 2^32: the kernel counts them in 32 bits)
+bool gated_norm_fits(const GatedNormArgs& a, int dt) {
+  return norm_blocks(a, norm_wide(a, dt) ? (dt == kElF32 ? 4 : 8) : 1) <= max_blocks(kGateThreads);
+}
+
+hipError_t launch_gated_norm(const GatedNormArgs& a, int dt, hipStream_t stream) {
+  const bool wide = norm_wide(a, dt);
   if (dt == kElF32) return wide ? gated_norm<kElF32, 4>(a, stream) : gated_norm<kElF32, 1>(a, stream);
   if (dt == kElF16) return wide ? gated_norm<kElF16, 8>(a, stream) : gated_norm<kElF16, 1>(a, stream);
   return wide ? gated_norm<kElBf16, 8>(a, stream) : gated_norm<kElBf16, 1>(a, stream);

@@ -134,10 +134,15 @@ int state_rows(int hd, int ln) {
   return r;
 }
 
+// workgroups of a head
+int few_parts(const ScanArgs& a, int ln) {
+  const int rows = kFewThreads / ln * state_rows(a.hd, ln);
+  return (a.hd + rows - 1) / rows;
+}
+
 template <bool F16, int LN>
 hipError_t scan_few(const ScanArgs& a, hipStream_t stream) {
-  const int rp = state_rows(a.hd, LN), rows = kFewThreads / LN * rp;
-  const int parts = (a.hd + rows - 1) / rows;
+  const int rp = state_rows(a.hd, LN), parts = few_parts(a, LN);
   const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.nh * parts)), wg(kFewThreads);
 #define FMX_FEW(RP) hipLaunchKernelGGL((scan_few_kernel<F16, LN, RP>), grid, wg, 0, stream, a, parts)
   if (rp == 1) FMX_FEW(1);
@@ -912,6 +917,18 @@ ScanPlan scan_plan(const ScanArgs& a) {
   return alone || a.rep * p.ck.tiles == 1 ? p : scan_plan(a, 2);
 }
 
+// a launch over `segs` segments: workgroups with work, neighbours on one XCD, and the grid
+struct ChunkGrid {
+  int64_t total, run, blocks;
+};
+ChunkGrid chunk_grid(const ScanArgs& a, const ChunkPlan& c, int segs) {
+  ChunkGrid g;
+  g.total = static_cast<int64_t>(a.B) * segs * a.groups * c.pairs;
+  g.run = std::max<int64_t>(1, std::min<int64_t>(c.pairs, g.total / 64));
+  g.blocks = (g.total + 8 * g.run - 1) / (8 * g.run) * (8 * g.run);
+  return g;
+}
+
 template <bool F16, int NK, int SLOTS>
 hipError_t scan_chunks(const ScanArgs& a, ScanPlan p, float* ws, hipStream_t stream) {
   ChunkPlan& c = p.ck;
@@ -919,10 +936,10 @@ hipError_t scan_chunks(const ScanArgs& a, ScanPlan p, float* ws, hipStream_t str
   float* decays = ws + p.states;
   for (int pass = c.segs > 1 ? 0 : 1; pass < 2; ++pass) {
     c.first_segs = pass ? c.segs : c.segs - 1;
-    c.total = static_cast<uint32_t>(static_cast<int64_t>(a.B) * c.first_segs * a.groups * c.pairs);
-    c.run = std::max(1, std::min<int>(c.pairs, c.total / 64));
-    const uint32_t round = 8 * c.run;
-    const dim3 grid((c.total + round - 1) / round * round), wg(kSlotThreads * SLOTS);
+    const ChunkGrid g = chunk_grid(a, c, c.first_segs);
+    c.total = static_cast<uint32_t>(g.total);
+    c.run = static_cast<int>(g.run);
+    const dim3 grid(static_cast<uint32_t>(g.blocks)), wg(kSlotThreads * SLOTS);
     if (pass)
       hipLaunchKernelGGL((scan_chunk_kernel<F16, NK, SLOTS, false>), grid, wg, 0, stream, a, c, ws, decays);
     else
@@ -958,11 +975,10 @@ bool scan_in_chunks(const ScanArgs& a) {
 size_t scan_workspace(const ScanArgs& a) { return scan_in_chunks(a) ? scan_plan(a).bytes : 0; }
 
 bool scan_fits(const ScanArgs& a) {
-  // (a part of the walk has at least 4 rows; workgroups of chunks have 512
-  // threads, as many as items, segments and a round to fill at most)
-  return static_cast<int64_t>(a.B) * a.nh * ((a.hd + 3) / 4) <= max_blocks(kFewThreads) &&
-         static_cast<int64_t>(a.B) * a.nh * ((a.hd + kTileRows - 1) / kTileRows) + kFullGrid + 8 * 65536 * 4 <=
-             max_blocks(2 * kSlotThreads);
+  if (!scan_in_chunks(a))
+    return static_cast<int64_t>(a.B) * a.nh * few_parts(a, state_lanes(a.N)) <= max_blocks(kFewThreads);
+  const ScanPlan p = scan_plan(a);
+  return chunk_grid(a, p.ck, p.ck.segs).blocks <= max_blocks(kSlotThreads * p.slots);
 }
 
 hipError_t launch_scan(const ScanArgs& a, bool f16, void* ws, hipStream_t stream) {

@@ -213,10 +213,15 @@ int step_rows(int hd, int ln) {
   return r;
 }
 
+// workgroups of a head
+int step_parts(const StepArgs& a, int ln) {
+  const int rows = kStepThreads / ln * step_rows(a.hd, ln);
+  return (a.hd + rows - 1) / rows;
+}
+
 template <bool F16, int LN, int K>
 hipError_t step_scan(const StepArgs& a, float* y, hipStream_t stream) {
-  const int rp = step_rows(a.hd, LN), rows = kStepThreads / LN * rp;
-  const int parts = (a.hd + rows - 1) / rows;
+  const int rp = step_rows(a.hd, LN), parts = step_parts(a, LN);
   const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.B) * a.nh * parts)), wg(kStepThreads);
 #define FMX_STEP(RP) hipLaunchKernelGGL((step_kernel<F16, LN, RP, K>), grid, wg, 0, stream, a, parts, y)
   if (rp == 1) FMX_STEP(1);
@@ -249,6 +254,13 @@ hipError_t step_norm(const StepArgs& a, float* y, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// vectors of 8 where every row starts on a word
+bool step_wide(const StepArgs& a) {
+  bool wide = a.C % 8 == 0 && a.nh * a.hd / a.norm_groups % 8 == 0 && on_words(a.norm_w);
+  for (const HeadsView* v : {&a.xbc, &a.z, &a.out}) wide = wide && on_words(*v, 2);
+  return wide;
+}
+
 template <bool F16>
 hipError_t step(const StepArgs& a, float* y, hipStream_t stream) {
   hipError_t e;
@@ -261,11 +273,7 @@ hipError_t step(const StepArgs& a, float* y, hipStream_t stream) {
     default: e = step_scan<F16, 64>(a, y, stream); break;
   }
   if (e != hipSuccess) return e;
-  // vectors of 8 where every row starts on a word
-  const int size = a.nh * a.hd / a.norm_groups;
-  bool wide = a.C % 8 == 0 && size % 8 == 0 && on_words(a.norm_w);
-  for (const HeadsView* v : {&a.xbc, &a.z, &a.out}) wide = wide && on_words(*v, 2);
-  return wide ? step_norm<F16, 8>(a, y, stream) : step_norm<F16, 1>(a, y, stream);
+  return step_wide(a) ? step_norm<F16, 8>(a, y, stream) : step_norm<F16, 1>(a, y, stream);
 }
 
 }  // namespace
@@ -273,8 +281,8 @@ hipError_t step(const StepArgs& a, float* y, hipStream_t stream) {
 size_t step_workspace(const StepArgs& a) { return static_cast<size_t>(a.B) * a.nh * a.hd * sizeof(float); }
 
 bool step_fits(const StepArgs& a) {
-  return static_cast<int64_t>(a.B) * a.nh * ((a.hd + 3) / 4) <= max_blocks(kStepThreads) &&
-         static_cast<int64_t>(a.B) * a.norm_groups + step_shifts(a, 1) <= max_blocks(kStepThreads);
+  return static_cast<int64_t>(a.B) * a.nh * step_parts(a, step_lanes(a.N)) <= max_blocks(kStepThreads) &&
+         static_cast<int64_t>(a.B) * a.norm_groups + step_shifts(a, step_wide(a) ? 8 : 1) <= max_blocks(kStepThreads);
 }
 
 hipError_t launch_step(const StepArgs& a, bool f16, void* ws, hipStream_t stream) {

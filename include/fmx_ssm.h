@@ -17,8 +17,10 @@
  * int32 [batch], clamped to [0, seq_len]; NULL: seq_len): the tokens of each
  * sequence, the first ones of its rows; what the rows behind them hold does
  * not reach any result, and the output's are left as they are. batch * seq_len at
- * most 2^24. An output must not lie between the first and last element of an
- * input or of another output, except where a call says so.
+ * most 2^24; work that takes launches of 2^32 threads or more (rows of 16-byte
+ * vectors go furthest) is FMX_ERR_UNSUPPORTED. An output must not lie between
+ * the first and last element of an input or of another output, except where a
+ * call says so.
  */
 #ifndef FMX_SSM_H
 #define FMX_SSM_H

@@ -278,3 +278,18 @@ def test_header_is_c(tmp_path):
     src = tmp_path / "h.c"
     src.write_text('#include "fmx_ssm.h"\nint main(void) { fmx_ssm_shape s = {FMX_BF16}; return s.dtype != FMX_BF16; }\n')
     subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-fsyntax-only", f"-I{include}", str(src)], check=True)
+
+
+def test_work_beyond_a_launch(lib):
+    """Workgroups are counted as the kernels deal the work out: one more than a
+    launch of fewer than 2^32 threads takes is refused."""
+    far = {k: Heads(0, 1 << 12, data=1 << at) for k, at in (("x", 50), ("out", 58))}
+    # groups of more than 128 vectors: a workgroup each; single elements: up to 192 of them in a wave's lanes, 4 a workgroup
+    assert _norm(lib, B=1, L=1 << 24, ch=2048, groups=1, **far) == UNSUP
+    assert _norm(lib, B=1, L=1 << 24, ch=600, groups=5, w=(1 << 33) + 2, **far) == UNSUP
+    # the walk: 2^24 workgroups of one head each; chunks: 2^23 of 512 threads
+    views = lambda: {k: Heads(1 << 17, 1 << 13, data=1 << at)  # noqa: E731
+                     for k, at in (("x", 50), ("b", 51), ("c", 52), ("dt", 53), ("out", 54))}
+    no = dict(s_in=None, s_out=None, n_slots=0)
+    assert _scan(lib, _shape(B=1 << 18, L=1, nh=64, g=1), **no, **views()) == UNSUP
+    assert _scan(lib, _shape(B=1 << 18, L=9, nh=64, g=1), **no, **views()) == UNSUP
