@@ -3,11 +3,13 @@
 //   out[t] = act(bias + sum over k of w[k] x[t - taps + 1 + k])  per channel
 //
 // Bound by HBM: every element is read and written once (8191 tokens of 6144
-// channels in fp32 81 us, 4.9 TB/s, a copy's rate; 2048 in bf16 17 us, 2.9 TB/s,
+// channels in fp32 79 us, 5.1 TB/s, a copy's rate; 2048 in bf16 15 us, 3.3 TB/s,
 // one round of workgroups that wait for their loads). A thread takes one
 // vector of channels over a run of tokens, whose taps - 1 rows before it it
 // reads again (from the caches); neighbouring threads take neighbouring
-// channels. The thread of a sequence's first run also keeps the state, so that
+// channels. In fp32 a run's loads are all in flight at once; 16-bit rows are
+// unpacked in the branch that loads them, which waits for each before the next.
+// The thread of a sequence's first run also keeps the state, so that
 // state_out may be state_in: nobody else reads it.
 #include "fmx_ssm_kernels.hpp"
 

@@ -31,7 +31,10 @@ struct alignas(sizeof(T) * N < 4 ? sizeof(T) * N : 4) Pack {
   T e[N];
 };
 
-// v sigmoid(v): hardware exponential and reciprocal, a few steps of 2^-24
+// v sigmoid(v), the argument of the exponential rounded once, hardware
+// exponential and reciprocal: off by (|v| + 4) 2^-23 of itself at most where v is
+// negative, by 4 2^-23 elsewhere; 0 from about -87 down, where the reciprocal is
+// no normal number
 __device__ inline float silu_f32(float v) {
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * 1.4426950408889634f));
 }

@@ -4,7 +4,7 @@
 //
 // scan_few_kernel walks the tokens one by one with the state in registers: the
 // state is read and written once, and that is its time while tokens are few (32
-// sequences of 5 tokens, 32 heads of 128 rows and 64 columns: 20.7 us in a
+// sequences of 5 tokens, 32 heads of 128 rows and 64 columns: 18.7 us in a
 // graph, 4.93 TB/s of a copy would be 14.2; each further token 0.75 us of
 // staging, a chain of adds across lanes and a barrier).
 //
@@ -870,14 +870,15 @@ __global__ __launch_bounds__(kSlotThreads* SLOTS, 2) void scan_chunk_kernel(Scan
 int chunk_steps(int N) { return N <= 32 ? 1 : N <= 64 ? 2 : N <= 128 ? 4 : 8; }
 
 // Tokens that the walk takes. One sequence of 64 heads of 64 rows and 128
-// columns: 8 tokens 12.3 us, 12 15.3, 16 18.1, a chunk 13.0; 16 of them 26, 33,
-// 38 and 33; 16 of 24 heads 18, 22, 26 and 18.
+// columns, in a graph: 8 tokens 9.9 us, 9 11.3, 12 13.1, 16 15.8, a chunk 9.9; 16
+// of them 20, 22, 27, 32 and 25; 16 of 24 heads 8 13.0, 12 16.8, 16 19.8 and 12.7.
 constexpr int kFewMost = 8;
 constexpr int kFullGrid = 256;    // workgroups that fill the CUs (one each, by its LDS)
 // Chunks of a segment up to which a workgroup takes one item rather than two
-// (which halve the reads of b and c and half hide each other's latencies): 64
-// heads of 200 tokens 25 us for 27, of 768 (3 chunks, 2 by two) 34 for 38, of
-// 1024 (4, 2) 39 for 38; 4 sequences of 200 (4, 2) 28 for 34.
+// (which halve the reads of b and c and half hide each other's latencies), in a
+// graph: 64 heads of 200 tokens 20.4 us for 22.8, of 768 (3 chunks, 2 by two)
+// 29.7 for 34.9, of 1024 (4, 2) 34.3 for 34.7; 4 sequences of 200 (4, 2) 23.0 for
+// 29.9.
 constexpr int kAloneChunks = 4;
 
 struct ScanPlan {
@@ -888,9 +889,10 @@ struct ScanPlan {
 };
 
 // Workgroups of `slots` items; as many segments as leave no CU without one and
-// none with two, of 2 chunks at least. (By one build: 16 ragged sequences of 24
-// heads, 192 workgroups, 129 us, in 2 segments 158, in 4 137; 8192 tokens of 64
-// heads in 6 155, in 8 127, in 16 141.)
+// none with two, of 2 chunks at least. (8192 tokens of 64 heads in a graph: whole
+// 584 us, in 2 segments 408, in 4 215, in 6 152, in 8 121, in 16 135; 16 ragged
+// sequences of 24 heads, 192 workgroups: whole 125, in 2 152, in 4 130, in 6 117,
+// in 8 144.)
 ScanPlan scan_plan(const ScanArgs& a, int slots) {
   ScanPlan p{};
   ChunkPlan& c = p.ck;

@@ -10,8 +10,8 @@
 //                     on (only now: the first launch reads it in many places)
 //
 // Bound by HBM: the state is read and written once (256 sequences of 64 heads of
-// 64 rows, 128 columns: 241 us, 4.6 TB/s, of which the second launch, in whose
-// place nothing else runs, takes 17; one sequence 9.8, two launches of one chain
+// 64 rows, 128 columns: 239 us, 4.6 TB/s, of which the second launch, in whose
+// place nothing else runs, takes 17; one sequence 8.1, two launches of one chain
 // of loads each).
 #include <algorithm>
 
@@ -24,7 +24,8 @@ namespace {
 constexpr int kStepThreads = 256;
 
 // Channel ch of the convolution of sequence b, before anything is rounded. K:
-// the taps, whose loads are then all in flight at once; 0: a.taps of them.
+// the taps, whose weights and state rows are then loaded before the first product
+// (behind the row's own element and the bias); 0: a.taps of them, one by one.
 template <bool F16, int K>
 __device__ inline float step_conv(const StepArgs& a, int b, int64_t slot, int ch) {
   const int taps = K ? K : a.taps;
@@ -108,7 +109,8 @@ __global__ __launch_bounds__(kStepThreads) void step_kernel(StepArgs a, int part
 
 // Workgroups [0, norms): a sequence's group each, its products kept in
 // registers (NV vectors of VEC a thread; 0: formed again); the others:
-// vectors of channels' states.
+// vectors of channels' states, whose rows, as many as there are taps at run time,
+// go through private memory where they are vectors of 8.
 template <bool F16, int VEC, int NV>
 __global__ __launch_bounds__(kStepThreads) void step_norm_kernel(StepArgs a, uint32_t norms, const float* y_in) {
   typedef Pack<uint16_t, VEC> V;

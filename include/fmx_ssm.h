@@ -51,7 +51,9 @@ typedef enum fmx_activation {
  *              state_in; NULL: not kept. (Both are ignored for one tap.)
  * x, out: [batch, seq_len, channels], head_stride unused. weight
  * [channels, taps] and bias [channels] (NULL: 0) contiguous. All of dtype:
- * FMX_BF16, FMX_F16 or FMX_F32; sums in fp32, rounded once. taps 1 ..
+ * FMX_BF16, FMX_F16 or FMX_F32; sums in fp32, rounded once. SiLU, v / (1 +
+ * e^-v), is off by 4 2^-23 of itself, and |v| 2^-23 more for negative v, and 0
+ * for v below about -87 (here and as a gate below). taps 1 ..
  * FMX_SSM_MAX_TAPS, channels at most 2^20. */
 int fmx_causal_conv(int dtype, int64_t batch, int64_t seq_len, int64_t channels, int64_t taps,
                     int activation, const fmx_heads* x, const void* weight, const void* bias,

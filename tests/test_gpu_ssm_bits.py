@@ -40,6 +40,21 @@ def _scan(fmx, p, dt_bias=None, state=None):
     return y.double().cpu()[0], after.double().cpu()[0]
 
 
+def test_silu(gpu, fmx):
+    """The documented bound, over the whole range: for negative v the rounded
+    argument of e^-v counts |v| log2 e 2^-24 ln 2 and log2 e's own rounding half of
+    that again, the exponential, the sum, the reciprocal and the product 3.5 2^-23."""
+    v = torch.cat([torch.linspace(-87, 87, 65536), 2.0 ** torch.arange(-60.0, 7), -2.0 ** torch.arange(-60.0, 7)])
+    y = fmx.causal_conv(v.cuda().view(1, -1, 1), torch.ones(1, 1, device="cuda")).double().cpu().flatten()
+    v = v.double()
+    want = v / (1 + torch.exp(-v))
+    off = want.abs() * 2.0 ** -23 * (4 + (-v).clamp(min=0))
+    live = v >= -87
+    assert ((y - want).abs() <= off)[live].all()
+    low = torch.tensor([-87.5, -88.0, -89.0, -100.0, -1e4, -3e38], device="cuda").view(1, -1, 1)
+    assert (fmx.causal_conv(low, torch.ones(1, 1, device="cuda")).abs() < 1e-35).all()
+
+
 SHAPES = [(6, 16, 2, 8), (6, 64, 2, 64), (4, 72, 1, 128), (2, 64, 1, 256)]
 
 
