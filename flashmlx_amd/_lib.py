@@ -419,7 +419,8 @@ _SIGS = {
         [C.c_int] + [C.c_int64] * 4 + [C.c_float, C.c_int, _H, _H] + [C.c_void_p] * 2 + [_H, C.c_void_p]),
     "fmx_ssm_prompt_check": (
         C.c_int,
-        [P(FmxSsmLayer)] + [C.c_int64] * 2 + [_H] * 3 + [C.c_void_p] * 4 + [C.c_int64] + [C.c_void_p] * 2 + [_H]),
+        [P(FmxSsmLayer)] + [C.c_int64] * 2 + [_H] * 3 + [C.c_void_p] * 3 + [C.c_int64, C.c_void_p, C.c_int64] +
+        [C.c_void_p] * 2 + [_H]),
     "fmx_ssm_step_workspace_size": (C.c_size_t, [P(FmxSsmLayer), C.c_int64]),
     "fmx_ssm_step": (
         C.c_int,

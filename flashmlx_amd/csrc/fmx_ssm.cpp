@@ -329,8 +329,8 @@ int fmx_gated_norm(int dtype, int64_t batch, int64_t seq_len, int64_t channels, 
 
 int fmx_ssm_prompt_check(const fmx_ssm_layer* layer, int64_t batch, int64_t seq_len, const fmx_heads* xbc,
                          const fmx_heads* dt, const fmx_heads* z, void* conv_rows, void* scan_rows, void* conv_state,
-                         float* state, int64_t n_slots, const int32_t* lengths, const int32_t* slots,
-                         const fmx_heads* out) {
+                         int64_t conv_slots, float* state, int64_t n_slots, const int32_t* lengths,
+                         const int32_t* slots, const fmx_heads* out) {
   if (!layer) return fail(FMX_ERR_ARG, "layer is NULL");
   const fmx_ssm_layer& l = *layer;
   const fmx_ssm_shape shape{l.dtype, batch, seq_len, l.n_heads, l.head_dim, l.n_groups, l.state_dim, l.dt_softplus,
@@ -346,14 +346,14 @@ int fmx_ssm_prompt_check(const fmx_ssm_layer* layer, int64_t batch, int64_t seq_
   GatedNormArgs norm;
   bool run;
   FMX_RC(plan_conv(l.dtype, batch, seq_len, C, l.taps, l.activation, xbc, l.conv_weight, l.conv_bias, conv_state,
-                   conv_state, n_slots, lengths, slots, &v_rows, &conv, &run));
+                   conv_state, conv_slots, lengths, slots, &v_rows, &conv, &run));
   FMX_RC(plan_scan(&shape, &x, dt, l.a, &b, &c, l.d, l.dt_bias, state, state, n_slots, lengths, slots, &y, &scan, &run));
   FMX_RC(plan_norm(l.dtype, batch, seq_len, d, l.norm_groups, l.eps, l.gate_first, &y_rows, z, l.norm_weight, lengths,
                    out, &norm, &run));
   if (!run) return ok();
   // each call has looked at its own arrays: here one's outputs against those of the others
   const int64_t rows = batch * seq_len;
-  const Named cs{"conv_state", bytes(l.taps > 1 ? conv_state : nullptr, n_slots * (l.taps - 1) * C * 2)};
+  const Named cs{"conv_state", bytes(l.taps > 1 ? conv_state : nullptr, conv_slots * (l.taps - 1) * C * 2)};
   const Named ss{"state", flat(state, n_slots * d * l.state_dim)};
   const Named vs{"conv_rows", bytes(v, rows * C * 2)}, ys{"scan_rows", bytes(scan_rows, rows * d * 2)};
   const fmx_heads dt_v{scan.dt.p, scan.dt.bs, scan.dt.ts, scan.dt.hs}, z_v{norm.z.p, norm.z.bs, norm.z.ts, 0};

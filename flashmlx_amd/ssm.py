@@ -231,12 +231,13 @@ class SsmLayer:
         n = self.groups * self.state_dim
         xbc_v, dt_v = _rows(xbc, "xbc", (B, L, ch), ty, dev), _steps(dt, "dt", (B, L, nh), ty, dev)
         z_v = None if z is None else _rows(z, "z", (B, L, inner), ty, dev)
-        some = conv_state if state is None else state
-        n_slots = 0
-        if some is not None:
-            _tensor(some, "state")
-            n_slots = some.shape[0] if some.dim() > 0 else -1
-        cs = _flat(conv_state, "conv_state", (n_slots, self.taps - 1, ch), ty, dev)
+        pools = []
+        for t, name, dims in ((conv_state, "conv_state", 3), (state, "state", 4)):
+            if t is not None:
+                _tensor(t, name)
+            pools.append(0 if t is None else t.shape[0] if t.dim() == dims else -1)
+        conv_slots, n_slots = pools
+        cs = _flat(conv_state, "conv_state", (conv_slots, self.taps - 1, ch), ty, dev)
         st = _flat(state, "state", (n_slots, nh, hd, self.state_dim), _F32, dev)
         lens, at = _flat(lengths, "lengths", (B,), _I32, dev), _flat(slots, "slots", (B,), _I32, dev)
         if out is None:
@@ -245,13 +246,14 @@ class SsmLayer:
         # between the calls: the convolution's rows and the scan's
         v, y = xbc.new_empty((B, L, ch)), xbc.new_empty((B, L, inner))
         vp, yp = v.data_ptr(), y.data_ptr()
-        _lib.check(lib.fmx_ssm_prompt_check(self._ref, B, L, xbc_v, dt_v, z_v, vp, yp, cs, st, n_slots, lens, at, out_v))
+        _lib.check(lib.fmx_ssm_prompt_check(self._ref, B, L, xbc_v, dt_v, z_v, vp, yp, cs, conv_slots, st, n_slots, lens, at,
+                                            out_v))
         c = self._c
         shape = _byref(FmxSsmShape(c.dtype, B, L, nh, hd, self.groups, self.state_dim, c.dt_softplus, c.dt_min, c.dt_max))
         ws = _workspace(None, lib.fmx_ssm_scan_workspace_size(shape), xbc)
         es, stream = xbc.element_size(), _stream(dev)
         _lib.check(lib.fmx_causal_conv(
-            c.dtype, B, L, ch, self.taps, c.activation, xbc_v, c.conv_weight, c.conv_bias, cs, cs, n_slots, lens, at,
+            c.dtype, B, L, ch, self.taps, c.activation, xbc_v, c.conv_weight, c.conv_bias, cs, cs, conv_slots, lens, at,
             _byref(FmxHeads(vp, L * ch, ch, 0)), stream))
         part = lambda first, size: _byref(FmxHeads(vp and vp + first * es, L * ch, ch, size))  # noqa: E731
         _lib.check(lib.fmx_ssm_scan(

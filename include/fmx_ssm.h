@@ -159,13 +159,14 @@ typedef struct fmx_ssm_layer {
  * of them moves a state: fmx_causal_conv of xbc into conv_rows, fmx_ssm_scan of
  * conv_rows' parts into scan_rows, fmx_gated_norm of scan_rows into out, states
  * in place; and outputs of one over what another reads. Launches nothing; taps
- * may be 1. conv_rows [batch, seq_len, channels] and scan_rows [batch, seq_len,
+ * may be 1, and conv_state's pool of conv_slots another size than state's of
+ * n_slots. conv_rows [batch, seq_len, channels] and scan_rows [batch, seq_len,
  * n_heads * head_dim] contiguous, 16-byte aligned. */
 int fmx_ssm_prompt_check(const fmx_ssm_layer* layer, int64_t batch, int64_t seq_len,
                          const fmx_heads* xbc, const fmx_heads* dt, const fmx_heads* z,
-                         void* conv_rows, void* scan_rows, void* conv_state, float* state,
-                         int64_t n_slots, const int32_t* lengths, const int32_t* slots,
-                         const fmx_heads* out);
+                         void* conv_rows, void* scan_rows, void* conv_state, int64_t conv_slots,
+                         float* state, int64_t n_slots, const int32_t* lengths,
+                         const int32_t* slots, const fmx_heads* out);
 
 /* fmx_causal_conv, fmx_ssm_scan and fmx_gated_norm of one token of each
  * sequence, states updated in place, in fp32 from the rows to the output,

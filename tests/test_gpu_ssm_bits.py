@@ -119,3 +119,12 @@ def test_tokens_keep_their_bits(gpu, fmx, dtype, L, first, second, nh, hd, group
     assert ((after[..., col + 1] - step[:, None]).abs() <= off).all()
     rest = [n for n in range(N) if n not in (col, col + 1)]
     assert (after[..., rest] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("first,second", [(3, 40), (70, 900), (300, 310), (511, 640)])
+@pytest.mark.parametrize("nh,hd,groups,N", [(258, 8, 2, 64), (130, 16, 130, 128), (132, 24, 66, 256)])
+def test_bits_over_many_chunks(gpu, fmx, dtype, first, second, nh, hd, groups, N):
+    """16 chunks in a row, two heads to a workgroup and one."""
+    test_tokens_keep_their_bits(gpu, fmx, dtype, 1000, first, second, nh, hd, groups, N)
+    test_a_state_keeps_its_bits_into_outputs(gpu, fmx, dtype, 1000, nh, hd, groups, N)

@@ -68,6 +68,12 @@ def test_a_prompt_is_its_three_calls(gpu, fmx, dtype, taps, L, lengths, slots, g
     want = fmx.gated_norm(y.flatten(2), layer.norm_weight, z, groups=2, gate_first=False, lengths=at[0],
                           out=torch.full_like(p["z"], 7.0))
     assert torch.equal(got, want) and torch.equal(conv_state, p["conv_state"]) and torch.equal(state, p["state"])
+    if taps > 1 and L:  # pools of two sizes: the second sequence's slot is in one of them alone
+        one, slot = torch.zeros_like(conv_state[:1]), torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+        layer.prompt(p["xbc"], p["dt"], z, one, state, at[0], slot, out=out)
+        both = torch.zeros_like(conv_state), p["state"]
+        assert torch.equal(layer.prompt(p["xbc"], p["dt"], z, *both, at[0], slot, out=want), out)
+        assert torch.equal(one[0], both[0][0]) and torch.equal(state, both[1])
     if lengths is None:
         assert torch.equal(layer.prompt(p["xbc"], p["dt"], z, torch.zeros_like(conv_state), torch.zeros_like(state)),
                            layer.prompt(p["xbc"], p["dt"], z, None, None))

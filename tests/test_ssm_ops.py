@@ -158,9 +158,9 @@ def test_step_refusals(lib):
 
 
 def _prompt(lib, layer=None, B=2, L=3, xbc=None, dt=None, z=None, v=1 << 48, y=1 << 49, cs=1 << 35, st=1 << 36, n_slots=4,
-            lens=None, slots=None, out=None):
-    return lib.fmx_ssm_prompt_check(layer or _layer(), B, L, xbc or Heads(), dt or Heads(hs=1), z, v, y, cs, st, n_slots,
-                                    lens, slots, out or Heads())
+            conv_slots=None, lens=None, slots=None, out=None):
+    return lib.fmx_ssm_prompt_check(layer or _layer(), B, L, xbc or Heads(), dt or Heads(hs=1), z, v, y, cs,
+                                    n_slots if conv_slots is None else conv_slots, st, n_slots, lens, slots, out or Heads())
 
 
 def test_prompt_refusals(lib):
@@ -178,8 +178,8 @@ def test_prompt_refusals(lib):
         assert _prompt(lib, bad) == UNSUP
     for bad in (_layer(act=5), _layer(eps=-1.0), _layer(w=None), _layer(a=None), _layer(lo=2.0, hi=1.0)):
         assert _prompt(lib, bad) == ARG
-    assert lib.fmx_ssm_prompt_check(None, 1, 1, *[None] * 7, 0, None, None, None) == ARG
-    for bad in (dict(B=-1), dict(L=1 << 25), dict(n_slots=1 << 25), dict(dt=Heads(ts=-1)), dict(out=Heads(bs=-1))):
+    assert lib.fmx_ssm_prompt_check(None, 1, 1, *[None] * 6, 0, None, 0, None, None, None) == ARG
+    for bad in (dict(B=-1), dict(L=1 << 25), dict(n_slots=1 << 25), dict(conv_slots=-1), dict(dt=Heads(ts=-1)), dict(out=Heads(bs=-1))):
         assert _prompt(lib, **bad) == SHAPE, bad
     for bad in (dict(xbc=Heads(data=0)), dict(dt=Heads(data=0)), dict(z=Heads(data=0)), dict(out=Heads(data=0)), dict(v=None),
                 dict(y=None), dict(v=(1 << 48) + 2), dict(y=(1 << 49) + 8), dict(st=(1 << 36) + 4), dict(cs=(1 << 35) + 1),
@@ -221,7 +221,7 @@ def test_a_refused_prompt_has_run_nothing(lib, monkeypatch):
     assert rec.launched == ["fmx_causal_conv", "fmx_ssm_scan", "fmx_gated_norm"]
     rec.launched.clear()
     wrong = [dict(dt=good["dt"][:, :4]), dict(dt=good["dt"].to(f)), dict(z=good["z"][..., :8]), dict(z=good["z"].half()),
-             dict(conv_state=good["conv_state"][:2]), dict(conv_state=good["conv_state"].half()),
+             dict(conv_state=good["conv_state"][:, :2]), dict(conv_state=good["conv_state"][0]), dict(conv_state=good["conv_state"].half()),
              dict(state=good["state"][:, :1]), dict(state=good["state"].double()),
              dict(state=torch.zeros(3 * 256 + 1)[1:].view(3, 2, 8, 16)), dict(state=good["state"].transpose(2, 3)),
              dict(out=torch.zeros(2, 5, 8, dtype=bf)), dict(out=torch.zeros(2, 5, 16)),
