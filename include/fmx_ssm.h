@@ -118,7 +118,8 @@ int fmx_ssm_scan(const fmx_ssm_shape* shape, const fmx_heads* x, const fmx_heads
  *   otherwise:               out = x / rms(x) weight gate
  * z NULL: no gate. x, z, out [batch, seq_len, channels], head_stride unused;
  * weight [channels] (NULL: 1); all of dtype: FMX_BF16, FMX_F16 or FMX_F32.
- * fp32 throughout, rounded once. channels a multiple of n_groups, at most
+ * fp32 throughout, rounded once (a sum of squares beyond fp32 makes its rms
+ * infinite). channels a multiple of n_groups, at most
  * 2^20; eps positive. out may be x or z, with the same strides. */
 int fmx_gated_norm(int dtype, int64_t batch, int64_t seq_len, int64_t channels,
                    int64_t n_groups, float eps, int gate_first, const fmx_heads* x,

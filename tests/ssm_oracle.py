@@ -81,9 +81,9 @@ def scan(x, dt, dt_rel, a, b, c, d=None, state=None, n_slots=0, lengths=None, sl
     2^-21, and a sum's roundings by 2^-22 of Sa; where 64 tokens are summed by
     matrix instructions, three products each (the incoming rows in three parts
     of 8 bits, 24 in all), 3 * 64 * 2^-23 of Sa once more. An output: sums of N
-    terms (2^-23 each), the state or the weights of a chunk's tokens in two
-    parts (16 bits: 2^-16 of the magnitudes with what they leave out of each
-    other)."""
+    terms (2^-23 each), and 2^-16 of the magnitudes, which is more than the
+    state and the weights of a chunk's tokens need, whose bits are held by
+    numbers that cancel in tests of their own."""
     B, L, nh, hd = x.shape
     N = b.shape[3]
     rep = nh // b.shape[2]
