@@ -229,7 +229,7 @@ def test_a_refused_prompt_has_run_nothing(lib, monkeypatch):
              dict(slots=torch.zeros(3, dtype=torch.int32)), dict(dt=None), dict(z=3)]
     shared = torch.zeros(1 << 14, dtype=torch.uint8)  # (the state at its start and what else the call writes there)
     at = shared[-shared.data_ptr() % 256:]
-    over = at[:3072].view(f).view(3, 2, 8, 16)
+    over = at[:good["state"].nbytes].view(f).view(3, 2, 8, 16)
     wrong += [dict(state=over, out=at[:320].view(bf).view(2, 5, 16)), dict(state=over, z=at[:320].view(bf).view(2, 5, 16)),
               dict(state=over, conv_state=at[:864].view(bf).view(3, 3, 48))]
     for bad in wrong:
